@@ -226,6 +226,52 @@ TF_API int tf_scatter_nd(const void* updates, void* data, const int64_t* indices
                          const int64_t* data_dims, int rank, int64_t num_index_rows,
                          int index_depth, int dtype, void* stream);
 
+/* C[M,N] = scale_a[m] * scale_b[n] * sum_k A[m,k] * B[n,k] of 8-bit integers: A [M,K] and B [N,K] int8, row-major; scale_a [M] and
+ * scale_b [N] fp32; C [M,N] of c_dtype (fp32, fp16 or bf16).  The sum is exact (int32), hence K <= 131071; it is scaled in fp32 and
+ * rounded once.  M = 0 and N = 0 are done at once.  (No counterpart in the reference.) */
+TF_API int tf_gemm_int8(const void* A, const void* B, const float* scale_a, const float* scale_b, void* C, int c_dtype,
+                        int64_t M, int64_t N, int64_t K, void* stream);
+/* Rows of x [rows,K] (fp16 or bf16) in 8 bits: scale[r] = max|x[r]| / 127 in fp32, q[r,k] the whole number nearest to
+ * x[r,k] / scale[r], the even one in the middle of two.  A row of zeros has scale 0 and q 0, a row with an infinity or a
+ * NaN scale NaN and q 0.  rows < 2^24. */
+TF_API int tf_quantize_rows(const void* x, void* q, float* scale, int dtype, int64_t rows, int64_t K, void* stream);
+
+/* act(g), g in fp32 */
+typedef enum {
+  TF_ACT_SILU = 0,     /* g / (1 + exp(-g)) */
+  TF_ACT_GELU = 1,     /* g * (1 + erf(g / sqrt(2))) / 2 */
+  TF_ACT_GELU_TANH = 2 /* g * (1 + tanh(sqrt(2 / pi) * (g + 0.044715 g^3))) / 2 */
+} tf_activation_t;
+
+/* h[M,F] = act(gate) * up, gate = x * w_gate^T, up = x * w_up^T: x [M,K], w_gate and w_up [F,K], all of dtype (fp16 or bf16),
+ * row-major.  gate and up are kept in fp32 up to the product and rounded to dtype where the caller hands over room for them ([M,F] each,
+ * both or neither), for tf_gated_ffn_backward.  M <= 2^22 - 64 and K <= 2^22 - 64, F <= 2^21 - 64. */
+TF_API int tf_gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up, int dtype,
+                        int activation, int64_t M, int64_t F, int64_t K, void* stream);
+/* Gradients of x [M,K], w_gate and w_up [F,K] from that of h (dh [M,F]) and the gate and up values that the forward call kept.  The
+ * workspace begins at a 16-byte boundary and may hold anything; it is done with when the call's work is.  w_up's gradient right behind
+ * w_gate's makes one product of the two.  M = 0: the weights' gradients are zero. */
+TF_API size_t tf_gated_ffn_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
+TF_API int tf_gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const void* gate,
+                                 const void* up, void* dx, void* dw_gate, void* dw_up, int dtype, int activation, int64_t M,
+                                 int64_t F, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of the logits hidden [T,K] * weight [V,K]^T, which are never in memory: lse[t] = log sum_v exp(logit[t,v]),
+ * loss[t] = lse[t] - logit[t,target[t]], both fp32; hidden and weight fp16 or bf16.  loss is 0 where target[t] == ignore_index and NaN where it
+ * is any other number outside 0 .. V-1.  T <= 2^22 - 64, V <= 2^30 - 64, K <= 2^22 - 64. */
+TF_API size_t tf_linear_cross_entropy_workspace_bytes(int64_t T, int64_t V, int64_t K);
+TF_API int tf_linear_cross_entropy(const void* hidden, const void* weight, const int64_t* target, float* loss, float* lse,
+                                   int dtype, int64_t T, int64_t V, int64_t K, int64_t ignore_index, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+/* Gradients of hidden and weight (both of dtype) from grad_loss [T] (fp32) and the lse of the forward call.  Ignored tokens have none,
+ * whatever their grad_loss; tokens with a target outside the vocabulary make NaN of every row of grad_weight and of their row of grad_hidden.
+ * The vocabulary is done in pieces, which the workspace has room for.  T = 0: grad_weight is zero. */
+TF_API size_t tf_linear_cross_entropy_backward_workspace_bytes(int64_t T, int64_t V, int64_t K);
+TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* hidden, const void* weight, const int64_t* target,
+                                            const float* lse, void* grad_hidden, void* grad_weight, int dtype, int64_t T,
+                                            int64_t V, int64_t K, int64_t ignore_index, void* workspace, size_t workspace_bytes,
+                                            void* stream);
+
 /* What a call would run, decided on the host from the sizes alone; nothing is launched.
  * tf_gemm_kernel_index, with operands at 16-byte boundaries: position of the kernel in the table kGemmKernels (csrc/gemm.hip), or behind
  * its end 0 for the bounds-checked kernel, from 1 on for the whole-line forms of kLinesKernels, then for the tile of 160 x 128, K a

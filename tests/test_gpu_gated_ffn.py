@@ -1,0 +1,239 @@
+"""The gated feed-forward block against its 64-bit form, forward and backward."""
+
+import pytest
+import torch
+
+from tests import product_ref as ref
+from tilefusion_amd import _capi, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float16, torch.bfloat16]
+ACTIVATIONS = ["silu", "gelu", "gelu_tanh"]
+
+
+def _randn(g, *shape, dtype, scale=1.0):
+    return (torch.randn(*shape, device=DEV, generator=g) * scale).to(dtype)
+
+
+def _block(m, f, k, dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed + m * 5 + f * 3 + k)
+    return _randn(g, m, k, dtype=dtype), _randn(g, f, k, dtype=dtype, scale=k ** -0.5), _randn(g, f, k, dtype=dtype, scale=k ** -0.5), g
+
+
+def _check_forward(x, w_gate, w_up, activation):
+    want, bounds = ref.gated_ffn(x.reshape(-1, x.shape[-1]), w_gate, w_up, activation)
+    shape = (*x.shape[:-1], w_gate.shape[0])
+    kept = ops.gated_ffn(x, w_gate, w_up, activation, keep=True)
+    alone = ops.gated_ffn(x, w_gate, w_up, activation)
+    assert alone.shape == shape and torch.equal(alone, kept[0])
+    for name, got, w, b in zip(("h", "gate", "up"), kept, want, bounds):
+        assert got.shape == shape and got.dtype == x.dtype
+        ref.assert_within(got.reshape(w.shape), w, b, f"{name} {tuple(x.shape)} F={w_gate.shape[0]} {x.dtype} {activation}")
+
+
+SIZES = [
+    (1, 1, 1), (1, 1, 8), (1, 16, 64), (1, 512, 4096), (2, 33, 40), (3, 257, 1000), (7, 100, 33), (16, 64, 256), (17, 96, 72), (32, 1000, 512), (64, 64, 64),
+    (65, 63, 127), (128, 64, 128), (129, 65, 136), (128, 256, 1024), (200, 128, 64), (255, 129, 264), (256, 128, 256), (257, 300, 520), (300, 1544, 1032),
+    (513, 1030, 96), (1111, 770, 328),
+]
+
+
+@pytest.mark.parametrize("m,f,k", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_forward_sizes(m, f, k, dtype):
+    x, w_gate, w_up, _ = _block(m, f, k, dtype)
+    _check_forward(x, w_gate, w_up, "silu")
+
+
+@pytest.mark.parametrize("m,f,k", [(1, 200, 128), (40, 136, 72), (150, 200, 264), (300, 256, 512), (9, 31, 15)])
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_forward_activations(m, f, k, activation, dtype):
+    x, w_gate, w_up, _ = _block(m, f, k, dtype, seed=1)
+    _check_forward(x * 3, w_gate, w_up, activation)
+
+
+def test_forward_shapes_strides_alignment():
+    g = torch.Generator(device=DEV).manual_seed(2)
+    base = _randn(g, 6, 5, 80, dtype=torch.float16)
+    w = _randn(g, 64, 100, dtype=torch.float16, scale=0.1)
+    _check_forward(base, w[:, :80], w[:, 20:], "silu")              # leading dimensions, strided weights
+    _check_forward(base.transpose(0, 1), w[:, :80], w[:, 20:], "silu")
+    _check_forward(base[0, 0], w[:, :80], w[:, 20:], "silu")         # one token, no leading dimension
+    flat = _randn(g, 70 * 128 + 1, dtype=torch.float16)
+    _check_forward(flat[1:].view(70, 128), flat[1:64 * 128 + 1].view(64, 128), flat[:64 * 128].view(64, 128), "gelu")   # odd addresses
+    both = _randn(g, 2 * 96, 128, dtype=torch.bfloat16, scale=0.1)   # one tensor that holds both weights
+    _check_forward(_randn(g, 130, 128, dtype=torch.bfloat16), both[:96], both[96:], "silu")
+    _check_forward(_randn(g, 130, 128, dtype=torch.bfloat16), both[96:], both[:96], "silu")
+    _check_forward(_randn(g, 130, 128, dtype=torch.bfloat16), both[:96], both[:96], "silu")   # the same weight twice
+
+
+def test_forward_infinities_and_nan_stay_in_their_rows():
+    x, w_gate, w_up, _ = _block(200, 160, 136, torch.bfloat16)
+    clean = ops.gated_ffn(x, w_gate, w_up)
+    x[3, 7] = float("nan")
+    x[150, 0] = float("inf")
+    x[199, 135] = -float("inf")
+    h = ops.gated_ffn(x, w_gate, w_up)
+    rows = torch.ones(200, dtype=torch.bool, device=DEV)
+    rows[[3, 150, 199]] = False
+    assert torch.equal(h[rows], clean[rows]) and h[3].isnan().all() and not h[[150, 199]].isfinite().all()
+
+
+def test_large_gates():
+    # far out on both sides the activations are 0 and the identity
+    x = torch.tensor([[1.0], [-1.0]], device=DEV, dtype=torch.bfloat16)
+    w_gate = torch.tensor([[50.0], [1e4], [1e20], [3e38]], device=DEV).bfloat16()
+    w_up = torch.ones(4, 1, device=DEV).bfloat16()
+    for activation in ACTIVATIONS:
+        h, gate, up = ops.gated_ffn(x, w_gate, w_up, activation, keep=True)
+        # (silu(-50) = -50 exp(-50) = -9.64e-21, the others' are smaller)
+        assert torch.equal(h[0], w_gate[:, 0]) and (h[1].abs() <= 9.7e-21).all()
+        one = torch.ones_like(h)
+        grads = ops.gated_ffn_backward(one, x, w_gate, w_up, gate, up, activation)
+        # (x[0]'s gradient is the sum of w_gate and of act(w_gate), 6e38, which is infinite in the type)
+        assert all(t.isfinite().all() for t in (grads[0][1], grads[1], grads[2])) and grads[0][0] == float("inf")
+
+
+# ---- backward ------------------------------------------------------------------------------
+def _check_backward(grad_h, x, w_gate, w_up, gate, up, activation):
+    got = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation)
+    f, k = w_gate.shape
+    want, bounds = ref.gated_ffn_backward(grad_h.reshape(-1, f), x.reshape(-1, k), w_gate, w_up, gate.reshape(-1, f), up.reshape(-1, f), activation)
+    for name, g, w, b, like in zip(("grad_x", "grad_w_gate", "grad_w_up"), got, want, bounds, (x, w_gate, w_up)):
+        assert g.shape == like.shape and g.dtype == x.dtype
+        what = f"{name} {tuple(x.shape)} F={f} {x.dtype} {activation}"
+        ref.assert_within(g.reshape(w.shape), w, b, what)
+        # errors of many roundings are independent: in all far less than every one at its largest
+        assert (g.reshape(w.shape).double() - w).norm() <= 2 * ref.half_step(x.dtype) * w.norm(), what
+
+
+BACKWARD_SIZES = [(1, 1, 1), (1, 64, 64), (3, 17, 9), (31, 100, 33), (64, 64, 64), (65, 127, 72), (130, 96, 200), (257, 136, 264), (400, 513, 104), (1000, 160, 1032)]
+
+
+@pytest.mark.parametrize("m,f,k", BACKWARD_SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_sizes(m, f, k, dtype):
+    x, w_gate, w_up, g = _block(m, f, k, dtype, seed=4)
+    _check_backward(*(_randn(g, m, f, dtype=dtype) for _ in range(1)), x, w_gate, w_up, _randn(g, m, f, dtype=dtype), _randn(g, m, f, dtype=dtype), "silu")
+
+
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_activations(activation, dtype):
+    x, w_gate, w_up, g = _block(150, 200, 88, dtype, seed=5)
+    grad_h = _randn(g, 150, 200, dtype=dtype)
+    _, gate, up = ops.gated_ffn(x * 2, w_gate, w_up, activation, keep=True)
+    _check_backward(grad_h, x * 2, w_gate, w_up, gate, up, activation)
+
+
+def test_backward_shapes_strides_and_empty():
+    g = torch.Generator(device=DEV).manual_seed(6)
+    dtype = torch.float16
+    x, w = _randn(g, 3, 11, 48, dtype=dtype), _randn(g, 2, 72, 48, dtype=dtype, scale=0.2)
+    tall = _randn(g, 3, 72, 11, dtype=dtype)
+    _check_backward(tall.transpose(1, 2), x, w[0], w[1], tall.transpose(1, 2) * 2, tall.flip(0).transpose(1, 2), "silu")
+    flat = _randn(g, 33 * 72 + 1, dtype=dtype)
+    odd = flat[1:].view(33, 72)
+    _check_backward(odd, x.reshape(33, 48), w[0], w[1], odd * 0.5, odd + 1, "gelu")
+    one = torch.ones(1, device=DEV, dtype=dtype)
+    _check_backward(one.expand(33, 72), x.reshape(33, 48), w[0], w[1], odd * 0.5, odd + 1, "gelu")   # the gradient of a sum: one number for all
+    empty = torch.empty(0, 72, device=DEV, dtype=dtype)
+    grads = ops.gated_ffn_backward(empty, torch.empty(0, 48, device=DEV, dtype=dtype), w[0], w[1], empty, empty)
+    assert grads[0].shape == (0, 48) and (grads[1] == 0).all() and (grads[2] == 0).all()
+    assert ops.gated_ffn(torch.empty(2, 0, 48, device=DEV, dtype=dtype), w[0], w[1]).shape == (2, 0, 72)
+
+
+def test_backward_with_any_workspace_and_gradients_apart():
+    # a workspace that holds NaN, one that is just large enough, and gradients of the weights that lie anywhere
+    m, f, k = 70, 40, 24
+    x, w_gate, w_up, g = _block(m, f, k, torch.bfloat16, seed=7)
+    grad_h, gate, up = (_randn(g, m, f, dtype=torch.bfloat16) for _ in range(3))
+    want = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up)
+    lib = _capi.load()
+    size = lib.tf_gated_ffn_backward_workspace_bytes(m, f, k)
+    room = torch.full((size + 64,), 0xFF, device=DEV, dtype=torch.uint8)
+    got = [torch.full_like(t, float("nan")) for t in (x, w_gate, w_up)]
+    _capi.check(lib.tf_gated_ffn_backward(*(t.data_ptr() for t in (grad_h, x, w_gate, w_up, gate, up, *got)), _capi.TF_DTYPE_BF16, _capi.TF_ACT_SILU,
+                                          m, f, k, room.data_ptr(), size, torch.cuda.current_stream().cuda_stream), "tf_gated_ffn_backward")
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert (room[size:] == 0xFF).all()
+
+
+def test_autograd_is_the_explicit_backward():
+    x, w_gate, w_up, g = _block(90, 72, 56, torch.bfloat16, seed=8)
+    grad_h = _randn(g, 90, 72, dtype=torch.bfloat16)
+    h0, gate, up = ops.gated_ffn(x, w_gate, w_up, "gelu", keep=True)
+    want = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, "gelu")
+    leaves = [t.clone().requires_grad_() for t in (x, w_gate, w_up)]
+    h = ops.gated_ffn(*leaves, "gelu")
+    assert torch.equal(h, h0)
+    h.backward(grad_h)
+    for leaf, w in zip(leaves, want):
+        assert torch.equal(leaf.grad, w)
+    # some leaves only, and a copy of x that is used twice
+    x2 = x.clone().requires_grad_()
+    h, gate, up = ops.gated_ffn(x2, w_gate, w_up, "gelu", keep=True)
+    assert not gate.requires_grad and not up.requires_grad
+    (grad,) = torch.autograd.grad(h, x2, grad_h)
+    assert torch.equal(grad, want[0])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(torch.autograd.grad(ops.gated_ffn(x2, w_gate, w_up).sum(), x2, create_graph=True)[0].sum(), x2)
+    with torch.no_grad():
+        assert not ops.gated_ffn(*leaves).requires_grad
+
+
+def test_replayed_and_on_two_streams():
+    x, w_gate, w_up, g = _block(140, 200, 96, torch.float16, seed=9)
+    grad_h = _randn(g, 140, 200, dtype=torch.float16)
+
+    def step():
+        h, gate, up = ops.gated_ffn(x, w_gate, w_up, keep=True)
+        return (h, *ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up))
+
+    want = [t.clone() for t in step()]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for side in sides:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(3):
+                results.append(step())
+    torch.cuda.synchronize()
+    for got in results:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for n in range(4):
+        x.mul_(0.5 if n % 2 else 2.0)
+        want = [t.clone() for t in step()]
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), n
+    leaf = w_gate.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.gated_ffn(x, leaf, w_up)
+
+
+def test_compiled_call():
+    x, w_gate, w_up, _ = _block(20, 48, 32, torch.bfloat16)
+    want = ops.gated_ffn(x, w_gate, w_up)
+    assert torch.equal(torch.compile(lambda *t: ops.gated_ffn(*t), backend="eager")(x, w_gate, w_up), want)
+
+
+def test_refusals():
+    x, w_gate, w_up, _ = _block(4, 16, 32, torch.float16)
+    h = torch.zeros(4, 16, device=DEV).half()
+    for bad in ((x, w_gate, w_up.bfloat16()), (x, w_gate, w_up[:8]), (x[:, :16], w_gate, w_up), (x, w_gate.cpu(), w_up), (x.float(), w_gate.float(), w_up.float()),
+                (x, w_gate, w_up, "relu"), (x, w_gate[0], w_up), (x[..., :0], w_gate[:, :0], w_up[:, :0])):
+        with pytest.raises(RuntimeError):
+            ops.gated_ffn(*bad)
+    for bad in ((h[:3], x, w_gate, w_up, h, h), (h, x, w_gate, w_up, h.float(), h), (h, x, w_gate, w_up, h, h[:, :8]), (h, x, w_gate, w_up, h, h, "tanh")):
+        with pytest.raises(RuntimeError):
+            ops.gated_ffn_backward(*bad)

@@ -1,0 +1,274 @@
+"""The cross entropy of a linear head against its 64-bit form, forward and backward."""
+
+import pytest
+import torch
+
+from tests import product_ref as ref
+from tilefusion_amd import _capi, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = [torch.float16, torch.bfloat16]
+
+
+def _head(t, v, k, dtype, seed=0, ignored=True):
+    g = torch.Generator(device=DEV).manual_seed(seed + t * 5 + v * 3 + k)
+    hidden = torch.randn(t, k, device=DEV, generator=g).to(dtype)
+    weight = (torch.randn(v, k, device=DEV, generator=g) * 2 * k ** -0.5).to(dtype)
+    target = torch.randint(0, v, (t,), device=DEV, generator=g)
+    if ignored:
+        target[torch.rand(t, device=DEV, generator=g) < 0.2] = -100
+    return hidden, weight, target, g
+
+
+def _check_forward(hidden, weight, target, ignore_index=-100):
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target, ignore_index)
+    (want_loss, want_lse), (b_loss, b_lse) = ref.linear_cross_entropy(hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), ignore_index)
+    assert loss.shape == target.shape == lse.shape and loss.dtype == lse.dtype == torch.float32
+    what = f"{tuple(hidden.shape)} V={weight.shape[0]} {hidden.dtype}"
+    ref.assert_within(lse.reshape(-1), want_lse, b_lse, "lse " + what)
+    ref.assert_within(loss.reshape(-1), want_loss, b_loss, "loss " + what)
+    assert (loss[target == ignore_index] == 0).all()
+    return lse
+
+
+def _check_backward(grad_loss, hidden, weight, target, ignore_index=-100):
+    lse = ops.linear_cross_entropy(hidden, weight, target, ignore_index)[1]
+    got = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index)
+    want, bounds = ref.linear_cross_entropy_backward(grad_loss.reshape(-1), hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), ignore_index)
+    for name, g, w, b, like in zip(("grad_hidden", "grad_weight"), got, want, bounds, (hidden, weight)):
+        assert g.shape == like.shape and g.dtype == like.dtype
+        what = f"{name} {tuple(hidden.shape)} V={weight.shape[0]} {hidden.dtype}"
+        ref.assert_within(g.reshape(w.shape), w, b, what)
+        if w.norm() > 0:
+            floor = w.numel() ** 0.5 * ref.TINY[hidden.dtype]   # results too small for the type
+            assert (g.reshape(w.shape).double() - w).norm() <= 2 * ref.half_step(hidden.dtype) * w.norm() + floor, what
+    return got
+
+
+SIZES = [
+    (1, 1, 1), (1, 2, 8), (1, 1000, 64), (1, 5003, 256), (2, 63, 40), (5, 65, 33), (16, 1000, 128), (37, 4099, 72), (64, 64, 64), (100, 129, 136), (128, 128, 128),
+    (130, 1000, 1000), (255, 2049, 96), (256, 256, 64), (257, 777, 264), (300, 3001, 520), (700, 300, 128), (1025, 513, 88),
+]
+
+
+@pytest.mark.parametrize("t,v,k", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_forward_sizes(t, v, k, dtype):
+    hidden, weight, target, _ = _head(t, v, k, dtype)
+    _check_forward(hidden, weight, target)
+
+
+@pytest.mark.parametrize("t,v,k", SIZES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_sizes(t, v, k, dtype):
+    hidden, weight, target, g = _head(t, v, k, dtype, seed=1)
+    scale = 4096.0 if dtype == torch.float16 else 1.0
+    _check_backward(torch.full((t,), scale / t, device=DEV), hidden, weight, target)
+    _check_backward((torch.rand(t, device=DEV, generator=g) - 0.5) * scale, hidden, weight, target)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_pieces_of_the_vocabulary(dtype):
+    # 40000 tokens: pieces of 4096 columns, the last one of an odd width
+    hidden, weight, target, g = _head(40000, 8195, 24, dtype, seed=2)
+    lib = _capi.load()
+    assert lib.tf_linear_cross_entropy_backward_workspace_bytes(40000, 8195, 24) < 2 * 40000 * 8195 * 2
+    _check_backward(torch.rand(40000, device=DEV, generator=g) / 40000 * (4096 if dtype == torch.float16 else 1), hidden, weight, target)
+
+
+def test_shapes_strides_and_alignment():
+    hidden, weight, target, g = _head(60, 300, 80, torch.float16, seed=3)
+    _check_forward(hidden.view(3, 20, 80), weight, target.view(3, 20))
+    _check_forward(hidden.view(3, 20, 80).transpose(0, 1), weight, target.view(3, 20).t())
+    wide = torch.randn(300, 100, device=DEV, generator=g).half()
+    _check_forward(hidden, wide[:, 20:], target)
+    flat = torch.randn(300 * 80 + 1, device=DEV, generator=g).half()
+    _check_forward(flat[1:60 * 80 + 1].view(60, 80), flat[1:].view(300, 80), target)
+    _check_backward(torch.rand(3, 20, device=DEV, generator=g), hidden.view(3, 20, 80), wide[:, 20:], target.view(3, 20))
+    _check_backward(torch.rand(60, device=DEV, generator=g), flat[1:60 * 80 + 1].view(60, 80), flat[1:].view(300, 80), target)
+    _check_backward(torch.ones(1, device=DEV).expand(60), hidden, weight, target)   # the gradient of a sum
+    one = hidden[0], weight, target[0] * 0
+    assert ops.linear_cross_entropy(*one)[0].shape == ()
+
+
+def test_ignored_and_invalid_targets():
+    hidden, weight, target, g = _head(200, 500, 64, torch.bfloat16, seed=4, ignored=False)
+    grad_loss = torch.rand(200, device=DEV, generator=g)
+    target[::3] = 7
+    _check_forward(hidden, weight, target, ignore_index=7)      # a word of the vocabulary may be the ignored one
+    _check_backward(grad_loss, hidden, weight, target, ignore_index=7)
+    # nothing of an ignored token's gradient is looked at
+    bad = grad_loss.clone()
+    bad[::3] = float("nan")
+    lse = ops.linear_cross_entropy(hidden, weight, target, 7)[1]
+    for a, b in zip(ops.linear_cross_entropy_backward(bad, hidden, weight, target, lse, 7),
+                    ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, 7)):
+        assert torch.equal(a, b)
+    everything = torch.full_like(target, -100)
+    loss, lse = ops.linear_cross_entropy(hidden, weight, everything)
+    assert (loss == 0).all() and lse.isfinite().all()
+    for grad in ops.linear_cross_entropy_backward(grad_loss, hidden, weight, everything, lse):
+        assert (grad == 0).all()
+    for word in (-1, 500, 1 << 40, -(1 << 40)):
+        target[5] = word
+        loss, lse = ops.linear_cross_entropy(hidden, weight, target, 7)
+        assert loss.isnan().nonzero().flatten().tolist() == [5] and lse.isfinite().all()
+        grad_hidden, grad_weight = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, 7)
+        assert grad_weight.isnan().all() and grad_hidden[5].isnan().all() and grad_hidden[:5].isfinite().all() and grad_hidden[6:].isfinite().all()
+
+
+def test_infinite_logits_and_nan_stay_with_their_token():
+    hidden, weight, target, _ = _head(150, 300, 64, torch.float16, seed=5, ignored=False)
+    clean = ops.linear_cross_entropy(hidden, weight, target)
+    bad = hidden.clone()
+    bad[4, 0] = float("nan")
+    bad[100] = 0
+    bad[100, 1] = float("inf")    # logits of both infinities
+    loss, lse = ops.linear_cross_entropy(bad, weight, target)
+    rows = torch.ones(150, dtype=torch.bool, device=DEV)
+    rows[[4, 100]] = False
+    assert torch.equal(loss[rows], clean[0][rows]) and torch.equal(lse[rows], clean[1][rows])
+    assert loss[4].isnan() and not lse[100].isfinite()
+    # words that cannot occur: logits of -inf take no part
+    weight[::2] = 0
+    weight[::2, 0] = -float("inf")
+    hidden[:, 0] = 1.0
+    target = target // 2 * 2 + 1
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    (want_loss, want_lse), bounds = ref.linear_cross_entropy(hidden, weight[1::2].contiguous(), target // 2, -100)
+    ref.assert_within(lse, want_lse, bounds[1])
+    ref.assert_within(loss, want_loss, bounds[0])
+    weight[:] = 0
+    weight[:, 0] = -float("inf")
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    assert (lse == -float("inf")).all()
+
+
+def test_large_logits_do_not_overflow():
+    hidden, weight, target, _ = _head(64, 200, 128, torch.bfloat16, seed=6)
+    _check_forward(hidden * 64, weight * 64, target)
+    _check_backward(torch.ones(64, device=DEV), hidden * 16, weight * 16, target)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [1e-30, 1e-7, 1.0, 1e4])
+def test_the_size_of_grad_loss_does_not_matter(dtype, size):
+    # exact powers of two apart, results are exact powers of two apart (bf16; fp16 as far as its results reach)
+    hidden, weight, target, g = _head(90, 400, 64, dtype, seed=7)
+    grad_loss = torch.rand(90, device=DEV, generator=g)
+    lse = ops.linear_cross_entropy(hidden, weight, target)[1]
+    by = 2.0 ** round(__import__("math").log2(size))
+    base = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse)
+    got = ops.linear_cross_entropy_backward(grad_loss * by, hidden, weight, target, lse)
+    for a, b in zip(got, base):
+        assert (a.double() - b.double() * by).abs().max() <= (ref.TINY[dtype] if dtype == torch.bfloat16 or by <= 1 else float("inf"))+ (
+            0 if dtype == torch.bfloat16 else 2 * ref.half_step(dtype) * (b.double() * by).abs().max())
+
+
+def test_gradient_against_differences():
+    # the loss itself along a direction: central differences of step 2^-4 on values that are multiples of it (exact in fp16)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    t, v, k = 40, 96, 48
+    grid = lambda *s: (torch.randint(-8, 9, s, device=DEV, generator=g) / 16).half()   # noqa: E731
+    hidden, weight, target = grid(t, k), grid(v, k), torch.randint(0, v, (t,), device=DEV, generator=g)
+    lse = ops.linear_cross_entropy(hidden, weight, target)[1]
+    grad_hidden, grad_weight = ops.linear_cross_entropy_backward(torch.ones(t, device=DEV), hidden, weight, target, lse)
+    step = 1.0 / 16
+    total = lambda h, w: ops.linear_cross_entropy(h, w, target)[0].double().sum().item()   # noqa: E731
+    for k_at in (0, 17, 47):
+        e = torch.zeros_like(hidden)
+        e[:, k_at] = step
+        along = grad_hidden[:, k_at].double().sum().item()
+        # the third derivative of lse along a coordinate is at most the largest |weight|^3 = 1/8, times step^2 / 6, each of t tokens
+        assert abs((total(hidden + e, weight) - total(hidden - e, weight)) / (2 * step) - along) <= t * (step ** 2 / 48 + 2.0 ** -11 + FAR / step)
+        e = torch.zeros_like(weight)
+        e[:5, k_at] = step
+        along = grad_weight[:5, k_at].double().sum().item()
+        assert abs((total(hidden, weight + e) - total(hidden, weight - e)) / (2 * step) - along) <= t * (step ** 2 / 48 + 2.0 ** -11 + FAR / step)
+
+
+FAR = 2.0 ** -19   # of a loss near 5: its fp32 error
+
+
+def test_any_workspace():
+    t, v, k = 150, 1000, 40
+    hidden, weight, target, g = _head(t, v, k, torch.bfloat16, seed=9)
+    grad_loss = torch.rand(t, device=DEV, generator=g)
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    grads = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse)
+    lib, st = _capi.load(), torch.cuda.current_stream().cuda_stream
+    size = lib.tf_linear_cross_entropy_workspace_bytes(t, v, k)
+    room = torch.full((size + 64,), 0xFF, device=DEV, dtype=torch.uint8)
+    got = [torch.full((t,), float("nan"), device=DEV) for _ in range(2)]
+    _capi.check(lib.tf_linear_cross_entropy(*(x.data_ptr() for x in (hidden, weight, target, *got)), _capi.TF_DTYPE_BF16, t, v, k, -100, room.data_ptr(),
+                                            size, st), "tf_linear_cross_entropy")
+    assert torch.equal(got[0], loss) and torch.equal(got[1], lse) and (room[size:] == 0xFF).all()
+    size = lib.tf_linear_cross_entropy_backward_workspace_bytes(t, v, k)
+    room = torch.full((size + 64,), 0xFF, device=DEV, dtype=torch.uint8)
+    got = [torch.full_like(x, float("nan")) for x in (hidden, weight)]
+    _capi.check(lib.tf_linear_cross_entropy_backward(*(x.data_ptr() for x in (grad_loss, hidden, weight, target, lse, *got)), _capi.TF_DTYPE_BF16, t, v, k,
+                                                     -100, room.data_ptr(), size, st), "tf_linear_cross_entropy_backward")
+    assert torch.equal(got[0], grads[0]) and torch.equal(got[1], grads[1]) and (room[size:] == 0xFF).all()
+
+
+def test_autograd_replay_streams_and_empty():
+    hidden, weight, target, g = _head(120, 900, 72, torch.bfloat16, seed=10)
+    leaves = [hidden.clone().requires_grad_(), weight.clone().requires_grad_()]
+    loss, lse = ops.linear_cross_entropy(*leaves, target)
+    assert not lse.requires_grad
+    valid = int((target != -100).sum())
+    (loss.sum() / valid).backward()
+    want = ops.linear_cross_entropy_backward(torch.full((120,), 1.0 / valid, device=DEV), hidden, weight, target, lse)
+    assert torch.equal(leaves[0].grad, want[0]) and torch.equal(leaves[1].grad, want[1])
+
+    grad_loss = torch.rand(120, device=DEV, generator=g)
+
+    def step():
+        loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+        return (loss, *ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse))
+
+    want = [x.clone() for x in step()]
+    results = []
+    for side in [torch.cuda.Stream() for _ in range(2)]:
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(3):
+                results.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for got in results for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for n in range(4):
+        hidden.mul_(0.5 if n % 2 else 2.0)
+        grad_loss.mul_(3.0)
+        want = [x.clone() for x in step()]
+        for x in out:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), n
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.linear_cross_entropy(leaves[0], weight, target)
+
+    none = hidden[:0], weight, target[:0]
+    loss, lse = ops.linear_cross_entropy(*none)
+    assert loss.shape == (0,) == lse.shape
+    grad_hidden, grad_weight = ops.linear_cross_entropy_backward(loss, *none, lse)
+    assert grad_hidden.shape == (0, 72) and (grad_weight == 0).all()
+
+
+def test_refusals():
+    hidden, weight, target, _ = _head(8, 32, 16, torch.float16)
+    for bad in ((hidden, weight.bfloat16(), target), (hidden, weight[:, :8], target), (hidden, weight, target[:4]), (hidden, weight, target.int()),
+                (hidden.float(), weight.float(), target), (hidden, weight.cpu(), target), (hidden, weight[0], target), (hidden[:, :0], weight[:, :0], target),
+                (hidden, weight[:0], target)):
+        with pytest.raises(RuntimeError):
+            ops.linear_cross_entropy(*bad)
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    for bad in ((loss.half(), hidden, weight, target, lse), (loss[:4], hidden, weight, target, lse), (loss, hidden, weight, target, lse.double()),
+                (loss, hidden, weight, target, lse[:2])):
+        with pytest.raises(RuntimeError):
+            ops.linear_cross_entropy_backward(*bad)

@@ -1,0 +1,156 @@
+"""CPU-only checks of gemm_int8, quantize_rows, gated_ffn and linear_cross_entropy: what the C ABI refuses before it touches the device, and
+the 64-bit forms that the GPU tests compare with, their gradients against differences."""
+
+import ctypes
+
+import pytest
+import torch
+
+from tests import product_ref as ref
+from tilefusion_amd import _capi, ops
+
+P = 0x1000   # never dereferenced: validation fails first
+F16, BF16, F32 = _capi.TF_DTYPE_F16, _capi.TF_DTYPE_BF16, _capi.TF_DTYPE_F32
+BAD, UNSUPPORTED, OK = _capi.TF_ERR_INVALID_ARG, _capi.TF_ERR_UNSUPPORTED, _capi.TF_OK
+
+
+def test_gemm_int8_arguments():
+    f = _capi.load().tf_gemm_int8
+    assert f(P, P, P, P, P, F32, 4, 4, 0, None) == BAD and f(P, P, P, P, P, F32, -1, 4, 4, None) == BAD
+    assert f(P, P, P, P, P, 3, 4, 4, 4, None) == UNSUPPORTED
+    assert f(P, P, P, P, P, F16, 4, 4, 131072, None) == BAD and b"131071" in _capi.load().tf_last_error()
+    assert f(P, P, P, P, P, F16, 1 << 30, 4, 4, None) == BAD
+    for at in range(5):
+        pointers = [P] * 5
+        pointers[at] = None
+        assert f(*pointers, F16, 4, 4, 4, None) == BAD
+    assert f(None, None, None, None, None, F16, 0, 4, 4, None) == OK == f(None, None, None, None, None, F16, 4, 0, 4, None)
+
+
+def test_quantize_rows_arguments():
+    f = _capi.load().tf_quantize_rows
+    assert f(P, P, P, F32, 4, 4, None) == UNSUPPORTED and f(P, P, P, F16, 4, 0, None) == BAD and f(P, P, P, F16, 1 << 24, 4, None) == BAD
+    assert f(None, P, P, F16, 4, 4, None) == BAD == f(P, None, P, F16, 4, 4, None) == f(P, P, None, F16, 4, 4, None) == f(P, P, P, F16, -1, 4, None)
+    assert f(None, None, None, F16, 0, 4, None) == OK
+
+
+def test_gated_ffn_arguments():
+    lib = _capi.load()
+    f = lib.tf_gated_ffn
+    assert f(P, P, P, P, None, None, F32, 0, 4, 4, 4, None) == UNSUPPORTED
+    assert f(P, P, P, P, None, None, F16, 3, 4, 4, 4, None) == BAD and b"activation" in lib.tf_last_error()
+    assert f(P, P, P, P, P, None, F16, 0, 4, 4, 4, None) == BAD and f(P, P, P, None, P, P, F16, 0, 4, 4, 4, None) == BAD
+    for m, n, k in ((-1, 4, 4), (4, 0, 4), (4, 4, 0), (1 << 22, 4, 4), (4, 1 << 21, 4), (4, 4, 1 << 22)):
+        assert f(P, P, P, P, None, None, F16, 0, m, n, k, None) == BAD
+    assert f(None, None, None, None, None, None, F16, 0, 0, 4, 4, None) == OK
+    size = lib.tf_gated_ffn_backward_workspace_bytes
+    assert size(0, 4, 4) == 0 == size(4, 0, 4) == size(1 << 22, 4, 4) and size(64, 64, 64) > 0
+    b = lib.tf_gated_ffn_backward
+    want = size(64, 64, 64)
+    assert b(*[P] * 9, F16, 0, 64, 64, 64, P, want - 1, None) == BAD and b"workspace" in lib.tf_last_error()
+    assert b(*[P] * 9, F16, 0, 64, 64, 64, P + 8, want, None) == BAD and b(*[P] * 9, F16, 0, 64, 64, 64, None, want, None) == BAD
+    for at in range(9):
+        pointers = [P] * 9
+        pointers[at] = None
+        assert b(*pointers, F16, 0, 64, 64, 64, P, want, None) == BAD
+
+
+def test_linear_cross_entropy_arguments():
+    lib = _capi.load()
+    for f, size, n in ((lib.tf_linear_cross_entropy, lib.tf_linear_cross_entropy_workspace_bytes, 5),
+                       (lib.tf_linear_cross_entropy_backward, lib.tf_linear_cross_entropy_backward_workspace_bytes, 7)):
+        want = size(8, 100, 64)
+        assert want > 0 and size(0, 100, 64) == 0 == size(8, 0, 64) == size(8, 100, 0) == size(1 << 22, 100, 64)
+        assert f(*[P] * n, F32, 8, 100, 64, -100, P, want, None) == UNSUPPORTED
+        assert f(*[P] * n, F16, 8, 100, 64, -100, P, want - 1, None) == BAD and b"workspace" in lib.tf_last_error()
+        assert f(*[P] * n, F16, 8, 100, 64, -100, P + 4, want, None) == BAD == f(*[P] * n, F16, 8, 100, 64, -100, None, want, None)
+        for sizes in ((-1, 100, 64), (8, 0, 64), (8, 100, 0), (8, 1 << 30, 64), (8, 100, 1 << 22)):
+            assert f(*[P] * n, F16, *sizes, -100, P, want, None) == BAD
+        for at in range(n):
+            pointers = [P] * n
+            pointers[at] = None
+            assert f(*pointers, F16, 8, 100, 64, -100, P, want, None) == BAD
+    assert lib.tf_linear_cross_entropy(*[None] * 5, F16, 0, 100, 64, -100, None, 0, None) == OK
+
+
+def test_workspace_of_the_backward_pass_is_a_piece_of_the_vocabulary():
+    size = _capi.load().tf_linear_cross_entropy_backward_workspace_bytes
+    # 8192 tokens x 131072 words: the logits are 2 GiB in 16 bits; and it does not grow with the vocabulary from some size on
+    assert size(8192, 131072, 1024) < 2 ** 30 and size(8192, 131072, 1024) == size(8192, 1 << 20, 1024)
+
+
+def test_wrappers_refuse_on_the_cpu():
+    x, w = torch.zeros(4, 8).half(), torch.zeros(6, 8).half()
+    for call in (lambda: ops.gated_ffn(x, w, w), lambda: ops.quantize_rows(x), lambda: ops.linear_cross_entropy(x, w, torch.zeros(4, dtype=torch.long)),
+                 lambda: ops.gemm_int8(x.char(), w.char(), torch.ones(4), torch.ones(6), torch.zeros(4, 6))):
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            call()
+    with pytest.raises(RuntimeError, match="must be"):
+        ops.gated_ffn(x, w[:, :4], w[:, :4])
+    with pytest.raises(RuntimeError, match="target"):
+        ops.linear_cross_entropy(x, w, torch.zeros(5, dtype=torch.long))
+
+
+def test_schemas():
+    want = {
+        "quantize_rows": "(Tensor x, Tensor(a!) q, Tensor(b!) scale) -> ()",
+        "gemm_int8": "(Tensor A, Tensor B, Tensor scale_a, Tensor scale_b, Tensor(a!) C) -> ()",
+        "gated_ffn": "(Tensor x, Tensor w_gate, Tensor w_up, str activation, Tensor(a!) h, Tensor(b!)? gate, Tensor(c!)? up) -> ()",
+        "gated_ffn_backward": "(Tensor grad_h, Tensor x, Tensor w_gate, Tensor w_up, Tensor gate, Tensor up, str activation, Tensor(a!) grad_x, Tensor(b!) grad_w) -> ()",
+        "linear_cross_entropy": "(Tensor hidden, Tensor weight, Tensor target, int ignore_index, Tensor(a!) loss, Tensor(b!) lse) -> ()",
+        "linear_cross_entropy_backward": "(Tensor grad_loss, Tensor hidden, Tensor weight, Tensor target, Tensor lse, int ignore_index, Tensor(a!) grad_hidden, Tensor(b!) grad_weight) -> ()",
+    }
+    for name, schema in want.items():
+        assert str(getattr(torch.ops.tilefusion, name).default._schema) == f"tilefusion::{name}{schema}"
+        assert callable(getattr(ops, name))
+
+
+# ---- the formulas --------------------------------------------------------------------------
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+def test_activation_slope_against_differences(activation):
+    g = torch.linspace(-9, 9, 1801, dtype=torch.float64)
+    step = 1e-5
+    differences = (ref.act(g + step, activation) - ref.act(g - step, activation)) / (2 * step)
+    assert (ref.act_slope(g, activation) - differences).abs().max() < 1e-9   # step^2 and 1e-16 / step
+    assert ref.act_slope(g, activation).abs().max() < 1.13                   # (what the bounds count with)
+    plain = {"silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu,
+             "gelu_tanh": lambda x: torch.nn.functional.gelu(x, approximate="tanh")}[activation]
+    assert (ref.act(g, activation) - plain(g)).abs().max() < 1e-13
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+def test_gated_ffn_gradients_against_autograd(activation):
+    gen = torch.Generator().manual_seed(1)
+    x, w_gate, w_up, grad_h = (torch.randn(*s, generator=gen).bfloat16() for s in ((7, 5), (6, 5), (6, 5), (7, 6)))
+    leaves = [t.double().requires_grad_() for t in (x, w_gate, w_up)]
+    gate, up = leaves[0] @ leaves[1].t(), leaves[0] @ leaves[2].t()
+    want = torch.autograd.grad((ref.act(gate, activation) * up * grad_h.double()).sum(), leaves)
+    got, bounds = ref.gated_ffn_backward(grad_h, x, w_gate, w_up, gate.detach(), up.detach(), activation)
+    for a, b, bound in zip(got, want, bounds):
+        assert (a - b).abs().max() < 1e-12 and (bound > 0).all()
+
+
+def test_linear_cross_entropy_gradients_against_autograd():
+    gen = torch.Generator().manual_seed(2)
+    hidden, weight = (torch.randn(*s, generator=gen).half() for s in ((9, 5), (11, 5)))
+    target, grad_loss = torch.randint(0, 11, (9,), generator=gen), torch.rand(9, generator=gen)
+    target[::4] = -100
+    leaves = [t.double().requires_grad_() for t in (hidden, weight)]
+    loss = torch.nn.functional.cross_entropy(leaves[0] @ leaves[1].t(), target, reduction="none")
+    (want_loss, _), _ = ref.linear_cross_entropy(hidden, weight, target, -100)
+    assert (loss - want_loss).abs().max() < 1e-12
+    want = torch.autograd.grad((loss * grad_loss.double()).sum(), leaves)
+    got, bounds = ref.linear_cross_entropy_backward(grad_loss, hidden, weight, target, -100)
+    for a, b, bound in zip(got, want, bounds):
+        assert (a - b).abs().max() < 1e-12 and (bound > 0).all()
+
+
+def test_the_comparison_sees_a_planted_mistake():
+    want, bounds = ref.gated_ffn(torch.randn(8, 64).half(), torch.randn(16, 64).half() / 8, torch.randn(16, 64).half() / 8, "silu")
+    good = want[0].to(torch.float16)
+    ref.assert_within(good, want[0], bounds[0])
+    for at, by in (((3, 5), 1.02), ((0, 0), 0.98)):
+        bad = good.clone()
+        bad[at] = (want[0][at] * by).half()
+        with pytest.raises(AssertionError, match="out of bounds"):
+            ref.assert_within(bad, want[0], bounds[0] + 0 * want[0])

@@ -12,6 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libtilefusion_hip.so")
 
 TF_OK, TF_ERR_INVALID_ARG, TF_ERR_UNSUPPORTED, TF_ERR_LDS, TF_ERR_HIP = range(5)
 TF_DTYPE_F32, TF_DTYPE_F16, TF_DTYPE_BF16 = range(3)
+TF_ACT_SILU, TF_ACT_GELU, TF_ACT_GELU_TANH = range(3)
 
 _vp, _i, _i64, _d, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double, ctypes.c_size_t
 
@@ -40,6 +41,15 @@ SIGNATURES = {
     "tf_flash_attention_fwd_split": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i, _d, _vp, _vp]),
     "tf_transpose_16bit": (_i, [_vp, _vp, _i64, _i64, _i64, _vp]),
     "tf_scatter_nd": (_i, [_vp, _vp, _vp, ctypes.POINTER(_i64), _i, _i64, _i, _i, _vp]),
+    "tf_gemm_int8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _vp]),
+    "tf_quantize_rows": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _vp]),
+    "tf_gated_ffn": (_i, [_vp] * 6 + [_i, _i, _i64, _i64, _i64, _vp]),
+    "tf_gated_ffn_backward_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "tf_gated_ffn_backward": (_i, [_vp] * 9 + [_i, _i, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "tf_linear_cross_entropy_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "tf_linear_cross_entropy": (_i, [_vp] * 5 + [_i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "tf_linear_cross_entropy_backward_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "tf_linear_cross_entropy_backward": (_i, [_vp] * 7 + [_i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "tf_gemm_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_flash_decode_plan": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_i)]),
     "tf_flash_attention_rows": (_i, [_i64, _i64, _i64, _i64, _i]),

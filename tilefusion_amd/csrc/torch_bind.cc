@@ -17,6 +17,7 @@
 #include <torch/library.h>
 
 #include <functional>
+#include <optional>
 #include <vector>
 
 #include "tilefusion_c.h"
@@ -390,6 +391,173 @@ TILEFUSION_EXPORT void scatter_nd(const at::Tensor& data, at::Tensor& updates, c
                "scatter_nd");
 }
 
+// ---- products whose results do not leave as they are -----------------------------------------
+// These take tensors of any one GPU, the current one or not: the call is made there, on that device's current stream.
+namespace {
+void check_operand(const at::Tensor& t, const char* name, const at::Tensor& like, const char* op) {
+  TORCH_CHECK(t.is_cuda(), "tilefusion::", op, ": ", name, " must be a CUDA tensor.");
+  TORCH_CHECK(t.device() == like.device(), "tilefusion::", op, ": ", name, " must be on the device of the other tensors.");
+  TORCH_CHECK(t.is_contiguous(), "tilefusion::", op, ": ", name, " must be contiguous.");
+}
+void check_like(const at::Tensor& t, const char* name, const at::Tensor& like, const char* op) {
+  check_operand(t, name, like, op);
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), "tilefusion::", op, ": ", name, " must have the dtype of the other tensors.");
+}
+void check_sizes(const at::Tensor& t, const char* name, int64_t rows, int64_t cols, const char* op) {
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, "tilefusion::", op, ": ", name, " must be [", rows, ", ", cols,
+              "], got ", t.sizes(), ".");
+}
+void check_vector(const at::Tensor& t, const char* name, at::ScalarType type, int64_t n, const at::Tensor& like, const char* op) {
+  check_operand(t, name, like, op);
+  TORCH_CHECK(t.scalar_type() == type, "tilefusion::", op, ": ", name, " must be of type ", toString(type), ".");
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n, "tilefusion::", op, ": ", name, " must be [", n, "], got ", t.sizes(), ".");
+}
+int activation_code(c10::string_view name, const char* op) {
+  const int code = name == "silu" ? TF_ACT_SILU : name == "gelu" ? TF_ACT_GELU : name == "gelu_tanh" ? TF_ACT_GELU_TANH : -1;
+  TORCH_CHECK(code >= 0, "tilefusion::", op, ": activation must be 'silu', 'gelu' or 'gelu_tanh', got '", name, "'.");
+  return code;
+}
+}  // namespace
+
+// quantize_rows(x [M,K] -> q [M,K] int8, scale [M] fp32)
+void quantize_rows(const at::Tensor& x, at::Tensor& q, at::Tensor& scale) {
+  constexpr const char* op = "quantize_rows";
+  check_operand(x, "x", x, op);
+  const int dtype = operand_dtype(x, op);
+  TORCH_CHECK(x.dim() == 2, "tilefusion::", op, ": x must be [M, K].");
+  check_operand(q, "q", x, op);
+  TORCH_CHECK(q.scalar_type() == at::kChar, "tilefusion::", op, ": q must be int8.");
+  check_sizes(q, "q", x.size(0), x.size(1), op);
+  check_vector(scale, "scale", at::kFloat, x.size(0), x, op);
+  const c10::DeviceGuard there(x.device());
+  check_status(tf_quantize_rows(x.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), dtype, x.size(0), x.size(1), current_stream()), op);
+}
+
+// gemm_int8(A [M,K] int8, B [N,K] int8, scale_a [M], scale_b [N], C [M,N] fp32, fp16 or bf16)
+void gemm_int8(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale_a, const at::Tensor& scale_b, at::Tensor& C) {
+  constexpr const char* op = "gemm_int8";
+  check_operand(A, "A", A, op);
+  TORCH_CHECK(A.scalar_type() == at::kChar && A.dim() == 2, "tilefusion::", op, ": A must be an int8 tensor [M, K].");
+  check_like(B, "B", A, op);
+  TORCH_CHECK(B.dim() == 2, "tilefusion::", op, ": B must be [N, K].");
+  const int64_t m = A.size(0), k = A.size(1), n = B.size(0);
+  check_sizes(B, "B", n, k, op);
+  check_vector(scale_a, "scale_a", at::kFloat, m, A, op);
+  check_vector(scale_b, "scale_b", at::kFloat, n, A, op);
+  check_operand(C, "C", A, op);
+  check_sizes(C, "C", m, n, op);
+  const at::ScalarType out = C.scalar_type();
+  TORCH_CHECK(out == at::kFloat || out == at::kHalf || out == at::kBFloat16, "tilefusion::", op, ": C must be float32, float16 or bfloat16.");
+  const int c_dtype = out == at::kFloat ? TF_DTYPE_F32 : out == at::kHalf ? TF_DTYPE_F16 : TF_DTYPE_BF16;
+  const c10::DeviceGuard there(A.device());
+  check_status(tf_gemm_int8(A.data_ptr(), B.data_ptr(), scale_a.data_ptr<float>(), scale_b.data_ptr<float>(), C.data_ptr(), c_dtype, m, n, k,
+                            current_stream()),
+               op);
+}
+
+// gated_ffn(x [M,K], w_gate [F,K], w_up [F,K] -> h [M,F], and gate and up [M,F] where they are given)
+void gated_ffn(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, c10::string_view activation, at::Tensor& h,
+               const std::optional<at::Tensor>& gate, const std::optional<at::Tensor>& up) {
+  constexpr const char* op = "gated_ffn";
+  check_operand(x, "x", x, op);
+  const int dtype = operand_dtype(x, op);
+  TORCH_CHECK(x.dim() == 2 && w_gate.dim() == 2, "tilefusion::", op, ": x must be [M, K], w_gate [F, K].");
+  const int64_t m = x.size(0), k = x.size(1), f = w_gate.size(0);
+  check_like(w_gate, "w_gate", x, op);
+  check_sizes(w_gate, "w_gate", f, k, op);
+  check_like(w_up, "w_up", x, op);
+  check_sizes(w_up, "w_up", f, k, op);
+  check_like(h, "h", x, op);
+  check_sizes(h, "h", m, f, op);
+  TORCH_CHECK(gate.has_value() == up.has_value(), "tilefusion::", op, ": gate and up are kept both or neither.");
+  if (gate.has_value()) {
+    check_like(*gate, "gate", x, op);
+    check_sizes(*gate, "gate", m, f, op);
+    check_like(*up, "up", x, op);
+    check_sizes(*up, "up", m, f, op);
+  }
+  const int act = activation_code(activation, op);
+  const c10::DeviceGuard there(x.device());
+  check_status(tf_gated_ffn(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(), gate.has_value() ? gate->data_ptr() : nullptr,
+                            up.has_value() ? up->data_ptr() : nullptr, dtype, act, m, f, k, current_stream()),
+               op);
+}
+
+// gated_ffn_backward(grad_h [M,F], x [M,K], w_gate, w_up [F,K], gate, up [M,F] -> grad_x [M,K], grad_w [2F,K]: gate's rows, then up's)
+void gated_ffn_backward(const at::Tensor& grad_h, const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, const at::Tensor& gate,
+                        const at::Tensor& up, c10::string_view activation, at::Tensor& grad_x, at::Tensor& grad_w) {
+  constexpr const char* op = "gated_ffn_backward";
+  check_operand(x, "x", x, op);
+  const int dtype = operand_dtype(x, op);
+  TORCH_CHECK(x.dim() == 2 && w_gate.dim() == 2, "tilefusion::", op, ": x must be [M, K], w_gate [F, K].");
+  const int64_t m = x.size(0), k = x.size(1), f = w_gate.size(0);
+  const struct { const at::Tensor& t; const char* name; int64_t rows, cols; } operands[] = {
+      {grad_h, "grad_h", m, f}, {w_gate, "w_gate", f, k}, {w_up, "w_up", f, k}, {gate, "gate", m, f},
+      {up, "up", m, f}, {grad_x, "grad_x", m, k}, {grad_w, "grad_w", 2 * f, k}};
+  for (const auto& o : operands) {
+    check_like(o.t, o.name, x, op);
+    check_sizes(o.t, o.name, o.rows, o.cols, op);
+  }
+  const int act = activation_code(activation, op);
+  const c10::DeviceGuard there(x.device());
+  const size_t bytes = tf_gated_ffn_backward_workspace_bytes(m, f, k);
+  c10::DataPtr ws;
+  if (bytes > 0) ws = scratch(bytes, x);
+  char* const to = static_cast<char*>(grad_w.data_ptr());
+  check_status(tf_gated_ffn_backward(grad_h.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), gate.data_ptr(), up.data_ptr(),
+                                     grad_x.data_ptr(), to, to + 2 * f * k, dtype, act, m, f, k, ws.get(), bytes, current_stream()),
+               op);
+}
+
+// linear_cross_entropy(hidden [T,K], weight [V,K], target [T] int64 -> loss [T], lse [T] fp32)
+void linear_cross_entropy(const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target, int64_t ignore_index, at::Tensor& loss,
+                          at::Tensor& lse) {
+  constexpr const char* op = "linear_cross_entropy";
+  check_operand(hidden, "hidden", hidden, op);
+  const int dtype = operand_dtype(hidden, op);
+  TORCH_CHECK(hidden.dim() == 2 && weight.dim() == 2, "tilefusion::", op, ": hidden must be [T, K], weight [V, K].");
+  const int64_t t = hidden.size(0), k = hidden.size(1), v = weight.size(0);
+  check_like(weight, "weight", hidden, op);
+  check_sizes(weight, "weight", v, k, op);
+  check_vector(target, "target", at::kLong, t, hidden, op);
+  check_vector(loss, "loss", at::kFloat, t, hidden, op);
+  check_vector(lse, "lse", at::kFloat, t, hidden, op);
+  const c10::DeviceGuard there(hidden.device());
+  const size_t bytes = tf_linear_cross_entropy_workspace_bytes(t, v, k);
+  c10::DataPtr ws;
+  if (bytes > 0) ws = scratch(bytes, hidden);
+  check_status(tf_linear_cross_entropy(hidden.data_ptr(), weight.data_ptr(), target.data_ptr<int64_t>(), loss.data_ptr<float>(),
+                                       lse.data_ptr<float>(), dtype, t, v, k, ignore_index, ws.get(), bytes, current_stream()),
+               op);
+}
+
+// linear_cross_entropy_backward(grad_loss [T] fp32, hidden, weight, target, lse [T] fp32 -> grad_hidden [T,K], grad_weight [V,K])
+void linear_cross_entropy_backward(const at::Tensor& grad_loss, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target,
+                                   const at::Tensor& lse, int64_t ignore_index, at::Tensor& grad_hidden, at::Tensor& grad_weight) {
+  constexpr const char* op = "linear_cross_entropy_backward";
+  check_operand(hidden, "hidden", hidden, op);
+  const int dtype = operand_dtype(hidden, op);
+  TORCH_CHECK(hidden.dim() == 2 && weight.dim() == 2, "tilefusion::", op, ": hidden must be [T, K], weight [V, K].");
+  const int64_t t = hidden.size(0), k = hidden.size(1), v = weight.size(0);
+  const struct { const at::Tensor& t; const char* name; int64_t rows, cols; } operands[] = {
+      {weight, "weight", v, k}, {grad_hidden, "grad_hidden", t, k}, {grad_weight, "grad_weight", v, k}};
+  for (const auto& o : operands) {
+    check_like(o.t, o.name, hidden, op);
+    check_sizes(o.t, o.name, o.rows, o.cols, op);
+  }
+  check_vector(target, "target", at::kLong, t, hidden, op);
+  check_vector(grad_loss, "grad_loss", at::kFloat, t, hidden, op);
+  check_vector(lse, "lse", at::kFloat, t, hidden, op);
+  const c10::DeviceGuard there(hidden.device());
+  const size_t bytes = tf_linear_cross_entropy_backward_workspace_bytes(t, v, k);
+  c10::DataPtr ws;
+  if (bytes > 0) ws = scratch(bytes, hidden);
+  check_status(tf_linear_cross_entropy_backward(grad_loss.data_ptr<float>(), hidden.data_ptr(), weight.data_ptr(), target.data_ptr<int64_t>(),
+                                                lse.data_ptr<float>(), grad_hidden.data_ptr(), grad_weight.data_ptr(), dtype, t, v, k, ignore_index,
+                                                ws.get(), bytes, current_stream()),
+               op);
+}
+
 }  // namespace kernels
 
 // Self-registering op table: each REGISTER_OP adds (schema, installer) at load time, and the
@@ -449,6 +617,25 @@ REGISTER_OP(flash_decode,
             "flash_decode(Tensor Q, Tensor K, Tensor V, Tensor(a!) O, "
             "int num_splits, float softmax_scale) -> ()",
             &kernels::flash_decode);
+
+REGISTER_OP(quantize_rows, "quantize_rows(Tensor x, Tensor(a!) q, Tensor(b!) scale) -> ()", &kernels::quantize_rows);
+REGISTER_OP(gemm_int8, "gemm_int8(Tensor A, Tensor B, Tensor scale_a, Tensor scale_b, Tensor(a!) C) -> ()", &kernels::gemm_int8);
+REGISTER_OP(gated_ffn,
+            "gated_ffn(Tensor x, Tensor w_gate, Tensor w_up, str activation, "
+            "Tensor(a!) h, Tensor(b!)? gate, Tensor(c!)? up) -> ()",
+            &kernels::gated_ffn);
+REGISTER_OP(gated_ffn_backward,
+            "gated_ffn_backward(Tensor grad_h, Tensor x, Tensor w_gate, Tensor w_up, Tensor gate, Tensor up, "
+            "str activation, Tensor(a!) grad_x, Tensor(b!) grad_w) -> ()",
+            &kernels::gated_ffn_backward);
+REGISTER_OP(linear_cross_entropy,
+            "linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target, int ignore_index, "
+            "Tensor(a!) loss, Tensor(b!) lse) -> ()",
+            &kernels::linear_cross_entropy);
+REGISTER_OP(linear_cross_entropy_backward,
+            "linear_cross_entropy_backward(Tensor grad_loss, Tensor hidden, Tensor weight, Tensor target, Tensor lse, "
+            "int ignore_index, Tensor(a!) grad_hidden, Tensor(b!) grad_weight) -> ()",
+            &kernels::linear_cross_entropy_backward);
 
 TORCH_LIBRARY(tilefusion, m) { KernelRegistry::instance().register_with_torch(m); }
 TORCH_LIBRARY_IMPL(tilefusion, CUDA, m) { KernelRegistry::instance().register_implementations(m); }
