@@ -44,27 +44,32 @@ struct GatedEpilogue {
   T *h, *gate, *up;   // gate, up: null where they are not kept
   int M, F, activation;
 
-  template <int TM, int TN>
-  TFK_DEVICE void operator()(float4_t (&acc)[TM][TN], const TileAt& at) const {
-    const int lr = at.lane & 15, lg = at.lane >> 4;
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    if (activation == TF_ACT_SILU) finish<kInside, TF_ACT_SILU>(acc, at);
+    else if (activation == TF_ACT_GELU) finish<kInside, TF_ACT_GELU>(acc, at);
+    else finish<kInside, TF_ACT_GELU_TANH>(acc, at);
+  }
+  template <bool kInside, int kActivation, int TM, int TN>
+  TFK_DEVICE void finish(float4_t (&acc)[TM][TN], const TileAt& at) const {
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      const int row = at.row + 16 * i + lr;
-      if (row >= M) continue;
+      const int row = at.row + 16 * i;
+      float4_t v[TN / 2];
+      if (gate != nullptr) {
 #pragma unroll
-      for (int j = 0; j < TN; j += 2)
+        for (int j = 0; j < TN / 2; ++j) v[j] = acc[i][2 * j];
+        store_blocks<kInside>(gate, (size_t)F, row, at.col, M, F, at.lane, v);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int col = at.col + 8 * j + 4 * lg + r;
-          if (col >= F) continue;
-          const float g = acc[i][j][r], u = acc[i][j + 1][r];
-          const size_t to = (size_t)row * F + col;
-          h[to] = (T)(act(g, activation) * u);
-          if (gate != nullptr) {
-            gate[to] = (T)g;
-            up[to] = (T)u;
-          }
-        }
+        for (int j = 0; j < TN / 2; ++j) v[j] = acc[i][2 * j + 1];
+        store_blocks<kInside>(up, (size_t)F, row, at.col, M, F, at.lane, v);
+      }
+#pragma unroll
+      for (int j = 0; j < TN / 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[j][r] = act(acc[i][2 * j][r], kActivation) * acc[i][2 * j + 1][r];
+      store_blocks<kInside>(h, (size_t)F, row, at.col, M, F, at.lane, v);
+      __builtin_amdgcn_sched_barrier(0);   // (a row of blocks at a time: registers)
     }
   }
 };
@@ -73,8 +78,8 @@ template <typename T>
 int gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up, int activation, int64_t M, int64_t F, int64_t K,
               hipStream_t st) {
   const Operands operands = {x, {w_gate, w_up}, (int)M, (int)F, (int)K};
-  return launch_product_any<T, true>(
-      "tf_gated_ffn", operands,
+  return launch_product<T, true>(
+      "tf_gated_ffn", operands, plan_product<T>(operands, true),
       GatedEpilogue<T>{static_cast<T*>(h), static_cast<T*>(gate), static_cast<T*>(up), (int)M, (int)F, activation}, st);
 }
 

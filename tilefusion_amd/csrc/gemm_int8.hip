@@ -14,23 +14,28 @@ struct Int8Epilogue {
   const float *scale_a, *scale_b;
   int M, N;
 
-  template <int TM, int TN>
-  TFK_DEVICE void operator()(float4_t (&acc)[TM][TN], const TileAt& at) const {
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
     const int lr = at.lane & 15, lg = at.lane >> 4;
+    // the lane's scales: of one row in each row of blocks, of four columns in each column of them
+    float4_t sb[TN];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sb[j][r] = scale_b[kInside ? at.col + 16 * j + 4 * lg + r : min(at.col + 16 * j + 4 * lg + r, N - 1)];
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      const int row = at.row + 16 * i + lr;
-      if (row >= M) continue;
-      const float sa = scale_a[row];
+      const int row = at.row + 16 * i;
+      const float sa = scale_a[kInside ? row + lr : min(row + lr, M - 1)];
+      float4_t v[TN];
 #pragma unroll
       for (int j = 0; j < TN; ++j) {
         const int4v_t sum = __builtin_bit_cast(int4v_t, acc[i][j]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int col = at.col + 16 * j + 4 * lg + r;
-          if (col < N) c[(size_t)row * N + col] = (OutT)((float)sum[r] * sa * scale_b[col]);
-        }
+        for (int r = 0; r < 4; ++r) v[j][r] = (float)sum[r] * sa * sb[j][r];
       }
+      store_blocks<kInside>(c, (size_t)N, row, at.col, M, N, at.lane, v);
+      __builtin_amdgcn_sched_barrier(0);   // (a row of blocks at a time: registers)
     }
   }
 };
@@ -38,7 +43,8 @@ struct Int8Epilogue {
 template <typename OutT>
 int gemm_int8(const void* A, const void* B, const float* sa, const float* sb, void* C, int64_t M, int64_t N, int64_t K, hipStream_t st) {
   const Operands x = {A, {B, nullptr}, (int)M, (int)N, (int)K};
-  return launch_product_any<int8_t, false>("tf_gemm_int8", x, Int8Epilogue<OutT>{static_cast<OutT*>(C), sa, sb, (int)M, (int)N}, st);
+  return launch_product<int8_t, false>("tf_gemm_int8", x, plan_product<int8_t>(x, false),
+                                       Int8Epilogue<OutT>{static_cast<OutT*>(C), sa, sb, (int)M, (int)N}, st);
 }
 
 // ---- quantize_rows -------------------------------------------------------------------------

@@ -29,6 +29,12 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(uint16_t* dst, int64_t c
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads) dst[i] = 0;
 }
 
+__global__ __launch_bounds__(kThreads) void zero_columns_kernel(uint16_t* dst, int64_t pitch, int64_t rows, int from, int width) {
+  const int64_t count = rows * width;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads)
+    dst[i / width * pitch + from + i % width] = 0;
+}
+
 }  // namespace
 
 int launch_transpose_padded(const char* who, const void* src, int64_t src_pitch, void* dst, int64_t pitch, int64_t rows, int64_t cols,
@@ -43,6 +49,12 @@ int launch_zero_16bit(void* dst, int64_t count, hipStream_t st) {
   if (count == 0) return TF_OK;
   const int64_t blocks = std::min<int64_t>(tiles_of(count, kThreads), 4096);
   return launch_kernel(zero_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, static_cast<uint16_t*>(dst), count);
+}
+
+int launch_zero_columns(const char*, void* dst, int64_t pitch, int64_t rows, int64_t from, int64_t to, hipStream_t st) {
+  const int64_t blocks = std::min<int64_t>(tiles_of(rows * (to - from), kThreads), 4096);
+  return launch_kernel(zero_columns_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, static_cast<uint16_t*>(dst), pitch, rows, (int)from,
+                       (int)(to - from));
 }
 
 }  // namespace tfk

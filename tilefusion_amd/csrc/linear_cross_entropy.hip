@@ -23,6 +23,8 @@ struct Part {
 // what a maximum is subtracted as: where there is none (every logit -inf), zero, so that the sum is zero and not a NaN
 TFK_DEVICE float as_origin(float top) { return top == -INFINITY ? 0.f : top; }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 struct LseEpilogue {
   Part* parts;            // [T][slots]
   int slots;
@@ -30,37 +32,49 @@ struct LseEpilogue {
   const int64_t* target;
   int M, N;
 
-  template <int TM, int TN>
-  TFK_DEVICE void operator()(float4_t (&acc)[TM][TN], const TileAt& at) const {
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    if (kInside && at.col >= at.col_from) reduce<false>(acc, at);
+    else reduce<true>(acc, at);
+  }
+  // kSome: columns in front of col_from and from N on do not count
+  template <bool kSome, int TM, int TN>
+  TFK_DEVICE void reduce(float4_t (&acc)[TM][TN], const TileAt& at) const {
     const int lr = at.lane & 15, lg = at.lane >> 4;
+    const auto counts = [&](int j, int r) __attribute__((always_inline)) {
+      const int col = at.col + 16 * j + 4 * lg + r;
+      return !kSome || (col >= at.col_from && col < N);
+    };
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int row = at.row + 16 * i + lr;
-      const int64_t wanted = row < M ? target[row] : -1;
+      const int64_t wanted = (row < M ? target[row] : -1) - at.col;   // counted from the tile's first column
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int col = at.col + 16 * j + 4 * lg + r;
-          if (col >= at.col_from && col < N) {
-            top = fmaxf(top, acc[i][j][r]);
-            if (col == wanted) at_target[row] = acc[i][j][r];
-          }
-        }
+        for (int r = 0; r < 4; ++r)
+          if (counts(j, r)) top = fmaxf(top, acc[i][j][r]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float origin = as_origin(top);
+      const float origin = as_origin(top) * kLog2e;
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int col = at.col + 16 * j + 4 * lg + r;
-          if (col >= at.col_from && col < N) sum += __expf(acc[i][j][r] - origin);
-        }
+        for (int r = 0; r < 4; ++r)
+          if (counts(j, r)) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -origin));
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
       if (lg == 0 && row < M) parts[(size_t)row * slots + at.slot] = Part{top, sum};
+      // few tiles hold a target of theirs
+      if (__any(wanted >= 0 && wanted < 16 * TN)) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (wanted == 16 * j + 4 * lg + r && counts(j, r)) at_target[row] = acc[i][j][r];
+      }
+      __builtin_amdgcn_sched_barrier(0);   // (a row of blocks at a time: registers)
     }
   }
 };
@@ -124,7 +138,7 @@ __global__ __launch_bounds__(kScaleThreads) void find_scale_kernel(const float* 
 
 template <typename T>
 struct ProbEpilogue {
-  T* p;                    // [tokens][pitch], zeros behind the piece's columns
+  T* p;                    // [tokens][pitch]
   int64_t pitch;
   const float *lse, *grad_loss;
   const Scale* scale;
@@ -133,61 +147,117 @@ struct ProbEpilogue {
   int M, N;                // tokens, columns of the piece
   int first, V;            // the piece's first column, columns of all
 
-  template <int TM, int TN>
-  TFK_DEVICE void operator()(float4_t (&acc)[TM][TN], const TileAt& at) const {
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
     const int lr = at.lane & 15, lg = at.lane >> 4;
     const float in = scale->in;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-      const int row = at.row + 16 * i + lr;
-      if (row >= M) continue;
+      const int row = kInside ? at.row + 16 * i + lr : min(at.row + 16 * i + lr, M - 1);
       const int64_t wanted = target[row];
       const bool ignored = wanted == ignore_index;
       const float origin = lse[row];
       // (a target outside the vocabulary: as the loss)
       const float weight = wanted >= 0 && wanted < V ? grad_loss[row] * in : __uint_as_float(0x7fc00000u);
-      const int64_t hot = wanted - first;
+      const int64_t hot = wanted - first - at.col;   // counted from the tile's first column
+      const float from = origin * kLog2e;
+      float4_t v[TN];
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int col = at.col + 16 * j + 4 * lg + r;
-          if (col >= pitch) continue;
-          const float value = (__expf(acc[i][j][r] - origin) - (col == hot ? 1.f : 0.f)) * weight;
-          p[(size_t)row * pitch + col] = (T)(ignored || col >= N ? 0.f : value);
-        }
+        for (int r = 0; r < 4; ++r) v[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -from)) * weight;
+      if (__any(hot >= 0 && hot < 16 * TN)) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (hot == 16 * j + 4 * lg + r) v[j][r] = (__builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -from)) - 1.f) * weight;
+      }
+      if (__any(ignored)) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[j][r] = ignored ? 0.f : v[j][r];
+      }
+      store_blocks<kInside>(p, (size_t)pitch, at.row + 16 * i, at.col, M, N, at.lane, v);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
 
-// A product that is summed over several calls in fp32, or leaves at once; the last call scales and rounds it.
+// A product that is scaled and rounded.
+template <typename T>
+struct ScaledEpilogue {
+  T* out;                  // [M][N]
+  const Scale* scale;
+  int M, N;
+
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    const float by = scale->out;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      float4_t v[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) v[j] = acc[i][j] * by;
+      store_blocks<kInside>(out, (size_t)N, at.row + 16 * i, at.col, M, N, at.lane, v);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+// One of several products that are summed in fp32; the last call scales and rounds the sum.
 template <typename T>
 struct SumEpilogue {
-  float* sum;              // [M][N], where there are several calls
+  float* sum;              // [M][N]
   T* out;                  // [M][N]
   const Scale* scale;
   bool first, last;
   int M, N;
 
-  template <int TM, int TN>
-  TFK_DEVICE void operator()(float4_t (&acc)[TM][TN], const TileAt& at) const {
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    if (kInside && at.row >= at.row_from && at.col >= at.col_from) add<true>(acc, at);
+    else add<false>(acc, at);
+  }
+  // kWhole: the tile overlaps none in front of it, and ends inside
+  template <bool kWhole, int TM, int TN>
+  TFK_DEVICE void add(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    typedef float4_t four_any_t __attribute__((aligned(4)));
     const int lr = at.lane & 15, lg = at.lane >> 4;
-    const float by = scale->out;
+    const float by = last ? scale->out : 1.f;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int row = at.row + 16 * i + lr;
-      if (row >= M || row < at.row_from) continue;
+      if (kWhole) {
+        float* const from = sum + (size_t)row * N + at.col + 4 * lg;
+        float4_t v[TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int col = at.col + 16 * j + 4 * lg + r;
-          if (col >= N || col < at.col_from) continue;
-          const size_t to = (size_t)row * N + col;
-          const float value = first ? acc[i][j][r] : acc[i][j][r] + sum[to];
-          if (last) out[to] = (T)(value * by);
-          else sum[to] = value;
+        for (int j = 0; j < TN; ++j) {
+          v[j] = acc[i][j];
+          if (!first) v[j] += *reinterpret_cast<const four_any_t*>(from + 16 * j);
+          v[j] *= by;
         }
+        if (last) {
+          store_blocks<true>(out, (size_t)N, at.row + 16 * i, at.col, M, N, at.lane, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < TN; ++j) *reinterpret_cast<four_any_t*>(from + 16 * j) = v[j];
+        }
+      } else if (row < M && row >= at.row_from) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int col = at.col + 16 * j + 4 * lg + r;
+            if (col >= N || col < at.col_from) continue;
+            const size_t to = (size_t)row * N + col;
+            const float value = (first ? acc[i][j][r] : acc[i][j][r] + sum[to]) * by;
+            if (last) out[to] = (T)value;
+            else sum[to] = value;
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -195,8 +265,9 @@ struct SumEpilogue {
 struct ForwardPlan {
   int64_t slots;
   size_t at_target, bytes;
-  ForwardPlan(int64_t T, int64_t V, int64_t) {
-    slots = any_slots(V);
+  ForwardPlan(int64_t T, int64_t V, int64_t K) {
+    // (which kernel runs also depends on where the operands start)
+    slots = std::max(product_slots(kAnyKernel, V), product_slots(pick_table_kernel(T, V, K, kOneAllowed), V));
     at_target = round_up_to(sizeof(Part) * T * slots, 256);
     bytes = at_target + round_up_to(sizeof(float) * T, 256);
   }
@@ -234,10 +305,11 @@ int forward(const void* hidden, const void* weight, const int64_t* target, float
   Part* const parts = reinterpret_cast<Part*>(ws);
   float* const at_target = reinterpret_cast<float*>(ws + plan.at_target);
   const Operands x = {hidden, {weight, nullptr}, (int)tokens, (int)V, (int)K};
-  if (int rc = launch_product_any<T, false>("tf_linear_cross_entropy", x,
-                                            LseEpilogue{parts, (int)plan.slots, at_target, target, (int)tokens, (int)V}, st))
+  const ProductPlan product = plan_product<T>(x, false);
+  if (int rc = launch_product<T, false>("tf_linear_cross_entropy", x, product,
+                                        LseEpilogue{parts, (int)product.slots, at_target, target, (int)tokens, (int)V}, st))
     return rc;
-  return launch_kernel(merge_parts_kernel, dim3((unsigned)tiles_of(tokens, kMergeRows)), dim3(kMergeThreads), 0, st, parts, (int)plan.slots,
+  return launch_kernel(merge_parts_kernel, dim3((unsigned)tiles_of(tokens, kMergeRows)), dim3(kMergeThreads), 0, st, parts, (int)product.slots,
                        at_target, target, ignore_index, (int)tokens, (int)V, loss, lse);
 }
 
@@ -258,21 +330,26 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
     const int64_t columns = std::min(plan.piece, V - first), pitch = round_up_to(columns, 64);
     const char* const w = static_cast<const char*>(weight) + 2 * first * K;
     const Operands logits = {hidden, {w, nullptr}, (int)tokens, (int)columns, (int)K};
-    if (int rc = launch_product_any<T, false>(who, logits,
+    if (int rc = launch_product<T, false>(who, logits, plan_product<T>(logits, false),
                                               ProbEpilogue<T>{p, pitch, lse, grad_loss, scale, target, ignore_index, (int)tokens, (int)columns,
                                                               (int)first, (int)V},
                                               st))
       return rc;
+    if (pitch > columns)
+      if (int rc = launch_zero_columns(who, p, pitch, tokens, columns, pitch, st)) return rc;
     if (int rc = launch_transpose_padded(who, p, pitch, ws + plan.pt, plan.Tp, tokens, columns, plan.Tp, st)) return rc;
     if (int rc = launch_transpose_padded(who, w, K, ws + plan.wt, pitch, columns, K, pitch, st)) return rc;
     const Operands of_hidden = {p, {ws + plan.wt, nullptr}, (int)tokens, (int)K, (int)pitch};
-    if (int rc = launch_product_any<T, false>(who, of_hidden,
-                                              SumEpilogue<T>{sum, static_cast<T*>(grad_hidden), scale, first == 0, first + columns == V, (int)tokens, (int)K},
-                                              st))
-      return rc;
+    const ProductPlan hidden_plan = plan_product<T>(of_hidden, false);
+    T* const to_hidden = static_cast<T*>(grad_hidden);
+    const int rc = plan.pieces == 1
+                       ? launch_product<T, false>(who, of_hidden, hidden_plan, ScaledEpilogue<T>{to_hidden, scale, (int)tokens, (int)K}, st)
+                       : launch_product<T, false>(who, of_hidden, hidden_plan,
+                                                  SumEpilogue<T>{sum, to_hidden, scale, first == 0, first + columns == V, (int)tokens, (int)K}, st);
+    if (rc) return rc;
     const Operands of_weight = {ws + plan.pt, {ws + plan.ht, nullptr}, (int)columns, (int)K, (int)plan.Tp};
-    if (int rc = launch_product_any<T, false>(
-            who, of_weight, SumEpilogue<T>{nullptr, static_cast<T*>(grad_weight) + first * K, scale, true, true, (int)columns, (int)K}, st))
+    if (int rc = launch_product<T, false>(who, of_weight, plan_product<T>(of_weight, false),
+                                          ScaledEpilogue<T>{static_cast<T*>(grad_weight) + first * K, scale, (int)columns, (int)K}, st))
       return rc;
   }
   return TF_OK;
