@@ -228,9 +228,12 @@ TF_API int tf_scatter_nd(const void* updates, void* data, const int64_t* indices
 
 /* C[M,N] = scale_a[m] * scale_b[n] * sum_k A[m,k] * B[n,k] of 8-bit integers: A [M,K] and B [N,K] int8, row-major; scale_a [M] and
  * scale_b [N] fp32; C [M,N] of c_dtype (fp32, fp16 or bf16).  The sum is exact (int32), hence K <= 131071; it is scaled in fp32 and
- * rounded once.  M = 0 and N = 0 are done at once.  (No counterpart in the reference.) */
+ * rounded once.  M = 0 and N = 0 are done at once.  A and B begin at 16-byte boundaries; where K is no multiple of 16 they may begin
+ * anywhere, and a workspace (at a 16-byte boundary, of the bytes that the function beside it says, otherwise 0) takes copies of them.
+ * (No counterpart in the reference.) */
+TF_API size_t tf_gemm_int8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 TF_API int tf_gemm_int8(const void* A, const void* B, const float* scale_a, const float* scale_b, void* C, int c_dtype,
-                        int64_t M, int64_t N, int64_t K, void* stream);
+                        int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 /* Rows of x [rows,K] (fp16 or bf16) in 8 bits: scale[r] = max|x[r]| / 127 in fp32, q[r,k] the whole number nearest to
  * x[r,k] / scale[r], the even one in the middle of two.  A row of zeros has scale 0 and q 0, a row with an infinity or a
  * NaN scale NaN and q 0.  rows < 2^24. */
@@ -245,11 +248,13 @@ typedef enum {
 
 /* h[M,F] = act(gate) * up, gate = x * w_gate^T, up = x * w_up^T: x [M,K], w_gate and w_up [F,K], all of dtype (fp16 or bf16),
  * row-major.  gate and up are kept in fp32 up to the product and rounded to dtype where the caller hands over room for them ([M,F] each,
- * both or neither), for tf_gated_ffn_backward.  M <= 2^22 - 64 and K <= 2^22 - 64, F <= 2^21 - 64. */
+ * both or neither), for tf_gated_ffn_backward.  M <= 2^22 - 64 and K <= 2^22 - 64, F <= 2^21 - 64.  x and the weights begin at 16-byte
+ * boundaries; where K is no multiple of 8 they may begin anywhere, and a workspace takes copies of them, as above. */
+TF_API size_t tf_gated_ffn_workspace_bytes(int64_t M, int64_t F, int64_t K);
 TF_API int tf_gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up, int dtype,
-                        int activation, int64_t M, int64_t F, int64_t K, void* stream);
-/* Gradients of x [M,K], w_gate and w_up [F,K] from that of h (dh [M,F]) and the gate and up values that the forward call kept.  The
- * workspace begins at a 16-byte boundary and may hold anything; it is done with when the call's work is.  w_up's gradient right behind
+                        int activation, int64_t M, int64_t F, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of x [M,K], w_gate and w_up [F,K] from that of h (dh [M,F]) and the gate and up values that the forward call kept; x and
+ * the weights as there, the others begin anywhere.  The workspace begins at a 16-byte boundary and may hold anything; it is done with when the call's work is.  w_up's gradient right behind
  * w_gate's makes one product of the two.  M = 0: the weights' gradients are zero. */
 TF_API size_t tf_gated_ffn_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
 TF_API int tf_gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const void* gate,
@@ -258,7 +263,8 @@ TF_API int tf_gated_ffn_backward(const void* dh, const void* x, const void* w_ga
 
 /* Softmax cross entropy of the logits hidden [T,K] * weight [V,K]^T, which are never in memory: lse[t] = log sum_v exp(logit[t,v]),
  * loss[t] = lse[t] - logit[t,target[t]], both fp32; hidden and weight fp16 or bf16.  loss is 0 where target[t] == ignore_index and NaN where it
- * is any other number outside 0 .. V-1.  T <= 2^22 - 64, V <= 2^30 - 64, K <= 2^22 - 64. */
+ * is any other number outside 0 .. V-1.  T <= 2^22 - 64, V <= 2^30 - 64, K <= 2^22 - 64.  hidden and weight begin at 16-byte boundaries, or, where K is
+ * no multiple of 8, anywhere. */
 TF_API size_t tf_linear_cross_entropy_workspace_bytes(int64_t T, int64_t V, int64_t K);
 TF_API int tf_linear_cross_entropy(const void* hidden, const void* weight, const int64_t* target, float* loss, float* lse,
                                    int dtype, int64_t T, int64_t V, int64_t K, int64_t ignore_index, void* workspace,

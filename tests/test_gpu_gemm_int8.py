@@ -164,4 +164,4 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             ops.quantize_rows(x)
     assert (c == 0).all()
-    assert _capi.load().tf_gemm_int8(a.data_ptr(), b.data_ptr(), s.data_ptr(), s.data_ptr(), c.data_ptr(), 0, 1, 1, 131072, None) == _capi.TF_ERR_INVALID_ARG
+    assert _capi.load().tf_gemm_int8(a.data_ptr(), b.data_ptr(), s.data_ptr(), s.data_ptr(), c.data_ptr(), 0, 1, 1, 131072, None, 0, None) == _capi.TF_ERR_INVALID_ARG

@@ -15,16 +15,23 @@ BAD, UNSUPPORTED, OK = _capi.TF_ERR_INVALID_ARG, _capi.TF_ERR_UNSUPPORTED, _capi
 
 
 def test_gemm_int8_arguments():
-    f = _capi.load().tf_gemm_int8
-    assert f(P, P, P, P, P, F32, 4, 4, 0, None) == BAD and f(P, P, P, P, P, F32, -1, 4, 4, None) == BAD
-    assert f(P, P, P, P, P, 3, 4, 4, 4, None) == UNSUPPORTED
-    assert f(P, P, P, P, P, F16, 4, 4, 131072, None) == BAD and b"131071" in _capi.load().tf_last_error()
-    assert f(P, P, P, P, P, F16, 1 << 30, 4, 4, None) == BAD
+    lib = _capi.load()
+    f, none = lib.tf_gemm_int8, (None, 0, None)
+    assert f(P, P, P, P, P, F32, 4, 4, 0, *none) == BAD and f(P, P, P, P, P, F32, -1, 4, 16, *none) == BAD
+    assert f(P, P, P, P, P, 3, 4, 4, 16, *none) == UNSUPPORTED
+    assert f(P, P, P, P, P, F16, 4, 4, 131072, *none) == BAD and b"131071" in lib.tf_last_error()
+    assert f(P, P, P, P, P, F16, 1 << 30, 4, 16, *none) == BAD
     for at in range(5):
         pointers = [P] * 5
         pointers[at] = None
-        assert f(*pointers, F16, 4, 4, 4, None) == BAD
-    assert f(None, None, None, None, None, F16, 0, 4, 4, None) == OK == f(None, None, None, None, None, F16, 4, 0, 4, None)
+        assert f(*pointers, F16, 4, 4, 16, *none) == BAD
+    assert f(None, None, None, None, None, F16, 0, 4, 4, *none) == OK == f(None, None, None, None, None, F16, 4, 0, 4, *none)
+    # rows that 16-byte requests cannot walk: room for copies of them
+    size = lib.tf_gemm_int8_workspace_bytes
+    assert size(7, 9, 160) == 0 == size(0, 9, 17) == size(7, 9, 131072) and size(7, 9, 17) == 16 * 128
+    assert f(P, P, P, P, P, F16, 7, 9, 17, P, size(7, 9, 17) - 1, None) == BAD and b"workspace" in lib.tf_last_error()
+    assert f(P, P, P, P, P, F16, 7, 9, 17, P + 8, size(7, 9, 17), None) == BAD == f(P, P, P, P, P, F16, 7, 9, 17, None, size(7, 9, 17), None)
+    assert f(P + 8, P, P, P, P, F16, 7, 9, 160, *none) == BAD == f(P, P + 1, P, P, P, F16, 7, 9, 160, *none)
 
 
 def test_quantize_rows_arguments():
@@ -36,13 +43,20 @@ def test_quantize_rows_arguments():
 
 def test_gated_ffn_arguments():
     lib = _capi.load()
-    f = lib.tf_gated_ffn
-    assert f(P, P, P, P, None, None, F32, 0, 4, 4, 4, None) == UNSUPPORTED
-    assert f(P, P, P, P, None, None, F16, 3, 4, 4, 4, None) == BAD and b"activation" in lib.tf_last_error()
-    assert f(P, P, P, P, P, None, F16, 0, 4, 4, 4, None) == BAD and f(P, P, P, None, P, P, F16, 0, 4, 4, 4, None) == BAD
-    for m, n, k in ((-1, 4, 4), (4, 0, 4), (4, 4, 0), (1 << 22, 4, 4), (4, 1 << 21, 4), (4, 4, 1 << 22)):
-        assert f(P, P, P, P, None, None, F16, 0, m, n, k, None) == BAD
-    assert f(None, None, None, None, None, None, F16, 0, 0, 4, 4, None) == OK
+    f, none = lib.tf_gated_ffn, (None, 0, None)
+    assert f(P, P, P, P, None, None, F32, 0, 4, 4, 8, *none) == UNSUPPORTED
+    assert f(P, P, P, P, None, None, F16, 3, 4, 4, 8, *none) == BAD and b"activation" in lib.tf_last_error()
+    assert f(P, P, P, P, P, None, F16, 0, 4, 4, 8, *none) == BAD and f(P, P, P, None, P, P, F16, 0, 4, 4, 8, *none) == BAD
+    for m, n, k in ((-1, 4, 8), (4, 0, 8), (4, 4, 0), (1 << 22, 4, 8), (4, 1 << 21, 8), (4, 4, 1 << 22)):
+        assert f(P, P, P, P, None, None, F16, 0, m, n, k, *none) == BAD
+    assert f(None, None, None, None, None, None, F16, 0, 0, 4, 4, *none) == OK
+    for at in range(3):
+        pointers = [P] * 4
+        pointers[at] = P + 2
+        assert f(*pointers, None, None, F16, 0, 4, 4, 8, *none) == BAD and b"boundaries" in lib.tf_last_error()
+    size = lib.tf_gated_ffn_workspace_bytes
+    assert size(4, 5, 8) == 0 == size(0, 5, 9) and size(4, 5, 9) == (4 + 10) * 128
+    assert f(P, P, P, P, None, None, F16, 0, 4, 5, 9, P, size(4, 5, 9) - 1, None) == BAD and b"workspace" in lib.tf_last_error()
     size = lib.tf_gated_ffn_backward_workspace_bytes
     assert size(0, 4, 4) == 0 == size(4, 0, 4) == size(1 << 22, 4, 4) and size(64, 64, 64) > 0
     b = lib.tf_gated_ffn_backward

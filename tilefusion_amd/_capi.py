@@ -41,9 +41,11 @@ SIGNATURES = {
     "tf_flash_attention_fwd_split": (_i, [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _i, _d, _vp, _vp]),
     "tf_transpose_16bit": (_i, [_vp, _vp, _i64, _i64, _i64, _vp]),
     "tf_scatter_nd": (_i, [_vp, _vp, _vp, ctypes.POINTER(_i64), _i, _i64, _i, _i, _vp]),
-    "tf_gemm_int8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _vp]),
+    "tf_gemm_int8_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "tf_gemm_int8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _vp, _sz, _vp]),
     "tf_quantize_rows": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _vp]),
-    "tf_gated_ffn": (_i, [_vp] * 6 + [_i, _i, _i64, _i64, _i64, _vp]),
+    "tf_gated_ffn_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "tf_gated_ffn": (_i, [_vp] * 6 + [_i, _i, _i64, _i64, _i64, _vp, _sz, _vp]),
     "tf_gated_ffn_backward_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "tf_gated_ffn_backward": (_i, [_vp] * 9 + [_i, _i, _i64, _i64, _i64, _vp, _sz, _vp]),
     "tf_linear_cross_entropy_workspace_bytes": (_sz, [_i64, _i64, _i64]),

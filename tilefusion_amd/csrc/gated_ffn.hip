@@ -7,9 +7,9 @@
 // Backward, from the gate and up values that were kept:
 //   dg = dh * up * act'(gate), du = dh * act(gate)
 //   dx = dg * Wg + du * Wu,  dWg = dg^T * x,  dWu = du^T * x
-// One pass over dh, gate and up leaves [dg | du] twice, as rows of tokens and transposed, both completed by zeros to multiples of 64; then
-// dx is one product over 2F and the weights' gradients are one (or two) over the tokens.  dg and du are rounded to the type once, as the operands of
-// the matrix instructions have to be.
+// One pass over dh, gate and up leaves [dg | du] as rows of tokens, each half completed by zeros to a multiple of 64 columns; dx is one product over the
+// 2F columns, the weights' gradients are one (or two) over the tokens.  dg and du are rounded to the type once, as operands of
+// matrix instructions have to be.
 #include "product.hpp"
 
 namespace tfk {
@@ -74,101 +74,165 @@ struct GatedEpilogue {
   }
 };
 
-template <typename T>
-int gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up, int activation, int64_t M, int64_t F, int64_t K,
-              hipStream_t st) {
-  const Operands operands = {x, {w_gate, w_up}, (int)M, (int)F, (int)K};
-  return launch_product<T, true>(
-      "tf_gated_ffn", operands, plan_product<T>(operands, true),
-      GatedEpilogue<T>{static_cast<T*>(h), static_cast<T*>(gate), static_cast<T*>(up), (int)M, (int)F, activation}, st);
-}
+// K is no multiple of 8: rows are copied, completed by zeros to whole lines.
+int64_t aligned_width(int64_t K) { return K % 8 == 0 ? K : round_up_to(K, 64); }
 
-// ---- backward ------------------------------------------------------------------------------
-constexpr int kTile = 64, kThreads = 256;
-
-// One 64 x 64 tile of dh, gate and up: dg and du to rows [dg | du] of pitch 2 * Fp, and transposed to rows of pitch Mp.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void gated_ffn_grads_kernel(const T* __restrict__ dh, const T* __restrict__ gate, const T* __restrict__ up,
-                                                                  T* __restrict__ rows, T* __restrict__ cols, int M, int F, int Mp, int Fp, int tiles_f,
-                                                                  int activation) {
-  __shared__ T s_dg[kTile][kTile + 2], s_du[kTile][kTile + 2];
-  const int m0 = blockIdx.x / tiles_f * kTile, f0 = blockIdx.x % tiles_f * kTile;
-  for (int e = threadIdx.x; e < kTile * kTile; e += kThreads) {
-    const int r = e / kTile, c = e % kTile;
-    float dg = 0.f, du = 0.f;
-    if (m0 + r < M && f0 + c < F) {
-      const size_t at = (size_t)(m0 + r) * F + f0 + c;
-      float value, slope;
-      act_both((float)gate[at], activation, value, slope);
-      const float d = (float)dh[at];
-      dg = d * (float)up[at] * slope;
-      du = d * value;
-    }
-    s_dg[r][c] = (T)dg;
-    s_du[r][c] = (T)du;
-    if (m0 + r < M) {
-      T* const to = rows + (size_t)(m0 + r) * 2 * Fp + f0 + c;
-      to[0] = (T)dg;
-      to[Fp] = (T)du;
-    }
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < kTile * kTile; e += kThreads) {
-    const int c = e / kTile, r = e % kTile;
-    if (f0 + c < F) {
-      cols[(size_t)(f0 + c) * Mp + m0 + r] = s_dg[r][c];
-      cols[(size_t)(F + f0 + c) * Mp + m0 + r] = s_du[r][c];
-    }
-  }
-}
-
-struct BackwardPlan {
-  int64_t Mp, Fp;
-  size_t rows, cols, weights, x, bytes;   // offsets in the workspace, its size
-  BackwardPlan(int64_t M, int64_t F, int64_t K) {
-    Mp = round_up_to(M, 64);
-    Fp = round_up_to(F, 64);
-    size_t at = 0;
-    auto take = [&](int64_t elements) {
-      const size_t from = at;
-      at += round_up_to(2 * elements, 256);
-      return from;
-    };
-    rows = take(M * 2 * Fp);      // [dg | du]
-    cols = take(2 * F * Mp);      // the same transposed
-    weights = take(K * 2 * Fp);   // [Wg^T | Wu^T]
-    x = take(K * Mp);             // x^T
-    bytes = at;
+struct ForwardPlan {
+  size_t w_gate = 0, w_up = 0, bytes = 0;   // copies: offsets (of x: 0), all
+  ForwardPlan(int64_t M, int64_t F, int64_t K) {
+    if (K % 8 == 0) return;
+    w_gate = 2 * M * aligned_width(K);
+    w_up = w_gate + 2 * F * aligned_width(K);
+    bytes = w_up + 2 * F * aligned_width(K);
   }
 };
 
 template <typename T>
+int gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up, int activation, int64_t M, int64_t F, int64_t K,
+              char* ws, hipStream_t st) {
+  constexpr const char* who = "tf_gated_ffn";
+  const ForwardPlan copy(M, F, K);
+  if (copy.bytes > 0) {
+    const int64_t pitch = 2 * aligned_width(K);
+    if (int rc = launch_copy_rows(who, x, 2 * K, M, ws, pitch, M, st)) return rc;
+    if (int rc = launch_copy_rows(who, w_gate, 2 * K, F, ws + copy.w_gate, pitch, F, st)) return rc;
+    if (int rc = launch_copy_rows(who, w_up, 2 * K, F, ws + copy.w_up, pitch, F, st)) return rc;
+    x = ws;
+    w_gate = ws + copy.w_gate;
+    w_up = ws + copy.w_up;
+  }
+  const Operands operands = {x, {w_gate, w_up}, (int)M, (int)F, (int)aligned_width(K)};
+  return launch_product<T, true>(
+      who, operands, plan_product(M, F, aligned_width(K), true),
+      GatedEpilogue<T>{static_cast<T*>(h), static_cast<T*>(gate), static_cast<T*>(up), (int)M, (int)F, activation}, st);
+}
+
+// ---- backward ------------------------------------------------------------------------------
+constexpr int kThreads = 256;
+
+// dg and du to rows [dg | du] of pitch 2 * Fp, zeros behind F columns of each.  Eight elements a lane; bound by memory (five streams of 16 bits an
+// element).
+template <typename T, int kActivation>
+__global__ __launch_bounds__(kThreads) void gated_ffn_grads_kernel(const T* __restrict__ dh, const T* __restrict__ gate, const T* __restrict__ up,
+                                                                  T* __restrict__ rows, int64_t count, int F, int Fp) {
+  typedef T eight_t __attribute__((ext_vector_type(8)));
+  typedef eight_t eight_any_t __attribute__((aligned(2)));
+  const int chunks = Fp / 8;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads) {
+    const int64_t row = i / chunks;
+    const int col = (int)(i - row * chunks) * 8;
+    const size_t at = (size_t)row * F + col;
+    eight_t d, g, u, dg, du;
+    if (col + 8 <= F) {
+      d = *reinterpret_cast<const eight_any_t*>(dh + at);
+      g = *reinterpret_cast<const eight_any_t*>(gate + at);
+      u = *reinterpret_cast<const eight_any_t*>(up + at);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const bool in = col + t < F;
+        d[t] = in ? dh[at + t] : (T)0.f;
+        g[t] = in ? gate[at + t] : (T)0.f;
+        u[t] = in ? up[at + t] : (T)0.f;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      float value, slope;
+      act_both((float)g[t], kActivation, value, slope);
+      dg[t] = (T)((float)d[t] * (float)u[t] * slope);
+      du[t] = (T)((float)d[t] * value);
+    }
+    T* const to = rows + (size_t)row * 2 * Fp + col;
+    *reinterpret_cast<eight_t*>(to) = dg;
+    *reinterpret_cast<eight_t*>(to + Fp) = du;
+  }
+}
+
+struct BackwardPlan {
+  int64_t Fp, Kp;
+  bool copy_weights, copy_x;
+  ColsPlan of_x, of_both, of_one; // products: dx, the weights' gradients together, one of them
+  size_t weights, x, parts, bytes;   // offsets in the workspace ([dg | du]: 0), its size
+  BackwardPlan(int64_t M, int64_t F, int64_t K) {
+    Fp = round_up_to(F, 64);
+    Kp = aligned_width(K);
+    // the sum over F goes on in the second weight at a whole k-tile
+    copy_weights = Kp != K || Fp != F;
+    copy_x = Kp != K;
+    of_x = plan_cols(M, K, 2 * Fp / 64);
+    of_both = plan_cols(2 * F, K, tiles_of(M, 64));
+    of_one = plan_cols(F, K, tiles_of(M, 64));
+    size_t at = 0;
+    auto take = [&](int64_t bytes_) {
+      const size_t from = at;
+      at += round_up_to(bytes_, 256);
+      return from;
+    };
+    take(2 * M * 2 * Fp);
+    weights = take(copy_weights ? 2 * 2 * Fp * Kp : 0);
+    x = take(copy_x ? 2 * M * Kp : 0);
+    const auto floats = [K](const ColsPlan& plan, int64_t rows) { return plan.splits > 1 ? PartsRoom(plan, rows, K).floats : 0; };
+    parts = take(4 * std::max({floats(of_x, M), floats(of_both, 2 * F), floats(of_one, F)}));
+    bytes = at;
+  }
+};
+
+// out [rows, K] = the product, in as many parts as its plan says
+template <typename T, bool kColA>
+int product_of_gradient(const char* who, const ColsProduct& product, const ColsPlan& plan, T* out, float* parts, hipStream_t st) {
+  const int rows = product.a.extent, cols = product.b.extent;
+  if (plan.splits == 1) return launch_cols<T, kColA>(who, product, plan, WholeEpilogue<T>{out, nullptr, rows, cols}, st);
+  const PartsRoom room(plan, rows, cols);
+  if (int rc = launch_cols<T, kColA>(who, product, plan, PartEpilogue{parts, room.rows, room.pitch, false}, st)) return rc;
+  return launch_sum_parts<T>(parts, room, plan.splits, 0, rows, cols, out, nullptr, st);
+}
+
+template <typename T>
 int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const void* gate, const void* up, void* dx, void* dw_gate,
-                       void* dw_up, int dtype, int activation, int64_t M, int64_t F, int64_t K, char* ws, hipStream_t st) {
+                       void* dw_up, int activation, int64_t M, int64_t F, int64_t K, char* ws, hipStream_t st) {
   constexpr const char* who = "tf_gated_ffn_backward";
   if (M == 0) {
     if (int rc = launch_zero_16bit(dw_gate, F * K, st)) return rc;
     return launch_zero_16bit(dw_up, F * K, st);
   }
   const BackwardPlan p(M, F, K);
-  T* const rows = reinterpret_cast<T*>(ws + p.rows);
-  T* const cols = reinterpret_cast<T*>(ws + p.cols);
-  const int64_t tiles_f = p.Fp / kTile, tiles = tiles_f * (p.Mp / kTile);
-  TFK_REQUIRE(tiles < (int64_t)1 << 24, TF_ERR_INVALID_ARG, "%s: gradient too large", who);
-  if (int rc = launch_kernel(gated_ffn_grads_kernel<T>, dim3((unsigned)tiles), dim3(kThreads), 0, st, static_cast<const T*>(dh),
-                             static_cast<const T*>(gate), static_cast<const T*>(up), rows, cols, (int)M, (int)F, (int)p.Mp, (int)p.Fp, (int)tiles_f,
-                             activation))
+  T* const rows = reinterpret_cast<T*>(ws);
+  const int64_t chunks = M * (p.Fp / 8);
+  const auto grads = activation == TF_ACT_SILU   ? gated_ffn_grads_kernel<T, TF_ACT_SILU>
+                     : activation == TF_ACT_GELU ? gated_ffn_grads_kernel<T, TF_ACT_GELU>
+                                                 : gated_ffn_grads_kernel<T, TF_ACT_GELU_TANH>;
+  if (int rc = launch_kernel(grads, dim3((unsigned)std::min<int64_t>(tiles_of(chunks, kThreads), 65536)), dim3(kThreads), 0, st,
+                             static_cast<const T*>(dh), static_cast<const T*>(gate), static_cast<const T*>(up), rows, chunks, (int)F, (int)p.Fp))
     return rc;
-  T* const weights = reinterpret_cast<T*>(ws + p.weights);
-  if (int rc = launch_transpose_padded(who, w_gate, K, weights, 2 * p.Fp, F, K, p.Fp, st)) return rc;
-  if (int rc = launch_transpose_padded(who, w_up, K, weights + p.Fp, 2 * p.Fp, F, K, p.Fp, st)) return rc;
-  if (int rc = launch_transpose_padded(who, x, K, ws + p.x, p.Mp, M, K, p.Mp, st)) return rc;
-  if (int rc = tf_gemm(rows, weights, dx, dtype, 0, M, K, 2 * p.Fp, 1, 1, 1, 1, 0, st)) return rc;
+  if (p.copy_weights) {
+    char* const to = ws + p.weights;
+    if (int rc = launch_copy_rows(who, w_gate, 2 * K, F, to, 2 * p.Kp, p.Fp, st)) return rc;
+    if (int rc = launch_copy_rows(who, w_up, 2 * K, F, to + 2 * p.Fp * p.Kp, 2 * p.Kp, p.Fp, st)) return rc;
+    w_gate = to;
+    w_up = to + 2 * p.Fp * p.Kp;
+  }
+  if (p.copy_x) {
+    if (int rc = launch_copy_rows(who, x, 2 * K, M, ws + p.x, 2 * p.Kp, M, st)) return rc;
+    x = ws + p.x;
+  }
+  float* const parts = reinterpret_cast<float*>(ws + p.parts);
+  const auto bits = [](const void* t) { return static_cast<const uint16_t*>(t); };
+  const uint16_t* const grads_at = bits(ws);
+  const ColsProduct of_x = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)M}, {bits(w_gate), p.Kp, (int)p.Kp, (int)K}, bits(w_up), (int)(p.Fp / 64), (int)(2 * p.Fp / 64), 0, 0};
+  if (int rc = product_of_gradient<T, false>(who, of_x, p.of_x, static_cast<T*>(dx), parts, st)) return rc;
+  const int m_tiles = (int)tiles_of(M, 64), m_pad = (int)(m_tiles * 64 - M);
+  const ColsOperand tokens = {bits(x), p.Kp, (int)p.Kp, (int)K};
   // (one product where the two gradients lie one behind the other)
-  const bool together = static_cast<char*>(dw_up) == static_cast<char*>(dw_gate) + 2 * F * K && 2 * F < (1 << 30);
-  if (together) return tf_gemm(cols, ws + p.x, dw_gate, dtype, 0, 2 * F, K, p.Mp, 1, 1, 1, 1, 0, st);
-  if (int rc = tf_gemm(cols, ws + p.x, dw_gate, dtype, 0, F, K, p.Mp, 1, 1, 1, 1, 0, st)) return rc;
-  return tf_gemm(cols + F * p.Mp, ws + p.x, dw_up, dtype, 0, F, K, p.Mp, 1, 1, 1, 1, 0, st);
+  if (p.Fp == F && static_cast<char*>(dw_up) == static_cast<char*>(dw_gate) + 2 * F * K) {
+    const ColsProduct both = {{grads_at, 2 * p.Fp, (int)(2 * F), (int)(2 * F)}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
+    return product_of_gradient<T, true>(who, both, p.of_both, static_cast<T*>(dw_gate), parts, st);
+  }
+  for (int half = 0; half < 2; ++half) {
+    const ColsProduct product = {{grads_at + half * p.Fp, 2 * p.Fp, (int)p.Fp, (int)F}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
+    if (int rc = product_of_gradient<T, true>(who, product, p.of_one, static_cast<T*>(half ? dw_up : dw_gate), parts, st)) return rc;
+  }
+  return TF_OK;
 }
 
 int check_sizes(const char* who, int dtype, int activation, int64_t M, int64_t F, int64_t K) {
@@ -183,16 +247,28 @@ int check_sizes(const char* who, int dtype, int activation, int64_t M, int64_t F
 }  // namespace
 }  // namespace tfk
 
+extern "C" size_t tf_gated_ffn_workspace_bytes(int64_t M, int64_t F, int64_t K) {
+  using namespace tfk;
+  if (M <= 0 || check_sizes("tf_gated_ffn_workspace_bytes", TF_DTYPE_F16, TF_ACT_SILU, M, F, K) != TF_OK) return 0;
+  return ForwardPlan(M, F, K).bytes;
+}
+
 extern "C" int tf_gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up, int dtype, int activation, int64_t M,
-                            int64_t F, int64_t K, void* stream) {
+                            int64_t F, int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace tfk;
   if (int rc = check_sizes("tf_gated_ffn", dtype, activation, M, F, K)) return rc;
   if (M == 0) return TF_OK;
   TFK_REQUIRE(x && w_gate && w_up && h, TF_ERR_INVALID_ARG, "tf_gated_ffn: null pointer");
   TFK_REQUIRE((gate == nullptr) == (up == nullptr), TF_ERR_INVALID_ARG, "tf_gated_ffn: gate and up are kept both or neither");
+  const size_t want = ForwardPlan(M, F, K).bytes;
+  TFK_REQUIRE(want > 0 || (at_16B(x) && at_16B(w_gate) && at_16B(w_up)), TF_ERR_INVALID_ARG,
+              "tf_gated_ffn: x and the weights must begin at 16-byte boundaries");
+  TFK_REQUIRE(want == 0 || (workspace && workspace_bytes >= want && at_16B(workspace)), TF_ERR_INVALID_ARG,
+              "tf_gated_ffn: workspace of %zu bytes at a 16-byte boundary needed, got %zu", want, workspace_bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == TF_DTYPE_F16) return gated_ffn<half_t>(x, w_gate, w_up, h, gate, up, activation, M, F, K, st);
-  return gated_ffn<bf16_t>(x, w_gate, w_up, h, gate, up, activation, M, F, K, st);
+  char* const ws = static_cast<char*>(workspace);
+  if (dtype == TF_DTYPE_F16) return gated_ffn<half_t>(x, w_gate, w_up, h, gate, up, activation, M, F, K, ws, st);
+  return gated_ffn<bf16_t>(x, w_gate, w_up, h, gate, up, activation, M, F, K, ws, st);
 }
 
 extern "C" size_t tf_gated_ffn_backward_workspace_bytes(int64_t M, int64_t F, int64_t K) {
@@ -209,6 +285,8 @@ extern "C" int tf_gated_ffn_backward(const void* dh, const void* x, const void* 
   TFK_REQUIRE(dw_gate && dw_up, TF_ERR_INVALID_ARG, "tf_gated_ffn_backward: null pointer");
   if (M > 0) {
     TFK_REQUIRE(dh && x && w_gate && w_up && gate && up && dx, TF_ERR_INVALID_ARG, "tf_gated_ffn_backward: null pointer");
+    TFK_REQUIRE(K % 8 != 0 || (at_16B(x) && at_16B(w_gate) && at_16B(w_up)), TF_ERR_INVALID_ARG,
+                "tf_gated_ffn_backward: x and the weights must begin at 16-byte boundaries");
     const size_t want = BackwardPlan(M, F, K).bytes;
     TFK_REQUIRE(workspace && workspace_bytes >= want && at_16B(workspace), TF_ERR_INVALID_ARG,
                 "tf_gated_ffn_backward: workspace of %zu bytes at a 16-byte boundary needed, got %zu", want, workspace_bytes);
@@ -216,6 +294,6 @@ extern "C" int tf_gated_ffn_backward(const void* dh, const void* x, const void* 
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* const ws = static_cast<char*>(workspace);
   if (dtype == TF_DTYPE_F16)
-    return gated_ffn_backward<half_t>(dh, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, dtype, activation, M, F, K, ws, st);
-  return gated_ffn_backward<bf16_t>(dh, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, dtype, activation, M, F, K, ws, st);
+    return gated_ffn_backward<half_t>(dh, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, activation, M, F, K, ws, st);
+  return gated_ffn_backward<bf16_t>(dh, x, w_gate, w_up, gate, up, dx, dw_gate, dw_up, activation, M, F, K, ws, st);
 }

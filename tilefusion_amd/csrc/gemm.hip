@@ -494,6 +494,8 @@ int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed) {
   return best;
 }
 
+float expected_table_us(int kernel, int64_t tiles, int64_t k_tiles) { return expected_us(kGemmKernels[kernel], tiles, (int)k_tiles, false, nullptr); }
+
 namespace {
 
 template <typename OutT, typename InT>

@@ -5,6 +5,8 @@
 // Forward.  A tile of the product is reduced, in the registers it was computed in, to a maximum and a sum of exp(z - maximum) for each of
 // its rows, and the lane that holds the target's logit writes that down; a second kernel merges the parts of a row.
 //
+// (rows of K that is no multiple of 8 are copied first, completed by zeros to whole lines)
+//
 // Backward, a piece of the vocabulary at a time: the product is computed again, and from lse
 //   P[t, v] = grad_loss[t] * (exp(z[t, v] - lse[t]) - [v = target[t]]),   dH += P * W,   dW = P^T * H.
 // P of a piece is rounded to 16 bits, as the operand of a matrix instruction has to be, divided by the smallest power of two that no
@@ -110,10 +112,6 @@ __global__ __launch_bounds__(kMergeThreads) void merge_parts_kernel(const Part* 
 }
 
 // ---- backward ------------------------------------------------------------------------------
-struct Scale {
-  float in, out;   // P holds grad_loss * in, sums are multiplied by out
-};
-
 constexpr int kScaleThreads = 1024;
 __global__ __launch_bounds__(kScaleThreads) void find_scale_kernel(const float* __restrict__ grad_loss, const int64_t* __restrict__ target,
                                                                    int64_t ignore_index, int T, int headroom, Scale* scale) {
@@ -138,7 +136,7 @@ __global__ __launch_bounds__(kScaleThreads) void find_scale_kernel(const float* 
 
 template <typename T>
 struct ProbEpilogue {
-  T* p;                    // [tokens][pitch]
+  T* p;                    // [tokens][pitch], the piece's first column
   int64_t pitch;
   const float *lse, *grad_loss;
   const Scale* scale;
@@ -185,131 +183,75 @@ struct ProbEpilogue {
   }
 };
 
-// A product that is scaled and rounded.
-template <typename T>
-struct ScaledEpilogue {
-  T* out;                  // [M][N]
-  const Scale* scale;
-  int M, N;
-
-  template <bool kInside, int TM, int TN>
-  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
-    const float by = scale->out;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      float4_t v[TN];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) v[j] = acc[i][j] * by;
-      store_blocks<kInside>(out, (size_t)N, at.row + 16 * i, at.col, M, N, at.lane, v);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-};
-
-// One of several products that are summed in fp32; the last call scales and rounds the sum.
-template <typename T>
-struct SumEpilogue {
-  float* sum;              // [M][N]
-  T* out;                  // [M][N]
-  const Scale* scale;
-  bool first, last;
-  int M, N;
-
-  template <bool kInside, int TM, int TN>
-  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
-    if (kInside && at.row >= at.row_from && at.col >= at.col_from) add<true>(acc, at);
-    else add<false>(acc, at);
-  }
-  // kWhole: the tile overlaps none in front of it, and ends inside
-  template <bool kWhole, int TM, int TN>
-  TFK_DEVICE void add(float4_t (&acc)[TM][TN], const TileAt& at) const {
-    typedef float4_t four_any_t __attribute__((aligned(4)));
-    const int lr = at.lane & 15, lg = at.lane >> 4;
-    const float by = last ? scale->out : 1.f;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const int row = at.row + 16 * i + lr;
-      if (kWhole) {
-        float* const from = sum + (size_t)row * N + at.col + 4 * lg;
-        float4_t v[TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          v[j] = acc[i][j];
-          if (!first) v[j] += *reinterpret_cast<const four_any_t*>(from + 16 * j);
-          v[j] *= by;
-        }
-        if (last) {
-          store_blocks<true>(out, (size_t)N, at.row + 16 * i, at.col, M, N, at.lane, v);
-        } else {
-#pragma unroll
-          for (int j = 0; j < TN; ++j) *reinterpret_cast<four_any_t*>(from + 16 * j) = v[j];
-        }
-      } else if (row < M && row >= at.row_from) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int col = at.col + 16 * j + 4 * lg + r;
-            if (col >= N || col < at.col_from) continue;
-            const size_t to = (size_t)row * N + col;
-            const float value = (first ? acc[i][j][r] : acc[i][j][r] + sum[to]) * by;
-            if (last) out[to] = (T)value;
-            else sum[to] = value;
-          }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-};
+int64_t aligned_width(int64_t K) { return K % 8 == 0 ? K : round_up_to(K, 64); }
 
 struct ForwardPlan {
-  int64_t slots;
-  size_t at_target, bytes;
+  ProductPlan product;
+  size_t at_target, hidden, weight, bytes;   // offsets in the workspace (of the parts: 0; hidden, weight: copies), its size
   ForwardPlan(int64_t T, int64_t V, int64_t K) {
-    // (which kernel runs also depends on where the operands start)
-    slots = std::max(product_slots(kAnyKernel, V), product_slots(pick_table_kernel(T, V, K, kOneAllowed), V));
-    at_target = round_up_to(sizeof(Part) * T * slots, 256);
-    bytes = at_target + round_up_to(sizeof(float) * T, 256);
-  }
-};
-
-// What is held for a piece of the vocabulary: P as it is and transposed, and W transposed; beside them H transposed and the sums of dH.
-struct BackwardPlan {
-  int64_t Tp, piece;   // tokens completed to a multiple of 64, columns of a piece
-  int64_t pieces;
-  size_t p, pt, wt, ht, sum, scale, bytes;
-  BackwardPlan(int64_t T, int64_t V, int64_t K) {
-    Tp = round_up_to(T, 64);
-    piece = std::min(round_up_to(V, 64), std::max<int64_t>(4096, ((int64_t)1 << 27) / Tp / 256 * 256));
-    pieces = tiles_of(V, piece);
+    const int64_t width = aligned_width(K);
+    product = plan_product(T, V, width, false);
     size_t at = 0;
     auto take = [&](int64_t bytes_) {
       const size_t from = at;
       at += round_up_to(bytes_, 256);
       return from;
     };
-    p = take(2 * T * piece);
-    pt = take(2 * piece * Tp);
-    wt = take(2 * K * piece);
-    ht = take(2 * K * Tp);
-    sum = take(pieces > 1 ? 4 * T * K : 0);
-    scale = take(sizeof(Scale));
+    take(sizeof(Part) * T * product.slots);
+    at_target = take(sizeof(float) * T);
+    hidden = take(width != K ? 2 * T * width : 0);
+    weight = take(width != K ? 2 * V * width : 0);
     bytes = at;
   }
+};
+
+// What is held for a piece of the vocabulary: P, completed by zeros in front of its columns to a multiple of 64 (they meet the rows of zeros that
+// the product over them begins with); and parts of the sums.
+struct BackwardPlan {
+  int64_t width, piece, pieces;      // K with its zeros, columns of a piece (the last may have fewer)
+  ColsPlan of_hidden, of_weight;     // (the last piece's are as those of the others)
+  size_t scale, hidden, weight, hidden_parts, weight_parts, bytes;   // offsets in the workspace (of P: 0), its size
+  BackwardPlan(int64_t T, int64_t V, int64_t K) {
+    width = aligned_width(K);
+    piece = std::min(round_up_to(V, 64), std::max<int64_t>(4096, kPieceElements / T / 256 * 256));
+    pieces = tiles_of(V, piece);
+    of_hidden = plan_cols(T, K, piece / 64);
+    of_weight = plan_cols(piece, K, tiles_of(T, 64));
+    size_t at = 0;
+    auto take = [&](int64_t bytes_) {
+      const size_t from = at;
+      at += round_up_to(bytes_, 256);
+      return from;
+    };
+    take(2 * T * piece);
+    scale = take(sizeof(Scale));
+    hidden = take(width != K ? 2 * T * width : 0);
+    weight = take(width != K ? 2 * piece * width : 0);
+    hidden_parts = take(pieces > 1 || of_hidden.splits > 1 ? 4 * PartsRoom(of_hidden, T, K).floats : 0);
+    weight_parts = take(of_weight.splits > 1 ? 4 * PartsRoom(of_weight, piece, K).floats : 0);
+    bytes = at;
+  }
+  static constexpr int64_t kPieceElements = (int64_t)1 << 27;   // of P, 256 MiB
 };
 
 template <typename T>
 int forward(const void* hidden, const void* weight, const int64_t* target, float* loss, float* lse, int64_t tokens, int64_t V, int64_t K,
             int64_t ignore_index, char* ws, hipStream_t st) {
+  constexpr const char* who = "tf_linear_cross_entropy";
   const ForwardPlan plan(tokens, V, K);
+  const int64_t width = aligned_width(K);
+  if (width != K) {
+    if (int rc = launch_copy_rows(who, hidden, 2 * K, tokens, ws + plan.hidden, 2 * width, tokens, st)) return rc;
+    if (int rc = launch_copy_rows(who, weight, 2 * K, V, ws + plan.weight, 2 * width, V, st)) return rc;
+    hidden = ws + plan.hidden;
+    weight = ws + plan.weight;
+  }
   Part* const parts = reinterpret_cast<Part*>(ws);
   float* const at_target = reinterpret_cast<float*>(ws + plan.at_target);
-  const Operands x = {hidden, {weight, nullptr}, (int)tokens, (int)V, (int)K};
-  const ProductPlan product = plan_product<T>(x, false);
-  if (int rc = launch_product<T, false>("tf_linear_cross_entropy", x, product,
-                                        LseEpilogue{parts, (int)product.slots, at_target, target, (int)tokens, (int)V}, st))
+  const Operands x = {hidden, {weight, nullptr}, (int)tokens, (int)V, (int)width};
+  if (int rc = launch_product<T, false>(who, x, plan.product, LseEpilogue{parts, (int)plan.product.slots, at_target, target, (int)tokens, (int)V}, st))
     return rc;
-  return launch_kernel(merge_parts_kernel, dim3((unsigned)tiles_of(tokens, kMergeRows)), dim3(kMergeThreads), 0, st, parts, (int)product.slots,
+  return launch_kernel(merge_parts_kernel, dim3((unsigned)tiles_of(tokens, kMergeRows)), dim3(kMergeThreads), 0, st, parts, (int)plan.product.slots,
                        at_target, target, ignore_index, (int)tokens, (int)V, loss, lse);
 }
 
@@ -319,40 +261,65 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
   constexpr const char* who = "tf_linear_cross_entropy_backward";
   if (tokens == 0) return launch_zero_16bit(grad_weight, V * K, st);
   const BackwardPlan plan(tokens, V, K);
-  T* const p = reinterpret_cast<T*>(ws + plan.p);
+  T* const p = reinterpret_cast<T*>(ws);
   Scale* const scale = reinterpret_cast<Scale*>(ws + plan.scale);
-  float* const sum = reinterpret_cast<float*>(ws + plan.sum);
+  float* const hidden_parts = reinterpret_cast<float*>(ws + plan.hidden_parts);
+  float* const weight_parts = reinterpret_cast<float*>(ws + plan.weight_parts);
   constexpr int kHeadroom = std::is_same_v<T, half_t> ? 14 : 0;
   if (int rc = launch_kernel(find_scale_kernel, dim3(1), dim3(kScaleThreads), 0, st, grad_loss, target, ignore_index, (int)tokens, kHeadroom, scale))
     return rc;
-  if (int rc = launch_transpose_padded(who, hidden, K, ws + plan.ht, plan.Tp, tokens, K, plan.Tp, st)) return rc;
+  if (plan.width != K) {
+    if (int rc = launch_copy_rows(who, hidden, 2 * K, tokens, ws + plan.hidden, 2 * plan.width, tokens, st)) return rc;
+    hidden = ws + plan.hidden;
+  }
+  const auto bits = [](const void* t) { return static_cast<const uint16_t*>(t); };
+  const int width = (int)plan.width;
+  const int t_tiles = (int)tiles_of(tokens, 64), t_pad = (int)(t_tiles * 64 - tokens);
+  const ColsOperand of_tokens = {bits(hidden), width, width, (int)K};
+  const PartsRoom hidden_room(plan.of_hidden, tokens, K), weight_room(plan.of_weight, plan.piece, K);
   for (int64_t first = 0; first < V; first += plan.piece) {
     const int64_t columns = std::min(plan.piece, V - first), pitch = round_up_to(columns, 64);
-    const char* const w = static_cast<const char*>(weight) + 2 * first * K;
-    const Operands logits = {hidden, {w, nullptr}, (int)tokens, (int)columns, (int)K};
-    if (int rc = launch_product<T, false>(who, logits, plan_product<T>(logits, false),
-                                              ProbEpilogue<T>{p, pitch, lse, grad_loss, scale, target, ignore_index, (int)tokens, (int)columns,
-                                                              (int)first, (int)V},
-                                              st))
+    const int pad = (int)(pitch - columns);
+    const char* w = static_cast<const char*>(weight) + 2 * first * K;
+    if (plan.width != K) {
+      if (int rc = launch_copy_rows(who, w, 2 * K, columns, ws + plan.weight, 2 * plan.width, columns, st)) return rc;
+      w = ws + plan.weight;
+    }
+    const Operands logits = {hidden, {w, nullptr}, (int)tokens, (int)columns, width};
+    if (int rc = launch_product<T, false>(who, logits, plan_product(tokens, columns, width, false),
+                                          ProbEpilogue<T>{p + pad, pitch, lse, grad_loss, scale, target, ignore_index, (int)tokens, (int)columns,
+                                                          (int)first, (int)V},
+                                          st))
       return rc;
-    if (pitch > columns)
-      if (int rc = launch_zero_columns(who, p, pitch, tokens, columns, pitch, st)) return rc;
-    if (int rc = launch_transpose_padded(who, p, pitch, ws + plan.pt, plan.Tp, tokens, columns, plan.Tp, st)) return rc;
-    if (int rc = launch_transpose_padded(who, w, K, ws + plan.wt, pitch, columns, K, pitch, st)) return rc;
-    const Operands of_hidden = {p, {ws + plan.wt, nullptr}, (int)tokens, (int)K, (int)pitch};
-    const ProductPlan hidden_plan = plan_product<T>(of_hidden, false);
-    T* const to_hidden = static_cast<T*>(grad_hidden);
-    const int rc = plan.pieces == 1
-                       ? launch_product<T, false>(who, of_hidden, hidden_plan, ScaledEpilogue<T>{to_hidden, scale, (int)tokens, (int)K}, st)
-                       : launch_product<T, false>(who, of_hidden, hidden_plan,
-                                                  SumEpilogue<T>{sum, to_hidden, scale, first == 0, first + columns == V, (int)tokens, (int)K}, st);
+    if (pad > 0)
+      if (int rc = launch_zero_columns(p, pitch, tokens, 0, pad, st)) return rc;
+
+    // dH += P * W
+    ColsPlan of_hidden = plan.of_hidden;
+    of_hidden.per_split = (int)tiles_of(pitch / 64, of_hidden.splits);
+    const int split_parts = (int)tiles_of(pitch / 64, of_hidden.per_split);   // (a short last piece may have fewer)
+    of_hidden.splits = split_parts;
+    const ColsProduct hidden_product = {{bits(p), pitch, (int)pitch, (int)tokens}, {bits(w), width, width, (int)K}, bits(w), INT_MAX, (int)(pitch / 64), pad, 0};
+    int rc;
+    if (plan.pieces == 1 && plan.of_hidden.splits == 1)
+      rc = launch_cols<T, false>(who, hidden_product, of_hidden, WholeEpilogue<T>{static_cast<T*>(grad_hidden), scale, (int)tokens, (int)K}, st);
+    else
+      rc = launch_cols<T, false>(who, hidden_product, of_hidden, PartEpilogue{hidden_parts, hidden_room.rows, hidden_room.pitch, first > 0}, st);
     if (rc) return rc;
-    const Operands of_weight = {ws + plan.pt, {ws + plan.ht, nullptr}, (int)columns, (int)K, (int)plan.Tp};
-    if (int rc = launch_product<T, false>(who, of_weight, plan_product<T>(of_weight, false),
-                                          ScaledEpilogue<T>{static_cast<T*>(grad_weight) + first * K, scale, (int)columns, (int)K}, st))
-      return rc;
+
+    // dW = P^T * H: the columns of P in front of the piece's are rows that are not stored
+    const ColsProduct weight_product = {{bits(p), pitch, (int)pitch, (int)pitch}, of_tokens, of_tokens.x, INT_MAX, t_tiles, t_pad, pad};
+    T* const out = static_cast<T*>(grad_weight) + first * K;
+    if (plan.of_weight.splits == 1) {
+      rc = launch_cols<T, true>(who, weight_product, plan.of_weight, WholeEpilogue<T>{out - (int64_t)pad * K, scale, (int)pitch, (int)K}, st);
+    } else {
+      rc = launch_cols<T, true>(who, weight_product, plan.of_weight, PartEpilogue{weight_parts, weight_room.rows, weight_room.pitch, false}, st);
+      if (rc == TF_OK) rc = launch_sum_parts<T>(weight_parts, weight_room, plan.of_weight.splits, pad, pitch, K, out, scale, st);
+    }
+    if (rc) return rc;
   }
-  return TF_OK;
+  if (plan.pieces == 1 && plan.of_hidden.splits == 1) return TF_OK;
+  return launch_sum_parts<T>(hidden_parts, hidden_room, plan.of_hidden.splits, 0, tokens, K, static_cast<T*>(grad_hidden), scale, st);
 }
 
 int check_sizes(const char* who, int dtype, int64_t T, int64_t V, int64_t K) {
@@ -377,6 +344,8 @@ extern "C" int tf_linear_cross_entropy(const void* hidden, const void* weight, c
   if (int rc = check_sizes("tf_linear_cross_entropy", dtype, T, V, K)) return rc;
   if (T == 0) return TF_OK;
   TFK_REQUIRE(hidden && weight && target && loss && lse, TF_ERR_INVALID_ARG, "tf_linear_cross_entropy: null pointer");
+  TFK_REQUIRE(K % 8 != 0 || (at_16B(hidden) && at_16B(weight)), TF_ERR_INVALID_ARG,
+              "tf_linear_cross_entropy: hidden and weight must begin at 16-byte boundaries");
   const size_t want = ForwardPlan(T, V, K).bytes;
   TFK_REQUIRE(workspace && workspace_bytes >= want && at_16B(workspace), TF_ERR_INVALID_ARG,
               "tf_linear_cross_entropy: workspace of %zu bytes at a 16-byte boundary needed, got %zu", want, workspace_bytes);
@@ -401,6 +370,8 @@ extern "C" int tf_linear_cross_entropy_backward(const float* grad_loss, const vo
   if (T > 0) {
     TFK_REQUIRE(grad_loss && hidden && weight && target && lse && grad_hidden, TF_ERR_INVALID_ARG,
                 "tf_linear_cross_entropy_backward: null pointer");
+    TFK_REQUIRE(K % 8 != 0 || (at_16B(hidden) && at_16B(weight)), TF_ERR_INVALID_ARG,
+                "tf_linear_cross_entropy_backward: hidden and weight must begin at 16-byte boundaries");
     const size_t want = BackwardPlan(T, V, K).bytes;
     TFK_REQUIRE(workspace && workspace_bytes >= want && at_16B(workspace), TF_ERR_INVALID_ARG,
                 "tf_linear_cross_entropy_backward: workspace of %zu bytes at a 16-byte boundary needed, got %zu", want, workspace_bytes);

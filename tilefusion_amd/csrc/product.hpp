@@ -8,15 +8,16 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 #include "common.hpp"
-#include "gemm_ring64.hpp"
+#include "gemm_ring64_cols.hpp"
 #include "gemm_split_k.hpp"
 
 namespace tfk {
 
-// The operands of a product.  With two matrices B (gate and up) the columns of the product alternate between them in blocks of 16:
+// The operands of a product, at 16-byte boundaries, K a multiple of 16 bytes (copy_rows makes such rows of others).  With two matrices B (gate and up) the columns of the product alternate between them in blocks of 16:
 // block 2 * j is columns 16 * j .. of b[0], block 2 * j + 1 the same columns of b[1].
 struct Operands {
   const void* a;
@@ -38,9 +39,11 @@ struct TileAt {
 // An epilogue is called as epilogue.run<kInside>(acc, at): kInside says that the whole tile lies inside the result.
 //
 // Two blocks side by side, columns `col` .. col + 31, rounded to T: 16 bytes a lane, four adjacent lanes a row, which is what leaves a wavefront as
-// one access (as gemm.hip's own store, with its reasons).  Rows and columns from `rows` and `cols` on are left out.
+// one access (as gemm.hip's own store, with its reasons).  Rows and columns from `rows` and `cols` on are left out,
+// and rows in front of `from`.
 template <bool kInside, typename T>
-TFK_DEVICE void store_block_pair(T* c, size_t pitch, int row, int col, int rows, int cols, int lane, float4_t left, float4_t right) {
+TFK_DEVICE void store_block_pair(T* c, size_t pitch, int row, int col, int rows, int cols, int lane, float4_t left, float4_t right,
+                                 int from) {
   typedef uint4_t out16B_t __attribute__((aligned(2)));
   typedef T two_t __attribute__((ext_vector_type(2)));
   const int st_row = lane >> 2, st_seg = lane & 3;
@@ -62,7 +65,7 @@ TFK_DEVICE void store_block_pair(T* c, size_t pitch, int row, int col, int rows,
   v[2] = (unsigned)__builtin_amdgcn_ds_bpermute(4 * src_lane, (int)y[0]);
   v[3] = (unsigned)__builtin_amdgcn_ds_bpermute(4 * src_lane, (int)y[1]);
   const int r = row + st_row, at = col + 8 * st_seg;
-  if (!kInside && r >= rows) return;
+  if (!kInside && (r >= rows || r < from)) return;
   T* const to = c + (size_t)r * pitch + at;
   if (kInside || at + 8 <= cols) {
     *reinterpret_cast<out16B_t*>(to) = v;
@@ -75,11 +78,11 @@ TFK_DEVICE void store_block_pair(T* c, size_t pitch, int row, int col, int rows,
 }
 // One block, rounded to T: four columns a lane.
 template <bool kInside, typename T>
-TFK_DEVICE void store_block(T* c, size_t pitch, int row, int col, int rows, int cols, int lane, float4_t v) {
+TFK_DEVICE void store_block(T* c, size_t pitch, int row, int col, int rows, int cols, int lane, float4_t v, int from) {
   typedef T four_t __attribute__((ext_vector_type(4)));
   typedef four_t four_any_t __attribute__((aligned(sizeof(T))));
   const int r = row + (lane & 15), at = col + 4 * (lane >> 4);
-  if (!kInside && r >= rows) return;
+  if (!kInside && (r >= rows || r < from)) return;
   T* const to = c + (size_t)r * pitch + at;
   if (kInside || at + 4 <= cols) {
     *reinterpret_cast<four_any_t*>(to) = four_t{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
@@ -91,93 +94,18 @@ TFK_DEVICE void store_block(T* c, size_t pitch, int row, int col, int rows, int 
 }
 // Row i of a wavefront's blocks: v[0 .. n)
 template <bool kInside, typename T, int kBlocks>
-TFK_DEVICE void store_blocks(T* c, size_t pitch, int row, int col, int rows, int cols, int lane, const float4_t (&v)[kBlocks]) {
+TFK_DEVICE void store_blocks(T* c, size_t pitch, int row, int col, int rows, int cols, int lane, const float4_t (&v)[kBlocks], int from = 0) {
   constexpr int kPairs = sizeof(T) == 2 ? kBlocks / 2 : 0;
   if constexpr (kPairs > 0) {
 #pragma unroll
-    for (int j = 0; j < kPairs; ++j) store_block_pair<kInside>(c, pitch, row, col + 32 * j, rows, cols, lane, v[2 * j], v[2 * j + 1]);
+    for (int j = 0; j < kPairs; ++j) store_block_pair<kInside>(c, pitch, row, col + 32 * j, rows, cols, lane, v[2 * j], v[2 * j + 1], from);
   }
 #pragma unroll
-  for (int j = 2 * kPairs; j < kBlocks; ++j) store_block<kInside>(c, pitch, row, col + 16 * j, rows, cols, lane, v[j]);
+  for (int j = 2 * kPairs; j < kBlocks; ++j) store_block<kInside>(c, pitch, row, col + 16 * j, rows, cols, lane, v[j], from);
 }
 
 // ------------------------------------------------------------------------------------------
-// Any M, N, K and any alignment: tiles of 64 x 64, 128 bytes of K at a time through registers into one LDS stage, every access checked.
-// What the other kernels' requests cannot fetch runs here: rows that do not start at 16-byte boundaries.
-// ------------------------------------------------------------------------------------------
-constexpr int kAnyTile = 64, kAnyThreads = 256;
-
-TFK_DEVICE int row_swizzle(int row, int c) { return c ^ ((row / 2) % 8); }   // 128-byte rows, 16-byte chunks: no bank conflicts
-
-template <typename InT>
-TFK_DEVICE uint4_t load_chunk_any(const InT* row, int k, int K, bool whole) {
-  constexpr int kElems = 16 / sizeof(InT);
-  uint4_t v = {0u, 0u, 0u, 0u};
-  if (whole) {
-    if (k < K) v = *reinterpret_cast<const uint4_t*>(row + k);
-    return v;
-  }
-  using bits_t = std::conditional_t<sizeof(InT) == 1, uint8_t, uint16_t>;
-  const bits_t* p = reinterpret_cast<const bits_t*>(row);
-#pragma unroll
-  for (int t = 0; t < kElems; ++t)
-    if (k + t < K) v[t * sizeof(InT) / 4] |= (unsigned)p[k + t] << (8 * (t * sizeof(InT) % 4));
-  return v;
-}
-
-template <typename InT, bool kTwo, typename Epilogue>
-__global__ __launch_bounds__(kAnyThreads) void product_any_kernel(Operands x, bool whole, int tiles_m, Epilogue epilogue) {
-  constexpr int kStep = 128 / sizeof(InT);   // elements of K at a time
-  __shared__ __attribute__((aligned(16))) char sa[kAnyTile * 128];
-  __shared__ __attribute__((aligned(16))) char sb[kAnyTile * 128];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tile_m = blockIdx.x % tiles_m, tile_n = blockIdx.x / tiles_m;
-  constexpr int kCols = kTwo ? kAnyTile / 2 : kAnyTile;   // columns of the result
-  const int m0 = tile_m * kAnyTile, n0 = tile_n * kCols;
-  const int wm = wave / 2, wn = wave % 2, fr = lane & 15, fg = lane >> 4;
-  const InT* const a = static_cast<const InT*>(x.a);
-
-  float4_t acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = float4_t{0.f, 0.f, 0.f, 0.f};
-
-  for (int k0 = 0; k0 < x.K; k0 += kStep) {
-    for (int f = tid; f < kAnyTile * 8; f += kAnyThreads) {
-      const int row = f / 8, c = f % 8;
-      const int k = k0 + c * (16 / (int)sizeof(InT));
-      uint4_t va = {0u, 0u, 0u, 0u}, vb = {0u, 0u, 0u, 0u};
-      if (m0 + row < x.M) va = load_chunk_any(a + (size_t)(m0 + row) * x.K, k, x.K, whole);
-      const int n = n0 + (kTwo ? row / 32 * 16 + row % 16 : row);
-      const InT* const b = static_cast<const InT*>(kTwo && row / 16 % 2 ? x.b[1] : x.b[0]);
-      if (n < x.N) vb = load_chunk_any(b + (size_t)n * x.K, k, x.K, whole);
-      *reinterpret_cast<uint4_t*>(sa + row * 128 + row_swizzle(row, c) * 16) = va;
-      *reinterpret_cast<uint4_t*>(sb + row * 128 + row_swizzle(row, c) * 16) = vb;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      uint4_t af[2], bf[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int ra = wm * 32 + i * 16 + fr, rb = wn * 32 + i * 16 + fr;
-        af[i] = *reinterpret_cast<const uint4_t*>(sa + ra * 128 + row_swizzle(ra, 4 * ks + fg) * 16);
-        bf[i] = *reinterpret_cast<const uint4_t*>(sb + rb * 128 + row_swizzle(rb, 4 * ks + fg) * 16);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma_rows<InT>(af[i], bf[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-  const int col = n0 + wn * (kTwo ? 16 : 32);
-  epilogue.template run<false>(acc, TileAt{m0 + wm * 32, col, m0, n0, lane, tile_n * 2 + wn});
-}
-
-// ------------------------------------------------------------------------------------------
-// Rows that start at 16-byte boundaries: the main loops of the GEMM.
+// A * B^T: the main loops of the GEMM.
 // ------------------------------------------------------------------------------------------
 // M >= BM, N >= BN (kTwo: BN / 2), K >= 128 bytes.  The last tile of a row or column of tiles ends where the result does: it overlaps its neighbour.
 template <typename S, typename InT, bool kTwo, typename Epilogue>
@@ -235,64 +163,54 @@ inline int64_t tiles_of(int64_t extent, int64_t tile) { return (extent + tile - 
 inline int64_t round_up_to(int64_t x, int64_t to) { return tiles_of(x, to) * to; }
 inline bool at_16B(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+constexpr int64_t kMaxTiles = ((int64_t)1 << 23) - 1;   // a launch has less than 2^32 threads, of which a workgroup has 512 at most
+
 // The kernel that gemm.hip's cost model expects to be done first with M x N outputs over K 16-bit elements, out of those of `allowed` (a bit per row of
 // its table kGemmKernels; bit 0 is among them): its position there.
 int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed);
 
 // Positions in that table, and the kernels here.  With two matrices B, tiles have an even number of 16-column blocks to a wavefront, a
 // wavefront's requests begin with a block (no tiles of 192 columns), and the smallest tile is 16 x 32.
-constexpr int kAnyKernel = -1;
 constexpr unsigned kOneAllowed = 0x7fff, kTwoAllowed = 0x7fff & ~(1u << 1 | 1u << 2 | 1u << 11 | 1u << 13);
 
 struct ProductPlan {
-  int kernel;       // position, or kAnyKernel
+  int kernel;       // position
   int64_t slots;    // of a row's partial results (TileAt)
 };
 // slots of a row's partial results
 inline int64_t product_slots(int kernel, int64_t N) {
   constexpr int kColumns[] = {16, 16, 16, 32, 32, 32, 64, 64, 64, 64, 64, 96, 64, 96, 128};   // a wavefront's (split K: a tile's)
-  if (kernel == kAnyKernel) return 2 * tiles_of(N, kAnyTile);
   // (the last tile has a slot for each of its wavefronts)
   return kernel < 7 ? tiles_of(N, kColumns[kernel]) : 2 * tiles_of(N, 2 * kColumns[kernel]);
 }
-
-template <typename InT>
-ProductPlan plan_product(const Operands& x, bool two) {
-  // rows that 16-byte requests can walk
-  const bool whole = x.K % (16 / (int)sizeof(InT)) == 0 && at_16B(x.a) && at_16B(x.b[0]) && (!two || at_16B(x.b[1]));
-  const int kernel = whole ? pick_table_kernel(x.M, two ? 2 * (int64_t)x.N : x.N, (int64_t)x.K * (int)sizeof(InT) / 2, two ? kTwoAllowed : kOneAllowed)
-                           : kAnyKernel;
-  return {kernel, product_slots(kernel, x.N)};
+// K: 16-bit elements (half the elements of 8)
+inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool two) {
+  const int kernel = pick_table_kernel(M, two ? 2 * N : N, K, two ? kTwoAllowed : kOneAllowed);
+  return {kernel, product_slots(kernel, N)};
 }
 
 template <typename S, typename InT, bool kTwo, typename Epilogue>
-int launch_ring64_product(const Operands& x, const Epilogue& epilogue, hipStream_t st) {
+int launch_ring64_product(const char* who, const Operands& x, const Epilogue& epilogue, hipStream_t st) {
   auto kern = product_ring64_kernel<S, InT, kTwo, Epilogue>;
   static_assert(S::kLdsBytes <= kMaxLdsBytes, "ring does not fit in LDS");
   TFK_LDS_OPT_IN(kern, S::kLdsBytes);
   const int64_t tiles_m = tiles_of(x.M, S::BM), tiles_n = tiles_of(x.N, kTwo ? S::BN / 2 : S::BN);
+  TFK_REQUIRE(tiles_m * tiles_n <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
   return launch_kernel(kern, dim3((unsigned)(tiles_m * tiles_n)), dim3(S::kThreads), S::kLdsBytes, st, x, (int)tiles_m, (int)tiles_n, epilogue);
 }
 template <typename S, typename InT, bool kTwo, typename Epilogue>
-int launch_split_k_product(const Operands& x, const Epilogue& epilogue, hipStream_t st) {
+int launch_split_k_product(const char* who, const Operands& x, const Epilogue& epilogue, hipStream_t st) {
   auto kern = product_split_k_kernel<S, InT, kTwo, Epilogue>;
   static_assert(S::kLdsBytes <= kMaxLdsBytes, "rings do not fit in LDS");
   if constexpr (S::kLdsBytes > 64 * 1024) TFK_LDS_OPT_IN(kern, S::kLdsBytes);
   const int64_t tiles_m = tiles_of(x.M, S::BM), tiles_n = tiles_of(x.N, kTwo ? S::BN / 2 : S::BN);
+  TFK_REQUIRE(tiles_m * tiles_n <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
   return launch_kernel(kern, dim3((unsigned)(tiles_m * tiles_n)), dim3(S::kThreads), S::kLdsBytes, st, x, (int)tiles_m, (int)tiles_n, epilogue);
 }
 
 template <typename InT, bool kTwo, typename Epilogue>
 int launch_product(const char* who, const Operands& x, const ProductPlan& plan, const Epilogue& epilogue, hipStream_t st) {
-  // (a launch has less than 2^32 threads: 2^24 workgroups of 256; no tile has fewer than 256 elements, or 512 of two matrices)
-  TFK_REQUIRE(tiles_of(x.M, 16) * tiles_of(x.N, 16) < (int64_t)1 << 27, TF_ERR_INVALID_ARG, "%s: result too large", who);
-  if (plan.kernel == kAnyKernel) {
-    const int64_t tiles_m = tiles_of(x.M, kAnyTile), tiles_n = tiles_of(x.N, kTwo ? kAnyTile / 2 : kAnyTile);
-    const bool whole = x.K % (16 / (int)sizeof(InT)) == 0 && at_16B(x.a) && at_16B(x.b[0]) && (!kTwo || at_16B(x.b[1]));
-    return launch_kernel(product_any_kernel<InT, kTwo, Epilogue>, dim3((unsigned)(tiles_m * tiles_n)), dim3(kAnyThreads), 0, st, x, whole, (int)tiles_m,
-                         epilogue);
-  }
-  using Launcher = int (*)(const Operands&, const Epilogue&, hipStream_t);
+  using Launcher = int (*)(const char*, const Operands&, const Epilogue&, hipStream_t);
   if constexpr (kTwo) {
     static constexpr Launcher kLaunchers[] = {
         launch_split_k_product<SplitKShape<1, 2, 4>, InT, kTwo, Epilogue>, nullptr, nullptr,
@@ -302,7 +220,7 @@ int launch_product(const char* who, const Operands& x, const ProductPlan& plan, 
         launch_ring64_product<Ring64Shape<128, 128, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<192, 128, 2>, InT, kTwo, Epilogue>,
         nullptr, launch_ring64_product<Ring64Shape<256, 128, 2>, InT, kTwo, Epilogue>, nullptr,
         launch_ring64_product<Ring64Shape<256, 256, 2>, InT, kTwo, Epilogue>};
-    return kLaunchers[plan.kernel](x, epilogue, st);
+    return kLaunchers[plan.kernel](who, x, epilogue, st);
   } else {
     static constexpr Launcher kLaunchers[] = {
         launch_split_k_product<SplitKShape<1, 1, 4>, InT, kTwo, Epilogue>, launch_split_k_product<SplitKShape<1, 1, 8>, InT, kTwo, Epilogue>,
@@ -313,18 +231,162 @@ int launch_product(const char* who, const Operands& x, const ProductPlan& plan, 
         launch_ring64_product<Ring64Shape<128, 128, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<192, 128, 2>, InT, kTwo, Epilogue>,
         launch_ring64_product<Ring64Shape<192, 192, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<256, 128, 2>, InT, kTwo, Epilogue>,
         launch_ring64_product<Ring64Shape<256, 192, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<256, 256, 2>, InT, kTwo, Epilogue>};
-    return kLaunchers[plan.kernel](x, epilogue, st);
+    return kLaunchers[plan.kernel](who, x, epilogue, st);
   }
 }
 
 // ------------------------------------------------------------------------------------------
-// Layout: what the products of a backward pass take transposed
+// A * B and A^T * B: the products of a backward pass, summed over tokens or over rows of a weight.
 // ------------------------------------------------------------------------------------------
-// dst[c * pitch + r] = src[r * src_pitch + c] of 16-bit elements, for c < cols and r < padded_rows, zeros from `rows` on.
-int launch_transpose_padded(const char* who, const void* src, int64_t src_pitch, void* dst, int64_t pitch, int64_t rows, int64_t cols,
-                            int64_t padded_rows, hipStream_t st);
+struct ColsProduct {
+  ColsOperand a, b;         // extents: rows and columns of the result
+  const uint16_t* b1;       // where b's rows continue from k-tile `turn` on
+  int turn;
+  int k_tiles, k_pad;       // 64 summed rows each; zeros in front of the first ones
+  int row_from;             // the result's first row that is stored
+};
+struct ColsPlan {
+  int shape;                // into kColsShapes
+  int splits, per_split;    // the sum is cut into that many parts of so many k-tiles (the last may be shorter)
+};
+struct ColsShape {
+  int bm, bn, table;        // tile, position in gemm.hip's table
+};
+constexpr ColsShape kColsShapes[] = {{256, 256, 14}, {256, 128, 12}, {128, 128, 7}, {128, 128, 9}};
+
+// What gemm.hip's cost model expects of a kernel of its table, in us.
+float expected_table_us(int kernel, int64_t tiles, int64_t k_tiles);
+
+// Cut, a product costs a launch more and its parts' way through memory (4 bytes written and
+// read for each element and part, at 4 TB/s).
+inline ColsPlan plan_cols(int64_t M, int64_t N, int64_t k_tiles) {
+  ColsPlan best = {0, 1, (int)k_tiles};
+  float best_us = INFINITY;
+  for (int s = 0; s < (int)(sizeof(kColsShapes) / sizeof(kColsShapes[0])); ++s) {
+    const int64_t tiles = tiles_of(M, kColsShapes[s].bm) * tiles_of(N, kColsShapes[s].bn);
+    for (int64_t splits = 1; splits <= 64 && (splits == 1 || tiles * splits <= 1024); ++splits) {
+      const int64_t per = tiles_of(k_tiles, splits);
+      if (tiles_of(k_tiles, per) != splits || (splits > 1 && per < 4)) continue;
+      const float parts = splits > 1 ? 3.f + (float)(8 * splits * M * N) / 4e6f : 0.f;
+      const float us = expected_table_us(kColsShapes[s].table, tiles * splits, per) + parts;
+      if (us < best_us) {
+        best = {s, (int)splits, (int)per};
+        best_us = us;
+      }
+    }
+  }
+  return best;
+}
+
+struct PartEpilogue;   // below; takes whole tiles
+
+template <typename S, typename InT, bool kColA, typename Epilogue>
+__global__ __launch_bounds__(S::kThreads) void product_cols_kernel(ColsProduct x, int tiles_m, int tiles_n, int per_split, Epilogue epilogue) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = tiles_m * tiles_n, split = blockIdx.x / tiles;
+  int tile_m, tile_n;
+  tile_of_block(blockIdx.x - split * tiles, tiles, tiles_m, tiles_n, tile_m, tile_n);
+  const int m0 = tile_m * S::BM, n0 = tile_n * S::BN, t0 = split * per_split;
+  const int wm = wave / S::WAVES_N, wn = wave % S::WAVES_N;
+  float4_t acc[S::TM][S::TN];
+  ring64_multiply_cols<S, InT, kColA>(x.a, x.b, x.b1, x.turn, m0, n0, t0, min(per_split, x.k_tiles - t0), x.k_pad, lane, wave, smem, acc);
+  int again = lane;
+  asm volatile("" : "+v"(again));
+  const TileAt at = {m0 + wm * S::WM, n0 + wn * S::WN, x.row_from, n0, again, split};
+  if (std::is_same_v<Epilogue, PartEpilogue>) epilogue.template run<true>(acc, at);
+  else if (m0 >= x.row_from && m0 + S::BM <= x.a.extent && n0 + S::BN <= x.b.extent) epilogue.template run<true>(acc, at);
+  else epilogue.template run<false>(acc, at);
+}
+
+template <typename S, typename InT, bool kColA, typename Epilogue>
+int launch_cols_shape(const char* who, const ColsProduct& x, const ColsPlan& plan, const Epilogue& epilogue, hipStream_t st) {
+  auto kern = product_cols_kernel<S, InT, kColA, Epilogue>;
+  TFK_LDS_OPT_IN(kern, S::kLdsBytes);
+  const int64_t tiles_m = tiles_of(x.a.extent, S::BM), tiles_n = tiles_of(x.b.extent, S::BN);
+  TFK_REQUIRE(tiles_m * tiles_n * plan.splits <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
+  return launch_kernel(kern, dim3((unsigned)(tiles_m * tiles_n * plan.splits)), dim3(S::kThreads), S::kLdsBytes, st, x, (int)tiles_m, (int)tiles_n,
+                       plan.per_split, epilogue);
+}
+template <typename InT, bool kColA, typename Epilogue>
+int launch_cols(const char* who, const ColsProduct& x, const ColsPlan& plan, const Epilogue& epilogue, hipStream_t st) {
+  switch (plan.shape) {
+    case 0: return launch_cols_shape<Ring64Shape<256, 256, 2>, InT, kColA>(who, x, plan, epilogue, st);
+    case 1: return launch_cols_shape<Ring64Shape<256, 128, 2>, InT, kColA>(who, x, plan, epilogue, st);
+    case 2: return launch_cols_shape<Ring64Shape<128, 128, 4>, InT, kColA>(who, x, plan, epilogue, st);
+    default: return launch_cols_shape<Ring64Shape<128, 128, 2>, InT, kColA>(who, x, plan, epilogue, st);
+  }
+}
+
+// ---- what gradients end in -----------------------------------------------------------------
+struct Scale {
+  float in, out;   // operands were multiplied by `in` where they were made, sums are by `out`
+};
+// A sum that is complete: scaled (where there is a scale), rounded to T.
+template <typename T>
+struct WholeEpilogue {
+  T* out;                  // [M][N]
+  const Scale* scale;      // or null
+  int M, N;
+
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    const float by = scale != nullptr ? scale->out : 1.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      float4_t v[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) v[j] = acc[i][j] * by;
+      store_blocks<kInside>(out, (size_t)N, at.row + 16 * i, at.col, M, N, at.lane, v, at.row_from);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+// A part of a sum: fp32, whole tiles (what lies behind the result's rows and columns is not looked at again), added to what an earlier launch left
+// there or in its place.
+struct PartEpilogue {
+  float* parts;
+  int64_t rows, pitch;     // whole tiles
+  bool add;
+
+  template <bool, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    if (add) leave<true>(acc, at);
+    else leave<false>(acc, at);
+  }
+  template <bool kAdd, int TM, int TN>
+  TFK_DEVICE void leave(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    float* const mine = parts + (at.slot * rows + at.row + (at.lane & 15)) * pitch + at.col + 4 * (at.lane >> 4);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        float4_t* const to = reinterpret_cast<float4_t*>(mine + 16 * i * pitch + 16 * j);
+        *to = kAdd ? acc[i][j] + *to : acc[i][j];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+// The room that the parts of a product with M x N results take, in floats, and its rows and pitch.
+struct PartsRoom {
+  int64_t rows, pitch, floats;
+  PartsRoom(const ColsPlan& plan, int64_t M, int64_t N)
+      : rows(round_up_to(M, kColsShapes[plan.shape].bm)), pitch(round_up_to(N, kColsShapes[plan.shape].bn)), floats(plan.splits * rows * pitch) {}
+};
+// out = T(by * the sum of the parts): rows `first` .. M - 1, of which the first is out's; N columns
+template <typename T>
+int launch_sum_parts(const float* parts, const PartsRoom& room, int splits, int64_t first, int64_t M, int64_t N, T* out, const Scale* scale,
+                     hipStream_t st);
+
+// ------------------------------------------------------------------------------------------
+// Layout
+// ------------------------------------------------------------------------------------------
+// dst: `padded_rows` rows of `pitch` bytes (a multiple of 16, from a 16-byte boundary on) with the `bytes` bytes of each of `rows` rows of src in
+// front, zeros behind them and in the rows that follow.
+int launch_copy_rows(const char* who, const void* src, int64_t bytes, int64_t rows, void* dst, int64_t pitch, int64_t padded_rows, hipStream_t st);
 // zeros in columns from .. to - 1 of rows of 16-bit elements
-int launch_zero_columns(const char* who, void* dst, int64_t pitch, int64_t rows, int64_t from, int64_t to, hipStream_t st);
+int launch_zero_columns(void* dst, int64_t pitch, int64_t rows, int64_t from, int64_t to, hipStream_t st);
 // count 16-bit elements of zero
 int launch_zero_16bit(void* dst, int64_t count, hipStream_t st);
 

@@ -412,6 +412,8 @@ void check_vector(const at::Tensor& t, const char* name, at::ScalarType type, in
   TORCH_CHECK(t.scalar_type() == type, "tilefusion::", op, ": ", name, " must be of type ", toString(type), ".");
   TORCH_CHECK(t.dim() == 1 && t.size(0) == n, "tilefusion::", op, ": ", name, " must be [", n, "], got ", t.sizes(), ".");
 }
+// at a 16-byte boundary, as the C ABI asks for (a slice of a flat buffer may begin elsewhere: then a copy)
+at::Tensor at_boundary(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(); }
 int activation_code(c10::string_view name, const char* op) {
   const int code = name == "silu" ? TF_ACT_SILU : name == "gelu" ? TF_ACT_GELU : name == "gelu_tanh" ? TF_ACT_GELU_TANH : -1;
   TORCH_CHECK(code >= 0, "tilefusion::", op, ": activation must be 'silu', 'gelu' or 'gelu_tanh', got '", name, "'.");
@@ -450,8 +452,12 @@ void gemm_int8(const at::Tensor& A, const at::Tensor& B, const at::Tensor& scale
   TORCH_CHECK(out == at::kFloat || out == at::kHalf || out == at::kBFloat16, "tilefusion::", op, ": C must be float32, float16 or bfloat16.");
   const int c_dtype = out == at::kFloat ? TF_DTYPE_F32 : out == at::kHalf ? TF_DTYPE_F16 : TF_DTYPE_BF16;
   const c10::DeviceGuard there(A.device());
-  check_status(tf_gemm_int8(A.data_ptr(), B.data_ptr(), scale_a.data_ptr<float>(), scale_b.data_ptr<float>(), C.data_ptr(), c_dtype, m, n, k,
-                            current_stream()),
+  const size_t bytes = tf_gemm_int8_workspace_bytes(m, n, k);
+  c10::DataPtr ws;
+  if (bytes > 0) ws = scratch(bytes, A);
+  const at::Tensor a = at_boundary(A), b = at_boundary(B);
+  check_status(tf_gemm_int8(a.data_ptr(), b.data_ptr(), scale_a.data_ptr<float>(), scale_b.data_ptr<float>(), C.data_ptr(), c_dtype, m, n, k, ws.get(),
+                            bytes, current_stream()),
                op);
 }
 
@@ -478,8 +484,12 @@ void gated_ffn(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& 
   }
   const int act = activation_code(activation, op);
   const c10::DeviceGuard there(x.device());
-  check_status(tf_gated_ffn(x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), h.data_ptr(), gate.has_value() ? gate->data_ptr() : nullptr,
-                            up.has_value() ? up->data_ptr() : nullptr, dtype, act, m, f, k, current_stream()),
+  const size_t bytes = tf_gated_ffn_workspace_bytes(m, f, k);
+  c10::DataPtr ws;
+  if (bytes > 0) ws = scratch(bytes, x);
+  const at::Tensor from = at_boundary(x), of_gate = at_boundary(w_gate), of_up = at_boundary(w_up);
+  check_status(tf_gated_ffn(from.data_ptr(), of_gate.data_ptr(), of_up.data_ptr(), h.data_ptr(), gate.has_value() ? gate->data_ptr() : nullptr,
+                            up.has_value() ? up->data_ptr() : nullptr, dtype, act, m, f, k, ws.get(), bytes, current_stream()),
                op);
 }
 
@@ -504,7 +514,8 @@ void gated_ffn_backward(const at::Tensor& grad_h, const at::Tensor& x, const at:
   c10::DataPtr ws;
   if (bytes > 0) ws = scratch(bytes, x);
   char* const to = static_cast<char*>(grad_w.data_ptr());
-  check_status(tf_gated_ffn_backward(grad_h.data_ptr(), x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), gate.data_ptr(), up.data_ptr(),
+  const at::Tensor from = at_boundary(x), of_gate = at_boundary(w_gate), of_up = at_boundary(w_up);
+  check_status(tf_gated_ffn_backward(grad_h.data_ptr(), from.data_ptr(), of_gate.data_ptr(), of_up.data_ptr(), gate.data_ptr(), up.data_ptr(),
                                      grad_x.data_ptr(), to, to + 2 * f * k, dtype, act, m, f, k, ws.get(), bytes, current_stream()),
                op);
 }
@@ -526,7 +537,8 @@ void linear_cross_entropy(const at::Tensor& hidden, const at::Tensor& weight, co
   const size_t bytes = tf_linear_cross_entropy_workspace_bytes(t, v, k);
   c10::DataPtr ws;
   if (bytes > 0) ws = scratch(bytes, hidden);
-  check_status(tf_linear_cross_entropy(hidden.data_ptr(), weight.data_ptr(), target.data_ptr<int64_t>(), loss.data_ptr<float>(),
+  const at::Tensor rows = at_boundary(hidden), table = at_boundary(weight);
+  check_status(tf_linear_cross_entropy(rows.data_ptr(), table.data_ptr(), target.data_ptr<int64_t>(), loss.data_ptr<float>(),
                                        lse.data_ptr<float>(), dtype, t, v, k, ignore_index, ws.get(), bytes, current_stream()),
                op);
 }
@@ -552,7 +564,8 @@ void linear_cross_entropy_backward(const at::Tensor& grad_loss, const at::Tensor
   const size_t bytes = tf_linear_cross_entropy_backward_workspace_bytes(t, v, k);
   c10::DataPtr ws;
   if (bytes > 0) ws = scratch(bytes, hidden);
-  check_status(tf_linear_cross_entropy_backward(grad_loss.data_ptr<float>(), hidden.data_ptr(), weight.data_ptr(), target.data_ptr<int64_t>(),
+  const at::Tensor rows = at_boundary(hidden), table = at_boundary(weight);
+  check_status(tf_linear_cross_entropy_backward(grad_loss.data_ptr<float>(), rows.data_ptr(), table.data_ptr(), target.data_ptr<int64_t>(),
                                                 lse.data_ptr<float>(), grad_hidden.data_ptr(), grad_weight.data_ptr(), dtype, t, v, k, ignore_index,
                                                 ws.get(), bytes, current_stream()),
                op);
