@@ -23,6 +23,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <optional>
+#include <string>
 
 namespace {
 
@@ -87,6 +89,12 @@ at::Tensor empty_output(at::IntArrayRef shape, const at::Tensor& like) {
   const auto& context = at::globalContext();
   if (context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory()) return at::empty(shape, like.options());
   return at::Tensor(at::detail::empty_cuda(shape, like.scalar_type(), like.device(), c10::nullopt));
+}
+
+at::Tensor empty_output(at::IntArrayRef shape, const at::Tensor& like, at::ScalarType type) {
+  const auto& context = at::globalContext();
+  if (context.deterministicAlgorithms() && context.deterministicFillUninitializedMemory()) return at::empty(shape, like.options().dtype(type));
+  return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), c10::nullopt));
 }
 
 // at::empty_like(like), which gives a dense tensor its strides, also the ones that address nothing (of extents of 1).
@@ -203,12 +211,120 @@ PyObject* flash_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- products whose results do not leave as they are: matrices, contiguous as they come -------
+bool matrices(const at::Tensor* t, int n) {
+  for (int i = 0; i < n; ++i)
+    if (t[i].dim() != 2 || !t[i].is_contiguous()) return false;
+  return true;
+}
+bool vectors(const at::Tensor* t, int n) {
+  for (int i = 0; i < n; ++i)
+    if (t[i].dim() != 1 || !t[i].is_contiguous()) return false;
+  return true;
+}
+bool text(PyObject* arg, c10::string_view* out) {
+  Py_ssize_t n = 0;
+  if (!PyUnicode_CheckExact(arg)) return false;
+  const char* const p = PyUnicode_AsUTF8AndSize(arg, &n);
+  if (p == nullptr) {
+    PyErr_Clear();
+    return false;
+  }
+  *out = c10::string_view(p, (size_t)n);
+  return true;
+}
+PyObject* tuple_of(std::initializer_list<at::Tensor> tensors) {
+  PyObject* const out = PyTuple_New((Py_ssize_t)tensors.size());
+  if (out == nullptr) return nullptr;
+  Py_ssize_t i = 0;
+  for (const at::Tensor& t : tensors) PyTuple_SET_ITEM(out, i++, THPVariable_Wrap(t));
+  return out;
+}
+
+// (x) -> (q, scale), or None
+PyObject* quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[1], q, scale;
+  static const auto op = find_op<void(const at::Tensor&, at::Tensor&, at::Tensor&)>("tilefusion::quantize_rows");
+  if (nargs != 1 || !plain(op, args, 1, t) || !matrices(t, 1)) Py_RETURN_NONE;
+  {
+    NoGil unlocked;
+    q = empty_output(t[0].sizes(), t[0], at::kChar);
+    scale = empty_output({t[0].size(0)}, t[0], at::kFloat);
+    op.redispatch(kCuda, t[0], q, scale);
+  }
+  return tuple_of({q, scale});
+  END_HANDLE_TH_ERRORS
+}
+
+// (A, B, scale_a, scale_b, C)
+PyObject* gemm_int8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[5];
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, at::Tensor&);
+  static const auto op = find_op<Op>("tilefusion::gemm_int8");
+  if (nargs != 5 || !plain(op, args, 5, t) || !matrices(t, 2) || !vectors(t + 2, 2)) Py_RETURN_FALSE;
+  {
+    NoGil unlocked;
+    op.redispatch(kCuda, t[0], t[1], t[2], t[3], t[4]);
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, w_gate, w_up, activation, keep) -> (h,) or (h, gate, up), or None
+PyObject* gated_ffn(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[3], h;
+  std::optional<at::Tensor> gate, up;
+  c10::string_view activation;
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, c10::string_view, at::Tensor&, const std::optional<at::Tensor>&,
+                  const std::optional<at::Tensor>&);
+  static const auto op = find_op<Op>("tilefusion::gated_ffn");
+  if (nargs != 5 || !plain(op, args, 3, t) || !matrices(t, 3) || !text(args[3], &activation) || !PyBool_Check(args[4])) Py_RETURN_NONE;
+  if (t[0].size(1) != t[1].size(1) || t[0].size(1) == 0) Py_RETURN_NONE;   // (the wrapper's own errors)
+  const bool keep = args[4] == Py_True;
+  {
+    NoGil unlocked;
+    const int64_t shape[2] = {t[0].size(0), t[1].size(0)};
+    h = empty_output(shape, t[0]);
+    if (keep) {
+      gate = empty_output(shape, t[0]);
+      up = empty_output(shape, t[0]);
+    }
+    op.redispatch(kCuda, t[0], t[1], t[2], activation, h, gate, up);
+  }
+  return keep ? tuple_of({h, *gate, *up}) : tuple_of({h});
+  END_HANDLE_TH_ERRORS
+}
+
+// (hidden, weight, target, ignore_index) -> (loss, lse), or None
+PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[3], loss, lse;
+  int64_t ignore_index;
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, at::Tensor&, at::Tensor&);
+  static const auto op = find_op<Op>("tilefusion::linear_cross_entropy");
+  if (nargs != 4 || !plain(op, args, 3, t) || !matrices(t, 2) || !vectors(t + 2, 1) || !ints(args + 3, 1, &ignore_index)) Py_RETURN_NONE;
+  if (t[0].size(1) != t[1].size(1) || t[0].size(1) == 0 || t[2].size(0) != t[0].size(0)) Py_RETURN_NONE;
+  {
+    NoGil unlocked;
+    loss = empty_output({t[0].size(0)}, t[0], at::kFloat);
+    lse = empty_output({t[0].size(0)}, t[0], at::kFloat);
+    op.redispatch(kCuda, t[0], t[1], t[2], ignore_index, loss, lse);
+  }
+  return tuple_of({loss, lse});
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*kFunction)(PyObject*, PyObject* const*, Py_ssize_t)>
 constexpr PyMethodDef method(const char* name) {
   return {name, (PyCFunction)(void (*)(void))kFunction, METH_FASTCALL, nullptr};
 }
 PyMethodDef methods[] = {method<gemm>("gemm"), method<fused_two_gemms>("fused_two_gemms"), method<scatter_nd>("scatter_nd"),
                          method<flash_attention>("flash_attention"), method<flash_decode>("flash_decode"),
+                         method<quantize_rows>("quantize_rows"), method<gemm_int8>("gemm_int8"), method<gated_ffn>("gated_ffn"),
+                         method<linear_cross_entropy>("linear_cross_entropy"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

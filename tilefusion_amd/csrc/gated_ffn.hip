@@ -8,32 +8,51 @@
 //   dg = dh * up * act'(gate), du = dh * act(gate)
 //   dx = dg * Wg + du * Wu,  dWg = dg^T * x,  dWu = du^T * x
 // One pass over dh, gate and up leaves [dg | du] as rows of tokens, each half completed by zeros to a multiple of 64 columns; dx is one product over the
-// 2F columns, the weights' gradients are one (or two) over the tokens.  dg and du are rounded to the type once, as operands of
+// 2F columns, the weights' gradients are one over the tokens.  dg and du are rounded to the type once, as operands of
 // matrix instructions have to be.
 #include "product.hpp"
 
 namespace tfk {
 namespace {
 
-// act(g) = g * phi(g)
-TFK_DEVICE float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
+// act(g) = g * phi(g), and phi's derivative
+TFK_DEVICE float exp_of(float x) { return __builtin_amdgcn_exp2f(1.4426950408889634f * x); }
+TFK_DEVICE float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x)); }
 constexpr float kGeluCubic = 0.044715f;
 constexpr float kGeluTwice = 1.5957691216057308f;   // 2 * sqrt(2 / pi): (1 + tanh(y)) / 2 = sigmoid(2y)
 
+// The normal distribution's weight below -|g|, from exp(-g^2 / 2): Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26
+// (within 1e-7, halved from their bound for erf), and without the difference from 1 that the tail would be lost in.  The library's erff takes both of its branches
+// for every wavefront: 250 cycles an element, 60 so (2999 x 1032 x 1544 with gate and up kept, fp16: 43 us with it).
+TFK_DEVICE float normal_tail(float g, float bell) {
+  const float t = __builtin_amdgcn_rcpf(1.f + (0.3275911f * 0.7071067811865476f) * fabsf(g));
+  float p = 0.5f * 1.061405429f;
+  p = __builtin_fmaf(p, t, 0.5f * -1.453152027f);
+  p = __builtin_fmaf(p, t, 0.5f * 1.421413741f);
+  p = __builtin_fmaf(p, t, 0.5f * -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.5f * 0.254829592f);
+  return p * t * bell;
+}
 TFK_DEVICE float act_phi(float g, int activation) {
   if (activation == TF_ACT_SILU) return sigmoid(g);
-  if (activation == TF_ACT_GELU) return 0.5f + 0.5f * erff(g * 0.7071067811865476f);
+  if (activation == TF_ACT_GELU) {
+    const float tail = normal_tail(g, exp_of(-0.5f * g * g));
+    return g < 0.f ? tail : 1.f - tail;
+  }
   return sigmoid(kGeluTwice * (g + kGeluCubic * g * g * g));
 }
 TFK_DEVICE float act(float g, int activation) { return g * act_phi(g, activation); }
 // act and its derivative
 TFK_DEVICE void act_both(float g, int activation, float& value, float& slope) {
-  const float p = act_phi(g, activation);
-  value = g * p;
   if (activation == TF_ACT_GELU) {
-    slope = p + g * 0.3989422804014327f * __expf(-0.5f * g * g);
+    const float bell = exp_of(-0.5f * g * g), tail = normal_tail(g, bell);
+    const float p = g < 0.f ? tail : 1.f - tail;
+    value = g * p;
+    slope = p + g * 0.3989422804014327f * bell;
     return;
   }
+  const float p = act_phi(g, activation);
+  value = g * p;
   const float inner = activation == TF_ACT_SILU ? 1.f : kGeluTwice * (1.f + 3.f * kGeluCubic * g * g);
   const float both = p * (1.f - p);
   slope = both > 0.f ? p + g * both * inner : p;   // (far out the square may be infinite; a NaN stays one)
@@ -94,9 +113,8 @@ int gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void
   const ForwardPlan copy(M, F, K);
   if (copy.bytes > 0) {
     const int64_t pitch = 2 * aligned_width(K);
-    if (int rc = launch_copy_rows(who, x, 2 * K, M, ws, pitch, M, st)) return rc;
-    if (int rc = launch_copy_rows(who, w_gate, 2 * K, F, ws + copy.w_gate, pitch, F, st)) return rc;
-    if (int rc = launch_copy_rows(who, w_up, 2 * K, F, ws + copy.w_up, pitch, F, st)) return rc;
+    const RowsToCopy all[] = {{x, M, ws, M}, {w_gate, F, ws + copy.w_gate, F}, {w_up, F, ws + copy.w_up, F}};
+    if (int rc = launch_copy_rows(all, 3, 2 * K, pitch, st)) return rc;
     x = ws;
     w_gate = ws + copy.w_gate;
     w_up = ws + copy.w_up;
@@ -152,7 +170,7 @@ __global__ __launch_bounds__(kThreads) void gated_ffn_grads_kernel(const T* __re
 struct BackwardPlan {
   int64_t Fp, Kp;
   bool copy_weights, copy_x;
-  ColsPlan of_x, of_both, of_one; // products: dx, the weights' gradients together, one of them
+  ColsPlan of_x, of_w;            // products: dx, the weights' gradients
   size_t weights, x, parts, bytes;   // offsets in the workspace ([dg | du]: 0), its size
   BackwardPlan(int64_t M, int64_t F, int64_t K) {
     Fp = round_up_to(F, 64);
@@ -161,8 +179,7 @@ struct BackwardPlan {
     copy_weights = Kp != K || Fp != F;
     copy_x = Kp != K;
     of_x = plan_cols(M, K, 2 * Fp / 64);
-    of_both = plan_cols(2 * F, K, tiles_of(M, 64));
-    of_one = plan_cols(F, K, tiles_of(M, 64));
+    of_w = plan_cols(Fp + F, K, tiles_of(M, 64));
     size_t at = 0;
     auto take = [&](int64_t bytes_) {
       const size_t from = at;
@@ -173,20 +190,33 @@ struct BackwardPlan {
     weights = take(copy_weights ? 2 * 2 * Fp * Kp : 0);
     x = take(copy_x ? 2 * M * Kp : 0);
     const auto floats = [K](const ColsPlan& plan, int64_t rows) { return plan.splits > 1 ? PartsRoom(plan, rows, K).floats : 0; };
-    parts = take(4 * std::max({floats(of_x, M), floats(of_both, 2 * F), floats(of_one, F)}));
+    parts = take(4 * std::max(floats(of_x, M), floats(of_w, Fp + F)));
     bytes = at;
   }
 };
 
-// out [rows, K] = the product, in as many parts as its plan says
-template <typename T, bool kColA>
-int product_of_gradient(const char* who, const ColsProduct& product, const ColsPlan& plan, T* out, float* parts, hipStream_t st) {
-  const int rows = product.a.extent, cols = product.b.extent;
-  if (plan.splits == 1) return launch_cols<T, kColA>(who, product, plan, WholeEpilogue<T>{out, nullptr, rows, cols}, st);
-  const PartsRoom room(plan, rows, cols);
-  if (int rc = launch_cols<T, kColA>(who, product, plan, PartEpilogue{parts, room.rows, room.pitch, false}, st)) return rc;
-  return launch_sum_parts<T>(parts, room, plan.splits, 0, rows, cols, out, nullptr, st);
-}
+// The weights' gradients out of one product over the columns of [dg | du]: rows from Fp on are the second one's.
+template <typename T>
+struct BothEpilogue {
+  WholeEpilogue<T> gate, up;   // M: F, Fp + F; up's `out` is Fp rows in front of it
+  int Fp;
+
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    constexpr int kRows = 16 * TM;
+    if (at.row + kRows <= Fp) {
+      if (kInside && at.row + kRows <= gate.M) gate.template run<kInside>(acc, at);
+      else gate.template run<false>(acc, at);
+    } else if (at.row >= Fp) {
+      up.template run<kInside>(acc, at);
+    } else {
+      gate.template run<false>(acc, at);
+      TileAt behind = at;
+      behind.row_from = Fp;
+      up.template run<false>(acc, behind);
+    }
+  }
+};
 
 template <typename T>
 int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const void* gate, const void* up, void* dx, void* dw_gate,
@@ -205,34 +235,45 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
   if (int rc = launch_kernel(grads, dim3((unsigned)std::min<int64_t>(tiles_of(chunks, kThreads), 65536)), dim3(kThreads), 0, st,
                              static_cast<const T*>(dh), static_cast<const T*>(gate), static_cast<const T*>(up), rows, chunks, (int)F, (int)p.Fp))
     return rc;
+  RowsToCopy copies[3];
+  int count = 0;
   if (p.copy_weights) {
     char* const to = ws + p.weights;
-    if (int rc = launch_copy_rows(who, w_gate, 2 * K, F, to, 2 * p.Kp, p.Fp, st)) return rc;
-    if (int rc = launch_copy_rows(who, w_up, 2 * K, F, to + 2 * p.Fp * p.Kp, 2 * p.Kp, p.Fp, st)) return rc;
+    copies[count++] = {w_gate, F, to, p.Fp};
+    copies[count++] = {w_up, F, to + 2 * p.Fp * p.Kp, p.Fp};
     w_gate = to;
     w_up = to + 2 * p.Fp * p.Kp;
   }
   if (p.copy_x) {
-    if (int rc = launch_copy_rows(who, x, 2 * K, M, ws + p.x, 2 * p.Kp, M, st)) return rc;
+    copies[count++] = {x, M, ws + p.x, M};
     x = ws + p.x;
   }
+  if (count > 0)
+    if (int rc = launch_copy_rows(copies, count, 2 * K, 2 * p.Kp, st)) return rc;
   float* const parts = reinterpret_cast<float*>(ws + p.parts);
   const auto bits = [](const void* t) { return static_cast<const uint16_t*>(t); };
   const uint16_t* const grads_at = bits(ws);
   const ColsProduct of_x = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)M}, {bits(w_gate), p.Kp, (int)p.Kp, (int)K}, bits(w_up), (int)(p.Fp / 64), (int)(2 * p.Fp / 64), 0, 0};
-  if (int rc = product_of_gradient<T, false>(who, of_x, p.of_x, static_cast<T*>(dx), parts, st)) return rc;
+  T* const to_x = static_cast<T*>(dx);
+  if (p.of_x.splits == 1) {
+    if (int rc = launch_cols<T, false>(who, of_x, p.of_x, WholeEpilogue<T>{to_x, nullptr, (int)M, (int)K}, st)) return rc;
+  } else {
+    const PartsRoom room(p.of_x, M, K);
+    if (int rc = launch_cols<T, false>(who, of_x, p.of_x, PartEpilogue{parts, room.rows, room.pitch, false}, st)) return rc;
+    if (int rc = launch_sum_parts<T>(parts, room, p.of_x.splits, 0, M, K, to_x, nullptr, st)) return rc;
+  }
   const int m_tiles = (int)tiles_of(M, 64), m_pad = (int)(m_tiles * 64 - M);
   const ColsOperand tokens = {bits(x), p.Kp, (int)p.Kp, (int)K};
-  // (one product where the two gradients lie one behind the other)
-  if (p.Fp == F && static_cast<char*>(dw_up) == static_cast<char*>(dw_gate) + 2 * F * K) {
-    const ColsProduct both = {{grads_at, 2 * p.Fp, (int)(2 * F), (int)(2 * F)}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
-    return product_of_gradient<T, true>(who, both, p.of_both, static_cast<T*>(dw_gate), parts, st);
+  const ColsProduct of_w = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)(p.Fp + F)}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
+  T *const to_gate = static_cast<T*>(dw_gate), *const to_up = static_cast<T*>(dw_up);
+  if (p.of_w.splits == 1) {
+    const BothEpilogue<T> both = {{to_gate, nullptr, (int)F, (int)K}, {to_up - p.Fp * K, nullptr, (int)(p.Fp + F), (int)K}, (int)p.Fp};
+    return launch_cols<T, true>(who, of_w, p.of_w, both, st);
   }
-  for (int half = 0; half < 2; ++half) {
-    const ColsProduct product = {{grads_at + half * p.Fp, 2 * p.Fp, (int)p.Fp, (int)F}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
-    if (int rc = product_of_gradient<T, true>(who, product, p.of_one, static_cast<T*>(half ? dw_up : dw_gate), parts, st)) return rc;
-  }
-  return TF_OK;
+  const PartsRoom room(p.of_w, p.Fp + F, K);
+  if (int rc = launch_cols<T, true>(who, of_w, p.of_w, PartEpilogue{parts, room.rows, room.pitch, false}, st)) return rc;
+  if (int rc = launch_sum_parts<T>(parts, room, p.of_w.splits, 0, F, K, to_gate, nullptr, st)) return rc;
+  return launch_sum_parts<T>(parts, room, p.of_w.splits, p.Fp, p.Fp + F, K, to_up, nullptr, st);
 }
 
 int check_sizes(const char* who, int dtype, int activation, int64_t M, int64_t F, int64_t K) {

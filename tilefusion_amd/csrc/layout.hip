@@ -6,33 +6,33 @@ namespace {
 
 constexpr int kThreads = 256;
 
+struct CopyArgs {
+  const char* src[3];
+  uint4_t* dst[3];
+  int64_t rows[3], end[3];   // rows of src; chunks of all matrices up to and with this one
+};
 // Bound by memory; 16 bytes a lane.  (Unaligned 16-byte loads are one instruction, of one or two lines.)
-__global__ __launch_bounds__(kThreads) void copy_rows_kernel(const char* __restrict__ src, int64_t bytes, int64_t rows, uint4_t* __restrict__ dst,
-                                                             int chunks, int64_t count) {
+__global__ __launch_bounds__(kThreads) void copy_rows_kernel(CopyArgs x, int64_t bytes, int chunks, int64_t count) {
   typedef uint4_t any16B_t __attribute__((aligned(1)));
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t row = i / chunks, at = (i - row * chunks) * 16;
-    const char* const from = src + row * bytes + at;
+    const int which = i < x.end[0] ? 0 : i < x.end[1] ? 1 : 2;
+    const int64_t in = which == 0 ? i : i - x.end[which - 1];
+    const int64_t row = in / chunks, at = (in - row * chunks) * 16;
+    const char* const from = x.src[which] + row * bytes + at;
     uint4_t v = {0u, 0u, 0u, 0u};
-    if (row < rows && at + 16 <= bytes) {
+    if (row < x.rows[which] && at + 16 <= bytes) {
       v = *reinterpret_cast<const any16B_t*>(from);
-    } else if (row < rows) {
+    } else if (row < x.rows[which]) {
 #pragma unroll
       for (int t = 0; t < 16; ++t)
         if (at + t < bytes) v[t / 4] |= (unsigned)(uint8_t)from[t] << (8 * (t % 4));
     }
-    dst[i] = v;
+    x.dst[which][in] = v;
   }
 }
 
 __global__ __launch_bounds__(kThreads) void zero_kernel(uint16_t* dst, int64_t count) {
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads) dst[i] = 0;
-}
-
-__global__ __launch_bounds__(kThreads) void zero_columns_kernel(uint16_t* dst, int64_t pitch, int64_t rows, int from, int width) {
-  const int64_t count = rows * width;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads)
-    dst[i / width * pitch + from + i % width] = 0;
 }
 
 // Four columns a lane; the parts are added in their order.
@@ -64,20 +64,24 @@ unsigned blocks_for(int64_t items) { return (unsigned)std::max<int64_t>(1, std::
 
 }  // namespace
 
-int launch_copy_rows(const char*, const void* src, int64_t bytes, int64_t rows, void* dst, int64_t pitch, int64_t padded_rows, hipStream_t st) {
-  const int64_t count = padded_rows * (pitch / 16);
-  return launch_kernel(copy_rows_kernel, dim3(blocks_for(count)), dim3(kThreads), 0, st, static_cast<const char*>(src), bytes, rows,
-                       static_cast<uint4_t*>(dst), (int)(pitch / 16), count);
+int launch_copy_rows(const RowsToCopy* matrices, int count, int64_t bytes, int64_t pitch, hipStream_t st) {
+  CopyArgs x{};
+  int64_t end = 0;
+  for (int m = 0; m < 3; ++m) {
+    if (m < count) {
+      x.src[m] = static_cast<const char*>(matrices[m].src);
+      x.dst[m] = static_cast<uint4_t*>(matrices[m].dst);
+      x.rows[m] = matrices[m].rows;
+      end += matrices[m].padded_rows * (pitch / 16);
+    }
+    x.end[m] = end;
+  }
+  return launch_kernel(copy_rows_kernel, dim3(blocks_for(end)), dim3(kThreads), 0, st, x, bytes, (int)(pitch / 16), end);
 }
 
 int launch_zero_16bit(void* dst, int64_t count, hipStream_t st) {
   if (count == 0) return TF_OK;
   return launch_kernel(zero_kernel, dim3(blocks_for(count)), dim3(kThreads), 0, st, static_cast<uint16_t*>(dst), count);
-}
-
-int launch_zero_columns(void* dst, int64_t pitch, int64_t rows, int64_t from, int64_t to, hipStream_t st) {
-  return launch_kernel(zero_columns_kernel, dim3(blocks_for(rows * (to - from))), dim3(kThreads), 0, st, static_cast<uint16_t*>(dst), pitch, rows,
-                       (int)from, (int)(to - from));
 }
 
 template <typename T>

@@ -81,30 +81,37 @@ struct LseEpilogue {
   }
 };
 
-// One wavefront a row.
-constexpr int kMergeThreads = 256, kMergeRows = kMergeThreads / 64;
+// A workgroup a row: the largest maximum first, then the sums relative to it.
+constexpr int kMergeThreads = 256;
 __global__ __launch_bounds__(kMergeThreads) void merge_parts_kernel(const Part* __restrict__ parts, int slots, const float* __restrict__ at_target,
-                                                                    const int64_t* __restrict__ target, int64_t ignore_index, int T, int V,
+                                                                    const int64_t* __restrict__ target, int64_t ignore_index, int V,
                                                                     float* __restrict__ loss, float* __restrict__ lse) {
-  const int row = blockIdx.x * kMergeRows + threadIdx.x / 64, lane = threadIdx.x % 64;
-  if (row >= T) return;
-  const Part* const mine = parts + (size_t)row * slots;
+  __shared__ float s_top[kMergeThreads / 64], s_sum[kMergeThreads / 64];
+  const size_t row = blockIdx.x;
+  const Part* const mine = parts + row * slots;
+  const int tid = threadIdx.x;
   float top = -INFINITY, sum = 0.f;
-  for (int s = lane; s < slots; s += 64) {
+  for (int s = tid; s < slots; s += kMergeThreads) top = fmaxf(top, mine[s].top);
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (tid % 64 == 0) s_top[tid / 64] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 64; ++w) top = fmaxf(top, s_top[w]);
+  const float origin = as_origin(top);
+  for (int s = tid; s < slots; s += kMergeThreads) {
     const Part p = mine[s];
-    const float next = fmaxf(top, p.top), origin = as_origin(next);
-    sum = sum * __expf(top - origin) + p.sum * __expf(p.top - origin);
-    top = next;
+    sum += p.sum * __expf(p.top - origin);
   }
 #pragma unroll
-  for (int d = 32; d >= 1; d /= 2) {
-    const float other_top = __shfl_xor(top, d), other_sum = __shfl_xor(sum, d);
-    const float next = fmaxf(top, other_top), origin = as_origin(next);
-    sum = sum * __expf(top - origin) + other_sum * __expf(other_top - origin);
-    top = next;
-  }
-  if (lane != 0) return;
-  const float value = as_origin(top) + logf(sum);
+  for (int d = 32; d >= 1; d /= 2) sum += __shfl_xor(sum, d);
+  if (tid % 64 == 0) s_sum[tid / 64] = sum;
+  __syncthreads();
+  if (tid != 0) return;
+  sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 64; ++w) sum += s_sum[w];
+  const float value = origin + logf(sum);
   const int64_t wanted = target[row];
   lse[row] = value;
   // a target outside the vocabulary is a mistake that must not pass for a number
@@ -138,6 +145,7 @@ template <typename T>
 struct ProbEpilogue {
   T* p;                    // [tokens][pitch], the piece's first column
   int64_t pitch;
+  int pad;                 // columns of zeros in front of it
   const float *lse, *grad_loss;
   const Scale* scale;
   const int64_t* target;
@@ -154,22 +162,29 @@ struct ProbEpilogue {
       const int row = kInside ? at.row + 16 * i + lr : min(at.row + 16 * i + lr, M - 1);
       const int64_t wanted = target[row];
       const bool ignored = wanted == ignore_index;
-      const float origin = lse[row];
+      const float origin = lse[row] * kLog2e;
       // (a target outside the vocabulary: as the loss)
       const float weight = wanted >= 0 && wanted < V ? grad_loss[row] * in : __uint_as_float(0x7fc00000u);
+      // exp(z - lse) * |weight| as one power of two: what a product for every element would cost is 3% of the kernel at K = 1024
+      const float from = origin - __builtin_amdgcn_logf(fabsf(weight));
       const int64_t hot = wanted - first - at.col;   // counted from the tile's first column
-      const float from = origin * kLog2e;
       float4_t v[TN];
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -from)) * weight;
+        for (int r = 0; r < 4; ++r) v[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -from));
+      if (__any(weight < 0.f)) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[j][r] = copysignf(v[j][r], weight);
+      }
       if (__any(hot >= 0 && hot < 16 * TN)) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (hot == 16 * j + 4 * lg + r) v[j][r] = (__builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -from)) - 1.f) * weight;
+            if (hot == 16 * j + 4 * lg + r) v[j][r] = (__builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -origin)) - 1.f) * weight;
       }
       if (__any(ignored)) {
 #pragma unroll
@@ -178,6 +193,8 @@ struct ProbEpilogue {
           for (int r = 0; r < 4; ++r) v[j][r] = ignored ? 0.f : v[j][r];
       }
       store_blocks<kInside>(p, (size_t)pitch, at.row + 16 * i, at.col, M, N, at.lane, v);
+      if (at.col == 0)
+        for (int z = lg; z < pad; z += 4) p[(int64_t)row * pitch - 1 - z] = (T)0.f;   // (the last row again where the tile ends behind it)
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -241,8 +258,8 @@ int forward(const void* hidden, const void* weight, const int64_t* target, float
   const ForwardPlan plan(tokens, V, K);
   const int64_t width = aligned_width(K);
   if (width != K) {
-    if (int rc = launch_copy_rows(who, hidden, 2 * K, tokens, ws + plan.hidden, 2 * width, tokens, st)) return rc;
-    if (int rc = launch_copy_rows(who, weight, 2 * K, V, ws + plan.weight, 2 * width, V, st)) return rc;
+    const RowsToCopy both[] = {{hidden, tokens, ws + plan.hidden, tokens}, {weight, V, ws + plan.weight, V}};
+    if (int rc = launch_copy_rows(both, 2, 2 * K, 2 * width, st)) return rc;
     hidden = ws + plan.hidden;
     weight = ws + plan.weight;
   }
@@ -251,8 +268,8 @@ int forward(const void* hidden, const void* weight, const int64_t* target, float
   const Operands x = {hidden, {weight, nullptr}, (int)tokens, (int)V, (int)width};
   if (int rc = launch_product<T, false>(who, x, plan.product, LseEpilogue{parts, (int)plan.product.slots, at_target, target, (int)tokens, (int)V}, st))
     return rc;
-  return launch_kernel(merge_parts_kernel, dim3((unsigned)tiles_of(tokens, kMergeRows)), dim3(kMergeThreads), 0, st, parts, (int)plan.product.slots,
-                       at_target, target, ignore_index, (int)tokens, (int)V, loss, lse);
+  return launch_kernel(merge_parts_kernel, dim3((unsigned)tokens), dim3(kMergeThreads), 0, st, parts, (int)plan.product.slots, at_target, target,
+                       ignore_index, (int)V, loss, lse);
 }
 
 template <typename T>
@@ -269,7 +286,8 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
   if (int rc = launch_kernel(find_scale_kernel, dim3(1), dim3(kScaleThreads), 0, st, grad_loss, target, ignore_index, (int)tokens, kHeadroom, scale))
     return rc;
   if (plan.width != K) {
-    if (int rc = launch_copy_rows(who, hidden, 2 * K, tokens, ws + plan.hidden, 2 * plan.width, tokens, st)) return rc;
+    const RowsToCopy copy = {hidden, tokens, ws + plan.hidden, tokens};
+    if (int rc = launch_copy_rows(&copy, 1, 2 * K, 2 * plan.width, st)) return rc;
     hidden = ws + plan.hidden;
   }
   const auto bits = [](const void* t) { return static_cast<const uint16_t*>(t); };
@@ -282,17 +300,16 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
     const int pad = (int)(pitch - columns);
     const char* w = static_cast<const char*>(weight) + 2 * first * K;
     if (plan.width != K) {
-      if (int rc = launch_copy_rows(who, w, 2 * K, columns, ws + plan.weight, 2 * plan.width, columns, st)) return rc;
+      const RowsToCopy copy = {w, columns, ws + plan.weight, columns};
+      if (int rc = launch_copy_rows(&copy, 1, 2 * K, 2 * plan.width, st)) return rc;
       w = ws + plan.weight;
     }
     const Operands logits = {hidden, {w, nullptr}, (int)tokens, (int)columns, width};
     if (int rc = launch_product<T, false>(who, logits, plan_product(tokens, columns, width, false),
-                                          ProbEpilogue<T>{p + pad, pitch, lse, grad_loss, scale, target, ignore_index, (int)tokens, (int)columns,
+                                          ProbEpilogue<T>{p + pad, pitch, pad, lse, grad_loss, scale, target, ignore_index, (int)tokens, (int)columns,
                                                           (int)first, (int)V},
                                           st))
       return rc;
-    if (pad > 0)
-      if (int rc = launch_zero_columns(p, pitch, tokens, 0, pad, st)) return rc;
 
     // dH += P * W
     ColsPlan of_hidden = plan.of_hidden;

@@ -166,7 +166,7 @@ inline bool at_16B(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 =
 constexpr int64_t kMaxTiles = ((int64_t)1 << 23) - 1;   // a launch has less than 2^32 threads, of which a workgroup has 512 at most
 
 // The kernel that gemm.hip's cost model expects to be done first with M x N outputs over K 16-bit elements, out of those of `allowed` (a bit per row of
-// its table kGemmKernels; bit 0 is among them): its position there.
+// its table kGemmKernels): its position there.
 int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed);
 
 // Positions in that table, and the kernels here.  With two matrices B, tiles have an even number of 16-column blocks to a wavefront, a
@@ -185,7 +185,8 @@ inline int64_t product_slots(int kernel, int64_t N) {
 }
 // K: 16-bit elements (half the elements of 8)
 inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool two) {
-  const int kernel = pick_table_kernel(M, two ? 2 * N : N, K, two ? kTwoAllowed : kOneAllowed);
+  // (the table has no tile of 16 x 32: up to 16 rows it is ahead of 32 x 32, 1 x 4096 x 11264 of two matrices 33.2 us / 38.4)
+  const int kernel = two && M <= 16 ? 0 : pick_table_kernel(M, two ? 2 * N : N, K, two ? kTwoAllowed & ~1u : kOneAllowed);
   return {kernel, product_slots(kernel, N)};
 }
 
@@ -382,11 +383,15 @@ int launch_sum_parts(const float* parts, const PartsRoom& room, int splits, int6
 // ------------------------------------------------------------------------------------------
 // Layout
 // ------------------------------------------------------------------------------------------
-// dst: `padded_rows` rows of `pitch` bytes (a multiple of 16, from a 16-byte boundary on) with the `bytes` bytes of each of `rows` rows of src in
-// front, zeros behind them and in the rows that follow.
-int launch_copy_rows(const char* who, const void* src, int64_t bytes, int64_t rows, void* dst, int64_t pitch, int64_t padded_rows, hipStream_t st);
-// zeros in columns from .. to - 1 of rows of 16-bit elements
-int launch_zero_columns(void* dst, int64_t pitch, int64_t rows, int64_t from, int64_t to, hipStream_t st);
+// `padded_rows` rows of `pitch` bytes (a multiple of 16, from a 16-byte boundary on) with the `bytes` bytes of each of `rows` rows of src in
+// front, zeros behind them and in the rows that follow: up to three matrices in one launch.
+struct RowsToCopy {
+  const void* src;
+  int64_t rows;
+  void* dst;
+  int64_t padded_rows;
+};
+int launch_copy_rows(const RowsToCopy* matrices, int count, int64_t bytes, int64_t pitch, hipStream_t st);
 // count 16-bit elements of zero
 int launch_zero_16bit(void* dst, int64_t count, hipStream_t st);
 

@@ -4,6 +4,7 @@ from typing import Any, Tuple, Union
 
 import torch
 
+from .. import _direct
 from ._autograd import records
 
 __all__ = ["gated_ffn", "gated_ffn_backward"]
@@ -57,6 +58,10 @@ def gated_ffn(
     Returns h [.., F], or (h, gate, up).  Everything is fp32 up to h, which is rounded once.  Under autograd h carries the backward
     pass (once: no gradient of a gradient), and gate and up none; calls that are captured into a graph are not recorded.
     """
+    if not torch.compiler.is_compiling():
+        direct = _direct.gated_ffn(x, w_gate, w_up, activation, keep)   # (no gradient is asked for)
+        if direct is not None:
+            return direct if keep else direct[0]
     if records("gated_ffn", x, w_gate, w_up):
         out = _GatedFfn.apply(x, w_gate, w_up, activation)
     else:

@@ -4,6 +4,8 @@ from typing import Tuple
 
 import torch
 
+from .. import _direct
+
 __all__ = ["gemm_int8", "quantize_rows"]
 
 
@@ -13,6 +15,10 @@ def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     scale = max|x| / 127 of a row (in fp32), q the whole number nearest to x / scale, the even one in the middle of two.
     A row of zeros has scale 0 and q 0; a row with an infinity or a NaN has scale NaN and q 0, so that every product of it is NaN.
     No gradient passes through a rounding: the results have none."""
+    if not torch.compiler.is_compiling():
+        direct = _direct.quantize_rows(x)
+        if direct is not None:
+            return direct
     if x.dim() < 1:
         raise RuntimeError("quantize_rows: x must have rows [.., K]")
     rows = x.detach().reshape(-1, x.size(-1)) if x.size(-1) > 0 else x.detach().reshape(0, 0)
@@ -40,6 +46,8 @@ def gemm_int8(
 
     The sum is exact (int32; K <= 131071), scaled in fp32 and rounded once.
     """
+    if not torch.compiler.is_compiling() and _direct.gemm_int8(tensor_a, tensor_b, scale_a, scale_b, tensor_c):
+        return
     torch.ops.tilefusion.gemm_int8(
         tensor_a.contiguous(), tensor_b.contiguous(), scale_a.contiguous(), scale_b.contiguous(), tensor_c
     )

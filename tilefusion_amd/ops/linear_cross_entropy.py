@@ -4,6 +4,7 @@ from typing import Any, Tuple
 
 import torch
 
+from .. import _direct
 from ._autograd import records
 
 __all__ = ["linear_cross_entropy", "linear_cross_entropy_backward"]
@@ -63,6 +64,10 @@ def linear_cross_entropy(
     exp(logits), which `linear_cross_entropy_backward` takes.  Under autograd the loss carries the backward pass (once: no
     gradient of a gradient), and lse none; calls that are captured into a graph are not recorded.
     """
+    if not torch.compiler.is_compiling():
+        direct = _direct.linear_cross_entropy(hidden, weight, target, ignore_index)   # (no gradient is asked for)
+        if direct is not None:
+            return direct
     if records("linear_cross_entropy", hidden, weight):
         return _LinearCrossEntropy.apply(hidden, weight, target, ignore_index)
     return _forward(hidden, weight, target, ignore_index)
