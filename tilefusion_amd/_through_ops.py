@@ -38,3 +38,11 @@ def gated_ffn(*args: Any) -> None:
 
 def linear_cross_entropy(*args: Any) -> None:
     return None
+
+
+def gated_ffn_backward(*args: Any) -> None:
+    return None
+
+
+def linear_cross_entropy_backward(*args: Any) -> None:
+    return None

@@ -317,6 +317,53 @@ PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t narg
   END_HANDLE_TH_ERRORS
 }
 
+// (grad_h, x, w_gate, w_up, gate, up, activation) -> (grad_x, grad_w [2, F, K]), or None
+PyObject* gated_ffn_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[6], grad_x, grad_w;
+  c10::string_view activation;
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, c10::string_view,
+                  at::Tensor&, at::Tensor&);
+  static const auto op = find_op<Op>("tilefusion::gated_ffn_backward");
+  if (nargs != 7 || !plain(op, args, 6, t) || !matrices(t, 6) || !text(args[6], &activation)) Py_RETURN_NONE;
+  const at::Tensor &x = t[1], &w = t[2];
+  if (x.size(1) != w.size(1) || x.size(1) == 0) Py_RETURN_NONE;   // (the wrapper's own errors)
+  for (int i : {0, 4, 5})
+    if (t[i].size(1) != w.size(0)) Py_RETURN_NONE;
+  {
+    NoGil unlocked;
+    grad_x = empty_output(x.sizes(), x);
+    grad_w = empty_output({2 * w.size(0), w.size(1)}, x);
+    op.redispatch(kCuda, t[0], x, w, t[3], t[4], t[5], activation, grad_x, grad_w);
+    grad_w = grad_w.view({2, w.size(0), w.size(1)});
+  }
+  return tuple_of({grad_x, grad_w});
+  END_HANDLE_TH_ERRORS
+}
+
+// (grad_loss, hidden, weight, target, lse, ignore_index) -> (grad_hidden, grad_weight), or None
+PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[5], grad_hidden, grad_weight;
+  int64_t ignore_index;
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, at::Tensor&, at::Tensor&);
+  static const auto op = find_op<Op>("tilefusion::linear_cross_entropy_backward");
+  if (nargs != 6 || !plain(op, args, 5, t) || !vectors(t, 1) || !matrices(t + 1, 2) || !vectors(t + 3, 2) || !ints(args + 5, 1, &ignore_index))
+    Py_RETURN_NONE;
+  const at::Tensor &hidden = t[1], &weight = t[2];
+  if (hidden.size(1) != weight.size(1) || hidden.size(1) == 0) Py_RETURN_NONE;
+  for (int i : {0, 3, 4})
+    if (t[i].size(0) != hidden.size(0)) Py_RETURN_NONE;
+  {
+    NoGil unlocked;
+    grad_hidden = empty_output(hidden.sizes(), hidden);
+    grad_weight = empty_output(weight.sizes(), weight);
+    op.redispatch(kCuda, t[0], hidden, weight, t[3], t[4], ignore_index, grad_hidden, grad_weight);
+  }
+  return tuple_of({grad_hidden, grad_weight});
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*kFunction)(PyObject*, PyObject* const*, Py_ssize_t)>
 constexpr PyMethodDef method(const char* name) {
   return {name, (PyCFunction)(void (*)(void))kFunction, METH_FASTCALL, nullptr};
@@ -324,7 +371,8 @@ constexpr PyMethodDef method(const char* name) {
 PyMethodDef methods[] = {method<gemm>("gemm"), method<fused_two_gemms>("fused_two_gemms"), method<scatter_nd>("scatter_nd"),
                          method<flash_attention>("flash_attention"), method<flash_decode>("flash_decode"),
                          method<quantize_rows>("quantize_rows"), method<gemm_int8>("gemm_int8"), method<gated_ffn>("gated_ffn"),
-                         method<linear_cross_entropy>("linear_cross_entropy"),
+                         method<gated_ffn_backward>("gated_ffn_backward"), method<linear_cross_entropy>("linear_cross_entropy"),
+                         method<linear_cross_entropy_backward>("linear_cross_entropy_backward"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

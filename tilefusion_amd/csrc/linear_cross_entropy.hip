@@ -9,9 +9,9 @@
 //
 // Backward, a piece of the vocabulary at a time: the product is computed again, and from lse
 //   P[t, v] = grad_loss[t] * (exp(z[t, v] - lse[t]) - [v = target[t]]),   dH += P * W,   dW = P^T * H.
-// P of a piece is rounded to 16 bits, as the operand of a matrix instruction has to be, divided by the smallest power of two that no
-// |grad_loss| is above (times 2^14 for fp16), so that the weights of a mean over many tokens do not fall below fp16's range; the sums are
-// multiplied by it again in 32 bits.  dH is summed over the pieces in fp32 and rounded once.
+// P of a piece is rounded to 16 bits, as the operand of a matrix instruction has to be; in fp16 divided by the smallest power of two that no
+// |grad_loss| is above, times 2^14, so that the weights of a mean over many tokens do not fall below the type's range: the sums are
+// multiplied by it again in 32 bits.  (bf16 has the range of fp32.)  dH is summed over the pieces in fp32 and rounded once.
 #include <cmath>
 
 #include "product.hpp"
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_parts_kernel(const Part* 
 // ---- backward ------------------------------------------------------------------------------
 constexpr int kScaleThreads = 1024;
 __global__ __launch_bounds__(kScaleThreads) void find_scale_kernel(const float* __restrict__ grad_loss, const int64_t* __restrict__ target,
-                                                                   int64_t ignore_index, int T, int headroom, Scale* scale) {
+                                                                   int64_t ignore_index, int T, Scale* scale) {
   __shared__ float s_top[kScaleThreads / 64];
   float top = 0.f;
   for (int t = threadIdx.x; t < T; t += kScaleThreads)
@@ -137,8 +137,8 @@ __global__ __launch_bounds__(kScaleThreads) void find_scale_kernel(const float* 
     const float m = frexpf(top, &e);   // top = m * 2^e, 0.5 <= m < 1
     if (m == 0.5f) --e;
   }
-  e = max(e, -110);   // (2^-e and the headroom have to fit as well)
-  *scale = Scale{ldexpf(1.f, headroom - e), ldexpf(1.f, e - headroom)};
+  e = max(e, -110);   // (2^(14 - e) has to fit as well)
+  *scale = Scale{ldexpf(1.f, 14 - e), ldexpf(1.f, e - 14)};
 }
 
 template <typename T>
@@ -147,7 +147,7 @@ struct ProbEpilogue {
   int64_t pitch;
   int pad;                 // columns of zeros in front of it
   const float *lse, *grad_loss;
-  const Scale* scale;
+  const Scale* scale;      // null: 1
   const int64_t* target;
   int64_t ignore_index;
   int M, N;                // tokens, columns of the piece
@@ -156,7 +156,7 @@ struct ProbEpilogue {
   template <bool kInside, int TM, int TN>
   TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
     const int lr = at.lane & 15, lg = at.lane >> 4;
-    const float in = scale->in;
+    const float in = scale != nullptr ? scale->in : 1.f;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int row = kInside ? at.row + 16 * i + lr : min(at.row + 16 * i + lr, M - 1);
@@ -165,20 +165,12 @@ struct ProbEpilogue {
       const float origin = lse[row] * kLog2e;
       // (a target outside the vocabulary: as the loss)
       const float weight = wanted >= 0 && wanted < V ? grad_loss[row] * in : __uint_as_float(0x7fc00000u);
-      // exp(z - lse) * |weight| as one power of two: what a product for every element would cost is 3% of the kernel at K = 1024
-      const float from = origin - __builtin_amdgcn_logf(fabsf(weight));
       const int64_t hot = wanted - first - at.col;   // counted from the tile's first column
       float4_t v[TN];
 #pragma unroll
       for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -from));
-      if (__any(weight < 0.f)) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[j][r] = copysignf(v[j][r], weight);
-      }
+        for (int r = 0; r < 4; ++r) v[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -origin)) * weight;
       if (__any(hot >= 0 && hot < 16 * TN)) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
@@ -279,12 +271,12 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
   if (tokens == 0) return launch_zero_16bit(grad_weight, V * K, st);
   const BackwardPlan plan(tokens, V, K);
   T* const p = reinterpret_cast<T*>(ws);
-  Scale* const scale = reinterpret_cast<Scale*>(ws + plan.scale);
+  constexpr bool kScaled = std::is_same_v<T, half_t>;
+  Scale* const scale = kScaled ? reinterpret_cast<Scale*>(ws + plan.scale) : nullptr;
   float* const hidden_parts = reinterpret_cast<float*>(ws + plan.hidden_parts);
   float* const weight_parts = reinterpret_cast<float*>(ws + plan.weight_parts);
-  constexpr int kHeadroom = std::is_same_v<T, half_t> ? 14 : 0;
-  if (int rc = launch_kernel(find_scale_kernel, dim3(1), dim3(kScaleThreads), 0, st, grad_loss, target, ignore_index, (int)tokens, kHeadroom, scale))
-    return rc;
+  if constexpr (kScaled)
+    if (int rc = launch_kernel(find_scale_kernel, dim3(1), dim3(kScaleThreads), 0, st, grad_loss, target, ignore_index, (int)tokens, scale)) return rc;
   if (plan.width != K) {
     const RowsToCopy copy = {hidden, tokens, ws + plan.hidden, tokens};
     if (int rc = launch_copy_rows(&copy, 1, 2 * K, 2 * plan.width, st)) return rc;

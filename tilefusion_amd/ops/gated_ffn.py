@@ -81,6 +81,10 @@ def gated_ffn_backward(
     """Gradients of x, w_gate and w_up, from that of h [.., F] and the gate and up [.., F] that `gated_ffn` kept.
 
     The gradients of gate and up are rounded to the type on the way, as operands of the products that follow."""
+    if not torch.compiler.is_compiling():
+        direct = _direct.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation)
+        if direct is not None:
+            return direct[0], direct[1][0], direct[1][1]
     if w_gate.dim() != 2 or w_up.dim() != 2:
         raise RuntimeError("gated_ffn_backward: w_gate and w_up must be [F, K]")
     f, k = w_gate.shape

@@ -86,6 +86,10 @@ def linear_cross_entropy_backward(
     The vocabulary is done in pieces; what is held of a piece are its softmax gradients in 16 bits, which is where they are
     rounded: relative to the largest |grad_loss|, so that no weight of a mean is too small for fp16.  A grad_loss of an
     ignored token is not looked at; tokens with a target outside the vocabulary make NaN of the gradients they have a part in."""
+    if not torch.compiler.is_compiling():
+        direct = _direct.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index)
+        if direct is not None:
+            return direct
     rows, table, words = _operands(hidden, weight, target, "linear_cross_entropy_backward")
     for name, t in (("grad_loss", grad_loss), ("lse", lse)):
         if t.shape != target.shape:
