@@ -228,7 +228,7 @@ TF_API int tf_scatter_nd(const void* updates, void* data, const int64_t* indices
 
 /* C[M,N] = scale_a[m] * scale_b[n] * sum_k A[m,k] * B[n,k] of 8-bit integers: A [M,K] and B [N,K] int8, row-major; scale_a [M] and
  * scale_b [N] fp32; C [M,N] of c_dtype (fp32, fp16 or bf16).  The sum is exact (int32), hence K <= 131071; it is scaled in fp32 and
- * rounded once.  M = 0 and N = 0 are done at once.  A and B begin at 16-byte boundaries; where K is no multiple of 16 they may begin
+ * rounded once.  M = 0 and N = 0 are done at once.  At most 2^23 tiles of 64 x 64 results.  A and B begin at 16-byte boundaries; where K is no multiple of 16 they may begin
  * anywhere, and a workspace (at a 16-byte boundary, of the bytes that the function beside it says, otherwise 0) takes copies of them.
  * (No counterpart in the reference.) */
 TF_API size_t tf_gemm_int8_workspace_bytes(int64_t M, int64_t N, int64_t K);
@@ -254,8 +254,8 @@ TF_API size_t tf_gated_ffn_workspace_bytes(int64_t M, int64_t F, int64_t K);
 TF_API int tf_gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void* gate, void* up, int dtype,
                         int activation, int64_t M, int64_t F, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients of x [M,K], w_gate and w_up [F,K] from that of h (dh [M,F]) and the gate and up values that the forward call kept; x and
- * the weights as there, the others begin anywhere.  The workspace begins at a 16-byte boundary and may hold anything; it is done with when the call's work is.  w_up's gradient right behind
- * w_gate's makes one product of the two.  M = 0: the weights' gradients are zero. */
+ * the weights as there, the others begin anywhere.  The workspace begins at a 16-byte boundary and may hold anything; it is done with when the call's work is.  A null dx, or
+ * null dw_gate and dw_up, are not computed.  M = 0: the weights' gradients are zero. */
 TF_API size_t tf_gated_ffn_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
 TF_API int tf_gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const void* gate,
                                  const void* up, void* dx, void* dw_gate, void* dw_up, int dtype, int activation, int64_t M,
@@ -263,7 +263,7 @@ TF_API int tf_gated_ffn_backward(const void* dh, const void* x, const void* w_ga
 
 /* Softmax cross entropy of the logits hidden [T,K] * weight [V,K]^T, which are never in memory: lse[t] = log sum_v exp(logit[t,v]),
  * loss[t] = lse[t] - logit[t,target[t]], both fp32; hidden and weight fp16 or bf16.  loss is 0 where target[t] == ignore_index and NaN where it
- * is any other number outside 0 .. V-1.  T <= 2^22 - 64, V <= 2^30 - 64, K <= 2^22 - 64.  hidden and weight begin at 16-byte boundaries, or, where K is
+ * is any other number outside 0 .. V-1.  T <= 2^22 - 64, V <= 2^28 - 64, K <= 2^22 - 64.  hidden and weight begin at 16-byte boundaries, or, where K is
  * no multiple of 8, anywhere. */
 TF_API size_t tf_linear_cross_entropy_workspace_bytes(int64_t T, int64_t V, int64_t K);
 TF_API int tf_linear_cross_entropy(const void* hidden, const void* weight, const int64_t* target, float* loss, float* lse,
@@ -271,7 +271,8 @@ TF_API int tf_linear_cross_entropy(const void* hidden, const void* weight, const
                                    size_t workspace_bytes, void* stream);
 /* Gradients of hidden and weight (both of dtype) from grad_loss [T] (fp32) and the lse of the forward call.  Ignored tokens have none,
  * whatever their grad_loss; tokens with a target outside the vocabulary make NaN of every row of grad_weight and of their row of grad_hidden.
- * The vocabulary is done in pieces, which the workspace has room for.  T = 0: grad_weight is zero. */
+ * The vocabulary is done in pieces, which the workspace has room for.  A null grad_hidden or grad_weight is not computed.  T = 0: grad_weight is
+ * zero. */
 TF_API size_t tf_linear_cross_entropy_backward_workspace_bytes(int64_t T, int64_t V, int64_t K);
 TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* hidden, const void* weight, const int64_t* target,
                                             const float* lse, void* grad_hidden, void* grad_weight, int dtype, int64_t T,
@@ -289,6 +290,11 @@ TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* 
  * `workspace_bytes`, runs the streaming kernel with operands at 16-byte boundaries, otherwise 0.  tf_scatter_nd_plan, `data` in ordinary memory of the
  * current device, it and 16-bit updates at 4-byte boundaries: updates that are sorted together (0: each goes straight to memory), and in
  * *words_a_lane the 32-bit words of an update that a lane adds; -1 for other arguments. */
+/* tf_product_kernel_index: position in kGemmKernels of what tf_gemm_int8 (K: half its own), tf_gated_ffn (two = 1, N: F) and tf_linear_cross_entropy
+ * and the first product of its backward pass (N: columns of the vocabulary or of a piece) run; -1 for other arguments.  tf_product_cols_plan: position in kColsShapes
+ * (csrc/product.hpp) of the tile of a gradient of M x N that is a sum over `rows` rows, and in *parts the parts that the sum is cut into. */
+TF_API int tf_product_kernel_index(int64_t M, int64_t N, int64_t K, int two);
+TF_API int tf_product_cols_plan(int64_t M, int64_t N, int64_t rows, int* parts);
 TF_API int tf_gemm_kernel_index(int64_t M, int64_t N, int64_t K, int c_is_f32);
 TF_API int tf_flash_decode_plan(int64_t batch_heads, int64_t Lkv, int64_t D, int num_splits, int* wavefronts);
 TF_API int tf_flash_attention_rows(int64_t batch, int64_t Lq, int64_t Lkv, int64_t D, int causal);

@@ -116,11 +116,17 @@ def linear_cross_entropy_backward(grad_loss, hidden, weight, target, ignore_inde
 
 
 def assert_within(got, want, bound, what=""):
+    """Returns where the result is a number: what may lie beyond the type's largest one may be that infinity, and nothing else may."""
+    largest = torch.finfo(got.dtype).max
     got = got.double()
     assert got.shape == want.shape, f"{what}: shape {tuple(got.shape)}, not {tuple(want.shape)}"
-    assert torch.isfinite(got).all(), f"{what}: not finite"
-    over = (got - want).abs() - bound
+    finite = torch.isfinite(got)
+    beyond = want.abs() + bound > largest
+    assert (finite | (beyond & (got == torch.sign(want) * float("inf")))).all(), f"{what}: not finite"
+    assert (~finite | (want.abs() - bound <= largest)).all(), f"{what}: finite"
+    over = torch.where(finite, (got - want).abs() - bound, torch.zeros_like(want))
     if (over > 0).any():
         at = int(over.argmax())
         raise AssertionError(f"{what}: {int((over > 0).sum())} of {got.numel()} out of bounds; element {at}: {got.flatten()[at]:.9g}, "
                              f"not {want.flatten()[at]:.9g} +- {bound.flatten()[at]:.3g}")
+    return finite

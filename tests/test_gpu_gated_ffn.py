@@ -39,7 +39,14 @@ SIZES = [
 ]
 
 
-@pytest.mark.parametrize("m,f,k", SIZES)
+# sizes that reach the kernels which those do not (tests/test_products_cpu.py looks)
+KERNELS = [
+    (35, 350, 64), (17, 1, 64), (37, 3004, 1984), (42, 3635, 728), (226, 2781, 448), (358, 1620, 72), (567, 5492, 64), (271, 5523, 64), (396, 5528, 72),
+    (658, 5679, 64),
+]
+
+
+@pytest.mark.parametrize("m,f,k", SIZES + KERNELS)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_forward_sizes(m, f, k, dtype):
     x, w_gate, w_up, _ = _block(m, f, k, dtype)
@@ -112,7 +119,14 @@ def _check_backward(grad_h, x, w_gate, w_up, gate, up, activation):
 BACKWARD_SIZES = [(1, 1, 1), (1, 64, 64), (3, 17, 9), (31, 100, 33), (64, 64, 64), (65, 127, 72), (130, 96, 200), (257, 136, 264), (400, 513, 104), (1000, 160, 1032)]
 
 
-@pytest.mark.parametrize("m,f,k", BACKWARD_SIZES)
+# sizes that reach the tiles, and sums in parts, which those do not (tests/test_products_cpu.py looks)
+BACKWARD_KERNELS = [
+    (3667, 1, 2320), (2442, 1, 1592), (3214, 3946, 8), (1810, 409, 2304), (130, 8700, 5936), (1, 6720, 1296), (1, 2186, 1800), (2, 3339, 520), (3951, 2907, 8),
+    (1, 3238, 1184), (26477, 548, 8), (34566, 1353, 144),
+]
+
+
+@pytest.mark.parametrize("m,f,k", BACKWARD_SIZES + BACKWARD_KERNELS)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_backward_sizes(m, f, k, dtype):
     x, w_gate, w_up, g = _block(m, f, k, dtype, seed=4)
@@ -126,6 +140,40 @@ def test_backward_activations(activation, dtype):
     grad_h = _randn(g, 150, 200, dtype=dtype)
     _, gate, up = ops.gated_ffn(x * 2, w_gate, w_up, activation, keep=True)
     _check_backward(grad_h, x * 2, w_gate, w_up, gate, up, activation)
+
+
+@pytest.mark.parametrize("f", [128, 130])
+def test_backward_of_some(f):
+    # what is not asked for is not computed, and changes nothing of what is
+    x, w_gate, w_up, g = _block(100, f, 72, torch.bfloat16, seed=11)
+    grad_h = _randn(g, 100, f, dtype=torch.bfloat16)
+    _, gate, up = ops.gated_ffn(x, w_gate, w_up, keep=True)
+    want = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up)
+    for asked in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        leaves = [t.clone().requires_grad_(i in asked) for i, t in enumerate((x, w_gate, w_up))]
+        ops.gated_ffn(*leaves).backward(grad_h)
+        for i, leaf in enumerate(leaves):
+            assert torch.equal(leaf.grad, want[i]) if i in asked else leaf.grad is None
+
+
+def test_offsets_that_pass_32_bits():
+    # h, gate and up of more than 4 GiB each, and gradients that are sums over them
+    m, f, k = 70000, 32768, 64
+    g = torch.Generator(device=DEV).manual_seed(12)
+    x, w = _randn(g, m, k, dtype=torch.bfloat16), _randn(g, 2, f, k, dtype=torch.bfloat16, scale=0.125)
+    h, gate, up = ops.gated_ffn(x, w[0], w[1], keep=True)
+    for rows in (slice(0, 200), slice(m - 200, m)):
+        want, bounds = ref.gated_ffn(x[rows], w[0], w[1], "silu")
+        for got, a, b in zip((h, gate, up), want, bounds):
+            ref.assert_within(got[rows], a, b)
+    # all but the last rows have no gradient: theirs is that of a small problem
+    h.zero_()
+    h[-200:] = _randn(g, 200, f, dtype=torch.bfloat16)
+    grad_x, grad_gate, grad_up = ops.gated_ffn_backward(h, x, w[0], w[1], gate, up)
+    want, bounds = ref.gated_ffn_backward(h[-200:], x[-200:], w[0], w[1], gate[-200:], up[-200:], "silu")
+    assert (grad_x[:-200] == 0).all()
+    for got, a, b in zip((grad_x[-200:], grad_gate, grad_up), want, bounds):
+        ref.assert_within(got, a, b)
 
 
 def test_backward_shapes_strides_and_empty():

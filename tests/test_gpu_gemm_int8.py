@@ -37,7 +37,14 @@ SIZES = [
 ]
 
 
-@pytest.mark.parametrize("m,n,k", SIZES)
+# sizes that reach the kernels which those do not (tests/test_products_cpu.py looks)
+KERNELS = [
+    (1, 1, 528), (889, 172, 144), (179, 583, 128), (334, 438, 144), (381, 792, 3968), (162, 2558, 1824), (746, 1748, 896), (358, 3187, 144), (2835, 5627, 192),
+    (1670, 2341, 128), (2120, 3587, 144), (1018, 5500, 128), (1974, 4508, 128), (2103, 5383, 144),
+]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES + KERNELS)
 @pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
 def test_sizes(m, n, k, out):
     g = torch.Generator(device=DEV).manual_seed(m * 7 + n * 3 + k)
@@ -55,6 +62,32 @@ def test_the_largest_sum_fits():
     one = torch.ones(5, device=DEV)
     ops.gemm_int8(a, b, one[:3].clone(), one, c)
     assert (c.double() == float(torch.tensor(k * 16384, dtype=torch.float32))).all()
+
+
+def test_offsets_that_pass_32_bits():
+    # operands and a result of more than 4 GiB each: the last rows
+    g = torch.Generator(device=DEV).manual_seed(4)
+    m, n, k = 70000, 33000, 65536
+    a = torch.randint(-128, 128, (m, k), device=DEV, dtype=torch.int8, generator=g)
+    b = torch.randint(-128, 128, (300, k), device=DEV, dtype=torch.int8, generator=g)
+    one = torch.ones(m, device=DEV)
+    c = torch.empty(m, 300, device=DEV)
+    ops.gemm_int8(a, b, one, one[:300], c)
+    assert torch.equal(c[-200:].double(), _expect(a[-200:], b, one[-200:], one[:300]).float().double())
+    c = torch.empty(300, m, device=DEV)
+    ops.gemm_int8(b, a, one[:300], one, c)
+    assert torch.equal(c[:, -200:].double(), _expect(b, a[-200:], one[:300], one[-200:]).float().double())
+    a, b = a[:, :64].contiguous(), a[:n, :64].contiguous()
+    c = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)
+    ops.gemm_int8(a, b, one, one[:n], c)
+    for rows in (slice(0, 300), slice(m // 2, m // 2 + 300), slice(m - 300, m)):
+        want = _expect(a[rows], b, one[rows], one[:n])
+        assert ((c[rows].double() - want).abs() <= want.abs() * half_step(torch.bfloat16)).all()
+    x = torch.randn(40000, 64000, device=DEV, generator=g, dtype=torch.bfloat16)
+    q, scale = ops.quantize_rows(x)
+    for rows in (slice(0, 4), slice(39990, 40000)):
+        want_q, want_scale = _quantized(x[rows])
+        assert torch.equal(q[rows], want_q) and torch.equal(scale[rows], want_scale)
 
 
 def test_strides_alignment_and_empty():

@@ -39,10 +39,10 @@ def _check_backward(grad_loss, hidden, weight, target, ignore_index=-100):
     for name, g, w, b, like in zip(("grad_hidden", "grad_weight"), got, want, bounds, (hidden, weight)):
         assert g.shape == like.shape and g.dtype == like.dtype
         what = f"{name} {tuple(hidden.shape)} V={weight.shape[0]} {hidden.dtype}"
-        ref.assert_within(g.reshape(w.shape), w, b, what)
+        number = ref.assert_within(g.reshape(w.shape), w, b, what)
         if w.norm() > 0:
             floor = w.numel() ** 0.5 * ref.TINY[hidden.dtype]   # results too small for the type
-            assert (g.reshape(w.shape).double() - w).norm() <= 2 * ref.half_step(hidden.dtype) * w.norm() + floor, what
+            assert (g.reshape(w.shape).double() - w)[number].norm() <= 2 * ref.half_step(hidden.dtype) * w.norm() + floor, what
     return got
 
 
@@ -52,14 +52,26 @@ SIZES = [
 ]
 
 
-@pytest.mark.parametrize("t,v,k", SIZES)
+# sizes that reach the kernels which those do not (tests/test_products_cpu.py looks)
+KERNELS = [
+    (1, 1, 264), (1883, 67, 72), (1752, 50, 64), (2319, 49, 72), (354, 855, 2048), (2411, 173, 712), (480, 2674, 448), (197, 5649, 72), (2891, 5564, 80),
+    (898, 4350, 64), (2865, 2786, 64), (967, 5420, 72), (2925, 3106, 64), (2206, 5545, 64),
+]
+# and the tiles, and sums in parts, of gradients
+BACKWARD_KERNELS = [
+    (3599, 1, 2208), (2522, 1, 1544), (1, 903, 8), (1849, 886, 2288), (130, 17395, 5936), (1175, 15938, 8), (1, 13431, 1296), (1, 3567, 2328), (1, 3263, 1168),
+    (898, 1, 8), (791, 3609, 1104), (22312, 129, 5776), (15938, 1175, 8), (33847, 1059, 8),
+]
+
+
+@pytest.mark.parametrize("t,v,k", SIZES + KERNELS)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_forward_sizes(t, v, k, dtype):
     hidden, weight, target, _ = _head(t, v, k, dtype)
     _check_forward(hidden, weight, target)
 
 
-@pytest.mark.parametrize("t,v,k", SIZES)
+@pytest.mark.parametrize("t,v,k", SIZES + KERNELS + BACKWARD_KERNELS)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_backward_sizes(t, v, k, dtype):
     hidden, weight, target, g = _head(t, v, k, dtype, seed=1)
@@ -75,6 +87,38 @@ def test_pieces_of_the_vocabulary(dtype):
     lib = _capi.load()
     assert lib.tf_linear_cross_entropy_backward_workspace_bytes(40000, 8195, 24) < 2 * 40000 * 8195 * 2
     _check_backward(torch.rand(40000, device=DEV, generator=g) / 40000 * (4096 if dtype == torch.float16 else 1), hidden, weight, target)
+
+
+def test_backward_of_some():
+    hidden, weight, target, g = _head(100, 500, 72, torch.bfloat16, seed=11)
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    want = ops.linear_cross_entropy_backward(torch.ones(100, device=DEV), hidden, weight, target, lse)
+    for asked in (0, 1):
+        leaves = [t.clone().requires_grad_(i == asked) for i, t in enumerate((hidden, weight))]
+        ops.linear_cross_entropy(*leaves, target)[0].sum().backward()
+        assert torch.equal(leaves[asked].grad, want[asked]) and leaves[1 - asked].grad is None
+
+
+def test_offsets_that_pass_32_bits():
+    # a table of more than 4 GiB and its gradient; the targets are its last words
+    t, v, k = 70, 600000, 4096
+    g = torch.Generator(device=DEV).manual_seed(12)
+    hidden = torch.randn(t, k, device=DEV, generator=g, dtype=torch.bfloat16)
+    weight = torch.zeros(v, k, device=DEV, dtype=torch.bfloat16)
+    weight[-500:] = torch.randn(500, k, device=DEV, generator=g) * 0.03
+    target = v - 1 - torch.arange(t, device=DEV)
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    z, off = ref.product(hidden, weight[-500:])
+    zeros = torch.full((t, 1), float(torch.tensor(float(v - 500)).double().log()), device=DEV, dtype=torch.float64)   # exp(0), v - 500 times
+    want_lse = torch.logsumexp(torch.cat([z, zeros], 1), 1)
+    bound = off.amax(1) + ref.FN * (1 + want_lse.abs())
+    ref.assert_within(lse, want_lse, bound)
+    ref.assert_within(loss, want_lse - z.gather(1, (target - v + 500)[:, None])[:, 0], 2 * bound)
+    grad_hidden, grad_weight = ops.linear_cross_entropy_backward(torch.ones(t, device=DEV), hidden, weight, target, lse)
+    p = torch.exp(z - want_lse[:, None]) - torch.nn.functional.one_hot(target - v + 500, 500).double()
+    for got, want in ((grad_hidden, p @ weight[-500:].double()), (grad_weight[-500:], p.t().contiguous() @ hidden.double()),
+                      (grad_weight[:3], torch.exp(-want_lse).sum(0) * 0 + (torch.exp(-want_lse)[:, None] * hidden.double()).sum(0).expand(3, k))):
+        assert (got.double() - want).norm() <= 2 * ref.half_step(torch.bfloat16) * want.norm() * 1.5
 
 
 def test_shapes_strides_and_alignment():

@@ -63,10 +63,10 @@ def test_gated_ffn_arguments():
     want = size(64, 64, 64)
     assert b(*[P] * 9, F16, 0, 64, 64, 64, P, want - 1, None) == BAD and b"workspace" in lib.tf_last_error()
     assert b(*[P] * 9, F16, 0, 64, 64, 64, P + 8, want, None) == BAD and b(*[P] * 9, F16, 0, 64, 64, 64, None, want, None) == BAD
-    for at in range(9):
-        pointers = [P] * 9
-        pointers[at] = None
-        assert b(*pointers, F16, 0, 64, 64, 64, P, want, None) == BAD
+    for gone in ([0], [1], [2], [3], [4], [5], [7], [8], [6, 7, 8], [6, 7]):   # (no gradient, or that of one weight)
+        pointers = [None if at in gone else P for at in range(9)]
+        assert b(*pointers, F16, 0, 64, 64, 64, P, want, None) == BAD, gone
+    assert b(*[P + 2] * 9, F16, 0, 64, 64, 64, P, want, None) == BAD and b"boundaries" in lib.tf_last_error()
 
 
 def test_linear_cross_entropy_arguments():
@@ -78,12 +78,12 @@ def test_linear_cross_entropy_arguments():
         assert f(*[P] * n, F32, 8, 100, 64, -100, P, want, None) == UNSUPPORTED
         assert f(*[P] * n, F16, 8, 100, 64, -100, P, want - 1, None) == BAD and b"workspace" in lib.tf_last_error()
         assert f(*[P] * n, F16, 8, 100, 64, -100, P + 4, want, None) == BAD == f(*[P] * n, F16, 8, 100, 64, -100, None, want, None)
-        for sizes in ((-1, 100, 64), (8, 0, 64), (8, 100, 0), (8, 1 << 30, 64), (8, 100, 1 << 22)):
+        for sizes in ((-1, 100, 64), (8, 0, 64), (8, 100, 0), (8, 1 << 28, 64), (8, 100, 1 << 22)):
             assert f(*[P] * n, F16, *sizes, -100, P, want, None) == BAD
-        for at in range(n):
-            pointers = [P] * n
-            pointers[at] = None
-            assert f(*pointers, F16, 8, 100, 64, -100, P, want, None) == BAD
+        for gone in [[at] for at in range(5)] + ([[5, 6]] if n == 7 else []):
+            pointers = [None if at in gone else P for at in range(n)]
+            assert f(*pointers, F16, 8, 100, 64, -100, P, want, None) == BAD, gone
+        assert f(*[P + 2] * n, F16, 8, 100, 64, -100, P, want, None) == BAD and b"boundaries" in lib.tf_last_error()
     assert lib.tf_linear_cross_entropy(*[None] * 5, F16, 0, 100, 64, -100, None, 0, None) == OK
 
 
@@ -110,9 +110,9 @@ def test_schemas():
         "quantize_rows": "(Tensor x, Tensor(a!) q, Tensor(b!) scale) -> ()",
         "gemm_int8": "(Tensor A, Tensor B, Tensor scale_a, Tensor scale_b, Tensor(a!) C) -> ()",
         "gated_ffn": "(Tensor x, Tensor w_gate, Tensor w_up, str activation, Tensor(a!) h, Tensor(b!)? gate, Tensor(c!)? up) -> ()",
-        "gated_ffn_backward": "(Tensor grad_h, Tensor x, Tensor w_gate, Tensor w_up, Tensor gate, Tensor up, str activation, Tensor(a!) grad_x, Tensor(b!) grad_w) -> ()",
+        "gated_ffn_backward": "(Tensor grad_h, Tensor x, Tensor w_gate, Tensor w_up, Tensor gate, Tensor up, str activation, Tensor(a!)? grad_x, Tensor(b!)? grad_w) -> ()",
         "linear_cross_entropy": "(Tensor hidden, Tensor weight, Tensor target, int ignore_index, Tensor(a!) loss, Tensor(b!) lse) -> ()",
-        "linear_cross_entropy_backward": "(Tensor grad_loss, Tensor hidden, Tensor weight, Tensor target, Tensor lse, int ignore_index, Tensor(a!) grad_hidden, Tensor(b!) grad_weight) -> ()",
+        "linear_cross_entropy_backward": "(Tensor grad_loss, Tensor hidden, Tensor weight, Tensor target, Tensor lse, int ignore_index, Tensor(a!)? grad_hidden, Tensor(b!)? grad_weight) -> ()",
     }
     for name, schema in want.items():
         assert str(getattr(torch.ops.tilefusion, name).default._schema) == f"tilefusion::{name}{schema}"
@@ -168,3 +168,53 @@ def test_the_comparison_sees_a_planted_mistake():
         bad[at] = (want[0][at] * by).half()
         with pytest.raises(AssertionError, match="out of bounds"):
             ref.assert_within(bad, want[0], bounds[0] + 0 * want[0])
+
+
+# ---- what a call runs, decided on the host ---------------------------------------------------
+def test_cases_reach_every_kernel():
+    """Every kernel that a call can run is run by a case of the GPU tests."""
+    import tests.test_gpu_gated_ffn as ffn
+    import tests.test_gpu_gemm_int8 as int8
+    import tests.test_gpu_linear_cross_entropy as loss
+    lib = _capi.load()
+
+    def padded(k, to, lines):
+        return k if k % to == 0 else -(-k // lines) * lines
+
+    one = set(range(15))
+    assert {lib.tf_product_kernel_index(m, n, padded(k, 16, 128) // 2, 0) for m, n, k in int8.SIZES + int8.KERNELS} == one
+    assert {lib.tf_product_kernel_index(t, v, padded(k, 8, 64), 0) for t, v, k in loss.SIZES + loss.KERNELS} == one
+    two = {0, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14}
+    assert {lib.tf_product_kernel_index(m, f, padded(k, 8, 64), 1) for m, f, k in ffn.SIZES + ffn.KERNELS} == two
+
+
+def _cols(m, n, rows):
+    parts = ctypes.c_int(0)
+    shape = _capi.load().tf_product_cols_plan(m, n, rows, ctypes.byref(parts))
+    return shape, parts.value > 1
+
+
+def test_cases_reach_every_form_of_a_gradient():
+    import tests.test_gpu_gated_ffn as ffn
+    import tests.test_gpu_linear_cross_entropy as loss
+
+    def up(x):
+        return -(-x // 64) * 64
+
+    every = {(shape, cut) for shape in range(4) for cut in (False, True)}
+    ffn_cases = ffn.BACKWARD_SIZES + ffn.BACKWARD_KERNELS
+    assert {_cols(m, k, 2 * up(f)) for m, f, k in ffn_cases} == every
+    assert {_cols(up(f) + f, k, m) for m, f, k in ffn_cases} == every
+    loss_cases = loss.SIZES + loss.BACKWARD_KERNELS
+    assert {_cols(t, k, up(v)) for t, v, k in loss_cases} == every
+    assert {_cols(up(v), k, t) for t, v, k in loss_cases} == every
+    plan = _capi.load().tf_product_cols_plan
+    assert plan(0, 4, 4, ctypes.byref(ctypes.c_int())) == -1 == plan(4, 4, 4, None) and _capi.load().tf_product_kernel_index(4, 4, 1 << 22, 0) == -1
+
+
+def test_no_plan_has_more_tiles_than_a_launch():
+    lib = _capi.load()
+    tile = [(16, 16), (16, 16), (32, 16), (32, 32), (32, 32), (64, 32), (64, 64)] + [(128, 128)] * 3 + [(192, 128), (192, 192), (256, 128), (256, 192), (256, 256)]
+    for m, n in ((1, (1 << 28) - 64), (16, (1 << 28) - 64), (100, (1 << 28) - 64), (1 << 20, 16), ((1 << 22) - 64, 64)):
+        bm, bn = tile[lib.tf_product_kernel_index(m, n, 64, 0)]
+        assert -(-m // bm) * -(-n // bn) < 1 << 23, (m, n)

@@ -52,6 +52,8 @@ SIGNATURES = {
     "tf_linear_cross_entropy": (_i, [_vp] * 5 + [_i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "tf_linear_cross_entropy_backward_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "tf_linear_cross_entropy_backward": (_i, [_vp] * 7 + [_i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "tf_product_kernel_index": (_i, [_i64, _i64, _i64, _i]),
+    "tf_product_cols_plan": (_i, [_i64, _i64, _i64, ctypes.POINTER(_i)]),
     "tf_gemm_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_flash_decode_plan": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_i)]),
     "tf_flash_attention_rows": (_i, [_i64, _i64, _i64, _i64, _i]),

@@ -323,7 +323,7 @@ PyObject* gated_ffn_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   at::Tensor t[6], grad_x, grad_w;
   c10::string_view activation;
   using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, c10::string_view,
-                  at::Tensor&, at::Tensor&);
+                  const std::optional<at::Tensor>&, const std::optional<at::Tensor>&);
   static const auto op = find_op<Op>("tilefusion::gated_ffn_backward");
   if (nargs != 7 || !plain(op, args, 6, t) || !matrices(t, 6) || !text(args[6], &activation)) Py_RETURN_NONE;
   const at::Tensor &x = t[1], &w = t[2];
@@ -346,7 +346,8 @@ PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssi
   HANDLE_TH_ERRORS
   at::Tensor t[5], grad_hidden, grad_weight;
   int64_t ignore_index;
-  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, at::Tensor&, at::Tensor&);
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, const std::optional<at::Tensor>&,
+                  const std::optional<at::Tensor>&);
   static const auto op = find_op<Op>("tilefusion::linear_cross_entropy_backward");
   if (nargs != 6 || !plain(op, args, 5, t) || !vectors(t, 1) || !matrices(t + 1, 2) || !vectors(t + 3, 2) || !ints(args + 5, 1, &ignore_index))
     Py_RETURN_NONE;

@@ -223,6 +223,7 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
                        void* dw_up, int activation, int64_t M, int64_t F, int64_t K, char* ws, hipStream_t st) {
   constexpr const char* who = "tf_gated_ffn_backward";
   if (M == 0) {
+    if (dw_gate == nullptr) return TF_OK;
     if (int rc = launch_zero_16bit(dw_gate, F * K, st)) return rc;
     return launch_zero_16bit(dw_up, F * K, st);
   }
@@ -237,14 +238,14 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
     return rc;
   RowsToCopy copies[3];
   int count = 0;
-  if (p.copy_weights) {
+  if (p.copy_weights && dx != nullptr) {
     char* const to = ws + p.weights;
     copies[count++] = {w_gate, F, to, p.Fp};
     copies[count++] = {w_up, F, to + 2 * p.Fp * p.Kp, p.Fp};
     w_gate = to;
     w_up = to + 2 * p.Fp * p.Kp;
   }
-  if (p.copy_x) {
+  if (p.copy_x && dw_gate != nullptr) {
     copies[count++] = {x, M, ws + p.x, M};
     x = ws + p.x;
   }
@@ -255,13 +256,16 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
   const uint16_t* const grads_at = bits(ws);
   const ColsProduct of_x = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)M}, {bits(w_gate), p.Kp, (int)p.Kp, (int)K}, bits(w_up), (int)(p.Fp / 64), (int)(2 * p.Fp / 64), 0, 0};
   T* const to_x = static_cast<T*>(dx);
-  if (p.of_x.splits == 1) {
+  if (dx == nullptr) {
+    // not asked for
+  } else if (p.of_x.splits == 1) {
     if (int rc = launch_cols<T, false>(who, of_x, p.of_x, WholeEpilogue<T>{to_x, nullptr, (int)M, (int)K}, st)) return rc;
   } else {
     const PartsRoom room(p.of_x, M, K);
     if (int rc = launch_cols<T, false>(who, of_x, p.of_x, PartEpilogue{parts, room.rows, room.pitch, false}, st)) return rc;
     if (int rc = launch_sum_parts<T>(parts, room, p.of_x.splits, 0, M, K, to_x, nullptr, st)) return rc;
   }
+  if (dw_gate == nullptr) return TF_OK;
   const int m_tiles = (int)tiles_of(M, 64), m_pad = (int)(m_tiles * 64 - M);
   const ColsOperand tokens = {bits(x), p.Kp, (int)p.Kp, (int)K};
   const ColsProduct of_w = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)(p.Fp + F)}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
@@ -323,9 +327,10 @@ extern "C" int tf_gated_ffn_backward(const void* dh, const void* x, const void* 
                                      size_t workspace_bytes, void* stream) {
   using namespace tfk;
   if (int rc = check_sizes("tf_gated_ffn_backward", dtype, activation, M, F, K)) return rc;
-  TFK_REQUIRE(dw_gate && dw_up, TF_ERR_INVALID_ARG, "tf_gated_ffn_backward: null pointer");
+  TFK_REQUIRE((dw_gate == nullptr) == (dw_up == nullptr) && (dx || dw_gate), TF_ERR_INVALID_ARG,
+              "tf_gated_ffn_backward: the gradients of both weights or of neither, and of something");
   if (M > 0) {
-    TFK_REQUIRE(dh && x && w_gate && w_up && gate && up && dx, TF_ERR_INVALID_ARG, "tf_gated_ffn_backward: null pointer");
+    TFK_REQUIRE(dh && x && w_gate && w_up && gate && up, TF_ERR_INVALID_ARG, "tf_gated_ffn_backward: null pointer");
     TFK_REQUIRE(K % 8 != 0 || (at_16B(x) && at_16B(w_gate) && at_16B(w_up)), TF_ERR_INVALID_ARG,
                 "tf_gated_ffn_backward: x and the weights must begin at 16-byte boundaries");
     const size_t want = BackwardPlan(M, F, K).bytes;

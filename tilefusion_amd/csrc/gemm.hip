@@ -484,7 +484,7 @@ int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed) {
     const GemmKernel& g = kGemmKernels[i];
     if (!(allowed >> i & 1) || (g.ring && (M < g.bm || N < g.bn || K < 64))) continue;
     const int64_t tiles = ((M + g.bm - 1) / g.bm) * ((N + g.bn - 1) / g.bn);
-    if (tiles < g.min_tiles || tiles > g.max_tiles) continue;
+    if (tiles < g.min_tiles || tiles > std::min(g.max_tiles, kMaxTiles)) continue;
     const float us = expected_us(g, tiles, ktiles, K % 64 != 0, nullptr);
     if (us < best_us) {
       best = i;
@@ -576,4 +576,16 @@ extern "C" int tf_gemm(const void* A, const void* B, void* C, int dtype, int c_i
 extern "C" int tf_gemm_kernel_index(int64_t M, int64_t N, int64_t K, int c_is_f32) {
   if (M <= 0 || N <= 0 || K <= 0 || M >= (1 << 30) || N >= (1 << 30) || K >= (1 << 22)) return -1;
   return tfk::pick_gemm_kernel((int)M, (int)N, (int)K, c_is_f32 != 0);
+}
+
+extern "C" int tf_product_kernel_index(int64_t M, int64_t N, int64_t K, int two) {
+  if (M <= 0 || N <= 0 || K <= 0 || M >= (1 << 30) || N >= (1 << 30) || K >= (1 << 22)) return -1;
+  return tfk::plan_product(M, N, K, two != 0).kernel;
+}
+
+extern "C" int tf_product_cols_plan(int64_t M, int64_t N, int64_t rows, int* parts) {
+  if (M <= 0 || N <= 0 || rows <= 0 || parts == nullptr) return -1;
+  const tfk::ColsPlan plan = tfk::plan_cols(M, N, tfk::tiles_of(rows, 64));
+  *parts = plan.splits;
+  return plan.shape;
 }

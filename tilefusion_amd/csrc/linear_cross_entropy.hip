@@ -268,7 +268,7 @@ template <typename T>
 int backward(const float* grad_loss, const void* hidden, const void* weight, const int64_t* target, const float* lse, void* grad_hidden,
              void* grad_weight, int64_t tokens, int64_t V, int64_t K, int64_t ignore_index, char* ws, hipStream_t st) {
   constexpr const char* who = "tf_linear_cross_entropy_backward";
-  if (tokens == 0) return launch_zero_16bit(grad_weight, V * K, st);
+  if (tokens == 0) return grad_weight != nullptr ? launch_zero_16bit(grad_weight, V * K, st) : TF_OK;
   const BackwardPlan plan(tokens, V, K);
   T* const p = reinterpret_cast<T*>(ws);
   constexpr bool kScaled = std::is_same_v<T, half_t>;
@@ -304,21 +304,25 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
       return rc;
 
     // dH += P * W
-    ColsPlan of_hidden = plan.of_hidden;
-    of_hidden.per_split = (int)tiles_of(pitch / 64, of_hidden.splits);
-    const int split_parts = (int)tiles_of(pitch / 64, of_hidden.per_split);   // (a short last piece may have fewer)
-    of_hidden.splits = split_parts;
-    const ColsProduct hidden_product = {{bits(p), pitch, (int)pitch, (int)tokens}, {bits(w), width, width, (int)K}, bits(w), INT_MAX, (int)(pitch / 64), pad, 0};
-    int rc;
-    if (plan.pieces == 1 && plan.of_hidden.splits == 1)
-      rc = launch_cols<T, false>(who, hidden_product, of_hidden, WholeEpilogue<T>{static_cast<T*>(grad_hidden), scale, (int)tokens, (int)K}, st);
-    else
-      rc = launch_cols<T, false>(who, hidden_product, of_hidden, PartEpilogue{hidden_parts, hidden_room.rows, hidden_room.pitch, first > 0}, st);
-    if (rc) return rc;
+    if (grad_hidden != nullptr) {
+      ColsPlan of_hidden = plan.of_hidden;
+      of_hidden.per_split = (int)tiles_of(pitch / 64, of_hidden.splits);
+      const int split_parts = (int)tiles_of(pitch / 64, of_hidden.per_split);   // (a short last piece may have fewer)
+      of_hidden.splits = split_parts;
+      const ColsProduct hidden_product = {{bits(p), pitch, (int)pitch, (int)tokens}, {bits(w), width, width, (int)K}, bits(w), INT_MAX, (int)(pitch / 64), pad, 0};
+      int rc;
+      if (plan.pieces == 1 && plan.of_hidden.splits == 1)
+        rc = launch_cols<T, false>(who, hidden_product, of_hidden, WholeEpilogue<T>{static_cast<T*>(grad_hidden), scale, (int)tokens, (int)K}, st);
+      else
+        rc = launch_cols<T, false>(who, hidden_product, of_hidden, PartEpilogue{hidden_parts, hidden_room.rows, hidden_room.pitch, first > 0}, st);
+      if (rc) return rc;
+    }
 
     // dW = P^T * H: the columns of P in front of the piece's are rows that are not stored
+    if (grad_weight == nullptr) continue;
     const ColsProduct weight_product = {{bits(p), pitch, (int)pitch, (int)pitch}, of_tokens, of_tokens.x, INT_MAX, t_tiles, t_pad, pad};
     T* const out = static_cast<T*>(grad_weight) + first * K;
+    int rc;
     if (plan.of_weight.splits == 1) {
       rc = launch_cols<T, true>(who, weight_product, plan.of_weight, WholeEpilogue<T>{out - (int64_t)pad * K, scale, (int)pitch, (int)K}, st);
     } else {
@@ -327,14 +331,14 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
     }
     if (rc) return rc;
   }
-  if (plan.pieces == 1 && plan.of_hidden.splits == 1) return TF_OK;
+  if (grad_hidden == nullptr || (plan.pieces == 1 && plan.of_hidden.splits == 1)) return TF_OK;
   return launch_sum_parts<T>(hidden_parts, hidden_room, plan.of_hidden.splits, 0, tokens, K, static_cast<T*>(grad_hidden), scale, st);
 }
 
 int check_sizes(const char* who, int dtype, int64_t T, int64_t V, int64_t K) {
   TFK_REQUIRE(dtype == TF_DTYPE_F16 || dtype == TF_DTYPE_BF16, TF_ERR_UNSUPPORTED, "%s: dtype must be TF_DTYPE_F16 or TF_DTYPE_BF16", who);
   TFK_REQUIRE(T >= 0 && V > 0 && K > 0, TF_ERR_INVALID_ARG, "%s: T must not be negative, V and K must be positive", who);
-  TFK_REQUIRE(T <= (1 << 22) - 64 && V <= (1 << 30) - 64 && K <= (1 << 22) - 64, TF_ERR_INVALID_ARG, "%s: dimension too large", who);
+  TFK_REQUIRE(T <= (1 << 22) - 64 && V <= (1 << 28) - 64 && K <= (1 << 22) - 64, TF_ERR_INVALID_ARG, "%s: dimension too large", who);
   return TF_OK;
 }
 
@@ -375,9 +379,9 @@ extern "C" int tf_linear_cross_entropy_backward(const float* grad_loss, const vo
                                                 void* workspace, size_t workspace_bytes, void* stream) {
   using namespace tfk;
   if (int rc = check_sizes("tf_linear_cross_entropy_backward", dtype, T, V, K)) return rc;
-  TFK_REQUIRE(grad_weight, TF_ERR_INVALID_ARG, "tf_linear_cross_entropy_backward: null pointer");
+  TFK_REQUIRE(grad_weight || grad_hidden, TF_ERR_INVALID_ARG, "tf_linear_cross_entropy_backward: no gradient asked for");
   if (T > 0) {
-    TFK_REQUIRE(grad_loss && hidden && weight && target && lse && grad_hidden, TF_ERR_INVALID_ARG,
+    TFK_REQUIRE(grad_loss && hidden && weight && target && lse, TF_ERR_INVALID_ARG,
                 "tf_linear_cross_entropy_backward: null pointer");
     TFK_REQUIRE(K % 8 != 0 || (at_16B(hidden) && at_16B(weight)), TF_ERR_INVALID_ARG,
                 "tf_linear_cross_entropy_backward: hidden and weight must begin at 16-byte boundaries");

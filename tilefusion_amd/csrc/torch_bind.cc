@@ -493,9 +493,11 @@ void gated_ffn(const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& 
                op);
 }
 
-// gated_ffn_backward(grad_h [M,F], x [M,K], w_gate, w_up [F,K], gate, up [M,F] -> grad_x [M,K], grad_w [2F,K]: gate's rows, then up's)
+// gated_ffn_backward(grad_h [M,F], x [M,K], w_gate, w_up [F,K], gate, up [M,F] -> grad_x [M,K], grad_w [2F,K]: gate's rows, then up's), the
+// gradients that are given
 void gated_ffn_backward(const at::Tensor& grad_h, const at::Tensor& x, const at::Tensor& w_gate, const at::Tensor& w_up, const at::Tensor& gate,
-                        const at::Tensor& up, c10::string_view activation, at::Tensor& grad_x, at::Tensor& grad_w) {
+                        const at::Tensor& up, c10::string_view activation, const std::optional<at::Tensor>& grad_x,
+                        const std::optional<at::Tensor>& grad_w) {
   constexpr const char* op = "gated_ffn_backward";
   check_operand(x, "x", x, op);
   const int dtype = operand_dtype(x, op);
@@ -503,20 +505,24 @@ void gated_ffn_backward(const at::Tensor& grad_h, const at::Tensor& x, const at:
   const int64_t m = x.size(0), k = x.size(1), f = w_gate.size(0);
   const struct { const at::Tensor& t; const char* name; int64_t rows, cols; } operands[] = {
       {grad_h, "grad_h", m, f}, {w_gate, "w_gate", f, k}, {w_up, "w_up", f, k}, {gate, "gate", m, f},
-      {up, "up", m, f}, {grad_x, "grad_x", m, k}, {grad_w, "grad_w", 2 * f, k}};
+      {up, "up", m, f}, {grad_x.has_value() ? *grad_x : x, "grad_x", m, k}};
   for (const auto& o : operands) {
     check_like(o.t, o.name, x, op);
     check_sizes(o.t, o.name, o.rows, o.cols, op);
+  }
+  if (grad_w.has_value()) {
+    check_like(*grad_w, "grad_w", x, op);
+    check_sizes(*grad_w, "grad_w", 2 * f, k, op);
   }
   const int act = activation_code(activation, op);
   const c10::DeviceGuard there(x.device());
   const size_t bytes = tf_gated_ffn_backward_workspace_bytes(m, f, k);
   c10::DataPtr ws;
   if (bytes > 0) ws = scratch(bytes, x);
-  char* const to = static_cast<char*>(grad_w.data_ptr());
+  char* const to = grad_w.has_value() ? static_cast<char*>(grad_w->data_ptr()) : nullptr;
   const at::Tensor from = at_boundary(x), of_gate = at_boundary(w_gate), of_up = at_boundary(w_up);
   check_status(tf_gated_ffn_backward(grad_h.data_ptr(), from.data_ptr(), of_gate.data_ptr(), of_up.data_ptr(), gate.data_ptr(), up.data_ptr(),
-                                     grad_x.data_ptr(), to, to + 2 * f * k, dtype, act, m, f, k, ws.get(), bytes, current_stream()),
+                                     grad_x.has_value() ? grad_x->data_ptr() : nullptr, to, to != nullptr ? to + 2 * f * k : nullptr, dtype, act, m, f, k, ws.get(), bytes, current_stream()),
                op);
 }
 
@@ -543,16 +549,19 @@ void linear_cross_entropy(const at::Tensor& hidden, const at::Tensor& weight, co
                op);
 }
 
-// linear_cross_entropy_backward(grad_loss [T] fp32, hidden, weight, target, lse [T] fp32 -> grad_hidden [T,K], grad_weight [V,K])
+// linear_cross_entropy_backward(grad_loss [T] fp32, hidden, weight, target, lse [T] fp32 -> grad_hidden [T,K], grad_weight [V,K]), the
+// gradients that are given
 void linear_cross_entropy_backward(const at::Tensor& grad_loss, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& target,
-                                   const at::Tensor& lse, int64_t ignore_index, at::Tensor& grad_hidden, at::Tensor& grad_weight) {
+                                   const at::Tensor& lse, int64_t ignore_index, const std::optional<at::Tensor>& grad_hidden,
+                                   const std::optional<at::Tensor>& grad_weight) {
   constexpr const char* op = "linear_cross_entropy_backward";
   check_operand(hidden, "hidden", hidden, op);
   const int dtype = operand_dtype(hidden, op);
   TORCH_CHECK(hidden.dim() == 2 && weight.dim() == 2, "tilefusion::", op, ": hidden must be [T, K], weight [V, K].");
   const int64_t t = hidden.size(0), k = hidden.size(1), v = weight.size(0);
   const struct { const at::Tensor& t; const char* name; int64_t rows, cols; } operands[] = {
-      {weight, "weight", v, k}, {grad_hidden, "grad_hidden", t, k}, {grad_weight, "grad_weight", v, k}};
+      {weight, "weight", v, k}, {grad_hidden.has_value() ? *grad_hidden : hidden, "grad_hidden", t, k},
+      {grad_weight.has_value() ? *grad_weight : weight, "grad_weight", v, k}};
   for (const auto& o : operands) {
     check_like(o.t, o.name, hidden, op);
     check_sizes(o.t, o.name, o.rows, o.cols, op);
@@ -566,7 +575,8 @@ void linear_cross_entropy_backward(const at::Tensor& grad_loss, const at::Tensor
   if (bytes > 0) ws = scratch(bytes, hidden);
   const at::Tensor rows = at_boundary(hidden), table = at_boundary(weight);
   check_status(tf_linear_cross_entropy_backward(grad_loss.data_ptr<float>(), rows.data_ptr(), table.data_ptr(), target.data_ptr<int64_t>(),
-                                                lse.data_ptr<float>(), grad_hidden.data_ptr(), grad_weight.data_ptr(), dtype, t, v, k, ignore_index,
+                                                lse.data_ptr<float>(), grad_hidden.has_value() ? grad_hidden->data_ptr() : nullptr,
+                                                grad_weight.has_value() ? grad_weight->data_ptr() : nullptr, dtype, t, v, k, ignore_index,
                                                 ws.get(), bytes, current_stream()),
                op);
 }
@@ -639,7 +649,7 @@ REGISTER_OP(gated_ffn,
             &kernels::gated_ffn);
 REGISTER_OP(gated_ffn_backward,
             "gated_ffn_backward(Tensor grad_h, Tensor x, Tensor w_gate, Tensor w_up, Tensor gate, Tensor up, "
-            "str activation, Tensor(a!) grad_x, Tensor(b!) grad_w) -> ()",
+            "str activation, Tensor(a!)? grad_x, Tensor(b!)? grad_w) -> ()",
             &kernels::gated_ffn_backward);
 REGISTER_OP(linear_cross_entropy,
             "linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target, int ignore_index, "
@@ -647,7 +657,7 @@ REGISTER_OP(linear_cross_entropy,
             &kernels::linear_cross_entropy);
 REGISTER_OP(linear_cross_entropy_backward,
             "linear_cross_entropy_backward(Tensor grad_loss, Tensor hidden, Tensor weight, Tensor target, Tensor lse, "
-            "int ignore_index, Tensor(a!) grad_hidden, Tensor(b!) grad_weight) -> ()",
+            "int ignore_index, Tensor(a!)? grad_hidden, Tensor(b!)? grad_weight) -> ()",
             &kernels::linear_cross_entropy_backward);
 
 TORCH_LIBRARY(tilefusion, m) { KernelRegistry::instance().register_with_torch(m); }

@@ -29,6 +29,37 @@ def _forward(
     return tuple(t.reshape(shape) for t in out)
 
 
+def _backward(
+    grad_h: torch.Tensor,
+    x: torch.Tensor,
+    w_gate: torch.Tensor,
+    w_up: torch.Tensor,
+    gate: torch.Tensor,
+    up: torch.Tensor,
+    activation: str,
+    of_x: bool,
+    of_weights: bool,
+) -> Tuple[Any, ...]:
+    """The gradients that are asked for, None in the place of the others."""
+    if w_gate.dim() != 2 or w_up.dim() != 2:
+        raise RuntimeError("gated_ffn_backward: w_gate and w_up must be [F, K]")
+    f, k = w_gate.shape
+    rows = _rows(x, k, "x", "gated_ffn_backward")
+    grad_h, gate, up = (
+        _rows(t, f, name, "gated_ffn_backward") for t, name in ((grad_h, "grad_h"), (gate, "gate"), (up, "up"))
+    )
+    grad_x = torch.empty_like(rows) if of_x else None
+    grad_w = torch.empty(2 * f, k, dtype=x.dtype, device=x.device) if of_weights else None
+    with torch.no_grad():
+        torch.ops.tilefusion.gated_ffn_backward(
+            grad_h, rows, w_gate.contiguous(), w_up.contiguous(), gate, up, activation, grad_x, grad_w
+        )
+    return (
+        grad_x.reshape(x.shape) if grad_x is not None else None,
+        *((grad_w[:f], grad_w[f:]) if grad_w is not None else (None, None)),
+    )
+
+
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str) -> Tuple[torch.Tensor, ...]:
@@ -41,7 +72,8 @@ class _GatedFfn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_h: torch.Tensor, *_: Any) -> Tuple[Any, ...]:
-        return (*gated_ffn_backward(grad_h, *ctx.saved_tensors, ctx.activation), None)
+        of_x, of_gate, of_up, _ = ctx.needs_input_grad
+        return (*_backward(grad_h, *ctx.saved_tensors, ctx.activation, of_x, of_gate or of_up), None)
 
 
 def gated_ffn(
@@ -85,17 +117,4 @@ def gated_ffn_backward(
         direct = _direct.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation)
         if direct is not None:
             return direct[0], direct[1][0], direct[1][1]
-    if w_gate.dim() != 2 or w_up.dim() != 2:
-        raise RuntimeError("gated_ffn_backward: w_gate and w_up must be [F, K]")
-    f, k = w_gate.shape
-    rows = _rows(x, k, "x", "gated_ffn_backward")
-    grad_h, gate, up = (
-        _rows(t, f, name, "gated_ffn_backward") for t, name in ((grad_h, "grad_h"), (gate, "gate"), (up, "up"))
-    )
-    grad_x = torch.empty_like(rows)
-    grad_w = torch.empty(2, f, k, dtype=x.dtype, device=x.device)
-    with torch.no_grad():
-        torch.ops.tilefusion.gated_ffn_backward(
-            grad_h, rows, w_gate.contiguous(), w_up.contiguous(), gate, up, activation, grad_x, grad_w.view(2 * f, k)
-        )
-    return grad_x.reshape(x.shape), grad_w[0], grad_w[1]
+    return _backward(grad_h, x, w_gate, w_up, gate, up, activation, True, True)

@@ -32,6 +32,30 @@ def _forward(
     return loss.reshape(target.shape), lse.reshape(target.shape)
 
 
+def _backward(
+    grad_loss: torch.Tensor,
+    hidden: torch.Tensor,
+    weight: torch.Tensor,
+    target: torch.Tensor,
+    lse: torch.Tensor,
+    ignore_index: int,
+    of_hidden: bool,
+    of_weight: bool,
+) -> Tuple[Any, Any]:
+    """The gradients that are asked for, None in the place of the others."""
+    rows, table, words = _operands(hidden, weight, target, "linear_cross_entropy_backward")
+    for name, t in (("grad_loss", grad_loss), ("lse", lse)):
+        if t.shape != target.shape:
+            raise RuntimeError(f"linear_cross_entropy_backward: {name} must be {list(target.shape)}, got {list(t.shape)}")
+    grad_hidden = torch.empty_like(rows) if of_hidden else None
+    grad_weight = torch.empty_like(table) if of_weight else None
+    with torch.no_grad():
+        torch.ops.tilefusion.linear_cross_entropy_backward(
+            grad_loss.reshape(-1).contiguous(), rows, table, words, lse.reshape(-1).contiguous(), ignore_index, grad_hidden, grad_weight
+        )
+    return grad_hidden.reshape(hidden.shape) if grad_hidden is not None else None, grad_weight
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(
@@ -46,7 +70,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_loss: torch.Tensor, _: Any) -> Tuple[Any, ...]:
-        return (*linear_cross_entropy_backward(grad_loss, *ctx.saved_tensors, ctx.ignore_index), None, None)
+        of_hidden, of_weight, _, _ = ctx.needs_input_grad
+        return (*_backward(grad_loss, *ctx.saved_tensors, ctx.ignore_index, of_hidden, of_weight), None, None)
 
 
 def linear_cross_entropy(
@@ -90,13 +115,4 @@ def linear_cross_entropy_backward(
         direct = _direct.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index)
         if direct is not None:
             return direct
-    rows, table, words = _operands(hidden, weight, target, "linear_cross_entropy_backward")
-    for name, t in (("grad_loss", grad_loss), ("lse", lse)):
-        if t.shape != target.shape:
-            raise RuntimeError(f"linear_cross_entropy_backward: {name} must be {list(target.shape)}, got {list(t.shape)}")
-    grad_hidden, grad_weight = torch.empty_like(rows), torch.empty_like(table)
-    with torch.no_grad():
-        torch.ops.tilefusion.linear_cross_entropy_backward(
-            grad_loss.reshape(-1).contiguous(), rows, table, words, lse.reshape(-1).contiguous(), ignore_index, grad_hidden, grad_weight
-        )
-    return grad_hidden.reshape(hidden.shape), grad_weight
+    return _backward(grad_loss, hidden, weight, target, lse, ignore_index, True, True)
