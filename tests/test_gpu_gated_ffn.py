@@ -42,7 +42,7 @@ SIZES = [
 # sizes that reach the kernels which those do not (tests/test_products_cpu.py looks)
 KERNELS = [
     (35, 350, 64), (17, 1, 64), (37, 3004, 1984), (42, 3635, 728), (226, 2781, 448), (358, 1620, 72), (567, 5492, 64), (271, 5523, 64), (396, 5528, 72),
-    (658, 5679, 64),
+    (658, 5679, 64), (34, 14236, 72), (127, 10001, 520), (33, 25751, 72), (100, 25801, 65),
 ]
 
 

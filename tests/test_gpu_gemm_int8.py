@@ -41,6 +41,7 @@ SIZES = [
 KERNELS = [
     (1, 1, 528), (889, 172, 144), (179, 583, 128), (334, 438, 144), (381, 792, 3968), (162, 2558, 1824), (746, 1748, 896), (358, 3187, 144), (2835, 5627, 192),
     (1670, 2341, 128), (2120, 3587, 144), (1018, 5500, 128), (1974, 4508, 128), (2103, 5383, 144),
+    (108, 12711, 144), (127, 20000, 1040), (33, 55674, 144), (100, 55673, 17),
 ]
 
 

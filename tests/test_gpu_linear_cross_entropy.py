@@ -55,7 +55,8 @@ SIZES = [
 # sizes that reach the kernels which those do not (tests/test_products_cpu.py looks)
 KERNELS = [
     (1, 1, 264), (1883, 67, 72), (1752, 50, 64), (2319, 49, 72), (354, 855, 2048), (2411, 173, 712), (480, 2674, 448), (197, 5649, 72), (2891, 5564, 80),
-    (898, 4350, 64), (2865, 2786, 64), (967, 5420, 72), (2925, 3106, 64), (2206, 5545, 64),
+    (898, 4350, 64), (2865, 2786, 64), (967, 5420, 72), (2925, 3106, 64), (2206, 5545, 64), (65, 17495, 80), (127, 30001, 264), (38, 54305, 72),
+    (100, 54305, 65),
 ]
 # and the tiles, and sums in parts, of gradients
 BACKWARD_KERNELS = [

@@ -181,10 +181,10 @@ def test_cases_reach_every_kernel():
     def padded(k, to, lines):
         return k if k % to == 0 else -(-k // lines) * lines
 
-    one = set(range(15))
+    one = set(range(17))
     assert {lib.tf_product_kernel_index(m, n, padded(k, 16, 128) // 2, 0) for m, n, k in int8.SIZES + int8.KERNELS} == one
     assert {lib.tf_product_kernel_index(t, v, padded(k, 8, 64), 0) for t, v, k in loss.SIZES + loss.KERNELS} == one
-    two = {0, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14}
+    two = {0, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14, 15, 16}
     assert {lib.tf_product_kernel_index(m, f, padded(k, 8, 64), 1) for m, f, k in ffn.SIZES + ffn.KERNELS} == two
 
 
@@ -214,7 +214,7 @@ def test_cases_reach_every_form_of_a_gradient():
 
 def test_no_plan_has_more_tiles_than_a_launch():
     lib = _capi.load()
-    tile = [(16, 16), (16, 16), (32, 16), (32, 32), (32, 32), (64, 32), (64, 64)] + [(128, 128)] * 3 + [(192, 128), (192, 192), (256, 128), (256, 192), (256, 256)]
+    tile = [(16, 16), (16, 16), (32, 16), (32, 32), (32, 32), (64, 32), (64, 64)] + [(128, 128)] * 3 + [(192, 128), (192, 192), (256, 128), (256, 192), (256, 256), (128, 128), (128, 128)]
     for m, n in ((1, (1 << 28) - 64), (16, (1 << 28) - 64), (100, (1 << 28) - 64), (1 << 20, 16), ((1 << 22) - 64, 64)):
         bm, bn = tile[lib.tf_product_kernel_index(m, n, 64, 0)]
         assert -(-m // bm) * -(-n // bn) < 1 << 23, (m, n)

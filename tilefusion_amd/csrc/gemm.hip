@@ -475,7 +475,7 @@ int pick_gemm_kernel(int M, int N, int K, bool c_is_f32) {
 
 }  // namespace
 
-int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed) {
+int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed, float* expected) {
   int best = 0;
   float best_us = INFINITY;
   const int ktiles = (int)((K + 63) / 64);
@@ -491,10 +491,13 @@ int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed) {
       best_us = us;
     }
   }
+  *expected = best_us;
   return best;
 }
 
-float expected_table_us(int kernel, int64_t tiles, int64_t k_tiles) { return expected_us(kGemmKernels[kernel], tiles, (int)k_tiles, false, nullptr); }
+float expected_table_us(int kernel, int64_t tiles, int64_t K) {
+  return expected_us(kGemmKernels[kernel], tiles, (int)((K + 63) / 64), K % 64 != 0, nullptr);
+}
 
 namespace {
 

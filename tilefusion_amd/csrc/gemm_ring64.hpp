@@ -138,9 +138,10 @@ __device__ const uint4_t kZeros[1] = {};   // what the chunks in front of a row 
 // InT is half_t, bf16_t or int8_t: they differ in the MFMA mnemonic, everything else moves 16 bits at a time without looking at them.
 // K counts these: half the elements of 8 bits.  int8_t: the accumulators are int32.
 // kTwo: the tile's columns alternate between rows of B and of B1 in blocks of 16, from row n0 of either on, BN / 2 of each.
-template <typename S, typename InT, bool kTwo = false>
+// kFew: A has only `rows` < BM rows (m0 = 0); what lies behind them in the tile is the last one again.
+template <typename S, typename InT, bool kTwo = false, bool kFew = false>
 TFK_DEVICE void ring64_multiply(const uint16_t* A, const uint16_t* B, const uint16_t* B1, int K, int m0, int n0, int lane, int wave, char* smem,
-                                float4_t (&acc)[S::TM][S::TN]) {
+                                float4_t (&acc)[S::TM][S::TN], int rows = 0) {
   const int wm = wave / S::WAVES_N, wn = wave % S::WAVES_N;
   // global -> LDS plan: request n of a wavefront covers rows (wave * kLoads + n) * 8 .. +7 of a
   // unit (consecutive 1 KiB blocks of LDS, so four requests share one M0 base and differ in the
@@ -164,15 +165,17 @@ TFK_DEVICE void ring64_multiply(const uint16_t* A, const uint16_t* B, const uint
     return (int)((in_line - (unsigned)pad_chunks - 1u) & 7u) + 1;
   };
   const int a_shift = shift_of(A, m0 + ld_row), b_shift = shift_of(B, n0 + ld_row);   // of the rows that this lane fetches
-  const char* a_tile = reinterpret_cast<const char*>(A + (size_t)(m0 + wave * 8 * S::kLoadsA) * K) - (kShift ? kLead : 2 * k_pad);
+  // (kTwo, kFew: offsets are counted from kLeadFar bytes in front: what an immediate offset takes off may be more than a row has)
+  constexpr int kLeadFar = 4096;
+  const char* a_tile = kFew ? reinterpret_cast<const char*>(A) - 2 * k_pad - kLeadFar
+                            : reinterpret_cast<const char*>(A + (size_t)(m0 + wave * 8 * S::kLoadsA) * K) - (kShift ? kLead : 2 * k_pad);
   // kTwo: block 2 * j of 16 rows of the unit are rows of B, block 2 * j + 1 the same rows of B1; a request's 8 rows are of one
-  // of them.  (Offsets are counted from kLeadTwo bytes in front: what an immediate offset takes off may be more than a row has.)
-  constexpr int kLeadTwo = 4096;
-  const char* b_tile = kTwo ? reinterpret_cast<const char*>(B + (size_t)(n0 + wave * 4 * S::kLoadsB) * K) - 2 * k_pad - kLeadTwo
+  // of them.
+  const char* b_tile = kTwo ? reinterpret_cast<const char*>(B + (size_t)(n0 + wave * 4 * S::kLoadsB) * K) - 2 * k_pad - kLeadFar
                             : reinterpret_cast<const char*>(B + (size_t)(n0 + wave * 8 * S::kLoadsB) * K) - (kShift ? kLead : 2 * k_pad);
-  const char* b1_tile = kTwo ? reinterpret_cast<const char*>(B1 + (size_t)(n0 + wave * 4 * S::kLoadsB) * K) - 2 * k_pad - kLeadTwo : nullptr;
+  const char* b1_tile = kTwo ? reinterpret_cast<const char*>(B1 + (size_t)(n0 + wave * 4 * S::kLoadsB) * K) - 2 * k_pad - kLeadFar : nullptr;
   unsigned g_off[S::kLoadsMax];
-  constexpr bool kOwnOffsetsB = S::kOwnOffsetsB || kTwo;
+  constexpr bool kOwnOffsetsB = S::kOwnOffsetsB || kTwo || kFew;
   unsigned g_off_b[kOwnOffsetsB ? S::kLoadsB : 1];
   // (an odd number of requests: every other wavefront's rows begin in the middle of the swizzle's sixteen)
   const int a_odd = S::kLoadsA % 2 ? wave & 1 : 0;
@@ -190,11 +193,18 @@ TFK_DEVICE void ring64_multiply(const uint16_t* A, const uint16_t* B, const uint
   for (int n = 0; n < S::kLoadsMax; ++n)
     g_off[n] = kShift ? segment_off(n, a_odd, a_shift)
                       : tile_off(n, a_odd);
+  if constexpr (kFew) {
+    static_assert(S::kLines == 0 && S::kLoadsA % 2 == 0, "");
+#pragma unroll
+    for (int n = 0; n < S::kLoadsA; ++n)
+      g_off[n] = (unsigned)min(wave * 8 * S::kLoadsA + ld_row + 8 * n, rows - 1) * (unsigned)K * 2u + (unsigned)S::swizzle(ld_row + 8 * n, ld_c) * 16u +
+                 kLeadFar - 1024u * (n % 4);
+  }
   if constexpr (kTwo) {
     static_assert(S::kLines == 0 && S::kLoadsB % 4 == 0, "a wavefront's requests begin with a block of B");
 #pragma unroll
     for (int n = 0; n < S::kLoadsB; ++n)
-      g_off_b[n] = (unsigned)(ld_row + n / 4 * 16 + n % 2 * 8) * (unsigned)K * 2u + (unsigned)S::swizzle(ld_row + 8 * n, ld_c) * 16u + kLeadTwo -
+      g_off_b[n] = (unsigned)(ld_row + n / 4 * 16 + n % 2 * 8) * (unsigned)K * 2u + (unsigned)S::swizzle(ld_row + 8 * n, ld_c) * 16u + kLeadFar -
                    1024u * (n % 4);
   } else if constexpr (kOwnOffsetsB) {
 #pragma unroll

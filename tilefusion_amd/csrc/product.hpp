@@ -107,23 +107,24 @@ TFK_DEVICE void store_blocks(T* c, size_t pitch, int row, int col, int rows, int
 // ------------------------------------------------------------------------------------------
 // A * B^T: the main loops of the GEMM.
 // ------------------------------------------------------------------------------------------
-// M >= BM, N >= BN (kTwo: BN / 2), K >= 128 bytes.  The last tile of a row or column of tiles ends where the result does: it overlaps its neighbour.
-template <typename S, typename InT, bool kTwo, typename Epilogue>
+// M >= BM (kFew: M < BM), N >= BN (kTwo: BN / 2), K >= 128 bytes.  The last tile of a row or column of tiles ends where the result does: it
+// overlaps its neighbour.
+template <typename S, typename InT, bool kTwo, bool kFew, typename Epilogue>
 __global__ __launch_bounds__(S::kThreads) void product_ring64_kernel(Operands x, int tiles_m, int tiles_n, Epilogue epilogue) {
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int kCols = kTwo ? S::BN / 2 : S::BN;   // columns of the result
   int tile_m, tile_n;
   tile_of_block(blockIdx.x, gridDim.x, tiles_m, tiles_n, tile_m, tile_n);
-  const int m0 = min(tile_m * S::BM, x.M - S::BM), n0 = min(tile_n * kCols, x.N - kCols);
+  const int m0 = kFew ? 0 : min(tile_m * S::BM, x.M - S::BM), n0 = min(tile_n * kCols, x.N - kCols);
   const int wm = wave / S::WAVES_N, wn = wave % S::WAVES_N;
   float4_t acc[S::TM][S::TN];
-  ring64_multiply<S, InT, kTwo>(static_cast<const uint16_t*>(x.a), static_cast<const uint16_t*>(x.b[0]), static_cast<const uint16_t*>(x.b[1]),
-                                x.K * (int)sizeof(InT) / 2, m0, n0, lane, wave, smem, acc);
+  ring64_multiply<S, InT, kTwo, kFew>(static_cast<const uint16_t*>(x.a), static_cast<const uint16_t*>(x.b[0]), static_cast<const uint16_t*>(x.b[1]),
+                                      x.K * (int)sizeof(InT) / 2, m0, n0, lane, wave, smem, acc, x.M);
   // nothing of the epilogue is worth a register of the main loop
   int again = lane;
   asm volatile("" : "+v"(again));
-  epilogue.template run<true>(acc, TileAt{m0 + wm * S::WM, n0 + wn * (kCols / S::WAVES_N), tile_m * S::BM, tile_n * kCols, again,
+  epilogue.template run<!kFew>(acc, TileAt{m0 + wm * S::WM, n0 + wn * (kCols / S::WAVES_N), tile_m * S::BM, tile_n * kCols, again,
                                           tile_n * S::WAVES_N + wn});
 }
 
@@ -167,7 +168,9 @@ constexpr int64_t kMaxTiles = ((int64_t)1 << 23) - 1;   // a launch has less tha
 
 // The kernel that gemm.hip's cost model expects to be done first with M x N outputs over K 16-bit elements, out of those of `allowed` (a bit per row of
 // its table kGemmKernels): its position there.
-int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed);
+int pick_table_kernel(int64_t M, int64_t N, int64_t K, unsigned allowed, float* expected_us);
+// What it expects of a kernel of its table, in us.
+float expected_table_us(int kernel, int64_t tiles, int64_t K);
 
 // Positions in that table, and the kernels here.  With two matrices B, tiles have an even number of 16-column blocks to a wavefront, a
 // wavefront's requests begin with a block (no tiles of 192 columns), and the smallest tile is 16 x 32.
@@ -177,22 +180,35 @@ struct ProductPlan {
   int kernel;       // position
   int64_t slots;    // of a row's partial results (TileAt)
 };
+// Behind the table's end: its tiles of 128 x 128 (requests 4 k-tiles ahead; in pairs on a CU) for fewer than 128 rows.
+constexpr int kFewAlone = 15, kFewPaired = 16;
 // slots of a row's partial results
 inline int64_t product_slots(int kernel, int64_t N) {
-  constexpr int kColumns[] = {16, 16, 16, 32, 32, 32, 64, 64, 64, 64, 64, 96, 64, 96, 128};   // a wavefront's (split K: a tile's)
+  constexpr int kColumns[] = {16, 16, 16, 32, 32, 32, 64, 64, 64, 64, 64, 96, 64, 96, 128, 64, 64};   // a wavefront's (split K: a tile's)
   // (the last tile has a slot for each of its wavefronts)
   return kernel < 7 ? tiles_of(N, kColumns[kernel]) : 2 * tiles_of(N, 2 * kColumns[kernel]);
 }
 // K: 16-bit elements (half the elements of 8)
 inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool two) {
+  const int64_t columns = two ? 2 * N : N;
   // (the table has no tile of 16 x 32: up to 16 rows it is ahead of 32 x 32, 1 x 4096 x 11264 of two matrices 33.2 us / 38.4)
-  const int kernel = two && M <= 16 ? 0 : pick_table_kernel(M, two ? 2 * N : N, K, two ? kTwoAllowed & ~1u : kOneAllowed);
+  if (two && M <= 16) return {0, product_slots(0, N)};
+  float us;
+  int kernel = pick_table_kernel(M, columns, K, two ? kTwoAllowed & ~1u : kOneAllowed, &us);
+  // Fewer than 128 rows and many columns: large tiles all the same where the model expects them sooner than the small ones, which read the
+  // weights once for every 32 or 64 rows.  us, small / large: loss of 100 x 1024 over 32000 words 33 / 20.5, of 37 22.3 / 19.4, gated
+  // block 100 x 4096 x 11264 57 / 44.5; 64 x 2048 x 8192 17.7 / 21.3 (where the small ones stay).
+  if (M < 128 && columns >= 128 && K >= 64) {
+    const int64_t tiles = tiles_of(columns, 128);
+    const int few = tiles <= 256 ? kFewAlone : kFewPaired;
+    if (tiles <= kMaxTiles && expected_table_us(few == kFewAlone ? 7 : 9, tiles, K) < us) kernel = few;
+  }
   return {kernel, product_slots(kernel, N)};
 }
 
-template <typename S, typename InT, bool kTwo, typename Epilogue>
+template <typename S, typename InT, bool kTwo, typename Epilogue, bool kFew = false>
 int launch_ring64_product(const char* who, const Operands& x, const Epilogue& epilogue, hipStream_t st) {
-  auto kern = product_ring64_kernel<S, InT, kTwo, Epilogue>;
+  auto kern = product_ring64_kernel<S, InT, kTwo, kFew, Epilogue>;
   static_assert(S::kLdsBytes <= kMaxLdsBytes, "ring does not fit in LDS");
   TFK_LDS_OPT_IN(kern, S::kLdsBytes);
   const int64_t tiles_m = tiles_of(x.M, S::BM), tiles_n = tiles_of(x.N, kTwo ? S::BN / 2 : S::BN);
@@ -220,7 +236,8 @@ int launch_product(const char* who, const Operands& x, const ProductPlan& plan, 
         launch_ring64_product<Ring64Shape<128, 128, 4>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<128, 128, 2>, InT, kTwo, Epilogue>,
         launch_ring64_product<Ring64Shape<128, 128, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<192, 128, 2>, InT, kTwo, Epilogue>,
         nullptr, launch_ring64_product<Ring64Shape<256, 128, 2>, InT, kTwo, Epilogue>, nullptr,
-        launch_ring64_product<Ring64Shape<256, 256, 2>, InT, kTwo, Epilogue>};
+        launch_ring64_product<Ring64Shape<256, 256, 2>, InT, kTwo, Epilogue>,
+        launch_ring64_product<Ring64Shape<128, 128, 4>, InT, kTwo, Epilogue, true>, launch_ring64_product<Ring64Shape<128, 128, 2>, InT, kTwo, Epilogue, true>};
     return kLaunchers[plan.kernel](who, x, epilogue, st);
   } else {
     static constexpr Launcher kLaunchers[] = {
@@ -231,7 +248,8 @@ int launch_product(const char* who, const Operands& x, const ProductPlan& plan, 
         launch_ring64_product<Ring64Shape<128, 128, 4>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<128, 128, 2>, InT, kTwo, Epilogue>,
         launch_ring64_product<Ring64Shape<128, 128, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<192, 128, 2>, InT, kTwo, Epilogue>,
         launch_ring64_product<Ring64Shape<192, 192, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<256, 128, 2>, InT, kTwo, Epilogue>,
-        launch_ring64_product<Ring64Shape<256, 192, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<256, 256, 2>, InT, kTwo, Epilogue>};
+        launch_ring64_product<Ring64Shape<256, 192, 2>, InT, kTwo, Epilogue>, launch_ring64_product<Ring64Shape<256, 256, 2>, InT, kTwo, Epilogue>,
+        launch_ring64_product<Ring64Shape<128, 128, 4>, InT, kTwo, Epilogue, true>, launch_ring64_product<Ring64Shape<128, 128, 2>, InT, kTwo, Epilogue, true>};
     return kLaunchers[plan.kernel](who, x, epilogue, st);
   }
 }
@@ -255,9 +273,6 @@ struct ColsShape {
 };
 constexpr ColsShape kColsShapes[] = {{256, 256, 14}, {256, 128, 12}, {128, 128, 7}, {128, 128, 9}};
 
-// What gemm.hip's cost model expects of a kernel of its table, in us.
-float expected_table_us(int kernel, int64_t tiles, int64_t k_tiles);
-
 // Cut, a product costs a launch more and its parts' way through memory (4 bytes written and read for each element and part, at 4 TB/s).
 // (Twelve numbers of parts are looked at, not all 64: choosing among these takes the calling thread 10 us a product.  Forced choices, backward pass of the
 // gated block and of the head over 11 problems: at most 6% ahead of it.)
@@ -271,7 +286,7 @@ inline ColsPlan plan_cols(int64_t M, int64_t N, int64_t k_tiles) {
       const int64_t per = tiles_of(k_tiles, splits);
       if (splits > 1 && (tiles * splits > 1024 || per < 4 || tiles_of(k_tiles, per) != splits)) continue;
       const float parts = splits > 1 ? 3.f + (float)(8 * splits * M * N) / 4e6f : 0.f;
-      const float us = expected_table_us(kColsShapes[s].table, tiles * splits, per) + parts;
+      const float us = expected_table_us(kColsShapes[s].table, tiles * splits, 64 * per) + parts;
       if (us < best_us) {
         best = {s, (int)splits, (int)per};
         best_us = us;
