@@ -23,7 +23,7 @@ constexpr float kGeluTwice = 1.5957691216057308f;   // 2 * sqrt(2 / pi): (1 + ta
 
 // The normal distribution's weight below -|g|, from exp(-g^2 / 2): Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26
 // (within 1e-7, halved from their bound for erf), and without the difference from 1 that the tail would be lost in.  The library's erff takes both of its branches
-// for every wavefront: 250 cycles an element, 60 so (2999 x 1032 x 1544 with gate and up kept, fp16: 43 us with it).
+// for every wavefront (2999 x 1032 x 1544 with gate and up kept, fp16: 43 us with it, 32 so).
 TFK_DEVICE float normal_tail(float g, float bell) {
   const float t = __builtin_amdgcn_rcpf(1.f + (0.3275911f * 0.7071067811865476f) * fabsf(g));
   float p = 0.5f * 1.061405429f;

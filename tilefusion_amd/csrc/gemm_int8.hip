@@ -40,7 +40,8 @@ struct Int8Epilogue {
   }
 };
 
-// K is no multiple of 16: rows are copied, completed by zeros to whole lines (131 us instead of 140 for 2999 x 1544 x 1032).
+// K is no multiple of 16: rows are copied, completed by zeros to whole lines.  2999 x 1544 x 1032: 7 us for the copies and 13 for the product, 131 by a kernel
+// that checks every access.
 struct CopyPlan {
   int64_t pitch = 0;
   size_t b = 0, bytes = 0;
