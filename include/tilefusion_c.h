@@ -255,7 +255,7 @@ TF_API int tf_gated_ffn(const void* x, const void* w_gate, const void* w_up, voi
                         int activation, int64_t M, int64_t F, int64_t K, void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients of x [M,K], w_gate and w_up [F,K] from that of h (dh [M,F]) and the gate and up values that the forward call kept; x and
  * the weights as there, the others begin anywhere.  The workspace begins at a 16-byte boundary and may hold anything; it is done with when the call's work is.  A null dx, or
- * null dw_gate and dw_up, are not computed.  M = 0: the weights' gradients are zero. */
+ * null dw_gate and dw_up, are not computed (the sums of the others may be cut otherwise than beside them).  M = 0: the weights' gradients are zero. */
 TF_API size_t tf_gated_ffn_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
 TF_API int tf_gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const void* gate,
                                  const void* up, void* dx, void* dw_gate, void* dw_up, int dtype, int activation, int64_t M,
@@ -292,9 +292,11 @@ TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* 
  * *words_a_lane the 32-bit words of an update that a lane adds; -1 for other arguments. */
 /* tf_product_kernel_index: position in kGemmKernels of what tf_gemm_int8 (K: half its own), tf_gated_ffn (two = 1, N: F) and tf_linear_cross_entropy
  * and the first product of its backward pass (N: columns of the vocabulary or of a piece) run; -1 for other arguments.  tf_product_cols_plan: position in kColsShapes
- * (csrc/product.hpp) of the tile of a gradient of M x N that is a sum over `rows` rows, and in *parts the parts that the sum is cut into. */
+ * (csrc/product.hpp) of the tile of a gradient of M x N that is a sum over `rows` rows, and in *parts the parts that the sum is cut into.
+ * tf_product_pair_plan: the same of two gradients that are asked for together and run in one launch; -1 where they run one after the other. */
 TF_API int tf_product_kernel_index(int64_t M, int64_t N, int64_t K, int two);
 TF_API int tf_product_cols_plan(int64_t M, int64_t N, int64_t rows, int* parts);
+TF_API int tf_product_pair_plan(int64_t M, int64_t N, int64_t rows, int64_t M2, int64_t N2, int64_t rows2, int* parts, int* parts2);
 TF_API int tf_gemm_kernel_index(int64_t M, int64_t N, int64_t K, int c_is_f32);
 TF_API int tf_flash_decode_plan(int64_t batch_heads, int64_t Lkv, int64_t D, int num_splits, int* wavefronts);
 TF_API int tf_flash_attention_rows(int64_t batch, int64_t Lq, int64_t Lkv, int64_t D, int causal);

@@ -1,5 +1,7 @@
 """The gated feed-forward block against its 64-bit form, forward and backward."""
 
+import importlib
+
 import pytest
 import torch
 
@@ -8,6 +10,7 @@ from tilefusion_amd import _capi, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+_one = importlib.import_module("tilefusion_amd.ops.gated_ffn")._backward   # of some gradients, as autograd asks for them
 TYPES = [torch.float16, torch.bfloat16]
 ACTIVATIONS = ["silu", "gelu", "gelu_tanh"]
 
@@ -104,16 +107,22 @@ def test_large_gates():
 
 
 # ---- backward ------------------------------------------------------------------------------
-def _check_backward(grad_h, x, w_gate, w_up, gate, up, activation):
-    got = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation)
+def _check_backward(grad_h, x, w_gate, w_up, gate, up, activation, alone=False):
+    results = [(ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation), (0, 1, 2))]
+    if alone:   # gradients that are asked for without the others: what runs is chosen for each
+        results += [(_one(grad_h, x, w_gate, w_up, gate, up, activation, of == (0,), of != (0,)), of) for of in ((0,), (1, 2))]
     f, k = w_gate.shape
     want, bounds = ref.gated_ffn_backward(grad_h.reshape(-1, f), x.reshape(-1, k), w_gate, w_up, gate.reshape(-1, f), up.reshape(-1, f), activation)
-    for name, g, w, b, like in zip(("grad_x", "grad_w_gate", "grad_w_up"), got, want, bounds, (x, w_gate, w_up)):
-        assert g.shape == like.shape and g.dtype == x.dtype
-        what = f"{name} {tuple(x.shape)} F={f} {x.dtype} {activation}"
-        ref.assert_within(g.reshape(w.shape), w, b, what)
-        # errors of many roundings are independent: in all far less than every one at its largest
-        assert (g.reshape(w.shape).double() - w).norm() <= 2 * ref.half_step(x.dtype) * w.norm(), what
+    for got, of in results:
+        for i, (name, g, w, b, like) in enumerate(zip(("grad_x", "grad_w_gate", "grad_w_up"), got, want, bounds, (x, w_gate, w_up))):
+            if i not in of:
+                assert g is None
+                continue
+            assert g.shape == like.shape and g.dtype == x.dtype
+            what = f"{name} {tuple(x.shape)} F={f} {x.dtype} {activation} of {of}"
+            ref.assert_within(g.reshape(w.shape), w, b, what)
+            # errors of many roundings are independent: in all far less than every one at its largest
+            assert (g.reshape(w.shape).double() - w).norm() <= 2 * ref.half_step(x.dtype) * w.norm(), what
 
 
 BACKWARD_SIZES = [(1, 1, 1), (1, 64, 64), (3, 17, 9), (31, 100, 33), (64, 64, 64), (65, 127, 72), (130, 96, 200), (257, 136, 264), (400, 513, 104), (1000, 160, 1032)]
@@ -124,13 +133,18 @@ BACKWARD_KERNELS = [
     (3667, 1, 2320), (2442, 1, 1592), (3214, 3946, 8), (1810, 409, 2304), (130, 8700, 5936), (1, 6720, 1296), (1, 2186, 1800), (2, 3339, 520), (3951, 2907, 8),
     (1, 3238, 1184), (26477, 548, 8), (34566, 1353, 144),
 ]
+# both products in one launch: every tile, with neither, either and both sums in parts
+BACKWARD_PAIRS = [
+    (960, 513, 3992), (4466, 497, 1056), (2, 2501, 3504), (5558, 4584, 152), (580, 200, 3880), (3057, 1, 2928), (1, 462, 3424), (2842, 2564, 8),
+    (836, 1, 8), (1, 385, 8), (964, 784, 8), (525, 271, 3536), (2493, 1, 3568), (1, 718, 2880), (4121, 5190, 8),
+]
 
 
-@pytest.mark.parametrize("m,f,k", BACKWARD_SIZES + BACKWARD_KERNELS)
+@pytest.mark.parametrize("m,f,k", BACKWARD_SIZES + BACKWARD_KERNELS + BACKWARD_PAIRS)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_backward_sizes(m, f, k, dtype):
     x, w_gate, w_up, g = _block(m, f, k, dtype, seed=4)
-    _check_backward(*(_randn(g, m, f, dtype=dtype) for _ in range(1)), x, w_gate, w_up, _randn(g, m, f, dtype=dtype), _randn(g, m, f, dtype=dtype), "silu")
+    _check_backward(*(_randn(g, m, f, dtype=dtype) for _ in range(1)), x, w_gate, w_up, _randn(g, m, f, dtype=dtype), _randn(g, m, f, dtype=dtype), "silu", alone=True)
 
 
 @pytest.mark.parametrize("activation", ACTIVATIONS)

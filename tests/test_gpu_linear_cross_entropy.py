@@ -1,5 +1,7 @@
 """The cross entropy of a linear head against its 64-bit form, forward and backward."""
 
+import importlib
+
 import pytest
 import torch
 
@@ -8,6 +10,7 @@ from tilefusion_amd import _capi, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+_one = importlib.import_module("tilefusion_amd.ops.linear_cross_entropy")._backward   # of some gradients, as autograd asks for them
 TYPES = [torch.float16, torch.bfloat16]
 
 
@@ -32,17 +35,24 @@ def _check_forward(hidden, weight, target, ignore_index=-100):
     return lse
 
 
-def _check_backward(grad_loss, hidden, weight, target, ignore_index=-100):
+def _check_backward(grad_loss, hidden, weight, target, ignore_index=-100, alone=False):
     lse = ops.linear_cross_entropy(hidden, weight, target, ignore_index)[1]
     got = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index)
     want, bounds = ref.linear_cross_entropy_backward(grad_loss.reshape(-1), hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), ignore_index)
-    for name, g, w, b, like in zip(("grad_hidden", "grad_weight"), got, want, bounds, (hidden, weight)):
-        assert g.shape == like.shape and g.dtype == like.dtype
-        what = f"{name} {tuple(hidden.shape)} V={weight.shape[0]} {hidden.dtype}"
-        number = ref.assert_within(g.reshape(w.shape), w, b, what)
-        if w.norm() > 0:
-            floor = w.numel() ** 0.5 * ref.TINY[hidden.dtype]   # results too small for the type
-            assert (g.reshape(w.shape).double() - w)[number].norm() <= 2 * ref.half_step(hidden.dtype) * w.norm() + floor, what
+    results = [(got, (0, 1))]
+    if alone:   # gradients that are asked for without the other: what runs is chosen for each
+        results += [(_one(grad_loss, hidden, weight, target, lse, ignore_index, of == 0, of == 1), (of,)) for of in (0, 1)]
+    for grads, of in results:
+        for i, (name, g, w, b, like) in enumerate(zip(("grad_hidden", "grad_weight"), grads, want, bounds, (hidden, weight))):
+            if i not in of:
+                assert g is None
+                continue
+            assert g.shape == like.shape and g.dtype == like.dtype
+            what = f"{name} {tuple(hidden.shape)} V={weight.shape[0]} {hidden.dtype} of {of}"
+            number = ref.assert_within(g.reshape(w.shape), w, b, what)
+            if w.norm() > 0:
+                floor = w.numel() ** 0.5 * ref.TINY[hidden.dtype]   # results too small for the type
+                assert (g.reshape(w.shape).double() - w)[number].norm() <= 2 * ref.half_step(hidden.dtype) * w.norm() + floor, what
     return got
 
 
@@ -63,6 +73,11 @@ BACKWARD_KERNELS = [
     (3599, 1, 2208), (2522, 1, 1544), (1, 903, 8), (1849, 886, 2288), (130, 17395, 5936), (1175, 15938, 8), (1, 13431, 1296), (1, 3567, 2328), (1, 3263, 1168),
     (898, 1, 8), (791, 3609, 1104), (22312, 129, 5776), (15938, 1175, 8), (33847, 1059, 8),
 ]
+# both products in one launch: every tile, with neither, either and both sums in parts
+BACKWARD_PAIRS = [
+    (1069, 1055, 3728), (5423, 1379, 928), (133, 8627, 2456), (5318, 9225, 152), (534, 464, 3624), (2989, 1, 3256), (1, 969, 3344), (2689, 5305, 8),
+    (839, 1, 8), (1, 835, 8), (1001, 1741, 8), (385, 579, 3608), (4635, 1, 3616), (1, 1421, 2712), (5816, 7434, 8),
+]
 
 
 @pytest.mark.parametrize("t,v,k", SIZES + KERNELS)
@@ -72,12 +87,12 @@ def test_forward_sizes(t, v, k, dtype):
     _check_forward(hidden, weight, target)
 
 
-@pytest.mark.parametrize("t,v,k", SIZES + KERNELS + BACKWARD_KERNELS)
+@pytest.mark.parametrize("t,v,k", SIZES + KERNELS + BACKWARD_KERNELS + BACKWARD_PAIRS)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_backward_sizes(t, v, k, dtype):
     hidden, weight, target, g = _head(t, v, k, dtype, seed=1)
     scale = 4096.0 if dtype == torch.float16 else 1.0
-    _check_backward(torch.full((t,), scale / t, device=DEV), hidden, weight, target)
+    _check_backward(torch.full((t,), scale / t, device=DEV), hidden, weight, target, alone=True)
     _check_backward((torch.rand(t, device=DEV, generator=g) - 0.5) * scale, hidden, weight, target)
 
 

@@ -194,6 +194,12 @@ def _cols(m, n, rows):
     return shape, parts.value > 1
 
 
+def _pair(one, other):
+    parts = ctypes.c_int(0), ctypes.c_int(0)
+    shape = _capi.load().tf_product_pair_plan(*one, *other, *(ctypes.byref(p) for p in parts))
+    return None if shape < 0 else (shape, parts[0].value > 1, parts[1].value > 1)
+
+
 def test_cases_reach_every_form_of_a_gradient():
     import tests.test_gpu_gated_ffn as ffn
     import tests.test_gpu_linear_cross_entropy as loss
@@ -202,12 +208,18 @@ def test_cases_reach_every_form_of_a_gradient():
         return -(-x // 64) * 64
 
     every = {(shape, cut) for shape in range(4) for cut in (False, True)}
-    ffn_cases = ffn.BACKWARD_SIZES + ffn.BACKWARD_KERNELS
+    ffn_cases = ffn.BACKWARD_SIZES + ffn.BACKWARD_KERNELS + ffn.BACKWARD_PAIRS   # (each runs with both gradients and with one)
     assert {_cols(m, k, 2 * up(f)) for m, f, k in ffn_cases} == every
     assert {_cols(up(f) + f, k, m) for m, f, k in ffn_cases} == every
-    loss_cases = loss.SIZES + loss.BACKWARD_KERNELS
+    loss_cases = loss.SIZES + loss.BACKWARD_KERNELS + loss.BACKWARD_PAIRS
     assert {_cols(t, k, up(v)) for t, v, k in loss_cases} == every
     assert {_cols(up(v), k, t) for t, v, k in loss_cases} == every
+
+    pairs = {(shape, one, other) for shape in range(4) for one in (False, True) for other in (False, True)}
+    assert {_pair((m, k, 2 * up(f)), (up(f) + f, k, m)) for m, f, k in ffn_cases} - {None} == pairs
+    assert {_pair((t, k, up(v)), (up(v), k, t)) for t, v, k in loss_cases} - {None} == pairs
+    parts = ctypes.byref(ctypes.c_int())
+    assert _capi.load().tf_product_pair_plan(4, 4, 0, 4, 4, 4, parts, parts) == -1 == _capi.load().tf_product_pair_plan(4, 4, 4, 4, 4, 4, None, parts)
     plan = _capi.load().tf_product_cols_plan
     assert plan(0, 4, 4, ctypes.byref(ctypes.c_int())) == -1 == plan(4, 4, 4, None) and _capi.load().tf_product_kernel_index(4, 4, 1 << 22, 0) == -1
 

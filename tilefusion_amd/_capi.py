@@ -54,6 +54,7 @@ SIGNATURES = {
     "tf_linear_cross_entropy_backward": (_i, [_vp] * 7 + [_i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "tf_product_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_product_cols_plan": (_i, [_i64, _i64, _i64, ctypes.POINTER(_i)]),
+    "tf_product_pair_plan": (_i, [_i64] * 6 + [ctypes.POINTER(_i)] * 2),
     "tf_gemm_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_flash_decode_plan": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_i)]),
     "tf_flash_attention_rows": (_i, [_i64, _i64, _i64, _i64, _i]),

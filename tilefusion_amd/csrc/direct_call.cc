@@ -8,7 +8,7 @@
 // torch.compile and torch.jit.script.  What is called is the dispatcher's CUDA kernel of the op, an implementation that a
 // program registers in place of the library's included.
 // us a call in a loop, through torch.ops / as here: gemm 128 x 64 x 256 4.6 / 3.7; fused 16384 x 128 x 128 x 128 4.7 / 4.4 and decoding
-// 32 x 1999 x 64 9.4 / 9.4, whose kernels take as long.
+// 32 x 1999 x 64 9.4 / 9.4, whose kernels take as long; rows of 16 x 4096 quantised and multiplied with 4096 channels in 8 bits 17.5 / 9.5.
 #include <Python.h>
 
 #include <ATen/ATen.h>

@@ -171,6 +171,8 @@ struct BackwardPlan {
   int64_t Fp, Kp;
   bool copy_weights, copy_x;
   ColsPlan of_x, of_w;            // products: dx, the weights' gradients
+  PairPlan both;                  // where both are asked for
+  int64_t x_floats;               // of dx's parts, which those of the weights' gradients lie behind
   size_t weights, x, parts, bytes;   // offsets in the workspace ([dg | du]: 0), its size
   BackwardPlan(int64_t M, int64_t F, int64_t K) {
     Fp = round_up_to(F, 64);
@@ -178,8 +180,10 @@ struct BackwardPlan {
     // the sum over F goes on in the second weight at a whole k-tile
     copy_weights = Kp != K || Fp != F;
     copy_x = Kp != K;
-    of_x = plan_cols(M, K, 2 * Fp / 64);
-    of_w = plan_cols(Fp + F, K, tiles_of(M, 64));
+    const ColsSize x_size = {M, K, 2 * Fp / 64}, w_size = {Fp + F, K, tiles_of(M, 64)};
+    of_x = plan_cols(x_size);
+    of_w = plan_cols(w_size);
+    both = plan_pair(of_x, x_size, of_w, w_size);
     size_t at = 0;
     auto take = [&](int64_t bytes_) {
       const size_t from = at;
@@ -190,7 +194,8 @@ struct BackwardPlan {
     weights = take(copy_weights ? 2 * 2 * Fp * Kp : 0);
     x = take(copy_x ? 2 * M * Kp : 0);
     const auto floats = [K](const ColsPlan& plan, int64_t rows) { return plan.splits > 1 ? PartsRoom(plan, rows, K).floats : 0; };
-    parts = take(4 * std::max(floats(of_x, M), floats(of_w, Fp + F)));
+    x_floats = floats(both.x, M);
+    parts = take(4 * std::max({floats(of_x, M), floats(of_w, Fp + F), both.together ? x_floats + floats(both.w, Fp + F) : 0}));
     bytes = at;
   }
 };
@@ -255,29 +260,33 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
   const auto bits = [](const void* t) { return static_cast<const uint16_t*>(t); };
   const uint16_t* const grads_at = bits(ws);
   const ColsProduct of_x = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)M}, {bits(w_gate), p.Kp, (int)p.Kp, (int)K}, bits(w_up), (int)(p.Fp / 64), (int)(2 * p.Fp / 64), 0, 0};
-  T* const to_x = static_cast<T*>(dx);
-  if (dx == nullptr) {
-    // not asked for
-  } else if (p.of_x.splits == 1) {
-    if (int rc = launch_cols<T, false>(who, of_x, p.of_x, WholeEpilogue<T>{to_x, nullptr, (int)M, (int)K}, st)) return rc;
-  } else {
-    const PartsRoom room(p.of_x, M, K);
-    if (int rc = launch_cols<T, false>(who, of_x, p.of_x, PartEpilogue{parts, room.rows, room.pitch, false}, st)) return rc;
-    if (int rc = launch_sum_parts<T>(parts, room, p.of_x.splits, 0, M, K, to_x, nullptr, st)) return rc;
-  }
-  if (dw_gate == nullptr) return TF_OK;
   const int m_tiles = (int)tiles_of(M, 64), m_pad = (int)(m_tiles * 64 - M);
   const ColsOperand tokens = {bits(x), p.Kp, (int)p.Kp, (int)K};
   const ColsProduct of_w = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)(p.Fp + F)}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
-  T *const to_gate = static_cast<T*>(dw_gate), *const to_up = static_cast<T*>(dw_up);
-  if (p.of_w.splits == 1) {
-    const BothEpilogue<T> both = {{to_gate, nullptr, (int)F, (int)K}, {to_up - p.Fp * K, nullptr, (int)(p.Fp + F), (int)K}, (int)p.Fp};
-    return launch_cols<T, true>(who, of_w, p.of_w, both, st);
+  T *const to_x = static_cast<T*>(dx), *const to_gate = static_cast<T*>(dw_gate), *const to_up = static_cast<T*>(dw_up);
+  const WholeEpilogue<T> whole_x = {to_x, nullptr, (int)M, (int)K};
+  const BothEpilogue<T> whole_w = {{to_gate, nullptr, (int)F, (int)K}, {to_up != nullptr ? to_up - p.Fp * K : nullptr, nullptr, (int)(p.Fp + F), (int)K}, (int)p.Fp};
+  const bool together = dx != nullptr && dw_gate != nullptr && p.both.together;
+  const ColsPlan &x_plan = together ? p.both.x : p.of_x, &w_plan = together ? p.both.w : p.of_w;
+  const PartsRoom x_room(x_plan, M, K), w_room(w_plan, p.Fp + F, K);
+  float* const w_parts = together ? parts + p.x_floats : parts;
+  const PartEpilogue part_x = {parts, x_room.rows, x_room.pitch, false}, part_w = {w_parts, w_room.rows, w_room.pitch, false};
+  if (together)
+    if (int rc = launch_pair<T>(who, of_x, x_plan, CutEpilogue<WholeEpilogue<T>>{whole_x, part_x, x_plan.splits > 1}, of_w, w_plan,
+                                CutEpilogue<BothEpilogue<T>>{whole_w, part_w, w_plan.splits > 1}, st))
+      return rc;
+  if (dx != nullptr) {
+    if (!together)
+      if (int rc = x_plan.splits == 1 ? launch_cols<T, false>(who, of_x, x_plan, whole_x, st) : launch_cols<T, false>(who, of_x, x_plan, part_x, st)) return rc;
+    if (x_plan.splits > 1)
+      if (int rc = launch_sum_parts<T>(parts, x_room, x_plan.splits, 0, M, K, to_x, nullptr, st)) return rc;
   }
-  const PartsRoom room(p.of_w, p.Fp + F, K);
-  if (int rc = launch_cols<T, true>(who, of_w, p.of_w, PartEpilogue{parts, room.rows, room.pitch, false}, st)) return rc;
-  if (int rc = launch_sum_parts<T>(parts, room, p.of_w.splits, 0, F, K, to_gate, nullptr, st)) return rc;
-  return launch_sum_parts<T>(parts, room, p.of_w.splits, p.Fp, p.Fp + F, K, to_up, nullptr, st);
+  if (dw_gate == nullptr) return TF_OK;
+  if (!together)
+    if (int rc = w_plan.splits == 1 ? launch_cols<T, true>(who, of_w, w_plan, whole_w, st) : launch_cols<T, true>(who, of_w, w_plan, part_w, st)) return rc;
+  if (w_plan.splits == 1) return TF_OK;
+  if (int rc = launch_sum_parts<T>(w_parts, w_room, w_plan.splits, 0, F, K, to_gate, nullptr, st)) return rc;
+  return launch_sum_parts<T>(w_parts, w_room, w_plan.splits, p.Fp, p.Fp + F, K, to_up, nullptr, st);
 }
 
 int check_sizes(const char* who, int dtype, int activation, int64_t M, int64_t F, int64_t K) {

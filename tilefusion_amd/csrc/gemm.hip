@@ -588,7 +588,16 @@ extern "C" int tf_product_kernel_index(int64_t M, int64_t N, int64_t K, int two)
 
 extern "C" int tf_product_cols_plan(int64_t M, int64_t N, int64_t rows, int* parts) {
   if (M <= 0 || N <= 0 || rows <= 0 || parts == nullptr) return -1;
-  const tfk::ColsPlan plan = tfk::plan_cols(M, N, tfk::tiles_of(rows, 64));
+  const tfk::ColsPlan plan = tfk::plan_cols({M, N, tfk::tiles_of(rows, 64)});
   *parts = plan.splits;
   return plan.shape;
+}
+
+extern "C" int tf_product_pair_plan(int64_t M, int64_t N, int64_t rows, int64_t M2, int64_t N2, int64_t rows2, int* parts, int* parts2) {
+  if (M <= 0 || N <= 0 || rows <= 0 || M2 <= 0 || N2 <= 0 || rows2 <= 0 || parts == nullptr || parts2 == nullptr) return -1;
+  const tfk::ColsSize one = {M, N, tfk::tiles_of(rows, 64)}, other = {M2, N2, tfk::tiles_of(rows2, 64)};
+  const tfk::PairPlan plan = tfk::plan_pair(tfk::plan_cols(one), one, tfk::plan_cols(other), other);
+  *parts = plan.x.splits;
+  *parts2 = plan.w.splits;
+  return plan.together ? plan.x.shape : -1;
 }

@@ -219,13 +219,16 @@ struct ForwardPlan {
 struct BackwardPlan {
   int64_t width, piece, pieces;      // K with its zeros, columns of a piece (the last may have fewer)
   ColsPlan of_hidden, of_weight;     // (the last piece's are as those of the others)
+  PairPlan both;                     // where both are asked for
   size_t scale, hidden, weight, hidden_parts, weight_parts, bytes;   // offsets in the workspace (of P: 0), its size
   BackwardPlan(int64_t T, int64_t V, int64_t K) {
     width = aligned_width(K);
     piece = std::min(round_up_to(V, 64), std::max<int64_t>(4096, kPieceElements / T / 256 * 256));
     pieces = tiles_of(V, piece);
-    of_hidden = plan_cols(T, K, piece / 64);
-    of_weight = plan_cols(piece, K, tiles_of(T, 64));
+    const ColsSize hidden_size = {T, K, piece / 64}, weight_size = {piece, K, tiles_of(T, 64)};
+    of_hidden = plan_cols(hidden_size);
+    of_weight = plan_cols(weight_size);
+    both = plan_pair(of_hidden, hidden_size, of_weight, weight_size);
     size_t at = 0;
     auto take = [&](int64_t bytes_) {
       const size_t from = at;
@@ -236,8 +239,11 @@ struct BackwardPlan {
     scale = take(sizeof(Scale));
     hidden = take(width != K ? 2 * T * width : 0);
     weight = take(width != K ? 2 * piece * width : 0);
-    hidden_parts = take(pieces > 1 || of_hidden.splits > 1 ? 4 * PartsRoom(of_hidden, T, K).floats : 0);
-    weight_parts = take(of_weight.splits > 1 ? 4 * PartsRoom(of_weight, piece, K).floats : 0);
+    const auto floats = [K](const ColsPlan& plan, bool cut, int64_t rows) { return cut ? PartsRoom(plan, rows, K).floats : 0; };
+    const auto hidden_floats = [&](const ColsPlan& plan) { return floats(plan, pieces > 1 || plan.splits > 1, T); };
+    const auto weight_floats = [&](const ColsPlan& plan) { return floats(plan, plan.splits > 1, piece); };
+    hidden_parts = take(4 * std::max(hidden_floats(of_hidden), hidden_floats(both.x)));
+    weight_parts = take(4 * std::max(weight_floats(of_weight), weight_floats(both.w)));
     bytes = at;
   }
   static constexpr int64_t kPieceElements = (int64_t)1 << 27;   // of P, 256 MiB
@@ -286,7 +292,10 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
   const int width = (int)plan.width;
   const int t_tiles = (int)tiles_of(tokens, 64), t_pad = (int)(t_tiles * 64 - tokens);
   const ColsOperand of_tokens = {bits(hidden), width, width, (int)K};
-  const PartsRoom hidden_room(plan.of_hidden, tokens, K), weight_room(plan.of_weight, plan.piece, K);
+  const bool together = grad_hidden != nullptr && grad_weight != nullptr && plan.both.together;
+  const ColsPlan &of_hidden = together ? plan.both.x : plan.of_hidden, &of_weight = together ? plan.both.w : plan.of_weight;
+  const PartsRoom hidden_room(of_hidden, tokens, K), weight_room(of_weight, plan.piece, K);
+  const bool cut_hidden = plan.pieces > 1 || of_hidden.splits > 1, cut_weight = of_weight.splits > 1;
   for (int64_t first = 0; first < V; first += plan.piece) {
     const int64_t columns = std::min(plan.piece, V - first), pitch = round_up_to(columns, 64);
     const int pad = (int)(pitch - columns);
@@ -303,36 +312,35 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
                                           st))
       return rc;
 
-    // dH += P * W
-    if (grad_hidden != nullptr) {
-      ColsPlan of_hidden = plan.of_hidden;
-      of_hidden.per_split = (int)tiles_of(pitch / 64, of_hidden.splits);
-      const int split_parts = (int)tiles_of(pitch / 64, of_hidden.per_split);   // (a short last piece may have fewer)
-      of_hidden.splits = split_parts;
-      const ColsProduct hidden_product = {{bits(p), pitch, (int)pitch, (int)tokens}, {bits(w), width, width, (int)K}, bits(w), INT_MAX, (int)(pitch / 64), pad, 0};
-      int rc;
-      if (plan.pieces == 1 && plan.of_hidden.splits == 1)
-        rc = launch_cols<T, false>(who, hidden_product, of_hidden, WholeEpilogue<T>{static_cast<T*>(grad_hidden), scale, (int)tokens, (int)K}, st);
-      else
-        rc = launch_cols<T, false>(who, hidden_product, of_hidden, PartEpilogue{hidden_parts, hidden_room.rows, hidden_room.pitch, first > 0}, st);
-      if (rc) return rc;
-    }
-
-    // dW = P^T * H: the columns of P in front of the piece's are rows that are not stored
-    if (grad_weight == nullptr) continue;
+    // dH += P * W (a short last piece may have fewer parts), dW = P^T * H: the columns of P in front of the piece's are rows that are not stored
+    ColsPlan hidden_plan = of_hidden;
+    hidden_plan.per_split = (int)tiles_of(pitch / 64, of_hidden.splits);
+    hidden_plan.splits = (int)tiles_of(pitch / 64, hidden_plan.per_split);
+    const ColsProduct hidden_product = {{bits(p), pitch, (int)pitch, (int)tokens}, {bits(w), width, width, (int)K}, bits(w), INT_MAX, (int)(pitch / 64), pad, 0};
     const ColsProduct weight_product = {{bits(p), pitch, (int)pitch, (int)pitch}, of_tokens, of_tokens.x, INT_MAX, t_tiles, t_pad, pad};
-    T* const out = static_cast<T*>(grad_weight) + first * K;
-    int rc;
-    if (plan.of_weight.splits == 1) {
-      rc = launch_cols<T, true>(who, weight_product, plan.of_weight, WholeEpilogue<T>{out - (int64_t)pad * K, scale, (int)pitch, (int)K}, st);
+    T* const out = grad_weight != nullptr ? static_cast<T*>(grad_weight) + first * K : nullptr;
+    const WholeEpilogue<T> whole_hidden = {static_cast<T*>(grad_hidden), scale, (int)tokens, (int)K};
+    const WholeEpilogue<T> whole_weight = {out != nullptr ? out - (int64_t)pad * K : nullptr, scale, (int)pitch, (int)K};
+    const PartEpilogue part_hidden = {hidden_parts, hidden_room.rows, hidden_room.pitch, first > 0};
+    const PartEpilogue part_weight = {weight_parts, weight_room.rows, weight_room.pitch, false};
+    int rc = TF_OK;
+    if (together) {
+      rc = launch_pair<T>(who, hidden_product, hidden_plan, CutEpilogue<WholeEpilogue<T>>{whole_hidden, part_hidden, cut_hidden}, weight_product, of_weight,
+                          CutEpilogue<WholeEpilogue<T>>{whole_weight, part_weight, cut_weight}, st);
     } else {
-      rc = launch_cols<T, true>(who, weight_product, plan.of_weight, PartEpilogue{weight_parts, weight_room.rows, weight_room.pitch, false}, st);
-      if (rc == TF_OK) rc = launch_sum_parts<T>(weight_parts, weight_room, plan.of_weight.splits, pad, pitch, K, out, scale, st);
+      if (grad_hidden != nullptr)
+        rc = cut_hidden ? launch_cols<T, false>(who, hidden_product, hidden_plan, part_hidden, st)
+                        : launch_cols<T, false>(who, hidden_product, hidden_plan, whole_hidden, st);
+      if (rc == TF_OK && grad_weight != nullptr)
+        rc = cut_weight ? launch_cols<T, true>(who, weight_product, of_weight, part_weight, st)
+                        : launch_cols<T, true>(who, weight_product, of_weight, whole_weight, st);
     }
+    if (rc == TF_OK && grad_weight != nullptr && cut_weight)
+      rc = launch_sum_parts<T>(weight_parts, weight_room, of_weight.splits, pad, pitch, K, out, scale, st);
     if (rc) return rc;
   }
-  if (grad_hidden == nullptr || (plan.pieces == 1 && plan.of_hidden.splits == 1)) return TF_OK;
-  return launch_sum_parts<T>(hidden_parts, hidden_room, plan.of_hidden.splits, 0, tokens, K, static_cast<T*>(grad_hidden), scale, st);
+  if (grad_hidden == nullptr || !cut_hidden) return TF_OK;
+  return launch_sum_parts<T>(hidden_parts, hidden_room, of_hidden.splits, 0, tokens, K, static_cast<T*>(grad_hidden), scale, st);
 }
 
 int check_sizes(const char* who, int dtype, int64_t T, int64_t V, int64_t K) {

@@ -267,6 +267,10 @@ struct ColsProduct {
 struct ColsPlan {
   int shape;                // into kColsShapes
   int splits, per_split;    // the sum is cut into that many parts of so many k-tiles (the last may be shorter)
+  float us;                 // expected
+};
+struct ColsSize {
+  int64_t M, N, k_tiles;    // rows and columns of the result, 64 summed rows each
 };
 struct ColsShape {
   int bm, bn, table;        // tile, position in gemm.hip's table
@@ -275,11 +279,11 @@ constexpr ColsShape kColsShapes[] = {{256, 256, 14}, {256, 128, 12}, {128, 128, 
 
 // Cut, a product costs a launch more and its parts' way through memory (4 bytes written and read for each element and part, at 4 TB/s).
 // (Twelve numbers of parts are looked at, not all 64: choosing among these takes the calling thread 10 us a product.  Forced choices, backward pass of the
-// gated block and of the head over 11 problems: at most 6% ahead of it.)
-inline ColsPlan plan_cols(int64_t M, int64_t N, int64_t k_tiles) {
+// gated block and of the head over 11 problems: at most 10% ahead of it.)
+inline ColsPlan plan_cols(const ColsSize& of) {
+  const auto [M, N, k_tiles] = of;
   constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
-  ColsPlan best = {0, 1, (int)k_tiles};
-  float best_us = INFINITY;
+  ColsPlan best = {0, 1, (int)k_tiles, INFINITY};
   for (int s = 0; s < (int)(sizeof(kColsShapes) / sizeof(kColsShapes[0])); ++s) {
     const int64_t tiles = tiles_of(M, kColsShapes[s].bm) * tiles_of(N, kColsShapes[s].bn);
     for (int64_t splits : kSplits) {
@@ -287,9 +291,50 @@ inline ColsPlan plan_cols(int64_t M, int64_t N, int64_t k_tiles) {
       if (splits > 1 && (tiles * splits > 1024 || per < 4 || tiles_of(k_tiles, per) != splits)) continue;
       const float parts = splits > 1 ? 3.f + (float)(8 * splits * M * N) / 4e6f : 0.f;
       const float us = expected_table_us(kColsShapes[s].table, tiles * splits, 64 * per) + parts;
-      if (us < best_us) {
-        best = {s, (int)splits, (int)per};
-        best_us = us;
+      if (us < best.us) best = {s, (int)splits, (int)per, us};
+    }
+  }
+  return best;
+}
+
+// Both products of a backward pass in one launch (product_pair_kernel), or one after the other as `x` and `w` are planned.  A launch's last round of tiles
+// leaves CUs idle, and together there is one such round.  us of the gated block's backward pass in bf16, one after the other / together: 100 x 2816 x 1024
+// (tokens x F x K) 25.6 / 18.8, 1337 x 1544 x 1032 52.7 / 42.8, 2048 x 1024 x 1024 42.8 / 28.3, 4096 x 5632 x 2048 360 / 325; 4096 x 2816 x 1024 135 / 133.
+// Of the head's in fp16: 1024 tokens x 8192 words x 512 55.4 / 48.4, 613 x 32003 x 1024 181 / 180.  Sums may be cut otherwise than in a product
+// that runs alone.
+struct PairPlan {
+  bool together;
+  ColsPlan x, w;            // where they run together
+};
+inline PairPlan plan_pair(const ColsPlan& x, const ColsSize& of_x, const ColsPlan& w, const ColsSize& of_w) {
+  constexpr int kXSplits[] = {1, 2, 3, 4, 6, 8}, kWSplits[] = {1, 2, 3, 4};
+  PairPlan best = {false, x, w};
+  float best_us = x.us + w.us;
+  const auto parts_us = [](const ColsSize& of, int splits) { return splits > 1 ? 3.f + (float)(8 * splits * of.M * of.N) / 4e6f : 0.f; };
+  const auto per_split = [](const ColsSize& of, int splits) -> int64_t {   // 0: not cut so
+    const int64_t per = tiles_of(of.k_tiles, splits);
+    return splits == 1 || (per >= 4 && tiles_of(of.k_tiles, per) == splits) ? per : 0;
+  };
+  for (int s = 0; s < (int)(sizeof(kColsShapes) / sizeof(kColsShapes[0])); ++s) {
+    const int bm = kColsShapes[s].bm, bn = kColsShapes[s].bn;
+    const int64_t x_tiles = tiles_of(of_x.M, bm) * tiles_of(of_x.N, bn), w_tiles = tiles_of(of_w.M, bm) * tiles_of(of_w.N, bn);
+    const int64_t at_once = s == 3 ? 512 : 256;
+    if (x_tiles + w_tiles > 8 * at_once) continue;   // the last of so many rounds does not pay
+    for (int xs : kXSplits) {
+      const int64_t x_per = per_split(of_x, xs);
+      if (x_per == 0 || parts_us(of_x, xs) >= best_us) continue;
+      for (int ws : kWSplits) {
+        const int64_t w_per = per_split(of_w, ws), blocks = x_tiles * xs + w_tiles * ws;
+        if (w_per == 0 || (s == 3 && blocks <= 256)) continue;
+        // what a workgroup of each takes where so many run at a time; the longest, or the whole work and half a workgroup more for the end
+        const int64_t round = std::min(blocks, at_once);
+        const float x_us = expected_table_us(kColsShapes[s].table, round, 64 * x_per), w_us = expected_table_us(kColsShapes[s].table, round, 64 * w_per);
+        const float longest = std::max(x_us, w_us), rounds_us = (x_tiles * xs * x_us + w_tiles * ws * w_us) / at_once + 0.5f * std::min(x_us, w_us);
+        const float us = (blocks > at_once ? std::max(longest, rounds_us) : longest) + parts_us(of_x, xs) + parts_us(of_w, ws);
+        if (us < best_us) {
+          best = {true, {s, xs, (int)x_per, us}, {s, ws, (int)w_per, us}};
+          best_us = us;
+        }
       }
     }
   }
@@ -299,12 +344,11 @@ inline ColsPlan plan_cols(int64_t M, int64_t N, int64_t k_tiles) {
 struct PartEpilogue;   // below; takes whole tiles
 
 template <typename S, typename InT, bool kColA, typename Epilogue>
-__global__ __launch_bounds__(S::kThreads) void product_cols_kernel(ColsProduct x, int tiles_m, int tiles_n, int per_split, Epilogue epilogue) {
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
+TFK_DEVICE void product_cols_tile(const ColsProduct& x, int index, int tiles_m, int tiles_n, int per_split, const Epilogue& epilogue, char* smem) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = tiles_m * tiles_n, split = blockIdx.x / tiles;
+  const int tiles = tiles_m * tiles_n, split = index / tiles;
   int tile_m, tile_n;
-  tile_of_block(blockIdx.x - split * tiles, tiles, tiles_m, tiles_n, tile_m, tile_n);
+  tile_of_block(index - split * tiles, tiles, tiles_m, tiles_n, tile_m, tile_n);
   const int m0 = tile_m * S::BM, n0 = tile_n * S::BN, t0 = split * per_split;
   const int wm = wave / S::WAVES_N, wn = wave % S::WAVES_N;
   float4_t acc[S::TM][S::TN];
@@ -315,6 +359,11 @@ __global__ __launch_bounds__(S::kThreads) void product_cols_kernel(ColsProduct x
   if (std::is_same_v<Epilogue, PartEpilogue>) epilogue.template run<true>(acc, at);
   else if (m0 >= x.row_from && m0 + S::BM <= x.a.extent && n0 + S::BN <= x.b.extent) epilogue.template run<true>(acc, at);
   else epilogue.template run<false>(acc, at);
+}
+template <typename S, typename InT, bool kColA, typename Epilogue>
+__global__ __launch_bounds__(S::kThreads) void product_cols_kernel(ColsProduct x, int tiles_m, int tiles_n, int per_split, Epilogue epilogue) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  product_cols_tile<S, InT, kColA>(x, blockIdx.x, tiles_m, tiles_n, per_split, epilogue, smem);
 }
 
 template <typename S, typename InT, bool kColA, typename Epilogue>
@@ -386,6 +435,65 @@ struct PartEpilogue {
     }
   }
 };
+// Either of them.
+template <typename Whole>
+struct CutEpilogue {
+  Whole whole;
+  PartEpilogue part;
+  bool cut;
+
+  template <bool kInside, int TM, int TN>
+  TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
+    if (cut) part.template run<true>(acc, at);
+    else whole.template run<kInside>(acc, at);
+  }
+};
+
+// Both products of a backward pass in one launch.
+template <typename Epilogue>
+struct ColsLaunch {
+  ColsProduct x;
+  int tiles_m, tiles_n, per_split, blocks;
+  Epilogue epilogue;
+};
+// Workgroups begin in the order of their numbers: those with the longer sums first.
+template <typename S, typename InT, typename RowsEpilogue, typename ColsEpilogue>
+__global__ __launch_bounds__(S::kThreads) void product_pair_kernel(ColsLaunch<RowsEpilogue> rows, ColsLaunch<ColsEpilogue> cols) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  int index = blockIdx.x;
+  bool of_rows;
+  if (rows.per_split >= cols.per_split) {
+    of_rows = index < rows.blocks;
+    if (!of_rows) index -= rows.blocks;
+  } else {
+    of_rows = index >= cols.blocks;
+    if (of_rows) index -= cols.blocks;
+  }
+  if (of_rows) product_cols_tile<S, InT, false>(rows.x, index, rows.tiles_m, rows.tiles_n, rows.per_split, rows.epilogue, smem);
+  else product_cols_tile<S, InT, true>(cols.x, index, cols.tiles_m, cols.tiles_n, cols.per_split, cols.epilogue, smem);
+}
+template <typename S, typename InT, typename RowsEpilogue, typename ColsEpilogue>
+int launch_pair_shape(const char* who, const ColsProduct& x, const ColsPlan& x_plan, const RowsEpilogue& x_epilogue, const ColsProduct& w,
+                      const ColsPlan& w_plan, const ColsEpilogue& w_epilogue, hipStream_t st) {
+  auto kern = product_pair_kernel<S, InT, RowsEpilogue, ColsEpilogue>;
+  TFK_LDS_OPT_IN(kern, S::kLdsBytes);
+  const auto tiles = [](const ColsOperand& t, int tile) { return tiles_of(t.extent, tile); };
+  const int64_t x_blocks = tiles(x.a, S::BM) * tiles(x.b, S::BN) * x_plan.splits, w_blocks = tiles(w.a, S::BM) * tiles(w.b, S::BN) * w_plan.splits;
+  TFK_REQUIRE(x_blocks + w_blocks <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
+  return launch_kernel(
+      kern, dim3((unsigned)(x_blocks + w_blocks)), dim3(S::kThreads), S::kLdsBytes, st,
+      ColsLaunch<RowsEpilogue>{x, (int)tiles(x.a, S::BM), (int)tiles(x.b, S::BN), x_plan.per_split, (int)x_blocks, x_epilogue},
+      ColsLaunch<ColsEpilogue>{w, (int)tiles(w.a, S::BM), (int)tiles(w.b, S::BN), w_plan.per_split, (int)w_blocks, w_epilogue});
+}
+template <typename InT, typename RowsEpilogue, typename ColsEpilogue>
+int launch_pair(const char* who, const ColsProduct& x, const ColsPlan& x_plan, const RowsEpilogue& x_epilogue, const ColsProduct& w,
+                const ColsPlan& w_plan, const ColsEpilogue& w_epilogue, hipStream_t st) {
+  if (x_plan.shape == 0) return launch_pair_shape<Ring64Shape<256, 256, 2>, InT>(who, x, x_plan, x_epilogue, w, w_plan, w_epilogue, st);
+  if (x_plan.shape == 1) return launch_pair_shape<Ring64Shape<256, 128, 2>, InT>(who, x, x_plan, x_epilogue, w, w_plan, w_epilogue, st);
+  if (x_plan.shape == 2) return launch_pair_shape<Ring64Shape<128, 128, 4>, InT>(who, x, x_plan, x_epilogue, w, w_plan, w_epilogue, st);
+  return launch_pair_shape<Ring64Shape<128, 128, 2>, InT>(who, x, x_plan, x_epilogue, w, w_plan, w_epilogue, st);
+}
+
 // The room that the parts of a product with M x N results take, in floats, and its rows and pitch.
 struct PartsRoom {
   int64_t rows, pitch, floats;

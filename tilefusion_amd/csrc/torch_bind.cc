@@ -1,5 +1,6 @@
 // PyTorch operator bindings: registers torch.ops.tilefusion.{gemm, fused_two_gemms,
-// flash_attention, flash_attention_fwd, flash_attention_fwd_kt, flash_decode} for the CUDA dispatch key (HIP tensors
+// flash_attention, flash_attention_fwd, flash_attention_fwd_kt, flash_decode, scatter_nd, quantize_rows, gemm_int8, gated_ffn, gated_ffn_backward,
+// linear_cross_entropy, linear_cross_entropy_backward} for the CUDA dispatch key (HIP tensors
 // are "cuda" tensors on PyTorch-ROCm) and forwards to the C ABI in tilefusion_c.h on the
 // caller's current stream.
 //
