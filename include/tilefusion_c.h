@@ -227,7 +227,7 @@ TF_API int tf_scatter_nd(const void* updates, void* data, const int64_t* indices
                          int index_depth, int dtype, void* stream);
 
 /* C[M,N] = scale_a[m] * scale_b[n] * sum_k A[m,k] * B[n,k] of 8-bit integers: A [M,K] and B [N,K] int8, row-major; scale_a [M] and
- * scale_b [N] fp32; C [M,N] of c_dtype (fp32, fp16 or bf16).  The sum is exact (int32), hence K <= 131071; it is scaled in fp32 and
+ * scale_b [N] fp32; C [M,N] of c_dtype (fp32, fp16 or bf16).  The sum is exact (int32), hence K <= 131071; it is multiplied by scale_a, then by scale_b in fp32, and
  * rounded once.  M = 0 and N = 0 are done at once.  At most 2^23 tiles of 64 x 64 results.  A and B begin at 16-byte boundaries; where K is no multiple of 16 they may begin
  * anywhere, and a workspace (at a 16-byte boundary, of the bytes that the function beside it says, otherwise 0) takes copies of them.
  * (No counterpart in the reference.) */

@@ -230,3 +230,21 @@ def test_no_plan_has_more_tiles_than_a_launch():
     for m, n in ((1, (1 << 28) - 64), (16, (1 << 28) - 64), (100, (1 << 28) - 64), (1 << 20, 16), ((1 << 22) - 64, 64)):
         bm, bn = tile[lib.tf_product_kernel_index(m, n, 64, 0)]
         assert -(-m // bm) * -(-n // bn) < 1 << 23, (m, n)
+
+
+def test_neither_a_recorded_call_nor_its_backward_pass_is_captured(monkeypatch):
+    import importlib
+    import types
+
+    leaf = torch.zeros(1, requires_grad=True)
+    autograd = importlib.import_module("tilefusion_amd.ops._autograd")
+    assert autograd.records("op", leaf) and not autograd.records("op", leaf.detach())
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert not autograd.records("op", leaf.detach())
+    with pytest.raises(RuntimeError, match="op: .*captured"):
+        autograd.records("op", leaf)
+    for name, function in (("gated_ffn", "_GatedFfn"), ("linear_cross_entropy", "_LinearCrossEntropy")):
+        backward = getattr(importlib.import_module("tilefusion_amd.ops." + name), function).backward
+        with pytest.raises(RuntimeError, match=name + ": .*captured"):
+            backward(types.SimpleNamespace(needs_input_grad=(True,) * 4), leaf.detach(), None)

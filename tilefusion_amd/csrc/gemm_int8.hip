@@ -1,6 +1,6 @@
 // Products of 8-bit integers with a scale for each row of either operand, and the quantisation of rows that makes the first of them:
 //
-//   C[m, n] = scale_a[m] * scale_b[n] * sum_k A[m, k] * B[n, k]
+//   C[m, n] = (sum_k A[m, k] * B[n, k]) * scale_a[m] * scale_b[n]
 //
 // The sum is exact in int32 (|A|, |B| <= 128: K <= 131071); it is converted to fp32, scaled, and rounded once to the result's type.
 #include "product.hpp"

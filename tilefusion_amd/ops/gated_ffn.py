@@ -5,7 +5,7 @@ from typing import Any, Tuple, Union
 import torch
 
 from .. import _direct
-from ._autograd import records
+from ._autograd import not_captured, records
 
 __all__ = ["gated_ffn", "gated_ffn_backward"]
 
@@ -72,6 +72,7 @@ class _GatedFfn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_h: torch.Tensor, *_: Any) -> Tuple[Any, ...]:
+        not_captured("gated_ffn")
         of_x, of_gate, of_up, _ = ctx.needs_input_grad
         return (*_backward(grad_h, *ctx.saved_tensors, ctx.activation, of_x, of_gate or of_up), None)
 
@@ -88,7 +89,7 @@ def gated_ffn(
         keep: also return x @ w_gate.T and x @ w_up.T, rounded to the type, for `gated_ffn_backward`.
 
     Returns h [.., F], or (h, gate, up).  Everything is fp32 up to h, which is rounded once.  Under autograd h carries the backward
-    pass (once: no gradient of a gradient), and gate and up none; calls that are captured into a graph are not recorded.
+    pass (once: no gradient of a gradient), and gate and up none; neither the call nor that pass is captured into a graph.
     """
     if not torch.compiler.is_compiling():
         direct = _direct.gated_ffn(x, w_gate, w_up, activation, keep)   # (no gradient is asked for)

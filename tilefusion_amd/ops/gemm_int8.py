@@ -44,7 +44,7 @@ def gemm_int8(
         scale_b: [N] fp32, one for each output channel.
         tensor_c: [M, N] fp32, fp16 or bf16.
 
-    The sum is exact (int32; K <= 131071), scaled in fp32 and rounded once.
+    The sum is exact (int32; K <= 131071), multiplied by scale_a, then by scale_b in fp32 and rounded once.  No gradient passes through.
     """
     if not torch.compiler.is_compiling() and _direct.gemm_int8(tensor_a, tensor_b, scale_a, scale_b, tensor_c):
         return

@@ -5,7 +5,7 @@ from typing import Any, Tuple
 import torch
 
 from .. import _direct
-from ._autograd import records
+from ._autograd import not_captured, records
 
 __all__ = ["linear_cross_entropy", "linear_cross_entropy_backward"]
 
@@ -70,6 +70,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad_loss: torch.Tensor, _: Any) -> Tuple[Any, ...]:
+        not_captured("linear_cross_entropy")
         of_hidden, of_weight, _, _ = ctx.needs_input_grad
         return (*_backward(grad_loss, *ctx.saved_tensors, ctx.ignore_index, of_hidden, of_weight), None, None)
 
@@ -87,7 +88,7 @@ def linear_cross_entropy(
 
     Returns (loss, lse), both [..] fp32: the loss of every token, for the caller to weigh and add up, and the logarithm of the sum of
     exp(logits), which `linear_cross_entropy_backward` takes.  Under autograd the loss carries the backward pass (once: no
-    gradient of a gradient), and lse none; calls that are captured into a graph are not recorded.
+    gradient of a gradient), and lse none; neither the call nor that pass is captured into a graph.
     """
     if not torch.compiler.is_compiling():
         direct = _direct.linear_cross_entropy(hidden, weight, target, ignore_index)   # (no gradient is asked for)
