@@ -96,7 +96,8 @@ def linear_cross_entropy(hidden, weight, target, ignore_index):
 
 
 def linear_cross_entropy_backward(grad_loss, hidden, weight, target, ignore_index):
-    """(grad_hidden, grad_weight) and their bounds: softmax gradients are rounded to the type, relative to the largest |grad_loss|."""
+    """(grad_hidden, grad_weight) and their bounds: softmax gradients are rounded to the type, relative to the largest |grad_loss|, and so
+    are the rows of hidden times what grad_loss is more than a power of two, m in (0.5, 1]."""
     dtype = hidden.dtype
     z, off = product(hidden, weight)
     lse = torch.logsumexp(z, dim=1, keepdim=True)
@@ -110,9 +111,14 @@ def linear_cross_entropy_backward(grad_loss, hidden, weight, target, ignore_inde
     signed = (p - one) * g
     top = g.abs().max()
     # rounded to the type; fp16 holds them times 2^14 relative to at least the largest |grad_loss|
-    off_p = off_p * g.abs() + (half_step(dtype) + 2.0 ** -23) * signed.abs() + (2.0 ** -38 * 2 * top if dtype == torch.float16 else 2.0 ** -120 * top)
+    # (and four roundings in fp32: grad_loss divided by a number, the power of two times the softmax gradient, the factor of the row, the sum times it)
+    off_p = off_p * g.abs() + (half_step(dtype) + 2.0 ** -22) * signed.abs() + (2.0 ** -38 * 2 * top if dtype == torch.float16 else 2.0 ** -120 * top)
     off_p = torch.where(valid.bool(), off_p, torch.zeros_like(off_p))
-    return _products([(signed, off_p, weight.t()), (signed.t(), off_p.t(), hidden.t())], dtype)
+    off_w = off_p + half_step(dtype) * (signed.abs() + off_p)   # m * hidden, rounded
+    values, bounds = _products([(signed, off_p, weight.t()), (signed.t(), off_w.t(), hidden.t())], dtype)
+    # m * hidden below the normal numbers is off by TINY / 2; what it is multiplied by is signed / m, less than twice as much
+    bounds[1] = bounds[1] + TINY[dtype] * signed.abs().sum(0)[:, None]
+    return values, bounds
 
 
 def assert_within(got, want, bound, what=""):

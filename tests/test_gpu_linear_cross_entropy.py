@@ -226,6 +226,28 @@ def test_the_size_of_grad_loss_does_not_matter(dtype, size):
             0 if dtype == torch.bfloat16 else 2 * ref.half_step(dtype) * (b.double() * by).abs().max())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["mean", "sequences"])
+def test_one_weight_for_many_tokens_is_not_rounded_as_one(dtype, kind):
+    """The largest term of a gradient is a token's grad_loss itself: rounded to 16 bits it would be off by the same for all tokens of the same
+    grad_loss, here just over halfway between two numbers of the type and just over a power of two, where that is most."""
+    t, v, k = 512, 4096, 256
+    hidden, weight, target, g = _head(t, v, k, dtype, seed=13, ignored=False)
+    step = 2 * ref.half_step(dtype)
+    grad_loss = torch.full((t,), 1 + step * 0.52, device=DEV)
+    if kind == "sequences":   # the last one's is another
+        grad_loss[-64:] = 0.8
+    lse = ops.linear_cross_entropy(hidden, weight, target)[1]
+    grads = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse)
+    want, _ = ref.linear_cross_entropy_backward(grad_loss, hidden, weight, target, -100)
+    # Errors that are independent from element to element: of rounding the result (1), of m * hidden (1, for the weight where m is not 1), and of softmax
+    # gradients, p - 1 at the target, p up to a few hundredths (under 0.6): at most sqrt(1 + 1 + 0.36) = 1.54 times the result's alone.  Rounded
+    # as one number: half a step over 1 is 2.4 times that (uniform errors: sqrt(3) times over their mean square, 1.4 for the binade), 2.6 in all.
+    for got, a in zip(grads, want):
+        alone = (a.to(dtype).double() - a).norm()
+        assert (got.double() - a).norm() <= 1.75 * alone, (got.double() - a).norm() / alone
+
+
 def test_gradient_against_differences():
     # the loss itself along a direction: central differences of step 2^-4 on values that are multiples of it (exact in fp16)
     g = torch.Generator(device=DEV).manual_seed(8)

@@ -264,8 +264,8 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
   const ColsOperand tokens = {bits(x), p.Kp, (int)p.Kp, (int)K};
   const ColsProduct of_w = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)(p.Fp + F)}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
   T *const to_x = static_cast<T*>(dx), *const to_gate = static_cast<T*>(dw_gate), *const to_up = static_cast<T*>(dw_up);
-  const WholeEpilogue<T> whole_x = {to_x, nullptr, (int)M, (int)K};
-  const BothEpilogue<T> whole_w = {{to_gate, nullptr, (int)F, (int)K}, {to_up != nullptr ? to_up - p.Fp * K : nullptr, nullptr, (int)(p.Fp + F), (int)K}, (int)p.Fp};
+  const WholeEpilogue<T> whole_x = {to_x, {}, (int)M, (int)K};
+  const BothEpilogue<T> whole_w = {{to_gate, {}, (int)F, (int)K}, {to_up != nullptr ? to_up - p.Fp * K : nullptr, {}, (int)(p.Fp + F), (int)K}, (int)p.Fp};
   const bool together = dx != nullptr && dw_gate != nullptr && p.both.together;
   const ColsPlan &x_plan = together ? p.both.x : p.of_x, &w_plan = together ? p.both.w : p.of_w;
   const PartsRoom x_room(x_plan, M, K), w_room(w_plan, p.Fp + F, K);
@@ -279,14 +279,14 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
     if (!together)
       if (int rc = x_plan.splits == 1 ? launch_cols<T, false>(who, of_x, x_plan, whole_x, st) : launch_cols<T, false>(who, of_x, x_plan, part_x, st)) return rc;
     if (x_plan.splits > 1)
-      if (int rc = launch_sum_parts<T>(parts, x_room, x_plan.splits, 0, M, K, to_x, nullptr, st)) return rc;
+      if (int rc = launch_sum_parts<T>(parts, x_room, x_plan.splits, 0, M, K, to_x, {}, st)) return rc;
   }
   if (dw_gate == nullptr) return TF_OK;
   if (!together)
     if (int rc = w_plan.splits == 1 ? launch_cols<T, true>(who, of_w, w_plan, whole_w, st) : launch_cols<T, true>(who, of_w, w_plan, part_w, st)) return rc;
   if (w_plan.splits == 1) return TF_OK;
-  if (int rc = launch_sum_parts<T>(w_parts, w_room, w_plan.splits, 0, F, K, to_gate, nullptr, st)) return rc;
-  return launch_sum_parts<T>(w_parts, w_room, w_plan.splits, p.Fp, p.Fp + F, K, to_up, nullptr, st);
+  if (int rc = launch_sum_parts<T>(w_parts, w_room, w_plan.splits, 0, F, K, to_gate, {}, st)) return rc;
+  return launch_sum_parts<T>(w_parts, w_room, w_plan.splits, p.Fp, p.Fp + F, K, to_up, {}, st);
 }
 
 int check_sizes(const char* who, int dtype, int activation, int64_t M, int64_t F, int64_t K) {

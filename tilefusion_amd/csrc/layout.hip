@@ -40,9 +40,9 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(uint16_t* dst, int64_t c
 constexpr int kSumChunks = 64, kSumWays = kThreads / kSumChunks;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sum_parts_kernel(const float* __restrict__ parts, int64_t part, int64_t pitch, int splits, int64_t first,
-                                                             int64_t count, int N, int chunks, T* __restrict__ out, const Scale* scale) {
+                                                             int64_t count, int N, int chunks, T* __restrict__ out, Factors factors) {
   __shared__ float4_t s_sum[kSumWays][kSumChunks];
-  const float by = scale != nullptr ? scale->out : 1.f;
+  const float common = factors.common();
   typedef T out4_t __attribute__((ext_vector_type(4)));
   typedef out4_t out4_any_t __attribute__((aligned(sizeof(T))));
   const int lane = threadIdx.x % kSumChunks, way = threadIdx.x / kSumChunks;
@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kThreads) void sum_parts_kernel(const float* __rest
     if (way == 0 && base + lane < count) {
 #pragma unroll
       for (int w = 1; w < kSumWays; ++w) v += s_sum[w][lane];
-      v *= by;
+      v *= common * factors.of_row(row);
       T* const to = out + row * N + col;
       if (col + 4 <= N) {
         *reinterpret_cast<out4_any_t*>(to) = out4_t{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
@@ -104,13 +104,13 @@ int launch_zero_16bit(void* dst, int64_t count, hipStream_t st) {
 }
 
 template <typename T>
-int launch_sum_parts(const float* parts, const PartsRoom& room, int splits, int64_t first, int64_t M, int64_t N, T* out, const Scale* scale,
+int launch_sum_parts(const float* parts, const PartsRoom& room, int splits, int64_t first, int64_t M, int64_t N, T* out, const Factors& factors,
                      hipStream_t st) {
   const int64_t chunks = tiles_of(N, 4), count = (M - first) * chunks;
   return launch_kernel(sum_parts_kernel<T>, dim3(blocks_for(tiles_of(count, kSumChunks) * kThreads)), dim3(kThreads), 0, st, parts, room.rows * room.pitch, room.pitch, splits, first, count,
-                       (int)N, (int)chunks, out, scale);
+                       (int)N, (int)chunks, out, factors);
 }
-template int launch_sum_parts<half_t>(const float*, const PartsRoom&, int, int64_t, int64_t, int64_t, half_t*, const Scale*, hipStream_t);
-template int launch_sum_parts<bf16_t>(const float*, const PartsRoom&, int, int64_t, int64_t, int64_t, bf16_t*, const Scale*, hipStream_t);
+template int launch_sum_parts<half_t>(const float*, const PartsRoom&, int, int64_t, int64_t, int64_t, half_t*, const Factors&, hipStream_t);
+template int launch_sum_parts<bf16_t>(const float*, const PartsRoom&, int, int64_t, int64_t, int64_t, bf16_t*, const Factors&, hipStream_t);
 
 }  // namespace tfk

@@ -8,10 +8,14 @@
 // (rows of K that is no multiple of 8 are copied first, completed by zeros to whole lines)
 //
 // Backward, a piece of the vocabulary at a time: the product is computed again, and from lse
-//   P[t, v] = grad_loss[t] * (exp(z[t, v] - lse[t]) - [v = target[t]]),   dH += P * W,   dW = P^T * H.
-// P of a piece is rounded to 16 bits, as the operand of a matrix instruction has to be; in fp16 divided by the smallest power of two that no
-// |grad_loss| is above, times 2^14, so that the weights of a mean over many tokens do not fall below the type's range: the sums are
-// multiplied by it again in 32 bits.  (bf16 has the range of fp32.)  dH is summed over the pieces in fp32 and rounded once.
+//   P[t, v] = w[t] * (exp(z[t, v] - lse[t]) - [v = target[t]]),   dH[t] += m[t] * (P * W)[t],   dW = P^T * (m * H),   grad_loss = w * m.
+// P of a piece is rounded to 16 bits, as the operand of a matrix instruction has to be.  At the target it is nearly -w[t], the largest part of both
+// gradients by far: with all of grad_loss in w, what 16 bits leave out of that one number would be an error of everything that a token (and with a
+// mean every token) adds, up to 2.5 times in all what rounding the results leaves out.  So w is a power of two, and m in (0.5, 1]: dH is
+// multiplied by it in 32 bits, and the rounding of m * H is another one for each element (1.4 times as much).  What m takes out of all tokens
+// is the mantissa of the last one's grad_loss: where they have the same, m is 1 and nothing is rounded.
+// In fp16 P is multiplied by a power of two as well by which the largest is 2^15 at most, so that the weights of a mean over many tokens do not fall
+// below the type's range; the sums are divided by it in 32 bits.  (bf16 has the range of fp32.)  dH is summed over the pieces in fp32 and rounded once.
 #include <cmath>
 
 #include "product.hpp"
@@ -119,26 +123,82 @@ __global__ __launch_bounds__(kMergeThreads) void merge_parts_kernel(const Part* 
 }
 
 // ---- backward ------------------------------------------------------------------------------
-constexpr int kScaleThreads = 1024;
-__global__ __launch_bounds__(kScaleThreads) void find_scale_kernel(const float* __restrict__ grad_loss, const int64_t* __restrict__ target,
-                                                                   int64_t ignore_index, int T, Scale* scale) {
-  __shared__ float s_top[kScaleThreads / 64];
+// x = power * m, power a power of two with x's sign and m in (0.5, 1]; numbers without a mantissa of their own (0, those below the normal ones,
+// infinities, NaN) keep m = 1.
+struct Split {
+  float power, m;
+};
+TFK_DEVICE Split split(float x) {
+  const unsigned bits = __float_as_uint(x), exponent = bits >> 23 & 0xff;
+  if (exponent == 0 || exponent == 0xff || (bits & 0x7fffffu) == 0) return {x, 1.f};
+  return {__uint_as_float((bits & 0x80000000u) | min(exponent + 1, 254u) << 23), __uint_as_float((bits & 0x7fffffu) | 126u << 23)};
+}
+
+// What a backward pass takes from grad_loss: w (0 for ignored tokens, NaN for targets outside the vocabulary, as the loss), m, and m * H in rows of `width`.
+// Everything is a quarter of grad_loss, divided by the last token's mantissa: factors[tokens] makes up for that, factors[t] has m as well.
+// The first workgroup looks for the largest as well, where there is a scale.
+constexpr int kWeighThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const float* __restrict__ grad_loss, const int64_t* __restrict__ target,
+                                                                     int64_t ignore_index, int tokens, int V, Scale* scale, float* __restrict__ weights,
+                                                                     float* __restrict__ factors, const T* __restrict__ hidden, T* __restrict__ weighted,
+                                                                     int K, int width) {
+  typedef T eight_t __attribute__((ext_vector_type(8)));
+  typedef eight_t eight_any_t __attribute__((aligned(2)));
+  const auto counts = [&](int64_t wanted) __attribute__((always_inline)) { return wanted != ignore_index && wanted >= 0 && wanted < V; };
+  // (every load of a thread is on its way before the first is waited for: a call of few tokens is as long as its latencies)
+  const int64_t wanted_last = target[tokens - 1];
+  const float grad_last = grad_loss[tokens - 1];
+  const int64_t first = (int64_t)blockIdx.x * kWeighThreads + threadIdx.x, step = (int64_t)gridDim.x * kWeighThreads;
+  const auto common_of = [&]() __attribute__((always_inline)) { return counts(wanted_last) ? split(grad_last).m : 1.f; };
+  if (weighted != nullptr) {
+    const unsigned chunks = (unsigned)width / 8;
+    const int64_t count = (int64_t)tokens * chunks;
+    for (int64_t i = first; i < count; i += step) {
+      const int64_t row = count < ((int64_t)1 << 32) ? (unsigned)i / chunks : i / chunks;
+      const int col = (int)(i - row * chunks) * 8;
+      const int64_t wanted = target[row];
+      const float grad = grad_loss[row];
+      eight_t v;
+      if (col + 8 <= K) {
+        v = *reinterpret_cast<const eight_any_t*>(hidden + row * K + col);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) v[t] = col + t < K ? hidden[row * K + col + t] : (T)0.f;
+      }
+      const float m = counts(wanted) ? split(grad * 0.25f / common_of()).m : 1.f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) v[t] = (T)((float)v[t] * m);
+      *reinterpret_cast<eight_t*>(weighted + i * 8) = v;
+    }
+  }
+  for (int64_t t = first; t < tokens; t += step) {
+    const int64_t wanted = target[t];
+    const float grad = grad_loss[t], common = common_of();
+    const Split s = counts(wanted) ? split(grad * 0.25f / common) : Split{wanted == ignore_index ? 0.f : __uint_as_float(0x7fc00000u), 1.f};
+    weights[t] = s.power;
+    factors[t] = 4.f * common * s.m;
+    if (t == 0) factors[tokens] = 4.f * common;
+  }
+  if (scale == nullptr || blockIdx.x != 0) return;
+  __shared__ float s_top[kWeighThreads / 64];
   float top = 0.f;
-  for (int t = threadIdx.x; t < T; t += kScaleThreads)
+  for (int t = threadIdx.x; t < tokens; t += kWeighThreads)
     if (target[t] != ignore_index) top = fmaxf(top, fabsf(grad_loss[t]));
 #pragma unroll
   for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
   if (threadIdx.x % 64 == 0) s_top[threadIdx.x / 64] = top;
   __syncthreads();
   if (threadIdx.x != 0) return;
-  for (int w = 1; w < kScaleThreads / 64; ++w) top = fmaxf(top, s_top[w]);
+  for (int w = 1; w < kWeighThreads / 64; ++w) top = fmaxf(top, s_top[w]);
   int e = 0;
   if (top > 0.f && top < INFINITY) {
     const float m = frexpf(top, &e);   // top = m * 2^e, 0.5 <= m < 1
     if (m == 0.5f) --e;
   }
-  e = max(e, -110);   // (2^(14 - e) has to fit as well)
-  *scale = Scale{ldexpf(1.f, 14 - e), ldexpf(1.f, e - 14)};
+  // A quarter of the largest, divided by a mantissa, is 2^(e - 1) at most, and so is its power of two.
+  e = max(e, -110);   // (2^(16 - e) has to fit as well)
+  *scale = Scale{ldexpf(1.f, 16 - e), ldexpf(1.f, e - 16)};
 }
 
 template <typename T>
@@ -146,12 +206,12 @@ struct ProbEpilogue {
   T* p;                    // [tokens][pitch], the piece's first column
   int64_t pitch;
   int pad;                 // columns of zeros in front of it
-  const float *lse, *grad_loss;
+  const float *lse, *weights;
   const Scale* scale;      // null: 1
   const int64_t* target;
   int64_t ignore_index;
   int M, N;                // tokens, columns of the piece
-  int first, V;            // the piece's first column, columns of all
+  int first;               // the piece's first column
 
   template <bool kInside, int TM, int TN>
   TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
@@ -163,8 +223,7 @@ struct ProbEpilogue {
       const int64_t wanted = target[row];
       const bool ignored = wanted == ignore_index;
       const float origin = lse[row] * kLog2e;
-      // (a target outside the vocabulary: as the loss)
-      const float weight = wanted >= 0 && wanted < V ? grad_loss[row] * in : __uint_as_float(0x7fc00000u);
+      const float weight = weights[row] * in;
       const int64_t hot = wanted - first - at.col;   // counted from the tile's first column
       float4_t v[TN];
 #pragma unroll
@@ -220,7 +279,7 @@ struct BackwardPlan {
   int64_t width, piece, pieces;      // K with its zeros, columns of a piece (the last may have fewer)
   ColsPlan of_hidden, of_weight;     // (the last piece's are as those of the others)
   PairPlan both;                     // where both are asked for
-  size_t scale, hidden, weight, hidden_parts, weight_parts, bytes;   // offsets in the workspace (of P: 0), its size
+  size_t scale, weights, factors, weighted, hidden, weight, hidden_parts, weight_parts, bytes;   // offsets in the workspace (of P: 0), its size
   BackwardPlan(int64_t T, int64_t V, int64_t K) {
     width = aligned_width(K);
     piece = std::min(round_up_to(V, 64), std::max<int64_t>(4096, kPieceElements / T / 256 * 256));
@@ -237,6 +296,9 @@ struct BackwardPlan {
     };
     take(2 * T * piece);
     scale = take(sizeof(Scale));
+    weights = take(4 * T);
+    factors = take(4 * (T + 1));
+    weighted = take(2 * T * width);
     hidden = take(width != K ? 2 * T * width : 0);
     weight = take(width != K ? 2 * piece * width : 0);
     const auto floats = [K](const ColsPlan& plan, bool cut, int64_t rows) { return cut ? PartsRoom(plan, rows, K).floats : 0; };
@@ -281,8 +343,12 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
   Scale* const scale = kScaled ? reinterpret_cast<Scale*>(ws + plan.scale) : nullptr;
   float* const hidden_parts = reinterpret_cast<float*>(ws + plan.hidden_parts);
   float* const weight_parts = reinterpret_cast<float*>(ws + plan.weight_parts);
-  if constexpr (kScaled)
-    if (int rc = launch_kernel(find_scale_kernel, dim3(1), dim3(kScaleThreads), 0, st, grad_loss, target, ignore_index, (int)tokens, scale)) return rc;
+  float *const weights = reinterpret_cast<float*>(ws + plan.weights), *const factors = reinterpret_cast<float*>(ws + plan.factors);
+  T* const weighted = grad_weight != nullptr ? reinterpret_cast<T*>(ws + plan.weighted) : nullptr;
+  const int64_t items = weighted != nullptr ? tokens * (plan.width / 8) : tokens;
+  if (int rc = launch_kernel(weigh_tokens_kernel<T>, dim3((unsigned)std::min<int64_t>(tiles_of(items, kWeighThreads), 4096)), dim3(kWeighThreads), 0, st, grad_loss,
+                             target, ignore_index, (int)tokens, (int)V, scale, weights, factors, static_cast<const T*>(hidden), weighted, (int)K, (int)plan.width))
+    return rc;
   if (plan.width != K) {
     const RowsToCopy copy = {hidden, tokens, ws + plan.hidden, tokens};
     if (int rc = launch_copy_rows(&copy, 1, 2 * K, 2 * plan.width, st)) return rc;
@@ -291,7 +357,8 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
   const auto bits = [](const void* t) { return static_cast<const uint16_t*>(t); };
   const int width = (int)plan.width;
   const int t_tiles = (int)tiles_of(tokens, 64), t_pad = (int)(t_tiles * 64 - tokens);
-  const ColsOperand of_tokens = {bits(hidden), width, width, (int)K};
+  const ColsOperand of_tokens = {bits(weighted), width, width, (int)K};
+  const Factors by_hidden = {scale, nullptr, factors}, by_weight = {scale, factors + tokens, nullptr};
   const bool together = grad_hidden != nullptr && grad_weight != nullptr && plan.both.together;
   const ColsPlan &of_hidden = together ? plan.both.x : plan.of_hidden, &of_weight = together ? plan.both.w : plan.of_weight;
   const PartsRoom hidden_room(of_hidden, tokens, K), weight_room(of_weight, plan.piece, K);
@@ -307,8 +374,8 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
     }
     const Operands logits = {hidden, {w, nullptr}, (int)tokens, (int)columns, width};
     if (int rc = launch_product<T, false>(who, logits, plan_product(tokens, columns, width, false),
-                                          ProbEpilogue<T>{p + pad, pitch, pad, lse, grad_loss, scale, target, ignore_index, (int)tokens, (int)columns,
-                                                          (int)first, (int)V},
+                                          ProbEpilogue<T>{p + pad, pitch, pad, lse, weights, scale, target, ignore_index, (int)tokens, (int)columns,
+                                                          (int)first},
                                           st))
       return rc;
 
@@ -319,8 +386,8 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
     const ColsProduct hidden_product = {{bits(p), pitch, (int)pitch, (int)tokens}, {bits(w), width, width, (int)K}, bits(w), INT_MAX, (int)(pitch / 64), pad, 0};
     const ColsProduct weight_product = {{bits(p), pitch, (int)pitch, (int)pitch}, of_tokens, of_tokens.x, INT_MAX, t_tiles, t_pad, pad};
     T* const out = grad_weight != nullptr ? static_cast<T*>(grad_weight) + first * K : nullptr;
-    const WholeEpilogue<T> whole_hidden = {static_cast<T*>(grad_hidden), scale, (int)tokens, (int)K};
-    const WholeEpilogue<T> whole_weight = {out != nullptr ? out - (int64_t)pad * K : nullptr, scale, (int)pitch, (int)K};
+    const WholeEpilogue<T> whole_hidden = {static_cast<T*>(grad_hidden), by_hidden, (int)tokens, (int)K};
+    const WholeEpilogue<T> whole_weight = {out != nullptr ? out - (int64_t)pad * K : nullptr, by_weight, (int)pitch, (int)K};
     const PartEpilogue part_hidden = {hidden_parts, hidden_room.rows, hidden_room.pitch, first > 0};
     const PartEpilogue part_weight = {weight_parts, weight_room.rows, weight_room.pitch, false};
     int rc = TF_OK;
@@ -336,11 +403,11 @@ int backward(const float* grad_loss, const void* hidden, const void* weight, con
                         : launch_cols<T, true>(who, weight_product, of_weight, whole_weight, st);
     }
     if (rc == TF_OK && grad_weight != nullptr && cut_weight)
-      rc = launch_sum_parts<T>(weight_parts, weight_room, of_weight.splits, pad, pitch, K, out, scale, st);
+      rc = launch_sum_parts<T>(weight_parts, weight_room, of_weight.splits, pad, pitch, K, out, by_weight, st);
     if (rc) return rc;
   }
   if (grad_hidden == nullptr || !cut_hidden) return TF_OK;
-  return launch_sum_parts<T>(hidden_parts, hidden_room, of_hidden.splits, 0, tokens, K, static_cast<T*>(grad_hidden), scale, st);
+  return launch_sum_parts<T>(hidden_parts, hidden_room, of_hidden.splits, 0, tokens, K, static_cast<T*>(grad_hidden), by_hidden, st);
 }
 
 int check_sizes(const char* who, int dtype, int64_t T, int64_t V, int64_t K) {

@@ -389,18 +389,28 @@ int launch_cols(const char* who, const ColsProduct& x, const ColsPlan& plan, con
 struct Scale {
   float in, out;   // operands were multiplied by `in` where they were made, sums are by `out`
 };
-// A sum that is complete: scaled (where there is a scale), rounded to T.
+// What sums are multiplied by, where it is not null: a scale, one number for all, one for each row.
+struct Factors {
+  const Scale* scale = nullptr;
+  const float *all = nullptr, *rows = nullptr;
+
+  TFK_DEVICE float common() const { return (scale != nullptr ? scale->out : 1.f) * (all != nullptr ? *all : 1.f); }
+  TFK_DEVICE float of_row(int64_t row) const { return rows != nullptr ? rows[row] : 1.f; }
+};
+// A sum that is complete: multiplied by its factors, rounded to T.
 template <typename T>
 struct WholeEpilogue {
   T* out;                  // [M][N]
-  const Scale* scale;      // or null
+  Factors factors;
   int M, N;
 
   template <bool kInside, int TM, int TN>
   TFK_DEVICE void run(float4_t (&acc)[TM][TN], const TileAt& at) const {
-    const float by = scale != nullptr ? scale->out : 1.f;
+    const float common = factors.common();
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
+      const int row = at.row + 16 * i + (at.lane & 15);
+      const float by = common * factors.of_row(kInside ? row : min(row, M - 1));
       float4_t v[TN];
 #pragma unroll
       for (int j = 0; j < TN; ++j) v[j] = acc[i][j] * by;
@@ -500,9 +510,9 @@ struct PartsRoom {
   PartsRoom(const ColsPlan& plan, int64_t M, int64_t N)
       : rows(round_up_to(M, kColsShapes[plan.shape].bm)), pitch(round_up_to(N, kColsShapes[plan.shape].bn)), floats(plan.splits * rows * pitch) {}
 };
-// out = T(by * the sum of the parts): rows `first` .. M - 1, of which the first is out's; N columns
+// out = T(the sum of the parts, times its factors): rows `first` .. M - 1, of which the first is out's and the factors'; N columns
 template <typename T>
-int launch_sum_parts(const float* parts, const PartsRoom& room, int splits, int64_t first, int64_t M, int64_t N, T* out, const Scale* scale,
+int launch_sum_parts(const float* parts, const PartsRoom& room, int splits, int64_t first, int64_t M, int64_t N, T* out, const Factors& factors,
                      hipStream_t st);
 
 // ------------------------------------------------------------------------------------------

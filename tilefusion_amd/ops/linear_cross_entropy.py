@@ -110,8 +110,9 @@ def linear_cross_entropy_backward(
     """Gradients of hidden and weight, of their type, from that of the loss [..] (fp32) and the lse of the forward call.
 
     The vocabulary is done in pieces; what is held of a piece are its softmax gradients in 16 bits, which is where they are
-    rounded: relative to the largest |grad_loss|, so that no weight of a mean is too small for fp16.  A grad_loss of an
-    ignored token is not looked at; tokens with a target outside the vocabulary make NaN of the gradients they have a part in."""
+    rounded: relative to the largest |grad_loss|, so that no weight of a mean is too small for fp16.  They have the power of two in
+    a token's grad_loss; what is left of it is rounded with hidden, where tokens differ in it.  A grad_loss of an ignored
+    token is not looked at; tokens with a target outside the vocabulary make NaN of the gradients they have a part in."""
     if not torch.compiler.is_compiling():
         direct = _direct.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index)
         if direct is not None:
