@@ -319,13 +319,13 @@ inline PairPlan plan_pair(const ColsPlan& x, const ColsSize& of_x, const ColsPla
     const int bm = kColsShapes[s].bm, bn = kColsShapes[s].bn;
     const int64_t x_tiles = tiles_of(of_x.M, bm) * tiles_of(of_x.N, bn), w_tiles = tiles_of(of_w.M, bm) * tiles_of(of_w.N, bn);
     const int64_t at_once = s == 3 ? 512 : 256;
-    if (x_tiles + w_tiles > 8 * at_once) continue;   // the last of so many rounds does not pay
     for (int xs : kXSplits) {
       const int64_t x_per = per_split(of_x, xs);
-      if (x_per == 0 || parts_us(of_x, xs) >= best_us) continue;
+      if (x_per == 0 || x_tiles * xs > 8 * at_once || parts_us(of_x, xs) >= best_us) continue;
       for (int ws : kWSplits) {
         const int64_t w_per = per_split(of_w, ws), blocks = x_tiles * xs + w_tiles * ws;
-        if (w_per == 0 || (s == 3 && blocks <= 256)) continue;
+        // (the last of more than eight rounds does not pay, and parts of so many tiles are half a gigabyte)
+        if (w_per == 0 || blocks > 8 * at_once || (s == 3 && blocks <= 256)) continue;
         // what a workgroup of each takes where so many run at a time; the longest, or the whole work and half a workgroup more for the end
         const int64_t round = std::min(blocks, at_once);
         const float x_us = expected_table_us(kColsShapes[s].table, round, 64 * x_per), w_us = expected_table_us(kColsShapes[s].table, round, 64 * w_per);
