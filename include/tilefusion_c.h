@@ -293,10 +293,12 @@ TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* 
 /* tf_product_kernel_index: position in kGemmKernels of what tf_gemm_int8 (K: half its own), tf_gated_ffn (two = 1, N: F) and tf_linear_cross_entropy
  * and the first product of its backward pass (N: columns of the vocabulary or of a piece) run; -1 for other arguments.  tf_product_cols_plan: position in kColsShapes
  * (csrc/product.hpp) of the tile of a gradient of M x N that is a sum over `rows` rows, and in *parts the parts that the sum is cut into.
- * tf_product_pair_plan: the same of two gradients that are asked for together and run in one launch; -1 where they run one after the other. */
+ * tf_product_pair_plan: the same of two gradients that are asked for together and run in one launch; -1 where they run one after the other.
+ * tf_linear_cross_entropy_backward_piece: columns of the vocabulary that the backward pass does at a time (the last piece may have fewer). */
 TF_API int tf_product_kernel_index(int64_t M, int64_t N, int64_t K, int two);
 TF_API int tf_product_cols_plan(int64_t M, int64_t N, int64_t rows, int* parts);
 TF_API int tf_product_pair_plan(int64_t M, int64_t N, int64_t rows, int64_t M2, int64_t N2, int64_t rows2, int* parts, int* parts2);
+TF_API int64_t tf_linear_cross_entropy_backward_piece(int64_t T, int64_t V, int64_t K);
 TF_API int tf_gemm_kernel_index(int64_t M, int64_t N, int64_t K, int c_is_f32);
 TF_API int tf_flash_decode_plan(int64_t batch_heads, int64_t Lkv, int64_t D, int num_splits, int* wavefronts);
 TF_API int tf_flash_attention_rows(int64_t batch, int64_t Lq, int64_t Lkv, int64_t D, int causal);

@@ -137,6 +137,31 @@ def test_offsets_that_pass_32_bits():
         assert (got.double() - want).norm() <= 2 * ref.half_step(torch.bfloat16) * want.norm() * 1.5
 
 
+@pytest.mark.parametrize("t", [1, 2, 3])
+def test_few_tokens_and_a_table_of_very_many_words(t):
+    # rows of softmax gradients that 32-bit offsets would not reach 63 of: pieces of the vocabulary
+    v, k, some = 34_100_001, 8, 500
+    assert _capi.load().tf_linear_cross_entropy_backward_piece(t, v, k) < v
+    g = torch.Generator(device=DEV).manual_seed(14)
+    hidden = torch.randn(t, k, device=DEV, generator=g, dtype=torch.bfloat16)
+    weight = torch.randn(v, k, device=DEV, generator=g, dtype=torch.bfloat16)
+    target = torch.tensor([v - 1, 7, 1 << 25], device=DEV)[:t]   # the last word, one in front, the first of the second piece
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    grad_hidden, grad_weight = ops.linear_cross_entropy_backward(torch.ones(t, device=DEV), hidden, weight, target, lse)
+    z, off = ref.product(hidden, weight)
+    want_lse = torch.logsumexp(z, 1)
+    bound = off.amax(1) + ref.FN * (1 + want_lse.abs())
+    ref.assert_within(lse, want_lse, bound)
+    ref.assert_within(loss, want_lse - z.gather(1, target[:, None])[:, 0], 2 * bound)
+    p = torch.exp(z - want_lse[:, None])
+    p[torch.arange(t, device=DEV), target] -= 1
+    want = p @ weight.double()
+    assert (grad_hidden.double() - want).norm() <= 3 * ref.half_step(torch.bfloat16) * want.norm()
+    for words in (slice(0, some), slice((1 << 25) - some, (1 << 25) + some), slice(v - some, v)):
+        want = p[:, words].t().contiguous() @ hidden.double()
+        assert (grad_weight[words].double() - want).norm() <= 3 * ref.half_step(torch.bfloat16) * want.norm()
+
+
 def test_shapes_strides_and_alignment():
     hidden, weight, target, g = _head(60, 300, 80, torch.float16, seed=3)
     _check_forward(hidden.view(3, 20, 80), weight, target.view(3, 20))

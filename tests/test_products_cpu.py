@@ -232,6 +232,26 @@ def test_no_plan_has_more_tiles_than_a_launch():
         assert -(-m // bm) * -(-n // bn) < 1 << 23, (m, n)
 
 
+def test_offsets_of_a_gradient_stay_within_32_bits():
+    """Lanes walk 64 rows of an operand that is summed over its rows, and up to 256 of one that is not, by 32-bit offsets: from kLead bytes
+    in front of the first row on, to its farthest 16 bytes of 512."""
+    piece = _capi.load().tf_linear_cross_entropy_backward_piece
+
+    def farthest(rows, pitch):
+        return 2 * (rows - 1) * pitch + 512 + 4096
+
+    most = (1 << 28) - 64
+    for t in (1, 2, 3, 4, 5, 31, 32, 33, 63, 64, 100, 256, 1000, 32768, (1 << 22) - 64):
+        for v in (1, 64, 65, 34_100_000, 34_100_224, 1 << 25, 1 << 26, 1 << 27, most):
+            columns = piece(t, v, 8)   # P's pitch
+            assert 0 < columns <= -(-v // 64) * 64 and columns % 64 == 0
+            assert farthest(64, columns) < 1 << 32 and farthest(min(t, 256), columns) < 1 << 32, (t, v)
+    # the gated block's: rows of [dg | du], of weights and of tokens
+    f, k = (1 << 21) - 64, (1 << 22) - 64
+    assert farthest(256, 2 * f) < 1 << 32 and farthest(64, k) < 1 << 32
+    assert piece(0, 4, 4) == -1 == piece(4, 0, 4) == piece(4, 4, 0) == piece(4, 1 << 28, 4)
+
+
 def test_neither_a_recorded_call_nor_its_backward_pass_is_captured(monkeypatch):
     import importlib
     import types

@@ -55,6 +55,7 @@ SIGNATURES = {
     "tf_product_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_product_cols_plan": (_i, [_i64, _i64, _i64, ctypes.POINTER(_i)]),
     "tf_product_pair_plan": (_i, [_i64] * 6 + [ctypes.POINTER(_i)] * 2),
+    "tf_linear_cross_entropy_backward_piece": (_i64, [_i64, _i64, _i64]),
     "tf_gemm_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_flash_decode_plan": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_i)]),
     "tf_flash_attention_rows": (_i, [_i64, _i64, _i64, _i64, _i]),

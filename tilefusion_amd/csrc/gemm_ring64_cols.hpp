@@ -24,12 +24,18 @@ struct ColsOperand {
   int extent;            // rows (A by rows) or columns of the result
 };
 
+// Lanes' offsets are counted from that many bytes in front: what an immediate offset takes off may be more than a row has.
+constexpr int kColsLead = 4096;
+// The farthest of them where `rows` rows of a tile are walked, `pitch` elements apart; it has to stay below 2^32.
+__host__ __device__ constexpr uint64_t cols_farthest(int64_t rows, int64_t pitch) { return 2 * (uint64_t)(rows - 1) * (uint64_t)pitch + 512 + kColsLead; }
+
 // The 16-column block that lies in place of block b in row `row` of a tile, and the other way round.
 __host__ __device__ constexpr int cols_swizzle(int row) { return (row & 3) | (row >> 3 & 1) << 2; }
 
 // acc += tile (m0, n0) over the k-tiles t0 .. t0 + num - 1 of 64; m0 and n0 are multiples of 8, and what lies behind the operands' extents
 // is some of theirs again (not to be stored).  The first k-tile begins k_pad rows in front of B (and of A, kColA;
 // otherwise A's rows hold zeros there), which are taken for zeros.  B's rows continue in `b1` from k-tile `turn` on.
+// cols_farthest of 64 rows of an operand by columns, and of the tile's rows of A by rows, is below 2^32.
 template <typename S, typename InT, bool kColA>
 TFK_DEVICE void ring64_multiply_cols(const ColsOperand& a, const ColsOperand& b, const uint16_t* b1, int turn, int m0, int n0, int t0, int num, int k_pad,
                                      int lane, int wave, char* smem, float4_t (&acc)[S::TM][S::TN]) {
@@ -37,7 +43,7 @@ TFK_DEVICE void ring64_multiply_cols(const ColsOperand& a, const ColsOperand& b,
   static_assert(S::free_gaps() >= 8, "a gap for every piece");
   constexpr int kPitchA = S::BM * 2, kPitchB = S::BN * 2;                 // bytes of a row in LDS
   constexpr int kRowsA = 1024 / kPitchA, kRowsB = 1024 / kPitchB;         // rows of a request
-  constexpr int kLead = 4096;   // offsets are counted from there in front: what an immediate offset takes off may be more than a row has
+  constexpr int kLead = kColsLead;
   const int wm = wave / S::WAVES_N, wn = wave % S::WAVES_N;
   const int fr = lane & 15, fg = lane >> 4;
 

@@ -282,7 +282,7 @@ struct BackwardPlan {
   size_t scale, weights, factors, weighted, hidden, weight, hidden_parts, weight_parts, bytes;   // offsets in the workspace (of P: 0), its size
   BackwardPlan(int64_t T, int64_t V, int64_t K) {
     width = aligned_width(K);
-    piece = std::min(round_up_to(V, 64), std::max<int64_t>(4096, kPieceElements / T / 256 * 256));
+    piece = piece_of(T, V);
     pieces = tiles_of(V, piece);
     const ColsSize hidden_size = {T, K, piece / 64}, weight_size = {piece, K, tiles_of(T, 64)};
     of_hidden = plan_cols(hidden_size);
@@ -308,7 +308,12 @@ struct BackwardPlan {
     weight_parts = take(4 * std::max(weight_floats(of_weight), weight_floats(both.w)));
     bytes = at;
   }
+  static int64_t piece_of(int64_t T, int64_t V) {
+    return std::min(round_up_to(V, 64), std::min(kPieceColumns, std::max<int64_t>(4096, kPieceElements / T / 256 * 256)));
+  }
   static constexpr int64_t kPieceElements = (int64_t)1 << 27;   // of P, 256 MiB
+  static constexpr int64_t kPieceColumns = (int64_t)1 << 25;    // P's rows are walked 64 at a time, by 32-bit offsets
+  static_assert(cols_farthest(64, kPieceColumns) < (uint64_t)1 << 32);
 };
 
 template <typename T>
@@ -469,4 +474,10 @@ extern "C" int tf_linear_cross_entropy_backward(const float* grad_loss, const vo
   if (dtype == TF_DTYPE_F16)
     return backward<half_t>(grad_loss, hidden, weight, target, lse, grad_hidden, grad_weight, T, V, K, ignore_index, ws, st);
   return backward<bf16_t>(grad_loss, hidden, weight, target, lse, grad_hidden, grad_weight, T, V, K, ignore_index, ws, st);
+}
+
+extern "C" int64_t tf_linear_cross_entropy_backward_piece(int64_t T, int64_t V, int64_t K) {
+  using namespace tfk;
+  if (T <= 0 || check_sizes("tf_linear_cross_entropy_backward_piece", TF_DTYPE_F16, T, V, K) != TF_OK) return -1;
+  return BackwardPlan::piece_of(T, V);
 }

@@ -367,12 +367,20 @@ __global__ __launch_bounds__(S::kThreads) void product_cols_kernel(ColsProduct x
   product_cols_tile<S, InT, kColA>(x, blockIdx.x, tiles_m, tiles_n, per_split, epilogue, smem);
 }
 
+// Whether 32-bit offsets reach the operands of a tile.
+template <typename S, bool kColA>
+bool cols_reach(const ColsProduct& x) {
+  constexpr uint64_t kEnd = (uint64_t)1 << 32;
+  return cols_farthest(kColA ? S::BK : std::min(S::BM, x.a.extent), x.a.pitch) < kEnd && cols_farthest(S::BK, x.b.pitch) < kEnd;
+}
+
 template <typename S, typename InT, bool kColA, typename Epilogue>
 int launch_cols_shape(const char* who, const ColsProduct& x, const ColsPlan& plan, const Epilogue& epilogue, hipStream_t st) {
   auto kern = product_cols_kernel<S, InT, kColA, Epilogue>;
   TFK_LDS_OPT_IN(kern, S::kLdsBytes);
   const int64_t tiles_m = tiles_of(x.a.extent, S::BM), tiles_n = tiles_of(x.b.extent, S::BN);
   TFK_REQUIRE(tiles_m * tiles_n * plan.splits <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
+  TFK_REQUIRE((cols_reach<S, kColA>(x)), TF_ERR_INVALID_ARG, "%s: rows too long", who);
   return launch_kernel(kern, dim3((unsigned)(tiles_m * tiles_n * plan.splits)), dim3(S::kThreads), S::kLdsBytes, st, x, (int)tiles_m, (int)tiles_n,
                        plan.per_split, epilogue);
 }
@@ -491,6 +499,7 @@ int launch_pair_shape(const char* who, const ColsProduct& x, const ColsPlan& x_p
   const auto tiles = [](const ColsOperand& t, int tile) { return tiles_of(t.extent, tile); };
   const int64_t x_blocks = tiles(x.a, S::BM) * tiles(x.b, S::BN) * x_plan.splits, w_blocks = tiles(w.a, S::BM) * tiles(w.b, S::BN) * w_plan.splits;
   TFK_REQUIRE(x_blocks + w_blocks <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
+  TFK_REQUIRE((cols_reach<S, false>(x) && cols_reach<S, true>(w)), TF_ERR_INVALID_ARG, "%s: rows too long", who);
   return launch_kernel(
       kern, dim3((unsigned)(x_blocks + w_blocks)), dim3(S::kThreads), S::kLdsBytes, st,
       ColsLaunch<RowsEpilogue>{x, (int)tiles(x.a, S::BM), (int)tiles(x.b, S::BN), x_plan.per_split, (int)x_blocks, x_epilogue},
