@@ -268,3 +268,39 @@ def test_neither_a_recorded_call_nor_its_backward_pass_is_captured(monkeypatch):
         backward = getattr(importlib.import_module("tilefusion_amd.ops." + name), function).backward
         with pytest.raises(RuntimeError, match=name + ": .*captured"):
             backward(types.SimpleNamespace(needs_input_grad=(True,) * 4), leaf.detach(), None)
+
+
+# ---- derivatives that there are not ---------------------------------------------------------
+def _differentiable():
+    gen = torch.Generator().manual_seed(3)
+    x, w, grad = (torch.randn(*s, generator=gen).bfloat16() for s in ((4, 8), (6, 8), (4, 6)))
+    target, one = torch.tensor([0, 5, 2, -100]), torch.ones(4)
+    return x, {
+        "gated_ffn": lambda x: ops.gated_ffn(x, w, w),
+        "gated_ffn_backward": lambda x: ops.gated_ffn_backward(grad, x, w, w, grad, grad)[0],
+        "linear_cross_entropy": lambda x: ops.linear_cross_entropy(x, w, target)[0],
+        "linear_cross_entropy_backward": lambda x: ops.linear_cross_entropy_backward(one, x, w, target, one)[0],
+    }
+
+
+@pytest.mark.parametrize("name", list(_differentiable()[1]))
+def test_forward_mode_and_transforms_are_refused(name):
+    # (their results are written into fresh tensors, whose tangent would be zero)
+    x, calls = _differentiable()
+    call = calls[name]
+    with pytest.raises(RuntimeError, match=f"{name}: there are no forward-mode"):
+        torch.func.jvp(call, (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError, match=f"{name}: there are no forward-mode"):
+        torch.func.jacfwd(call)(x)
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(RuntimeError, match=f"{name}: there are no forward-mode"):
+            call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(RuntimeError, match=f"{name}: does not work under torch.func"):
+        torch.func.grad(lambda x: call(x).float().sum())(x)
+    with pytest.raises(RuntimeError, match=f"{name}: does not work under torch.func"):
+        torch.func.vmap(call)(torch.stack([x, x]))
+    # inside a dual level or a transform, on tensors that have no part in it, the call goes on (to an op that has no kernel on the CPU)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        call(x)
+    with pytest.raises(NotImplementedError):
+        torch.func.grad(lambda y: (y * call(x).float().sum()).sum())(torch.ones(3))

@@ -1,6 +1,9 @@
 """When the operators with a backward pass record it."""
 
+from typing import Any
+
 import torch
+from torch.autograd import forward_ad
 
 
 def not_captured(op: str) -> None:
@@ -15,8 +18,22 @@ def not_captured(op: str) -> None:
         )
 
 
+def refuse_transforms(op: str, *tensors: Any) -> None:
+    """Refuses inputs that carry a derivative which nothing here passes on: a tangent, or the wrapper of a transform of torch.func.
+
+    The operators write into tensors of their own, whose derivative would be zero without a word."""
+    functorch = torch._C._functorch
+    for t in tensors:
+        if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{op}: there are no forward-mode derivatives")
+        # (compiled code can ask whether a transform is at work, and not whether it is on t)
+        if functorch.maybe_current_level() is not None and (torch.compiler.is_compiling() or functorch.is_functorch_wrapped_tensor(t)):
+            raise RuntimeError(f"{op}: does not work under torch.func's transforms")
+
+
 def records(op: str, *tensors: torch.Tensor) -> bool:
     """Whether a call on `tensors` is to be recorded for autograd."""
+    refuse_transforms(op, *tensors)
     if not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
         return False
     not_captured(op)

@@ -5,7 +5,7 @@ from typing import Any, Tuple, Union
 import torch
 
 from .. import _direct
-from ._autograd import not_captured, records
+from ._autograd import not_captured, records, refuse_transforms
 
 __all__ = ["gated_ffn", "gated_ffn_backward"]
 
@@ -89,7 +89,7 @@ def gated_ffn(
         keep: also return x @ w_gate.T and x @ w_up.T, rounded to the type, for `gated_ffn_backward`.
 
     Returns h [.., F], or (h, gate, up).  Everything is fp32 up to h, which is rounded once.  Under autograd h carries the backward
-    pass (once: no gradient of a gradient), and gate and up none; neither the call nor that pass is captured into a graph.
+    pass (once: no gradient of a gradient, no forward mode), and gate and up none; neither the call nor that pass is captured into a graph.
     """
     if not torch.compiler.is_compiling():
         direct = _direct.gated_ffn(x, w_gate, w_up, activation, keep)   # (no gradient is asked for)
@@ -118,4 +118,5 @@ def gated_ffn_backward(
         direct = _direct.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation)
         if direct is not None:
             return direct[0], direct[1][0], direct[1][1]
+    refuse_transforms("gated_ffn_backward", grad_h, x, w_gate, w_up, gate, up)
     return _backward(grad_h, x, w_gate, w_up, gate, up, activation, True, True)

@@ -5,7 +5,7 @@ from typing import Any, Tuple
 import torch
 
 from .. import _direct
-from ._autograd import not_captured, records
+from ._autograd import not_captured, records, refuse_transforms
 
 __all__ = ["linear_cross_entropy", "linear_cross_entropy_backward"]
 
@@ -88,7 +88,7 @@ def linear_cross_entropy(
 
     Returns (loss, lse), both [..] fp32: the loss of every token, for the caller to weigh and add up, and the logarithm of the sum of
     exp(logits), which `linear_cross_entropy_backward` takes.  Under autograd the loss carries the backward pass (once: no
-    gradient of a gradient), and lse none; neither the call nor that pass is captured into a graph.
+    gradient of a gradient, no forward mode), and lse none; neither the call nor that pass is captured into a graph.
     """
     if not torch.compiler.is_compiling():
         direct = _direct.linear_cross_entropy(hidden, weight, target, ignore_index)   # (no gradient is asked for)
@@ -117,4 +117,5 @@ def linear_cross_entropy_backward(
         direct = _direct.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse, ignore_index)
         if direct is not None:
             return direct
+    refuse_transforms("linear_cross_entropy_backward", grad_loss, hidden, weight, lse)
     return _backward(grad_loss, hidden, weight, target, lse, ignore_index, True, True)
