@@ -207,6 +207,14 @@ def test_backward_shapes_strides_and_empty():
     assert ops.gated_ffn(torch.empty(2, 0, 48, device=DEV, dtype=dtype), w[0], w[1]).shape == (2, 0, 72)
 
 
+@pytest.mark.parametrize("asked", [(0,), (1,), (2,), (0, 1, 2)])
+def test_autograd_of_no_tokens(asked):
+    leaves = [torch.randn(*s, device=DEV).half().requires_grad_(i in asked) for i, s in enumerate(((0, 48), (72, 48), (72, 48)))]
+    ops.gated_ffn(*leaves).sum().backward()
+    for i, leaf in enumerate(leaves):
+        assert (leaf.grad == 0).all() and leaf.grad.shape == leaf.shape if i in asked else leaf.grad is None
+
+
 def test_backward_with_any_workspace_and_gradients_apart():
     # a workspace that holds NaN, one that is just large enough, and gradients of the weights that lie anywhere
     m, f, k = 70, 40, 24

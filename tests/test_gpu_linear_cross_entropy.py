@@ -367,6 +367,14 @@ def test_autograd_replay_streams_and_empty():
     assert grad_hidden.shape == (0, 72) and (grad_weight == 0).all()
 
 
+@pytest.mark.parametrize("asked", [(0,), (1,), (0, 1)])
+def test_autograd_of_no_tokens(asked):
+    leaves = [torch.randn(*s, device=DEV).bfloat16().requires_grad_(i in asked) for i, s in enumerate(((0, 24), (100, 24)))]
+    ops.linear_cross_entropy(*leaves, torch.empty(0, device=DEV, dtype=torch.int64))[0].sum().backward()
+    for i, leaf in enumerate(leaves):
+        assert (leaf.grad == 0).all() and leaf.grad.shape == leaf.shape if i in asked else leaf.grad is None
+
+
 def test_refusals():
     hidden, weight, target, _ = _head(8, 32, 16, torch.float16)
     for bad in ((hidden, weight.bfloat16(), target), (hidden, weight[:, :8], target), (hidden, weight, target[:4]), (hidden, weight, target.int()),

@@ -87,6 +87,15 @@ def test_linear_cross_entropy_arguments():
     assert lib.tf_linear_cross_entropy(*[None] * 5, F16, 0, 100, 64, -100, None, 0, None) == OK
 
 
+def test_gradients_of_no_tokens_alone():
+    # a tensor without elements has no address: that of grad_x, asked for without the weights' (as where they are frozen), is null
+    lib = _capi.load()
+    for f in (F16, BF16):
+        assert lib.tf_gated_ffn_backward(*[None] * 9, f, 0, 0, 64, 64, None, 0, None) == OK
+        assert lib.tf_linear_cross_entropy_backward(*[None] * 7, f, 0, 100, 64, -100, None, 0, None) == OK
+    assert lib.tf_gated_ffn_backward(*[None] * 8, P, F16, 0, 0, 64, 64, None, 0, None) == BAD   # of one weight
+
+
 def test_workspace_of_the_backward_pass_is_a_piece_of_the_vocabulary():
     size = _capi.load().tf_linear_cross_entropy_backward_workspace_bytes
     # 8192 tokens x 131072 words: the logits are 2 GiB in 16 bits; and it does not grow with the vocabulary from some size on

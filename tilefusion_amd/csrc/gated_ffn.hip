@@ -336,9 +336,9 @@ extern "C" int tf_gated_ffn_backward(const void* dh, const void* x, const void* 
                                      size_t workspace_bytes, void* stream) {
   using namespace tfk;
   if (int rc = check_sizes("tf_gated_ffn_backward", dtype, activation, M, F, K)) return rc;
-  TFK_REQUIRE((dw_gate == nullptr) == (dw_up == nullptr) && (dx || dw_gate), TF_ERR_INVALID_ARG,
-              "tf_gated_ffn_backward: the gradients of both weights or of neither, and of something");
-  if (M > 0) {
+  TFK_REQUIRE((dw_gate == nullptr) == (dw_up == nullptr), TF_ERR_INVALID_ARG, "tf_gated_ffn_backward: the gradients of both weights or of neither");
+  if (M > 0) {   // (dx of no tokens may be null all the same)
+    TFK_REQUIRE(dx || dw_gate, TF_ERR_INVALID_ARG, "tf_gated_ffn_backward: no gradient asked for");
     TFK_REQUIRE(dh && x && w_gate && w_up && gate && up, TF_ERR_INVALID_ARG, "tf_gated_ffn_backward: null pointer");
     TFK_REQUIRE(K % 8 != 0 || (at_16B(x) && at_16B(w_gate) && at_16B(w_up)), TF_ERR_INVALID_ARG,
                 "tf_gated_ffn_backward: x and the weights must begin at 16-byte boundaries");

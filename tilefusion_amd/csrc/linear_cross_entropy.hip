@@ -459,8 +459,8 @@ extern "C" int tf_linear_cross_entropy_backward(const float* grad_loss, const vo
                                                 void* workspace, size_t workspace_bytes, void* stream) {
   using namespace tfk;
   if (int rc = check_sizes("tf_linear_cross_entropy_backward", dtype, T, V, K)) return rc;
-  TFK_REQUIRE(grad_weight || grad_hidden, TF_ERR_INVALID_ARG, "tf_linear_cross_entropy_backward: no gradient asked for");
-  if (T > 0) {
+  if (T > 0) {   // (grad_hidden of no tokens may be null all the same)
+    TFK_REQUIRE(grad_weight || grad_hidden, TF_ERR_INVALID_ARG, "tf_linear_cross_entropy_backward: no gradient asked for");
     TFK_REQUIRE(grad_loss && hidden && weight && target && lse, TF_ERR_INVALID_ARG,
                 "tf_linear_cross_entropy_backward: null pointer");
     TFK_REQUIRE(K % 8 != 0 || (at_16B(hidden) && at_16B(weight)), TF_ERR_INVALID_ARG,
