@@ -203,6 +203,28 @@ def test_ignored_and_invalid_targets():
         assert grad_weight.isnan().all() and grad_hidden[5].isnan().all() and grad_hidden[:5].isfinite().all() and grad_hidden[6:].isfinite().all()
 
 
+@pytest.mark.parametrize("t,v,k", [(1, 100, 64), (37, 1000, 72), (200, 513, 65), (613, 3001, 128), (1100, 700, 264)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_whatever_stands_in_an_ignored_tokens_row(t, v, k, dtype):
+    # a padded batch: rows that nothing was ever written to
+    hidden, weight, target, g = _head(t, v, k, dtype, seed=15, ignored=False)
+    grad_loss = torch.rand(t, device=DEV, generator=g)
+    target[::3] = -100
+    clean = hidden.clone()
+    clean[::3] = 0
+    hidden[::3, ::2], hidden[::3, 1::2] = float("nan"), float("inf")
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    want_loss, want_lse = ops.linear_cross_entropy(clean, weight, target)
+    counted = target != -100
+    assert torch.equal(loss, want_loss) and torch.equal(lse[counted], want_lse[counted]) and (loss[::3] == 0).all()
+    want = ops.linear_cross_entropy_backward(grad_loss, clean, weight, target, want_lse)
+    for of_hidden, of_weight in ((True, True), (True, False), (False, True)):
+        got = _one(grad_loss, hidden, weight, target, lse, -100, of_hidden, of_weight)
+        for a, b in zip(got, want if of_hidden and of_weight else _one(grad_loss, clean, weight, target, want_lse, -100, of_hidden, of_weight)):
+            assert b is None if a is None else a.isfinite().all() and torch.equal(a, b)
+    assert (want[0][::3] == 0).all()
+
+
 def test_infinite_logits_and_nan_stay_with_their_token():
     hidden, weight, target, _ = _head(150, 300, 64, torch.float16, seed=5, ignored=False)
     clean = ops.linear_cross_entropy(hidden, weight, target)

@@ -134,7 +134,8 @@ TFK_DEVICE Split split(float x) {
   return {__uint_as_float((bits & 0x80000000u) | min(exponent + 1, 254u) << 23), __uint_as_float((bits & 0x7fffffu) | 126u << 23)};
 }
 
-// What a backward pass takes from grad_loss: w (0 for ignored tokens, NaN for targets outside the vocabulary, as the loss), m, and m * H in rows of `width`.
+// What a backward pass takes from grad_loss: w (0 for ignored tokens, NaN for targets outside the vocabulary, as the loss), m, and m * H in rows of `width`,
+// zeros for ignored tokens.
 // Everything is a quarter of grad_loss, divided by the last token's mantissa: factors[tokens] makes up for that, factors[t] has m as well.
 // The first workgroup looks for the largest as well, where there is a scale.
 constexpr int kWeighThreads = 256;
@@ -167,8 +168,10 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const float
         for (int t = 0; t < 8; ++t) v[t] = col + t < K ? hidden[row * K + col + t] : (T)0.f;
       }
       const float m = counts(wanted) ? split(grad * 0.25f / common_of()).m : 1.f;
+      // (an ignored token's row is what its P, zeros, are multiplied by: it may hold anything, and zero times a NaN is one)
+      const bool ignored = wanted == ignore_index;
 #pragma unroll
-      for (int t = 0; t < 8; ++t) v[t] = (T)((float)v[t] * m);
+      for (int t = 0; t < 8; ++t) v[t] = ignored ? (T)0.f : (T)((float)v[t] * m);
       *reinterpret_cast<eight_t*>(weighted + i * 8) = v;
     }
   }
