@@ -1,6 +1,7 @@
 """The gated feed-forward block against its 64-bit form, forward and backward."""
 
 import importlib
+import math
 
 import pytest
 import torch
@@ -104,6 +105,43 @@ def test_large_gates():
         grads = ops.gated_ffn_backward(one, x, w_gate, w_up, gate, up, activation)
         # (x[0]'s gradient is the sum of w_gate and of act(w_gate), 6e38, which is infinite in the type)
         assert all(t.isfinite().all() for t in (grads[0][1], grads[1], grads[2])) and grads[0][0] == float("inf")
+
+
+def _far(g, activation):
+    """How far an activation in fp32 may be off, relative to its terms: a few roundings, and exp's argument, which is off by its own rounding."""
+    return 2.0 ** -20 + 2.0 ** -21 * {"silu": g.abs(), "gelu": g * g / 2, "gelu_tanh": 1.6 * (g + 0.044715 * g ** 3).abs()}[activation]
+
+
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_activations_are_right_in_their_leading_digits(dtype, activation):
+    # every number of the type from -14 to 14 as a gate that is no sum, far out on the left as well, where the activation is small
+    values = torch.arange(0, 0x8000, device=DEV, dtype=torch.int16).view(dtype)
+    values = values[values.abs() <= 14]
+    values = torch.cat([values, -values])
+    step, tiny, g = ref.half_step(dtype), ref.TINY[dtype], values.double()
+    up = 1024.0 if dtype == torch.float16 else 1.0   # (h reaches further down in fp16 so)
+    x = torch.zeros(len(values), 8, device=DEV, dtype=dtype)
+    x[:, 0], x[:, 1] = values, 1.0
+    w_gate, w_up = torch.zeros(2, 1, 8, device=DEV, dtype=dtype)
+    w_gate[0, 0], w_up[0, 1] = 1.0, up
+    h = ops.gated_ffn(x, w_gate, w_up, activation)[:, 0].double()
+    far = _far(g, activation)
+    # (torch.special.ndtr is (1 + erf) / 2, without leading digits from -8 on)
+    phi = torch.special.erfc(-g / math.sqrt(2)) / 2 if activation == "gelu" else ref.phi(g, activation)
+    rest = ref.act_slope(g, activation) - ref.phi(g, activation)   # g * phi'(g)
+    if activation == "gelu":
+        rest = g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    want, small = up * g * phi, 2.0 ** -120 * up   # (fp32 below its normal numbers)
+    assert ((h - want).abs() <= (far + step * (1 + far)) * want.abs() + tiny + small).all()
+    # the gradients of gate and up, each through a weight of one number
+    gate, ones = values[:, None], torch.ones(len(values), 1, device=DEV, dtype=dtype)
+    one, none = torch.ones(1, 8, device=DEV, dtype=dtype), torch.zeros(1, 8, device=DEV, dtype=dtype)
+    grad_gate = ops.gated_ffn_backward(ones * up, x, one, none, gate, ones, activation)[0][:, 3].double()
+    grad_up = ops.gated_ffn_backward(ones * up, x, none, one, gate, ones, activation)[0][:, 3].double()
+    assert ((grad_up - want).abs() <= (far + step * (1 + far)) * want.abs() + tiny + small).all()
+    slope, terms = up * (phi + rest), up * (phi + rest.abs())
+    assert ((grad_gate - slope).abs() <= far * terms + step * (slope.abs() + far * terms) + tiny + small * 16).all()
 
 
 # ---- backward ------------------------------------------------------------------------------

@@ -21,16 +21,22 @@ TFK_DEVICE float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + exp_of(-x
 constexpr float kGeluCubic = 0.044715f;
 constexpr float kGeluTwice = 1.5957691216057308f;   // 2 * sqrt(2 / pi): (1 + tanh(y)) / 2 = sigmoid(2y)
 
-// The normal distribution's weight below -|g|, from exp(-g^2 / 2): Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26
-// (within 1e-7, halved from their bound for erf), and without the difference from 1 that the tail would be lost in.  The library's erff takes both of its branches
-// for every wavefront (2999 x 1032 x 1544 with gate and up kept, fp16: 43 us with it, 32 so).
+// The normal distribution's weight below -|g|, from exp(-g^2 / 2): bell * t * p(t), t = 1 / (1 + 0.28 |g|), where t * p(t) stands for
+// erfcx(|g| / sqrt(2)) / 2.  p is the polynomial of degree 8 whose largest relative error over all g is least (Remez' exchange): 1.7e-7, so that the
+// tail, which is not taken from 1, is right in its leading digits as far out as it is a number of the type.  In fp32 5e-7 up to |g| = 1, and g^2 * 2^-23 further
+// out, by the argument of bell.  The library's erff takes both of its branches for every wavefront (2999 x 1032 x 1544 with gate and up kept, fp16:
+// 43 us with it, 32 so).
 TFK_DEVICE float normal_tail(float g, float bell) {
-  const float t = __builtin_amdgcn_rcpf(1.f + (0.3275911f * 0.7071067811865476f) * fabsf(g));
-  float p = 0.5f * 1.061405429f;
-  p = __builtin_fmaf(p, t, 0.5f * -1.453152027f);
-  p = __builtin_fmaf(p, t, 0.5f * 1.421413741f);
-  p = __builtin_fmaf(p, t, 0.5f * -0.284496736f);
-  p = __builtin_fmaf(p, t, 0.5f * 0.254829592f);
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.28f * fabsf(g));
+  float p = 0.024719954f;
+  p = __builtin_fmaf(p, t, -0.093593046f);
+  p = __builtin_fmaf(p, t, 0.092428006f);
+  p = __builtin_fmaf(p, t, -0.0064490973f);
+  p = __builtin_fmaf(p, t, 0.072774976f);
+  p = __builtin_fmaf(p, t, 0.0836308f);
+  p = __builtin_fmaf(p, t, 0.10308466f);
+  p = __builtin_fmaf(p, t, 0.1116998f);
+  p = __builtin_fmaf(p, t, 0.11170386f);
   return p * t * bell;
 }
 TFK_DEVICE float act_phi(float g, int activation) {
