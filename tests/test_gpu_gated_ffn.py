@@ -144,6 +144,24 @@ def test_activations_are_right_in_their_leading_digits(dtype, activation):
     assert ((grad_gate - slope).abs() <= far * terms + step * (slope.abs() + far * terms) + tiny + small * 16).all()
 
 
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+def test_gates_beyond_the_largest_number_of_fp16(activation):
+    # kept as infinities, they still say which side of the activation they are on: 0 with a slope of 0, the identity with a slope of 1
+    x = torch.tensor([[256.0], [-256.0], [1.0]], device=DEV).half()
+    w_gate, w_up = torch.tensor([[512.0]], device=DEV).half(), torch.tensor([[0.25]], device=DEV).half()
+    h, gate, up = ops.gated_ffn(x, w_gate, w_up, activation, keep=True)
+    assert gate[:2, 0].tolist() == [float("inf"), -float("inf")] and h[1:, 0].tolist() == [0.0, 128.0]
+    grad_h = torch.tensor([[0.0], [0.5], [0.25]], device=DEV).half()
+    grad_x, grad_gate, grad_up = ops.gated_ffn_backward(grad_h[1:], x[1:], w_gate, w_up, gate[1:], up[1:], activation)
+    # token 1: nothing; token 2: dg = 0.25 * 0.25 and du = 0.25 * 512
+    assert grad_x[:, 0].tolist() == [0.0, 0.0625 * 512 + 128 * 0.25] and grad_gate.item() == 0.0625 and grad_up.item() == 128.0
+    # the other side: dg = 0.5 * 64 of a gate that is infinite, in the gradient of the gate's weight
+    one = torch.ones(1, 1, device=DEV).half()
+    grads = ops.gated_ffn_backward(one * 0.5, x[:1], w_gate * 0, w_up * 0, gate[:1], up[:1], activation)
+    assert grads[1].item() == 0.5 * 64 * 256 and grads[2].item() == float("inf")
+    assert ops.gated_ffn_backward(one, one, one, one, one * float("nan"), one, activation)[0].isnan().all()
+
+
 # ---- backward ------------------------------------------------------------------------------
 def _check_backward(grad_h, x, w_gate, w_up, gate, up, activation, alone=False):
     results = [(ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation), (0, 1, 2))]

@@ -48,17 +48,17 @@ TFK_DEVICE float act_phi(float g, int activation) {
   return sigmoid(kGeluTwice * (g + kGeluCubic * g * g * g));
 }
 TFK_DEVICE float act(float g, int activation) { return g * act_phi(g, activation); }
-// act and its derivative
+// act and its derivative; at infinities, which a kept gate beyond the largest number of its type has become, their limits
 TFK_DEVICE void act_both(float g, int activation, float& value, float& slope) {
   if (activation == TF_ACT_GELU) {
     const float bell = exp_of(-0.5f * g * g), tail = normal_tail(g, bell);
     const float p = g < 0.f ? tail : 1.f - tail;
-    value = g * p;
-    slope = p + g * 0.3989422804014327f * bell;
+    value = g == -INFINITY ? 0.f : g * p;
+    slope = bell > 0.f ? p + g * 0.3989422804014327f * bell : p;
     return;
   }
   const float p = act_phi(g, activation);
-  value = g * p;
+  value = g == -INFINITY ? 0.f : g * p;
   const float inner = activation == TF_ACT_SILU ? 1.f : kGeluTwice * (1.f + 3.f * kGeluCubic * g * g);
   const float both = p * (1.f - p);
   slope = both > 0.f ? p + g * both * inner : p;   // (far out the square may be infinite; a NaN stays one)
