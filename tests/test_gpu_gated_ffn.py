@@ -203,6 +203,78 @@ def test_backward_sizes(m, f, k, dtype):
     _check_backward(*(_randn(g, m, f, dtype=dtype) for _ in range(1)), x, w_gate, w_up, _randn(g, m, f, dtype=dtype), _randn(g, m, f, dtype=dtype), "silu", alone=True)
 
 
+def _scaled_backward(grad_h, x, w_gate, w_up, gate, up, activation):
+    """The gradients and their bounds where dg and du have a power of two in common by which the largest is 2^14 to 2^15: what fp16's smallest numbers
+    leave out of one is 2^-25, 2^-39 of the largest."""
+    d, g, u = grad_h.double(), gate.double(), up.double()
+    grads = d * u * ref.act_slope(g, activation), d * ref.act(g, activation)
+    most = 2.0 ** -39 * max(t.abs().max() for t in grads)
+    offs = [ref.FN * size + ref.half_step(x.dtype) * t.abs() + most for t, size in zip(grads, ((d * u).abs() * (1 + g.abs()), (d * g).abs()))]
+    (dg, du), (off_g, off_u) = grads, offs
+    return ref._products([(torch.cat([dg, du], 1), torch.cat([off_g, off_u], 1), torch.cat([w_gate, w_up]).t()), (dg.t(), off_g.t(), x.t()),
+                          (du.t(), off_u.t(), x.t())], x.dtype)
+
+
+# grad_h, up, weights and tokens: dg and du beyond 65504, and below fp16's smallest number, where the gradients that they add up to are not
+RANGES = {"large": (300.0, 300.0, 2.0 ** -10, 2.0 ** -10), "small": (2.0 ** -13, 2.0 ** -9, 1024.0, 1024.0)}
+
+
+@pytest.mark.parametrize("m,f,k", [(1, 64, 64), (70, 40, 24), (130, 96, 200), (257, 136, 264), (31, 100, 33), (2, 2501, 3504), (2493, 1, 3568)])
+@pytest.mark.parametrize("span", list(RANGES))
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+def test_backward_beyond_the_range_of_fp16(m, f, k, span, activation):
+    of_h, of_up, of_w, of_x = RANGES[span]
+    g = torch.Generator(device=DEV).manual_seed(16 + m + f + k)
+    dtype = torch.float16
+    grad_h, gate, up = _randn(g, m, f, dtype=dtype, scale=of_h), _randn(g, m, f, dtype=dtype), _randn(g, m, f, dtype=dtype, scale=of_up)
+    x, w_gate, w_up = _randn(g, m, k, dtype=dtype, scale=of_x), *(_randn(g, f, k, dtype=dtype, scale=of_w) for _ in range(2))
+    if span == "small":   # (du has no part of up, and would be the largest)
+        w_up.zero_()
+        gate *= 2.0 ** -9
+    want, bounds = _scaled_backward(grad_h, x, w_gate, w_up, gate, up, activation)
+    assert (want[0].abs() < 65504).all() and (want[0].abs().max() > 2.0 ** -14)
+    got = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation)
+    some = [_one(grad_h, x, w_gate, w_up, gate, up, activation, of, not of) for of in (True, False)]
+    for grads, of in ((got, (0, 1, 2)), (some[0], (0,)), (some[1], (1, 2))):
+        for i in of:
+            ref.assert_within(grads[i], want[i], bounds[i], f"{i} of {of}")
+            floor = want[i].numel() ** 0.5 * ref.TINY[dtype]
+            assert (grads[i].double() - want[i]).norm() <= 2 * ref.half_step(dtype) * want[i].norm() + floor
+
+
+def test_an_infinite_gradient_does_not_take_the_others_range():
+    # one token's grad_h is infinite (a step that a loss scaler leaves out): the other tokens' gradients are as without it
+    m, f, k = 200, 72, 96
+    x, w_gate, w_up, g = _block(m, f, k, torch.float16, seed=17)
+    grad_h, gate, up = (_randn(g, m, f, dtype=torch.float16, scale=s) for s in (300.0, 1.0, 300.0))
+    w_gate, w_up = w_gate * 2.0 ** -8, w_up * 2.0 ** -8
+    grad_h[7] = 0
+    clean = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up)
+    assert clean[0].isfinite().all()
+    grad_h[7, 5], grad_h[7, 6] = float("inf"), float("nan")
+    grads = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up)
+    others = torch.arange(m, device=DEV) != 7
+    assert torch.equal(grads[0][others], clean[0][others]) and not grads[0][7].isfinite().any()
+
+
+def test_ranges_that_change_between_replays():
+    m, f, k = 140, 72, 96
+    x, w_gate, w_up, g = _block(m, f, k, torch.float16, seed=18)
+    grad_h, gate, up = (_randn(g, m, f, dtype=torch.float16) for _ in range(3))
+    start = grad_h.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up)
+    for by in (1.0, 2.0 ** 14, 2.0 ** -9, 1.0, 0.0):
+        grad_h.copy_(start * by)
+        want = [t.clone() for t in ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up)]
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), by
+
+
 @pytest.mark.parametrize("activation", ACTIVATIONS)
 @pytest.mark.parametrize("dtype", TYPES)
 def test_backward_activations(activation, dtype):

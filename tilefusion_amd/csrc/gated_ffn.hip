@@ -9,7 +9,7 @@
 //   dx = dg * Wg + du * Wu,  dWg = dg^T * x,  dWu = du^T * x
 // One pass over dh, gate and up leaves [dg | du] as rows of tokens, each half completed by zeros to a multiple of 64 columns; dx is one product over the
 // 2F columns, the weights' gradients are one over the tokens.  dg and du are rounded to the type once, as operands of
-// matrix instructions have to be.
+// matrix instructions have to be; in fp16 times a power of two where their own range is not the type's, by which the sums are divided in fp32.
 #include "product.hpp"
 
 namespace tfk {
@@ -133,44 +133,113 @@ int gated_ffn(const void* x, const void* w_gate, const void* w_up, void* h, void
 
 // ---- backward ------------------------------------------------------------------------------
 constexpr int kThreads = 256;
+// dg and du have a power of two in common.  (bf16 has the range of fp32.)
+template <typename T>
+constexpr bool kScaled = std::is_same_v<T, half_t>;
+constexpr int kMostTops = 1024;   // workgroups that look for the largest
 
-// dg and du to rows [dg | du] of pitch 2 * Fp, zeros behind F columns of each.  Eight elements a lane; bound by memory (five streams of 16 bits an
-// element).
+// The largest of the workgroup's numbers, in every thread.
+TFK_DEVICE float largest_of_block(float top) {
+  __shared__ float s_top[kThreads / 64];
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (threadIdx.x % 64 == 0) s_top[threadIdx.x / 64] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) top = fmaxf(top, s_top[w]);
+  return top;
+}
+
+// Elements i * 8 .. of dg and du to rows [dg | du] of pitch 2 * Fp, zeros behind F columns of each, times `in`; the largest finite one of them in `top`.
 template <typename T, int kActivation>
-__global__ __launch_bounds__(kThreads) void gated_ffn_grads_kernel(const T* __restrict__ dh, const T* __restrict__ gate, const T* __restrict__ up,
-                                                                  T* __restrict__ rows, int64_t count, int F, int Fp) {
+TFK_DEVICE void leave_grads(const T* __restrict__ dh, const T* __restrict__ gate, const T* __restrict__ up, T* __restrict__ rows, int64_t i, int chunks, int F,
+                            int Fp, float in, float& top) {
   typedef T eight_t __attribute__((ext_vector_type(8)));
   typedef eight_t eight_any_t __attribute__((aligned(2)));
-  const int chunks = Fp / 8;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t row = i / chunks;
-    const int col = (int)(i - row * chunks) * 8;
-    const size_t at = (size_t)row * F + col;
-    eight_t d, g, u, dg, du;
-    if (col + 8 <= F) {
-      d = *reinterpret_cast<const eight_any_t*>(dh + at);
-      g = *reinterpret_cast<const eight_any_t*>(gate + at);
-      u = *reinterpret_cast<const eight_any_t*>(up + at);
-    } else {
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const bool in = col + t < F;
-        d[t] = in ? dh[at + t] : (T)0.f;
-        g[t] = in ? gate[at + t] : (T)0.f;
-        u[t] = in ? up[at + t] : (T)0.f;
-      }
-    }
+  const int64_t row = i / chunks;
+  const int col = (int)(i - row * chunks) * 8;
+  const size_t at = (size_t)row * F + col;
+  eight_t d, g, u, dg, du;
+  if (col + 8 <= F) {
+    d = *reinterpret_cast<const eight_any_t*>(dh + at);
+    g = *reinterpret_cast<const eight_any_t*>(gate + at);
+    u = *reinterpret_cast<const eight_any_t*>(up + at);
+  } else {
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      float value, slope;
-      act_both((float)g[t], kActivation, value, slope);
-      dg[t] = (T)((float)d[t] * (float)u[t] * slope);
-      du[t] = (T)((float)d[t] * value);
+      const bool inside = col + t < F;
+      d[t] = inside ? dh[at + t] : (T)0.f;
+      g[t] = inside ? gate[at + t] : (T)0.f;
+      u[t] = inside ? up[at + t] : (T)0.f;
     }
-    T* const to = rows + (size_t)row * 2 * Fp + col;
-    *reinterpret_cast<eight_t*>(to) = dg;
-    *reinterpret_cast<eight_t*>(to + Fp) = du;
   }
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    float value, slope;
+    act_both((float)g[t], kActivation, value, slope);
+    const float of_gate = (float)d[t] * (float)u[t] * slope, of_up = (float)d[t] * value;
+    if constexpr (kScaled<T>) {
+      const float most = fmaxf(fabsf(of_gate), fabsf(of_up)), least = fminf(fabsf(of_gate), fabsf(of_up));
+      top = fmaxf(top, most < INFINITY ? most : least < INFINITY ? least : 0.f);
+    }
+    dg[t] = (T)(of_gate * in);
+    du[t] = (T)(of_up * in);
+  }
+  T* const to = rows + (size_t)row * 2 * Fp + col;
+  *reinterpret_cast<eight_t*>(to) = dg;
+  *reinterpret_cast<eight_t*>(to + Fp) = du;
+}
+
+// [dg | du].  Eight elements a lane; bound by memory (five streams of 16 bits an element).  fp16: tops, the largest of each workgroup.
+template <typename T, int kActivation>
+__global__ __launch_bounds__(kThreads) void gated_ffn_grads_kernel(const T* __restrict__ dh, const T* __restrict__ gate, const T* __restrict__ up,
+                                                                  T* __restrict__ rows, float* __restrict__ tops, int64_t count, int F, int Fp) {
+  float top = 0.f;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads)
+    leave_grads<T, kActivation>(dh, gate, up, rows, i, Fp / 8, F, Fp, 1.f, top);
+  if constexpr (kScaled<T>) {
+    top = largest_of_block(top);
+    if (threadIdx.x == 0) tops[blockIdx.x] = top;
+  }
+}
+
+// fp16: where the largest is beyond the type, or so small that fp16's smallest number leaves more out of the others than a rounding of the largest in
+// fp32 would (2^-25 of it: below 1), [dg | du] once more, times a power of two by which the largest is 2^14 to 2^15.  Elsewhere, as with a loss whose scale
+// suits the type, there is nothing to do, and the launch is what it costs: backward passes of 1337 x 1544 x 1032 42.8 -> 46.6 us, 2048 x 1024 x 1024 28.4 -> 31.8,
+// 8192 x 11264 x 4096 2374 -> 2391 (with 4096 workgroups looking and 2048 here 2435: each of these reads what all of those found).
+template <typename T, int kActivation>
+__global__ __launch_bounds__(kThreads) void gated_ffn_rescale_kernel(const T* __restrict__ dh, const T* __restrict__ gate, const T* __restrict__ up,
+                                                                    T* __restrict__ rows, const float* __restrict__ tops, int num_tops, Scale* scale,
+                                                                    int64_t count, int F, int Fp) {
+  float top = 0.f;
+  for (int i = threadIdx.x; i < num_tops; i += kThreads) top = fmaxf(top, tops[i]);
+  top = largest_of_block(top);
+  const bool again = top > 0.f && (top < 1.f || top > 65504.f);
+  int e = 0;
+  frexpf(top, &e);                                  // top = m * 2^e, 0.5 <= m < 1
+  const int by = again ? min(15 - e, 110) : 0;      // (2^-by has to be a number as well)
+  const float in = ldexpf(1.f, by);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *scale = Scale{in, ldexpf(1.f, -by)};
+  if (!again) return;
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < count; i += (int64_t)gridDim.x * kThreads)
+    leave_grads<T, kActivation>(dh, gate, up, rows, i, Fp / 8, F, Fp, in, top);
+}
+
+template <typename T>
+struct GradsKernels {
+  decltype(&gated_ffn_grads_kernel<T, TF_ACT_SILU>) grads;
+  void (*rescale)(const T*, const T*, const T*, T*, const float*, int, Scale*, int64_t, int, int);   // null: not scaled
+};
+template <typename T, int kActivation>
+GradsKernels<T> grads_kernels_of() {
+  if constexpr (kScaled<T>) return {gated_ffn_grads_kernel<T, kActivation>, gated_ffn_rescale_kernel<T, kActivation>};
+  else return {gated_ffn_grads_kernel<T, kActivation>, nullptr};
+}
+template <typename T>
+GradsKernels<T> grads_kernels(int activation) {
+  if (activation == TF_ACT_SILU) return grads_kernels_of<T, TF_ACT_SILU>();
+  if (activation == TF_ACT_GELU) return grads_kernels_of<T, TF_ACT_GELU>();
+  return grads_kernels_of<T, TF_ACT_GELU_TANH>();
 }
 
 struct BackwardPlan {
@@ -179,7 +248,7 @@ struct BackwardPlan {
   ColsPlan of_x, of_w;            // products: dx, the weights' gradients
   PairPlan both;                  // where both are asked for
   int64_t x_floats;               // of dx's parts, which those of the weights' gradients lie behind
-  size_t weights, x, parts, bytes;   // offsets in the workspace ([dg | du]: 0), its size
+  size_t tops, scale, weights, x, parts, bytes;   // offsets in the workspace ([dg | du]: 0), its size
   BackwardPlan(int64_t M, int64_t F, int64_t K) {
     Fp = round_up_to(F, 64);
     Kp = aligned_width(K);
@@ -197,6 +266,8 @@ struct BackwardPlan {
       return from;
     };
     take(2 * M * 2 * Fp);
+    tops = take(sizeof(float) * kMostTops);
+    scale = take(sizeof(Scale));
     weights = take(copy_weights ? 2 * 2 * Fp * Kp : 0);
     x = take(copy_x ? 2 * M * Kp : 0);
     const auto floats = [K](const ColsPlan& plan, int64_t rows) { return plan.splits > 1 ? PartsRoom(plan, rows, K).floats : 0; };
@@ -241,12 +312,17 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
   const BackwardPlan p(M, F, K);
   T* const rows = reinterpret_cast<T*>(ws);
   const int64_t chunks = M * (p.Fp / 8);
-  const auto grads = activation == TF_ACT_SILU   ? gated_ffn_grads_kernel<T, TF_ACT_SILU>
-                     : activation == TF_ACT_GELU ? gated_ffn_grads_kernel<T, TF_ACT_GELU>
-                                                 : gated_ffn_grads_kernel<T, TF_ACT_GELU_TANH>;
-  if (int rc = launch_kernel(grads, dim3((unsigned)std::min<int64_t>(tiles_of(chunks, kThreads), 65536)), dim3(kThreads), 0, st,
-                             static_cast<const T*>(dh), static_cast<const T*>(gate), static_cast<const T*>(up), rows, chunks, (int)F, (int)p.Fp))
+  float* const tops = reinterpret_cast<float*>(ws + p.tops);
+  Scale* const scale = kScaled<T> ? reinterpret_cast<Scale*>(ws + p.scale) : nullptr;
+  const GradsKernels<T> kernels = grads_kernels<T>(activation);
+  const T *const of_h = static_cast<const T*>(dh), *const of_gate = static_cast<const T*>(gate), *const of_up = static_cast<const T*>(up);
+  const int64_t blocks = std::min<int64_t>(tiles_of(chunks, kThreads), kScaled<T> ? kMostTops : 65536);
+  if (int rc = launch_kernel(kernels.grads, dim3((unsigned)blocks), dim3(kThreads), 0, st, of_h, of_gate, of_up, rows, tops, chunks, (int)F, (int)p.Fp))
     return rc;
+  if (scale != nullptr)
+    if (int rc = launch_kernel(kernels.rescale, dim3((unsigned)std::min<int64_t>(blocks, 512)), dim3(kThreads), 0, st, of_h, of_gate, of_up, rows, tops,
+                               (int)blocks, scale, chunks, (int)F, (int)p.Fp))
+      return rc;
   RowsToCopy copies[3];
   int count = 0;
   if (p.copy_weights && dx != nullptr) {
@@ -270,8 +346,9 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
   const ColsOperand tokens = {bits(x), p.Kp, (int)p.Kp, (int)K};
   const ColsProduct of_w = {{grads_at, 2 * p.Fp, (int)(2 * p.Fp), (int)(p.Fp + F)}, tokens, tokens.x, INT_MAX, m_tiles, m_pad, 0};
   T *const to_x = static_cast<T*>(dx), *const to_gate = static_cast<T*>(dw_gate), *const to_up = static_cast<T*>(dw_up);
-  const WholeEpilogue<T> whole_x = {to_x, {}, (int)M, (int)K};
-  const BothEpilogue<T> whole_w = {{to_gate, {}, (int)F, (int)K}, {to_up != nullptr ? to_up - p.Fp * K : nullptr, {}, (int)(p.Fp + F), (int)K}, (int)p.Fp};
+  const Factors by = {scale, nullptr, nullptr};
+  const WholeEpilogue<T> whole_x = {to_x, by, (int)M, (int)K};
+  const BothEpilogue<T> whole_w = {{to_gate, by, (int)F, (int)K}, {to_up != nullptr ? to_up - p.Fp * K : nullptr, by, (int)(p.Fp + F), (int)K}, (int)p.Fp};
   const bool together = dx != nullptr && dw_gate != nullptr && p.both.together;
   const ColsPlan &x_plan = together ? p.both.x : p.of_x, &w_plan = together ? p.both.w : p.of_w;
   const PartsRoom x_room(x_plan, M, K), w_room(w_plan, p.Fp + F, K);
@@ -285,14 +362,14 @@ int gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const 
     if (!together)
       if (int rc = x_plan.splits == 1 ? launch_cols<T, false>(who, of_x, x_plan, whole_x, st) : launch_cols<T, false>(who, of_x, x_plan, part_x, st)) return rc;
     if (x_plan.splits > 1)
-      if (int rc = launch_sum_parts<T>(parts, x_room, x_plan.splits, 0, M, K, to_x, {}, st)) return rc;
+      if (int rc = launch_sum_parts<T>(parts, x_room, x_plan.splits, 0, M, K, to_x, by, st)) return rc;
   }
   if (dw_gate == nullptr) return TF_OK;
   if (!together)
     if (int rc = w_plan.splits == 1 ? launch_cols<T, true>(who, of_w, w_plan, whole_w, st) : launch_cols<T, true>(who, of_w, w_plan, part_w, st)) return rc;
   if (w_plan.splits == 1) return TF_OK;
-  if (int rc = launch_sum_parts<T>(w_parts, w_room, w_plan.splits, 0, F, K, to_gate, {}, st)) return rc;
-  return launch_sum_parts<T>(w_parts, w_room, w_plan.splits, p.Fp, p.Fp + F, K, to_up, {}, st);
+  if (int rc = launch_sum_parts<T>(w_parts, w_room, w_plan.splits, 0, F, K, to_gate, by, st)) return rc;
+  return launch_sum_parts<T>(w_parts, w_room, w_plan.splits, p.Fp, p.Fp + F, K, to_up, by, st);
 }
 
 int check_sizes(const char* who, int dtype, int activation, int64_t M, int64_t F, int64_t K) {

@@ -113,7 +113,9 @@ def gated_ffn_backward(
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients of x, w_gate and w_up, from that of h [.., F] and the gate and up [.., F] that `gated_ffn` kept.
 
-    The gradients of gate and up are rounded to the type on the way, as operands of the products that follow."""
+    The gradients of gate and up are rounded to the type on the way, as operands of the products that follow (in fp16 times a power of two
+    where their own range is not the type's, which the products are divided by).  gate and up are taken as they were kept: an up beyond 65504,
+    infinite in fp16, makes its gradients so."""
     if not torch.compiler.is_compiling():
         direct = _direct.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up, activation)
         if direct is not None:
