@@ -228,7 +228,7 @@ TF_API int tf_scatter_nd(const void* updates, void* data, const int64_t* indices
 
 /* C[M,N] = scale_a[m] * scale_b[n] * sum_k A[m,k] * B[n,k] of 8-bit integers: A [M,K] and B [N,K] int8, row-major; scale_a [M] and
  * scale_b [N] fp32; C [M,N] of c_dtype (fp32, fp16 or bf16).  The sum is exact (int32), hence K <= 131071; it is multiplied by scale_a, then by scale_b in fp32, and
- * rounded once.  M = 0 and N = 0 are done at once.  At most 2^23 tiles of 64 x 64 results.  A and B begin at 16-byte boundaries; where K is no multiple of 16 they may begin
+ * rounded once.  M = 0 and N = 0 are done at once.  M < 2^30, N <= 2^29 - 64.  A and B begin at 16-byte boundaries; where K is no multiple of 16 they may begin
  * anywhere, and a workspace (at a 16-byte boundary, of the bytes that the function beside it says, otherwise 0) takes copies of them.
  * (No counterpart in the reference.) */
 TF_API size_t tf_gemm_int8_workspace_bytes(int64_t M, int64_t N, int64_t K);
@@ -292,7 +292,7 @@ TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* 
  * `workspace_bytes`, runs the streaming kernel with operands at 16-byte boundaries, otherwise 0.  tf_scatter_nd_plan, `data` in ordinary memory of the
  * current device, it and 16-bit updates at 4-byte boundaries: updates that are sorted together (0: each goes straight to memory), and in
  * *words_a_lane the 32-bit words of an update that a lane adds; -1 for other arguments. */
-/* tf_product_kernel_index: position in kGemmKernels of what tf_gemm_int8 (K: half its own), tf_gated_ffn (two = 1, N: F) and tf_linear_cross_entropy
+/* tf_product_kernel_index: position in kGemmKernels, or behind its 15 entries for tiles of 128 x 128 of fewer than 128 rows (15: one on a CU, 16: two), of what tf_gemm_int8 (K: half its own), tf_gated_ffn (two = 1, N: F) and tf_linear_cross_entropy
  * and the first product of its backward pass (N: columns of the vocabulary or of a piece) run; -1 for other arguments.  tf_product_cols_plan: position in kColsShapes
  * (csrc/product.hpp) of the tile of a gradient of M x N that is a sum over `rows` rows, and in *parts the parts that the sum is cut into.
  * tf_product_pair_plan: the same of two gradients that are asked for together and run in one launch; -1 where they run one after the other.

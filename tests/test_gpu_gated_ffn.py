@@ -318,6 +318,17 @@ def test_offsets_that_pass_32_bits():
         ref.assert_within(got, a, b)
 
 
+def test_more_tiles_than_a_launch_has():
+    # 2^23 + 1024 tiles of 64 x 32, the only ones for so few columns
+    m, f, k = (1 << 19) + 5, 1 << 15, 8
+    x, w_gate, w_up, _ = _block(m, f, k, torch.bfloat16, seed=19)
+    h = ops.gated_ffn(x, w_gate, w_up)
+    for at in (0, 8191 * 64 - 40, m - 60):
+        rows = slice(at, at + 60)
+        want, bounds = ref.gated_ffn(x[rows], w_gate, w_up, "silu")
+        ref.assert_within(h[rows], want[0], bounds[0], f"{at}")
+
+
 def test_backward_shapes_strides_and_empty():
     g = torch.Generator(device=DEV).manual_seed(6)
     dtype = torch.float16

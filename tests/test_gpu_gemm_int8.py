@@ -91,6 +91,19 @@ def test_offsets_that_pass_32_bits():
         assert torch.equal(q[rows], want_q) and torch.equal(scale[rows], want_scale)
 
 
+def test_more_tiles_than_a_launch_has():
+    # more than 2^23 tiles of 64 x 64, the largest for so few columns
+    g = torch.Generator(device=DEV).manual_seed(5)
+    m, n, k = (1 << 18) + 3, (1 << 17) + 1, 16
+    a, b = _ints(g, m, k), _ints(g, n, k)
+    sa, sb = torch.rand(m, device=DEV, generator=g), torch.rand(n, device=DEV, generator=g)
+    c = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)
+    ops.gemm_int8(a, b, sa, sb, c)
+    for at in (0, 4093 * 64 - 50, 4094 * 64 - 50, 4095 * 64 - 50, m - 100):
+        want = _expect(a[at:at + 100], b, sa[at:at + 100], sb)
+        assert ((c[at:at + 100].double() - want).abs() <= want.abs() * (4 * 2.0 ** -24 + half_step(torch.bfloat16)) + TINY[torch.bfloat16]).all(), at
+
+
 def test_strides_alignment_and_empty():
     g = torch.Generator(device=DEV).manual_seed(3)
     wide = _ints(g, 130, 400)

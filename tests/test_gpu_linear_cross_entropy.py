@@ -162,6 +162,18 @@ def test_few_tokens_and_a_table_of_very_many_words(t):
         assert (grad_weight[words].double() - want).norm() <= 3 * ref.half_step(torch.bfloat16) * want.norm()
 
 
+def test_more_tiles_than_a_launch_has():
+    # 2^24 tiles of 64 x 64, the only ones for so few columns: 511 rows of them at a time
+    t, v, k = 65530, 1 << 20, 8
+    hidden, weight, target, _ = _head(t, v, k, torch.bfloat16, seed=19)
+    loss, lse = ops.linear_cross_entropy(hidden, weight, target)
+    for at in (0, 511 * 64 - 20, 2 * 511 * 64 - 20, t - 40):
+        rows = slice(at, at + 40)
+        (want_loss, want_lse), bounds = ref.linear_cross_entropy(hidden[rows], weight, target[rows], -100)
+        ref.assert_within(lse[rows], want_lse, bounds[1], f"lse {at}")
+        ref.assert_within(loss[rows], want_loss, bounds[0], f"loss {at}")
+
+
 def test_shapes_strides_and_alignment():
     hidden, weight, target, g = _head(60, 300, 80, torch.float16, seed=3)
     _check_forward(hidden.view(3, 20, 80), weight, target.view(3, 20))

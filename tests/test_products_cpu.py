@@ -241,6 +241,20 @@ def test_no_plan_has_more_tiles_than_a_launch():
         assert -(-m // bm) * -(-n // bn) < 1 << 23, (m, n)
 
 
+def test_columns_of_tiles_fit_a_launch():
+    """Rows of tiles may take several launches, a row of them may not."""
+    lib = _capi.load()
+    width = [16, 16, 16, 32, 32, 32, 64, 128, 128, 128, 128, 192, 128, 192, 256, 128, 128]
+    for n in ((1 << 28) - 64, (1 << 29) - 64):
+        for m in (1, 16, 17, 64, 65, 100, 128, 1000, 1 << 16, 1 << 22, (1 << 30) - 1):
+            for k in (8, 32, 64, 72, 1024):
+                assert -(-n // width[lib.tf_product_kernel_index(m, n, k, 0)]) < 1 << 23, (m, n, k)
+    for m in (1, 17, 1 << 16, (1 << 22) - 64):
+        assert lib.tf_product_kernel_index(m, (1 << 21) - 64, 8, 1) in (0, 3, 4, 5, 6)
+    assert lib.tf_gemm_int8(P, P, P, P, P, F16, 1, (1 << 29) - 63, 16, None, 0, None) == BAD and b"too large" in lib.tf_last_error()
+    assert lib.tf_gemm_int8_workspace_bytes(1, (1 << 29) - 63, 17) == 0
+
+
 def test_offsets_of_a_gradient_stay_within_32_bits():
     """Lanes walk 64 rows of an operand that is summed over its rows, and up to 256 of one that is not, by 32-bit offsets: from kLead bytes
     in front of the first row on, to its farthest 16 bytes of 512."""

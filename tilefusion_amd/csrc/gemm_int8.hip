@@ -191,7 +191,7 @@ int quantize_rows(const void* x, void* q, float* scales, int64_t rows, int64_t K
 }  // namespace tfk
 
 extern "C" size_t tf_gemm_int8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > 131071 || M >= (1 << 30) || N >= (1 << 30)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || K > 131071 || M >= (1 << 30) || N > (1 << 29) - 64) return 0;
   return tfk::CopyPlan(M, N, K).bytes;
 }
 
@@ -202,7 +202,7 @@ extern "C" int tf_gemm_int8(const void* A, const void* B, const float* scale_a, 
   TFK_REQUIRE(c_dtype >= TF_DTYPE_F32 && c_dtype <= TF_DTYPE_BF16, TF_ERR_UNSUPPORTED,
               "tf_gemm_int8: the result must be TF_DTYPE_F32, TF_DTYPE_F16 or TF_DTYPE_BF16");
   TFK_REQUIRE(K <= 131071, TF_ERR_INVALID_ARG, "tf_gemm_int8: a sum of more than 131071 products does not fit 32 bits (K = %lld)", (long long)K);
-  TFK_REQUIRE(M < (1 << 30) && N < (1 << 30), TF_ERR_INVALID_ARG, "tf_gemm_int8: dimension too large");
+  TFK_REQUIRE(M < (1 << 30) && N <= (1 << 29) - 64, TF_ERR_INVALID_ARG, "tf_gemm_int8: dimension too large");   // (tiles of 64 columns: kMaxTiles)
   if (M == 0 || N == 0) return TF_OK;
   TFK_REQUIRE(A && B && scale_a && scale_b && C, TF_ERR_INVALID_ARG, "tf_gemm_int8: null pointer");
   const CopyPlan copy(M, N, K);

@@ -24,6 +24,7 @@ struct Operands {
   const void* b[2];
   int M, N;          // rows of a, rows of each b
   int K;
+  int tile_row = 0;  // of the result's rows of tiles, the first that a launch does
 };
 
 // Where a wavefront's tile lies: its first row and column (of b[0] where there are two), and the first that no tile in front of it
@@ -117,6 +118,7 @@ __global__ __launch_bounds__(S::kThreads) void product_ring64_kernel(Operands x,
   constexpr int kCols = kTwo ? S::BN / 2 : S::BN;   // columns of the result
   int tile_m, tile_n;
   tile_of_block(blockIdx.x, gridDim.x, tiles_m, tiles_n, tile_m, tile_n);
+  tile_m += x.tile_row;
   const int m0 = kFew ? 0 : min(tile_m * S::BM, x.M - S::BM), n0 = min(tile_n * kCols, x.N - kCols);
   const int wm = wave / S::WAVES_N, wn = wave % S::WAVES_N;
   float4_t acc[S::TM][S::TN];
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(S::kThreads) void product_split_k_kernel(Operands x
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int kCols = kTwo ? S::BN / 2 : S::BN;
   const int pid = xcd_major(blockIdx.x, tiles_m * tiles_n);
-  const int m0 = pid % tiles_m * S::BM, n0 = pid / tiles_m * kCols;
+  const int m0 = (x.tile_row + pid % tiles_m) * S::BM, n0 = pid / tiles_m * kCols;
   split_k_multiply<S, InT, kTwo>(static_cast<const uint16_t*>(x.a), static_cast<const uint16_t*>(x.b[0]), static_cast<const uint16_t*>(x.b[1]), x.M,
                                  x.N, x.K * (int)sizeof(InT) / 2, m0, n0, lane, wave, smem);
   const float* const parts = reinterpret_cast<const float*>(smem);
@@ -165,7 +167,7 @@ inline int64_t tiles_of(int64_t extent, int64_t tile) { return (extent + tile - 
 inline int64_t round_up_to(int64_t x, int64_t to) { return tiles_of(x, to) * to; }
 inline bool at_16B(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-constexpr int64_t kMaxTiles = ((int64_t)1 << 23) - 1;   // a launch has less than 2^32 threads, of which a workgroup has 512 at most
+constexpr int64_t kMaxTiles = ((int64_t)1 << 23) - 1;   // of a launch: it has less than 2^32 threads, of which a workgroup has 512 at most
 
 // The kernel that gemm.hip's cost model expects to be done first with M x N outputs over K 16-bit elements, out of those of `allowed` (a bit per row of
 // its table kGemmKernels): its position there.
@@ -195,7 +197,13 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool two) {
   // (the table has no tile of 16 x 32: up to 16 rows it is ahead of 32 x 32, 1 x 4096 x 11264 of two matrices 33.2 us / 38.4)
   if (two && M <= 16) return {0, product_slots(0, N)};
   float us;
-  int kernel = pick_table_kernel(M, columns, K, two ? kTwoAllowed & ~1u : kOneAllowed, &us);
+  const unsigned allowed = two ? kTwoAllowed & ~1u : kOneAllowed;
+  int kernel = pick_table_kernel(M, columns, K, allowed, &us);
+  // More tiles than a launch has, of whatever size: what is best for as many rows as a launch does.
+  for (int64_t m = M; !(us < INFINITY) && m > 64;) {
+    m = round_up_to(m / 2, 64);
+    kernel = pick_table_kernel(m, columns, K, allowed, &us);
+  }
   // Fewer than 128 rows and many columns: large tiles all the same where the model expects them sooner than the small ones, which read the
   // weights once for every 32 or 64 rows.  us, small / large: loss of 100 x 1024 over 32000 words 33 / 20.5, of 37 22.3 / 19.4, gated
   // block 100 x 4096 x 11264 57 / 44.5; 64 x 2048 x 8192 17.7 / 21.3 (where the small ones stay).
@@ -207,23 +215,32 @@ inline ProductPlan plan_product(int64_t M, int64_t N, int64_t K, bool two) {
   return {kernel, product_slots(kernel, N)};
 }
 
+// As many rows of tiles at a time as a launch has room for: all of them where the result is not enormous.
+template <typename S, typename Epilogue>
+int launch_tiles(const char* who, void (*kern)(Operands, int, int, Epilogue), Operands x, int64_t tiles_m, int64_t tiles_n, const Epilogue& epilogue,
+                 hipStream_t st) {
+  TFK_REQUIRE(tiles_n <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
+  const int64_t most = kMaxTiles / tiles_n;
+  for (int64_t from = 0; from < tiles_m; from += most) {
+    const int64_t rows = std::min(most, tiles_m - from);
+    x.tile_row = (int)from;
+    if (int rc = launch_kernel(kern, dim3((unsigned)(rows * tiles_n)), dim3(S::kThreads), S::kLdsBytes, st, x, (int)rows, (int)tiles_n, epilogue)) return rc;
+  }
+  return TF_OK;
+}
 template <typename S, typename InT, bool kTwo, typename Epilogue, bool kFew = false>
 int launch_ring64_product(const char* who, const Operands& x, const Epilogue& epilogue, hipStream_t st) {
   auto kern = product_ring64_kernel<S, InT, kTwo, kFew, Epilogue>;
   static_assert(S::kLdsBytes <= kMaxLdsBytes, "ring does not fit in LDS");
   TFK_LDS_OPT_IN(kern, S::kLdsBytes);
-  const int64_t tiles_m = tiles_of(x.M, S::BM), tiles_n = tiles_of(x.N, kTwo ? S::BN / 2 : S::BN);
-  TFK_REQUIRE(tiles_m * tiles_n <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
-  return launch_kernel(kern, dim3((unsigned)(tiles_m * tiles_n)), dim3(S::kThreads), S::kLdsBytes, st, x, (int)tiles_m, (int)tiles_n, epilogue);
+  return launch_tiles<S>(who, kern, x, tiles_of(x.M, S::BM), tiles_of(x.N, kTwo ? S::BN / 2 : S::BN), epilogue, st);
 }
 template <typename S, typename InT, bool kTwo, typename Epilogue>
 int launch_split_k_product(const char* who, const Operands& x, const Epilogue& epilogue, hipStream_t st) {
   auto kern = product_split_k_kernel<S, InT, kTwo, Epilogue>;
   static_assert(S::kLdsBytes <= kMaxLdsBytes, "rings do not fit in LDS");
   if constexpr (S::kLdsBytes > 64 * 1024) TFK_LDS_OPT_IN(kern, S::kLdsBytes);
-  const int64_t tiles_m = tiles_of(x.M, S::BM), tiles_n = tiles_of(x.N, kTwo ? S::BN / 2 : S::BN);
-  TFK_REQUIRE(tiles_m * tiles_n <= kMaxTiles, TF_ERR_INVALID_ARG, "%s: result too large", who);
-  return launch_kernel(kern, dim3((unsigned)(tiles_m * tiles_n)), dim3(S::kThreads), S::kLdsBytes, st, x, (int)tiles_m, (int)tiles_n, epilogue);
+  return launch_tiles<S>(who, kern, x, tiles_of(x.M, S::BM), tiles_of(x.N, kTwo ? S::BN / 2 : S::BN), epilogue, st);
 }
 
 template <typename InT, bool kTwo, typename Epilogue>
