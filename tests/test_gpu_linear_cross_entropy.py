@@ -307,6 +307,27 @@ def test_one_weight_for_many_tokens_is_not_rounded_as_one(dtype, kind):
         assert (got.double() - a).norm() <= 1.75 * alone, (got.double() - a).norm() / alone
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("padding", [1, 3, 4, 64, 255, 256, 257, 700])
+def test_one_weight_for_the_tokens_of_a_padded_batch(dtype, padding):
+    # as above, of a mean, with tokens behind the last one that counts: nothing is rounded with hidden, whose part would be 1.4 times the result's
+    t, v, k = 512, 4096, 256
+    hidden, weight, target, g = _head(t + padding, v, k, dtype, seed=20, ignored=False)
+    target[t:] = -100
+    grad_loss = torch.full((t + padding,), 1 + 2 * ref.half_step(dtype) * 0.52, device=DEV)
+    lse = ops.linear_cross_entropy(hidden, weight, target)[1]
+    grads = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse)
+    want, _ = ref.linear_cross_entropy_backward(grad_loss, hidden, weight, target, -100)
+    for got, a in zip(grads, want):
+        # the result's rounding, and that of the softmax gradients (0.6 of it at most): sqrt(1 + 0.36) = 1.17
+        alone = (a.to(dtype).double() - a).norm()
+        assert (got.double() - a).norm() <= 1.25 * alone, (got.double() - a).norm() / alone
+    alike = ops.linear_cross_entropy_backward(grad_loss[:t], hidden[:t], weight, target[:t], lse[:t])
+    assert (grads[0][t:] == 0).all()
+    for got, a in zip((grads[0][:t], grads[1]), alike):   # (sums may be cut otherwise)
+        assert (got.double() - a.double()).norm() <= 2 * ref.half_step(dtype) * a.double().norm()
+
+
 def test_gradient_against_differences():
     # the loss itself along a direction: central differences of step 2^-4 on values that are multiples of it (exact in fp16)
     g = torch.Generator(device=DEV).manual_seed(8)

@@ -13,7 +13,7 @@
 // gradients by far: with all of grad_loss in w, what 16 bits leave out of that one number would be an error of everything that a token (and with a
 // mean every token) adds, up to 2.5 times in all what rounding the results leaves out.  So w is a power of two, and m in (0.5, 1]: dH is
 // multiplied by it in 32 bits, and the rounding of m * H is another one for each element (1.4 times as much).  What m takes out of all tokens
-// is the mantissa of the last one's grad_loss: where they have the same, m is 1 and nothing is rounded.
+// is the mantissa of the grad_loss of the last one that counts (of the last 8192): where they have the same, m is 1 and nothing is rounded.
 // In fp16 P is multiplied by a power of two as well by which the largest is 2^15 at most, so that the weights of a mean over many tokens do not fall
 // below the type's range; the sums are divided by it in 32 bits.  (bf16 has the range of fp32.)  dH is summed over the pieces in fp32 and rounded once.
 #include <cmath>
@@ -136,9 +136,10 @@ TFK_DEVICE Split split(float x) {
 
 // What a backward pass takes from grad_loss: w (0 for ignored tokens, NaN for targets outside the vocabulary, as the loss), m, and m * H in rows of `width`,
 // zeros for ignored tokens.
-// Everything is a quarter of grad_loss, divided by the last token's mantissa: factors[tokens] makes up for that, factors[t] has m as well.
+// Everything is a quarter of grad_loss, divided by that mantissa: factors[tokens] makes up for that, factors[t] has m as well.
 // The first workgroup looks for the largest as well, where there is a scale.
 constexpr int kWeighThreads = 256;
+constexpr int kSearched = 8192;   // tokens at the end of which one is to count
 template <typename T>
 __global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const float* __restrict__ grad_loss, const int64_t* __restrict__ target,
                                                                      int64_t ignore_index, int tokens, int V, Scale* scale, float* __restrict__ weights,
@@ -147,11 +148,25 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const float
   typedef T eight_t __attribute__((ext_vector_type(8)));
   typedef eight_t eight_any_t __attribute__((aligned(2)));
   const auto counts = [&](int64_t wanted) __attribute__((always_inline)) { return wanted != ignore_index && wanted >= 0 && wanted < V; };
-  // (every load of a thread is on its way before the first is waited for: a call of few tokens is as long as its latencies)
-  const int64_t wanted_last = target[tokens - 1];
-  const float grad_last = grad_loss[tokens - 1];
+  // The mantissa of the last token that counts: the batch may be padded behind it.  A wavefront looks at 256 tokens at a time.
+  float common = 1.f;
+  for (int end = tokens; end > 0 && end > tokens - kSearched; end -= 256) {
+    const int t = end - 4 * (int)(threadIdx.x % 64) - 1;   // the lane's last one
+    int64_t wanted[4];
+    float grad[4], mine = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) wanted[n] = target[max(t - n, 0)], grad[n] = grad_loss[max(t - n, 0)];
+    bool found = false;
+#pragma unroll
+    for (int n = 3; n >= 0; --n)
+      if (t - n >= 0 && counts(wanted[n])) found = true, mine = grad[n];
+    const unsigned long long lanes = __ballot(found);
+    if (lanes != 0) {
+      common = split(__shfl(mine, __ffsll(lanes) - 1)).m;
+      break;
+    }
+  }
   const int64_t first = (int64_t)blockIdx.x * kWeighThreads + threadIdx.x, step = (int64_t)gridDim.x * kWeighThreads;
-  const auto common_of = [&]() __attribute__((always_inline)) { return counts(wanted_last) ? split(grad_last).m : 1.f; };
   if (weighted != nullptr) {
     const unsigned chunks = (unsigned)width / 8;
     const int64_t count = (int64_t)tokens * chunks;
@@ -167,7 +182,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const float
 #pragma unroll
         for (int t = 0; t < 8; ++t) v[t] = col + t < K ? hidden[row * K + col + t] : (T)0.f;
       }
-      const float m = counts(wanted) ? split(grad * 0.25f / common_of()).m : 1.f;
+      const float m = counts(wanted) ? split(grad * 0.25f / common).m : 1.f;
       // (an ignored token's row is what its P, zeros, are multiplied by: it may hold anything, and zero times a NaN is one)
       const bool ignored = wanted == ignore_index;
 #pragma unroll
@@ -177,7 +192,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const float
   }
   for (int64_t t = first; t < tokens; t += step) {
     const int64_t wanted = target[t];
-    const float grad = grad_loss[t], common = common_of();
+    const float grad = grad_loss[t];
     const Split s = counts(wanted) ? split(grad * 0.25f / common) : Split{wanted == ignore_index ? 0.f : __uint_as_float(0x7fc00000u), 1.f};
     weights[t] = s.power;
     factors[t] = 4.f * common * s.m;
