@@ -285,6 +285,21 @@ def test_the_size_of_grad_loss_does_not_matter(dtype, size):
             0 if dtype == torch.bfloat16 else 2 * ref.half_step(dtype) * (b.double() * by).abs().max())
 
 
+@pytest.mark.parametrize("size", [2.0 ** -20, 1.0, 4096.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_an_infinite_grad_loss_does_not_take_the_others_range(dtype, size):
+    hidden, weight, target, g = _head(90, 400, 64, dtype, seed=21, ignored=False)
+    grad_loss = (torch.rand(90, device=DEV, generator=g) + 0.25) * size
+    lse = ops.linear_cross_entropy(hidden, weight, target)[1]
+    want, bounds = ref.linear_cross_entropy_backward(grad_loss, hidden, weight, target, -100)
+    others = torch.arange(90, device=DEV) != 7
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        grad_loss[7] = bad
+        grad_hidden, grad_weight = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse)
+        ref.assert_within(grad_hidden[others], want[0][others], bounds[0][others], str(bad))
+        assert not grad_hidden[7].isfinite().any()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", ["mean", "sequences"])
 def test_one_weight_for_many_tokens_is_not_rounded_as_one(dtype, kind):

@@ -137,7 +137,7 @@ TFK_DEVICE Split split(float x) {
 // What a backward pass takes from grad_loss: w (0 for ignored tokens, NaN for targets outside the vocabulary, as the loss), m, and m * H in rows of `width`,
 // zeros for ignored tokens.
 // Everything is a quarter of grad_loss, divided by that mantissa: factors[tokens] makes up for that, factors[t] has m as well.
-// The first workgroup looks for the largest as well, where there is a scale.
+// The first workgroup looks for the largest finite one as well, where there is a scale.
 constexpr int kWeighThreads = 256;
 constexpr int kSearched = 8192;   // tokens at the end of which one is to count
 template <typename T>
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const float
   __shared__ float s_top[kWeighThreads / 64];
   float top = 0.f;
   for (int t = threadIdx.x; t < tokens; t += kWeighThreads)
-    if (target[t] != ignore_index) top = fmaxf(top, fabsf(grad_loss[t]));
+    if (target[t] != ignore_index && fabsf(grad_loss[t]) < INFINITY) top = fmaxf(top, fabsf(grad_loss[t]));
 #pragma unroll
   for (int d = 32; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d));
   if (threadIdx.x % 64 == 0) s_top[threadIdx.x / 64] = top;
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const float
   if (threadIdx.x != 0) return;
   for (int w = 1; w < kWeighThreads / 64; ++w) top = fmaxf(top, s_top[w]);
   int e = 0;
-  if (top > 0.f && top < INFINITY) {
+  if (top > 0.f) {
     const float m = frexpf(top, &e);   // top = m * 2^e, 0.5 <= m < 1
     if (m == 0.5f) --e;
   }
