@@ -301,6 +301,22 @@ def test_an_infinite_grad_loss_does_not_take_the_others_range(dtype, size):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [2.0 ** -40, 2.0 ** -10, 1.0, 2.0 ** 13, 2.0 ** 15])
+def test_backward_within_bounds_at_any_size_of_grad_loss(dtype, size):
+    # large ones in fp16 as well, up to results beyond the type, which are infinities of their sign and nothing else
+    hidden, weight, target, g = _head(90, 400, 64, dtype, seed=22)
+    grad_loss = (torch.rand(90, device=DEV, generator=g) - 0.5) * size
+    lse = ops.linear_cross_entropy(hidden, weight, target)[1]
+    grads = ops.linear_cross_entropy_backward(grad_loss, hidden, weight, target, lse)
+    want, bounds = ref.linear_cross_entropy_backward(grad_loss, hidden, weight, target, -100)
+    for got, a, bound in zip(grads, want, bounds):
+        number = ref.assert_within(got, a, bound, str(size))
+        rest = torch.where(number, got.double() - a, torch.zeros_like(a))
+        assert rest.norm() <= 2 * ref.half_step(dtype) * a.norm() + a.numel() ** 0.5 * ref.TINY[dtype]
+        assert number.float().mean() > 0.5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", ["mean", "sequences"])
 def test_one_weight_for_many_tokens_is_not_rounded_as_one(dtype, kind):
     """The largest term of a gradient is a token's grad_loss itself: rounded to 16 bits it would be off by the same for all tokens of the same
