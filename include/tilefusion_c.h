@@ -256,7 +256,7 @@ TF_API int tf_gated_ffn(const void* x, const void* w_gate, const void* w_up, voi
 /* Gradients of x [M,K], w_gate and w_up [F,K] from that of h (dh [M,F]) and the gate and up values that the forward call kept; x and
  * the weights as there, the others begin anywhere.  The workspace begins at a 16-byte boundary and may hold anything; it is done with when the call's work is.  A null dx, or
  * null dw_gate and dw_up, are not computed (the sums of the others may be cut otherwise than beside them).  M = 0: the weights' gradients are zero.
- * The gradients of gate and up are rounded to dtype on the way; in fp16, where the largest finite one of them is below 1 or above 65504, times a power of two by
+ * The gradients of gate and up are rounded to dtype on the way; in fp16, where the largest finite one of them is below 2^-6 or above 65504, times a power of two by
  * which it is 2^14 to 2^15, so that neither end of the type's range is lost from sums that lie within it. */
 TF_API size_t tf_gated_ffn_backward_workspace_bytes(int64_t M, int64_t F, int64_t K);
 TF_API int tf_gated_ffn_backward(const void* dh, const void* x, const void* w_gate, const void* w_up, const void* gate,

@@ -204,11 +204,12 @@ def test_backward_sizes(m, f, k, dtype):
 
 
 def _scaled_backward(grad_h, x, w_gate, w_up, gate, up, activation):
-    """The gradients and their bounds where dg and du have a power of two in common by which the largest is 2^14 to 2^15: what fp16's smallest numbers
-    leave out of one is 2^-25, 2^-39 of the largest."""
+    """The gradients and their bounds in fp16.  Where the largest of dg and du is below 2^-6 or above 65504 they have a power of two in common by which
+    it is 2^14 to 2^15.  What fp16's smallest numbers leave out of one is 2^-25, 2^-39 of the largest then."""
     d, g, u = grad_h.double(), gate.double(), up.double()
     grads = d * u * ref.act_slope(g, activation), d * ref.act(g, activation)
-    most = 2.0 ** -39 * max(t.abs().max() for t in grads)
+    top = max(t.abs().max() for t in grads)
+    most = 2.0 ** -25 if 2.0 ** -6 <= top <= 65504 else 2.0 ** -39 * top
     offs = [ref.FN * size + ref.half_step(x.dtype) * t.abs() + most for t, size in zip(grads, ((d * u).abs() * (1 + g.abs()), (d * g).abs()))]
     (dg, du), (off_g, off_u) = grads, offs
     return ref._products([(torch.cat([dg, du], 1), torch.cat([off_g, off_u], 1), torch.cat([w_gate, w_up]).t()), (dg.t(), off_g.t(), x.t()),
@@ -240,6 +241,20 @@ def test_backward_beyond_the_range_of_fp16(m, f, k, span, activation):
             ref.assert_within(grads[i], want[i], bounds[i], f"{i} of {of}")
             floor = want[i].numel() ** 0.5 * ref.TINY[dtype]
             assert (grads[i].double() - want[i]).norm() <= 2 * ref.half_step(dtype) * want[i].norm() + floor
+
+
+@pytest.mark.parametrize("power", list(range(-22, 14)))
+def test_backward_at_every_size_of_its_gradients(power):
+    m, f, k = 60, 72, 40
+    x, w_gate, w_up, g = _block(m, f, k, torch.float16, seed=23)
+    grad_h, gate, up = (_randn(g, m, f, dtype=torch.float16) for _ in range(3))
+    grad_h *= 2.0 ** power
+    by = 2.0 ** max(0, -power // 2 - 4)   # (results within the type)
+    x, w_gate, w_up = (t * by if power < 0 else t * 2.0 ** -6 for t in (x, w_gate, w_up))
+    want, bounds = _scaled_backward(grad_h, x, w_gate, w_up, gate, up, "silu")
+    for got, a, bound in zip(ops.gated_ffn_backward(grad_h, x, w_gate, w_up, gate, up), want, bounds):
+        ref.assert_within(got, a, bound, str(power))
+        assert (got.double() - a).norm() <= 2 * ref.half_step(torch.float16) * a.norm() + a.numel() ** 0.5 * ref.TINY[torch.float16]
 
 
 def test_an_infinite_gradient_does_not_take_the_others_range():

@@ -203,8 +203,9 @@ __global__ __launch_bounds__(kThreads) void gated_ffn_grads_kernel(const T* __re
   }
 }
 
-// fp16: where the largest is beyond the type, or so small that fp16's smallest number leaves more out of the others than a rounding of the largest in
-// fp32 would (2^-25 of it: below 1), [dg | du] once more, times a power of two by which the largest is 2^14 to 2^15.  Elsewhere, as with a loss whose scale
+// fp16: where the largest is beyond the type, or so small (below 2^-6) that numbers a 256th of it are below fp16's normal ones, [dg | du] once more, times a
+// power of two by which the largest is 2^14 to 2^15.  In between, fp16's smallest number leaves 2^-19 of the largest out of the others at most: less than rounding
+// leaves out of numbers that are a 64th of it.  Elsewhere, as with a loss whose scale
 // suits the type, there is nothing to do, and the launch is what it costs: backward passes of 1337 x 1544 x 1032 42.8 -> 46.6 us, 2048 x 1024 x 1024 28.4 -> 31.8,
 // 8192 x 11264 x 4096 2374 -> 2391 (with 4096 workgroups looking and 2048 here 2435: each of these reads what all of those found).
 template <typename T, int kActivation>
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void gated_ffn_rescale_kernel(const T* __
   float top = 0.f;
   for (int i = threadIdx.x; i < num_tops; i += kThreads) top = fmaxf(top, tops[i]);
   top = largest_of_block(top);
-  const bool again = top > 0.f && (top < 1.f || top > 65504.f);
+  const bool again = top > 0.f && (top < 0.015625f || top > 65504.f);
   int e = 0;
   frexpf(top, &e);                                  // top = m * 2^e, 0.5 <= m < 1
   const int by = again ? min(15 - e, 110) : 0;      // (2^-by has to be a number as well)
