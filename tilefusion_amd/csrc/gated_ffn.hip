@@ -25,7 +25,7 @@ constexpr float kGeluTwice = 1.5957691216057308f;   // 2 * sqrt(2 / pi): (1 + ta
 // erfcx(|g| / sqrt(2)) / 2.  p is the polynomial of degree 8 whose largest relative error over all g is least (Remez' exchange): 1.7e-7, so that the
 // tail, which is not taken from 1, is right in its leading digits as far out as it is a number of the type.  In fp32 5e-7 up to |g| = 1, and g^2 * 2^-23 further
 // out, by the argument of bell.  The library's erff takes both of its branches for every wavefront (2999 x 1032 x 1544 with gate and up kept, fp16:
-// 43 us with it, 32 so).
+// 43 us with it, 33 so).
 TFK_DEVICE float normal_tail(float g, float bell) {
   const float t = __builtin_amdgcn_rcpf(1.f + 0.28f * fabsf(g));
   float p = 0.024719954f;
