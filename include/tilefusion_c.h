@@ -281,6 +281,46 @@ TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* 
                                             int64_t V, int64_t K, int64_t ignore_index, void* workspace, size_t workspace_bytes,
                                             void* stream);
 
+/* A cache of keys and values in pages: token p of sequence b is row p % page_size of page page_table[b][p / page_size].  key and value
+ * [pages, page_size, kv_heads, D] of dtype (fp16 or bf16), D 64 or 128, in any order of the first three dimensions: strides in elements from page to
+ * page, token to token and head to head, multiples of 8; both begin at 16-byte boundaries.  page_table [sequences, table_width] int32, rows table_stride
+ * apart, and lengths [sequences] int32 are in device memory and may hold anything: a page that the cache does not have is
+ * never read or written.  Table entries beyond a sequence's length are not looked at.  (No counterpart in the reference.) */
+typedef struct {
+  void* key;
+  void* value;
+  int64_t key_strides[3], value_strides[3];
+  int64_t pages, page_size, kv_heads, D;
+  const int32_t* page_table;
+  int64_t table_width, table_stride;
+  const int32_t* lengths;
+  int64_t sequences;
+  int dtype;
+} tf_paged_cache_t;
+
+/* New tokens enter a cache: query [tokens, heads, D] and key [tokens, kv_heads, D] are rotated by their positions, key and value go to their pages.
+ * `strides`: of query, key and value, in elements, from token to token and head to head (multiples of 8; 16-byte boundaries).
+ * lengths holds the sequences' lengths with the new tokens.  offsets [sequences + 1] int32 on the device, ascending: sequence b's new tokens
+ * are offsets[b] .. offsets[b+1] - 1, the last of them at position lengths[b] - 1; without offsets (null) token b is the one new token of sequence b.
+ * The first `rotated` elements (even) of a head are turned in pairs, two neighbours (interleaved) or elements i and i + rotated / 2: (x, y) becomes
+ * (x cos - y sin, x sin + y cos) in fp32, rounded once, with cos and sin [positions, rotated / 2] fp32 of the token's position.
+ * The rotated queries go to query_out [tokens, heads, D], the keys to key_out [tokens, kv_heads, D] as well unless it is null.
+ * A token whose position has no page in the cache or no row in the tables changes nothing in the cache; its rows of query_out and key_out are NaN.  Tokens that
+ * belong to no sequence, and those of a sequence that is not as long as its new tokens, change nothing either, and their rows are zero.
+ * Pages that new tokens go to belong to one sequence.  tokens < 2^24. */
+TF_API int tf_append_paged_kv(const tf_paged_cache_t* cache, const void* query, const void* key, const void* value, const int64_t* strides,
+                              const float* cos, const float* sin, int64_t positions, int64_t rotated, int interleaved, const int32_t* offsets,
+                              int64_t tokens, int64_t heads, void* query_out, void* key_out, void* stream);
+
+/* out[b, h] = softmax(softmax_scale * query[b, h] K^T) V over the lengths[b] keys and values of sequence b in the cache, for the head h / (heads /
+ * kv_heads) of it: one new token a sequence.  query [sequences, heads, D] (query_strides: from sequence to sequence and head to head, multiples of 8
+ * elements), out [sequences, heads, D].  fp32 scores, maximum and sums.  page_size is a multiple of 16.  A sequence without a key (length 0 or
+ * below) has rows of zeros; one that is longer than its row of the table, or has a page that the cache does not have, NaN.
+ * The workspace begins at a 16-byte boundary, is ordinary memory of the current device and may hold anything; two calls at a time need one each. */
+TF_API size_t tf_flash_decode_paged_workspace_bytes(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t D);
+TF_API int tf_flash_decode_paged(const tf_paged_cache_t* cache, const void* query, const int64_t* query_strides, void* out, int64_t heads,
+                                 double softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+
 /* What a call would run, decided on the host from the sizes alone; nothing is launched.
  * tf_gemm_kernel_index, with operands at 16-byte boundaries: position of the kernel in the table kGemmKernels (csrc/gemm.hip), or behind
  * its end 0 for the bounds-checked kernel, from 1 on for the whole-line forms of kLinesKernels, then for the tile of 160 x 128, K a

@@ -16,6 +16,15 @@ TF_ACT_SILU, TF_ACT_GELU, TF_ACT_GELU_TANH = range(3)
 
 _vp, _i, _i64, _d, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double, ctypes.c_size_t
 
+
+class PagedCache(ctypes.Structure):
+    """tf_paged_cache_t"""
+
+    _fields_ = [("key", _vp), ("value", _vp), ("key_strides", _i64 * 3), ("value_strides", _i64 * 3), ("pages", _i64), ("page_size", _i64),
+                ("kv_heads", _i64), ("D", _i64), ("page_table", _vp), ("table_width", _i64), ("table_stride", _i64), ("lengths", _vp),
+                ("sequences", _i64), ("dtype", _i)]
+
+
 # name -> (restype, argtypes); every symbol include/tilefusion_c.h declares
 SIGNATURES = {
     "tf_gemm_f16": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _i64, _i, _i, _i, _i, _i, _vp]),
@@ -52,6 +61,9 @@ SIGNATURES = {
     "tf_linear_cross_entropy": (_i, [_vp] * 5 + [_i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
     "tf_linear_cross_entropy_backward_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "tf_linear_cross_entropy_backward": (_i, [_vp] * 7 + [_i, _i64, _i64, _i64, _i64, _vp, _sz, _vp]),
+    "tf_append_paged_kv": (_i, [ctypes.POINTER(PagedCache), _vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _vp, _i64, _i64, _i, _vp, _i64, _i64, _vp, _vp, _vp]),
+    "tf_flash_decode_paged_workspace_bytes": (_sz, [_i64] * 4),
+    "tf_flash_decode_paged": (_i, [ctypes.POINTER(PagedCache), _vp, ctypes.POINTER(_i64), _vp, _i64, _d, _vp, _sz, _vp]),
     "tf_product_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_product_cols_plan": (_i, [_i64, _i64, _i64, ctypes.POINTER(_i)]),
     "tf_product_pair_plan": (_i, [_i64] * 6 + [ctypes.POINTER(_i)] * 2),

@@ -1,6 +1,6 @@
 // PyTorch operator bindings: registers torch.ops.tilefusion.{gemm, fused_two_gemms,
 // flash_attention, flash_attention_fwd, flash_attention_fwd_kt, flash_decode, scatter_nd, quantize_rows, gemm_int8, gated_ffn, gated_ffn_backward,
-// linear_cross_entropy, linear_cross_entropy_backward} for the CUDA dispatch key (HIP tensors
+// linear_cross_entropy, linear_cross_entropy_backward, append_paged_kv, flash_decode_paged} for the CUDA dispatch key (HIP tensors
 // are "cuda" tensors on PyTorch-ROCm) and forwards to the C ABI in tilefusion_c.h on the
 // caller's current stream.
 //
@@ -582,6 +582,127 @@ void linear_cross_entropy_backward(const at::Tensor& grad_loss, const at::Tensor
                op);
 }
 
+// ---- a paged cache ----------------------------------------------------------------------------
+namespace {
+// Tensors [n, heads, D] whose rows the kernels read where they are: `strides` takes those of the first two dimensions.
+void check_rows(const at::Tensor& t, const char* name, int64_t n, int64_t heads, int64_t d, const at::Tensor& like, const char* op, int64_t* strides) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "tilefusion::", op, ": ", name, " must be a CUDA tensor on the device of the other tensors.");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), "tilefusion::", op, ": ", name, " must have the dtype of the other tensors.");
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == d, "tilefusion::", op, ": ", name, " must be [", n, ", ", heads, ", ",
+              d, "], got ", t.sizes(), ".");
+  if (t.numel() == 0) {
+    strides[0] = strides[1] = 0;
+    return;
+  }
+  // (the stride of one row alone addresses nothing)
+  strides[0] = t.size(0) > 1 ? t.stride(0) : 0;
+  strides[1] = t.size(1) > 1 ? t.stride(1) : 0;
+  TORCH_CHECK(t.stride(2) == 1 && strides[0] % 8 == 0 && strides[1] % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "tilefusion::", op,
+              ": rows of ", name, " must lie in one piece each, at 16-byte boundaries.");
+}
+// Contiguous results [n, heads, D].
+void check_result(const at::Tensor& t, const char* name, int64_t n, int64_t heads, int64_t d, const at::Tensor& like, const char* op) {
+  check_like(t, name, like, op);
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == d, "tilefusion::", op, ": ", name, " must be [", n, ", ", heads, ", ",
+              d, "], got ", t.sizes(), ".");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "tilefusion::", op, ": ", name, " must begin at a 16-byte boundary.");
+}
+void check_int32(const at::Tensor& t, const char* name, const at::Tensor& like, const char* op) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "tilefusion::", op, ": ", name, " must be a CUDA tensor on the device of the other tensors.");
+  TORCH_CHECK(t.scalar_type() == at::kInt, "tilefusion::", op, ": ", name, " must be int32.");
+}
+tf_paged_cache_t paged_cache(const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& page_table, const at::Tensor& lengths,
+                             const at::Tensor& query, const char* op) {
+  tf_paged_cache_t c = {};
+  c.dtype = operand_dtype(query, op);
+  TORCH_CHECK(key_cache.dim() == 4 && key_cache.numel() > 0, "tilefusion::", op, ": key_cache must be [pages, page_size, kv_heads, D], got ", key_cache.sizes(), ".");
+  TORCH_CHECK(value_cache.sizes() == key_cache.sizes(), "tilefusion::", op, ": value_cache must have the shape of key_cache.");
+  const struct { const at::Tensor& t; const char* name; int64_t* strides; } caches[] = {{key_cache, "key_cache", c.key_strides}, {value_cache, "value_cache", c.value_strides}};
+  for (const auto& x : caches) {
+    TORCH_CHECK(x.t.is_cuda() && x.t.device() == query.device(), "tilefusion::", op, ": ", x.name, " must be a CUDA tensor on the device of the other tensors.");
+    TORCH_CHECK(x.t.scalar_type() == query.scalar_type(), "tilefusion::", op, ": ", x.name, " must have the dtype of the other tensors.");
+    bool whole = x.t.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.t.data_ptr()) % 16 == 0;
+    for (int i = 0; i < 3; ++i) {
+      x.strides[i] = x.t.size(i) > 1 ? x.t.stride(i) : 0;
+      whole = whole && x.strides[i] % 8 == 0 && (x.t.size(i) == 1 || x.strides[i] > 0);
+    }
+    TORCH_CHECK(whole, "tilefusion::", op, ": rows of ", x.name, " must lie in one piece each, in places of their own at 16-byte boundaries.");
+  }
+  c.key = key_cache.data_ptr();
+  c.value = value_cache.data_ptr();
+  c.pages = key_cache.size(0);
+  c.page_size = key_cache.size(1);
+  c.kv_heads = key_cache.size(2);
+  c.D = key_cache.size(3);
+  check_int32(page_table, "page_table", query, op);
+  check_int32(lengths, "lengths", query, op);
+  TORCH_CHECK(lengths.dim() == 1 && lengths.is_contiguous(), "tilefusion::", op, ": lengths must be [sequences] and contiguous.");
+  TORCH_CHECK(page_table.dim() == 2 && page_table.size(0) == lengths.size(0) && (page_table.size(1) < 2 || page_table.stride(1) == 1), "tilefusion::", op,
+              ": page_table must be [", lengths.size(0), ", pages of a sequence], each row in one piece, got ", page_table.sizes(), ".");
+  c.sequences = lengths.size(0);
+  c.table_width = page_table.size(1);
+  c.table_stride = page_table.stride(0);
+  // (a table of no entries has no address)
+  c.page_table = page_table.numel() > 0 ? page_table.data_ptr<int32_t>() : static_cast<const int32_t*>(key_cache.data_ptr());
+  c.lengths = lengths.numel() > 0 ? lengths.data_ptr<int32_t>() : static_cast<const int32_t*>(key_cache.data_ptr());
+  return c;
+}
+}  // namespace
+
+// append_paged_kv(query [T,H,D], key, value [T,Hkv,D], cos, sin [positions, rotated / 2] fp32, the cache, its table and lengths, offsets [sequences + 1]
+// int32 or none -> query_out [T,H,D], key_out [T,Hkv,D] where it is given)
+void append_paged_kv(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const at::Tensor& cos, const at::Tensor& sin,
+                     at::Tensor& key_cache, at::Tensor& value_cache, const at::Tensor& page_table, const at::Tensor& lengths,
+                     const std::optional<at::Tensor>& offsets, bool interleaved, at::Tensor& query_out, const std::optional<at::Tensor>& key_out) {
+  constexpr const char* op = "append_paged_kv";
+  const tf_paged_cache_t cache = paged_cache(key_cache, value_cache, page_table, lengths, query, op);
+  TORCH_CHECK(query.dim() == 3, "tilefusion::", op, ": query must be [tokens, heads, D], got ", query.sizes(), ".");
+  const int64_t t = query.size(0), h = query.size(1), d = cache.D;
+  int64_t strides[6];
+  check_rows(query, "query", t, h, d, query, op, strides);
+  check_rows(key, "key", t, cache.kv_heads, d, query, op, strides + 2);
+  check_rows(value, "value", t, cache.kv_heads, d, query, op, strides + 4);
+  TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), "tilefusion::", op, ": cos and sin must be [positions, rotated / 2].");
+  const struct { const at::Tensor& t; const char* name; } tables[] = {{cos, "cos"}, {sin, "sin"}};
+  for (const auto& x : tables) {
+    check_operand(x.t, x.name, query, op);
+    TORCH_CHECK(x.t.scalar_type() == at::kFloat, "tilefusion::", op, ": ", x.name, " must be float32.");
+  }
+  if (offsets.has_value()) {
+    check_int32(*offsets, "offsets", query, op);
+    TORCH_CHECK(offsets->dim() == 1 && offsets->size(0) == cache.sequences + 1 && offsets->is_contiguous(), "tilefusion::", op, ": offsets must be [",
+                cache.sequences + 1, "] and contiguous.");
+  } else {
+    TORCH_CHECK(t == cache.sequences, "tilefusion::", op, ": without offsets there is one token for each of the ", cache.sequences, " sequences, got ", t, ".");
+  }
+  check_result(query_out, "query_out", t, h, d, query, op);
+  if (key_out.has_value()) check_result(*key_out, "key_out", t, cache.kv_heads, d, query, op);
+  if (t == 0) return;
+  const c10::DeviceGuard there(query.device());
+  check_status(tf_append_paged_kv(&cache, query.data_ptr(), key.data_ptr(), value.data_ptr(), strides, cos.data_ptr<float>(), sin.data_ptr<float>(),
+                                  cos.size(0), 2 * cos.size(1), interleaved ? 1 : 0, offsets.has_value() ? offsets->data_ptr<int32_t>() : nullptr, t, h,
+                                  query_out.data_ptr(), key_out.has_value() ? key_out->data_ptr() : nullptr, current_stream()),
+               op);
+}
+
+// flash_decode_paged(query [sequences,H,D], the cache, its table and lengths -> out [sequences,H,D])
+void flash_decode_paged(const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& page_table,
+                        const at::Tensor& lengths, double softmax_scale, at::Tensor& out) {
+  constexpr const char* op = "flash_decode_paged";
+  const tf_paged_cache_t cache = paged_cache(key_cache, value_cache, page_table, lengths, query, op);
+  TORCH_CHECK(query.dim() == 3, "tilefusion::", op, ": query must be [sequences, heads, D], got ", query.sizes(), ".");
+  const int64_t h = query.size(1);
+  int64_t strides[2];
+  check_rows(query, "query", cache.sequences, h, cache.D, query, op, strides);
+  check_result(out, "out", cache.sequences, h, cache.D, query, op);
+  TORCH_CHECK(h > 0 && h % cache.kv_heads == 0, "tilefusion::", op, ": the heads of query (", h, ") must be a multiple of those of the cache (", cache.kv_heads, ").");
+  if (cache.sequences == 0) return;
+  const c10::DeviceGuard there(query.device());
+  const size_t bytes = tf_flash_decode_paged_workspace_bytes(cache.sequences, h, cache.kv_heads, cache.D);
+  const c10::DataPtr ws = scratch(bytes, query);
+  check_status(tf_flash_decode_paged(&cache, query.data_ptr(), strides, out.data_ptr(), h, softmax_scale, ws.get(), bytes, current_stream()), op);
+}
+
 }  // namespace kernels
 
 // Self-registering op table: each REGISTER_OP adds (schema, installer) at load time, and the
@@ -660,6 +781,15 @@ REGISTER_OP(linear_cross_entropy_backward,
             "linear_cross_entropy_backward(Tensor grad_loss, Tensor hidden, Tensor weight, Tensor target, Tensor lse, "
             "int ignore_index, Tensor(a!)? grad_hidden, Tensor(b!)? grad_weight) -> ()",
             &kernels::linear_cross_entropy_backward);
+
+REGISTER_OP(append_paged_kv,
+            "append_paged_kv(Tensor query, Tensor key, Tensor value, Tensor cos, Tensor sin, Tensor(a!) key_cache, Tensor(b!) value_cache, "
+            "Tensor page_table, Tensor lengths, Tensor? offsets, bool interleaved, Tensor(c!) query_out, Tensor(d!)? key_out) -> ()",
+            &kernels::append_paged_kv);
+REGISTER_OP(flash_decode_paged,
+            "flash_decode_paged(Tensor query, Tensor key_cache, Tensor value_cache, Tensor page_table, Tensor lengths, "
+            "float softmax_scale, Tensor(a!) out) -> ()",
+            &kernels::flash_decode_paged);
 
 TORCH_LIBRARY(tilefusion, m) { KernelRegistry::instance().register_with_torch(m); }
 TORCH_LIBRARY_IMPL(tilefusion, CUDA, m) { KernelRegistry::instance().register_implementations(m); }

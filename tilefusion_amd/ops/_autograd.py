@@ -38,3 +38,18 @@ def records(op: str, *tensors: torch.Tensor) -> bool:
         return False
     not_captured(op)
     return True
+
+
+def refuse_gradients(op: str, *tensors: torch.Tensor) -> None:
+    """Refuses a call whose inputs ask for a gradient: `op` has none, and results without one would end the graph without a word."""
+    refuse_transforms(op, *tensors)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op}: there is no gradient; call it under torch.no_grad()")
+
+
+def rows_in_place(t: torch.Tensor) -> torch.Tensor:
+    """t [.., heads, D] as it is where every row lies in one piece at a 16-byte boundary (elements of 16 bits), otherwise a copy that does."""
+    if t.dim() == 3 and t.stride(2) == 1 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
