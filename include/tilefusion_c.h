@@ -321,6 +321,25 @@ TF_API size_t tf_flash_decode_paged_workspace_bytes(int64_t sequences, int64_t h
 TF_API int tf_flash_decode_paged(const tf_paged_cache_t* cache, const void* query, const int64_t* query_strides, void* out, int64_t heads,
                                  double softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention over sequences packed one behind the other.  query [tokens, heads, D], key and value [kv_tokens, kv_heads, D] of dtype (fp16 or bf16), D 64
+ * or 128; head h attends head h / (heads / kv_heads) of the keys; strides in elements from token to token and head to head, multiples of 8 below
+ * 2^24, 16-byte boundaries.  offsets and kv_offsets [sequences + 1] int32 in device memory, ascending: sequence b is queries offsets[b] .. offsets[b+1] - 1
+ * and keys kv_offsets[b] .. kv_offsets[b+1] - 1 (null: the same as the queries).  What they name beyond the tensors is cut off.  causal: query i of a
+ * sequence of m queries and n keys sees keys up to i + n - m, the last one all.  tokens and kv_tokens < 2^24.  (No counterpart in the reference, whose attention has one
+ * length and one head count, include/kernels/ops.hpp:47-52.) */
+typedef struct {
+  const void *query, *key, *value;
+  int64_t query_strides[2], key_strides[2], value_strides[2];
+  int64_t tokens, kv_tokens, sequences, heads, kv_heads, D;
+  const int32_t *offsets, *kv_offsets;
+  double softmax_scale;
+  int causal, dtype;
+} tf_packed_attention_t;
+/* out [tokens, heads, D] = softmax(softmax_scale * Q K^T) V per sequence and head, and where lse is not null lse [heads, tokens] fp32 = log sum exp of the
+ * scaled scores.  Scores, maxima and sums in fp32; the weights are rounded to dtype for the product with V.  Rows that see no key, and rows of no
+ * sequence, are zero and their lse -inf. */
+TF_API int tf_flash_attention_packed(const tf_packed_attention_t* p, void* out, float* lse, void* stream);
+
 /* What a call would run, decided on the host from the sizes alone; nothing is launched.
  * tf_gemm_kernel_index, with operands at 16-byte boundaries: position of the kernel in the table kGemmKernels (csrc/gemm.hip), or behind
  * its end 0 for the bounds-checked kernel, from 1 on for the whole-line forms of kLinesKernels, then for the tile of 160 x 128, K a
@@ -328,7 +347,7 @@ TF_API int tf_flash_decode_paged(const tf_paged_cache_t* cache, const void* quer
  * *wavefronts those of a workgroup; 0 for arguments that tf_flash_decode rejects.  tf_flash_attention_rows:
  * query rows per workgroup of the tuned kernels for D = 64, 96, 128 (0 for other arguments); tf_flash_attention_pairs: 1 where
  * a workgroup of them takes two query tiles of a causal slice; tf_flash_attention_wide_rows: the rows of
- * tf_flash_attention_fwd_wide, twice that for pairs.  tf_fused_two_gemms_rows: rows per workgroup (64 or 128) where a problem, handed
+ * tf_flash_attention_fwd_wide, twice that for pairs.  tf_flash_attention_packed_rows: rows (queries of a group's heads) per workgroup (256, 128 or 64).  tf_fused_two_gemms_rows: rows per workgroup (64 or 128) where a problem, handed
  * `workspace_bytes`, runs the streaming kernel with operands at 16-byte boundaries, otherwise 0.  tf_scatter_nd_plan, `data` in ordinary memory of the
  * current device, it and 16-bit updates at 4-byte boundaries: updates that are sorted together (0: each goes straight to memory), and in
  * *words_a_lane the 32-bit words of an update that a lane adds; -1 for other arguments. */
@@ -346,6 +365,7 @@ TF_API int tf_flash_decode_plan(int64_t batch_heads, int64_t Lkv, int64_t D, int
 TF_API int tf_flash_attention_rows(int64_t batch, int64_t Lq, int64_t Lkv, int64_t D, int causal);
 TF_API int tf_flash_attention_pairs(int64_t batch, int64_t Lq, int64_t Lkv, int64_t D, int causal);
 TF_API int tf_flash_attention_wide_rows(int64_t batch, int64_t Lq, int causal);
+TF_API int tf_flash_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads);
 TF_API int tf_scatter_nd_plan(int64_t num_index_rows, int64_t targets, int64_t slice, int dtype, int* words_a_lane);
 TF_API int tf_fused_two_gemms_rows(int64_t batch, int64_t M, int64_t N, int64_t K, int64_t P, size_t workspace_bytes);
 

@@ -25,6 +25,14 @@ class PagedCache(ctypes.Structure):
                 ("sequences", _i64), ("dtype", _i)]
 
 
+class PackedAttention(ctypes.Structure):
+    """tf_packed_attention_t"""
+
+    _fields_ = [("query", _vp), ("key", _vp), ("value", _vp), ("query_strides", _i64 * 2), ("key_strides", _i64 * 2), ("value_strides", _i64 * 2),
+                ("tokens", _i64), ("kv_tokens", _i64), ("sequences", _i64), ("heads", _i64), ("kv_heads", _i64), ("D", _i64), ("offsets", _vp),
+                ("kv_offsets", _vp), ("softmax_scale", _d), ("causal", _i), ("dtype", _i)]
+
+
 # name -> (restype, argtypes); every symbol include/tilefusion_c.h declares
 SIGNATURES = {
     "tf_gemm_f16": (_i, [_vp, _vp, _vp, _i, _i64, _i64, _i64, _i, _i, _i, _i, _i, _vp]),
@@ -64,6 +72,7 @@ SIGNATURES = {
     "tf_append_paged_kv": (_i, [ctypes.POINTER(PagedCache), _vp, _vp, _vp, ctypes.POINTER(_i64), _vp, _vp, _i64, _i64, _i, _vp, _i64, _i64, _vp, _vp, _vp]),
     "tf_flash_decode_paged_workspace_bytes": (_sz, [_i64] * 4),
     "tf_flash_decode_paged": (_i, [ctypes.POINTER(PagedCache), _vp, ctypes.POINTER(_i64), _vp, _i64, _d, _vp, _sz, _vp]),
+    "tf_flash_attention_packed": (_i, [ctypes.POINTER(PackedAttention), _vp, _vp, _vp]),
     "tf_product_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_product_cols_plan": (_i, [_i64, _i64, _i64, ctypes.POINTER(_i)]),
     "tf_product_pair_plan": (_i, [_i64] * 6 + [ctypes.POINTER(_i)] * 2),
@@ -73,6 +82,7 @@ SIGNATURES = {
     "tf_flash_attention_rows": (_i, [_i64, _i64, _i64, _i64, _i]),
     "tf_flash_attention_pairs": (_i, [_i64, _i64, _i64, _i64, _i]),
     "tf_flash_attention_wide_rows": (_i, [_i64, _i64, _i]),
+    "tf_flash_attention_packed_rows": (_i, [_i64] * 4),
     "tf_scatter_nd_plan": (_i, [_i64, _i64, _i64, _i, ctypes.POINTER(_i)]),
     "tf_fused_two_gemms_rows": (_i, [_i64, _i64, _i64, _i64, _i64, _sz]),
     "tf_jit_compile": (_i, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p), _i,

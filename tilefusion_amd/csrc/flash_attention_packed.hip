@@ -1,0 +1,64 @@
+// Attention over packed sequences: the C entry points, and which instance of the kernels a call runs.
+#include <algorithm>
+
+#include "flash_attention_packed.hpp"
+
+namespace tfk {
+namespace {
+
+int check_packed(const char* who, const tf_packed_attention_t* p) {
+  TFK_REQUIRE(p, TF_ERR_INVALID_ARG, "%s: null pointer", who);
+  TFK_REQUIRE(p->dtype == TF_DTYPE_F16 || p->dtype == TF_DTYPE_BF16, TF_ERR_UNSUPPORTED, "%s: dtype must be TF_DTYPE_F16 or TF_DTYPE_BF16", who);
+  TFK_REQUIRE(p->D == 64 || p->D == 128, TF_ERR_UNSUPPORTED, "%s: head dim must be 64 or 128 (got %lld)", who, (long long)p->D);
+  TFK_REQUIRE(p->tokens >= 0 && p->kv_tokens >= 0 && p->tokens < (1 << 24) && p->kv_tokens < (1 << 24) && p->sequences >= 0 && p->sequences <= 65536,
+              TF_ERR_INVALID_ARG, "%s: tokens and kv_tokens must be below 2^24, sequences at most 65536", who);
+  TFK_REQUIRE(p->heads > 0 && p->heads <= 1024 && p->kv_heads > 0 && p->heads % p->kv_heads == 0, TF_ERR_INVALID_ARG,
+              "%s: heads must be a multiple of kv_heads, at most 1024 (got %lld and %lld)", who, (long long)p->heads, (long long)p->kv_heads);
+  TFK_REQUIRE(std::max(p->tokens, p->kv_tokens) * (p->heads / p->kv_heads) < (1ll << 31) - 256, TF_ERR_INVALID_ARG,
+              "%s: tokens times the heads of a group must be below 2^31 - 256", who);
+  TFK_REQUIRE(p->softmax_scale == p->softmax_scale && p->softmax_scale - p->softmax_scale == 0.0, TF_ERR_INVALID_ARG,
+              "%s: softmax_scale must be finite", who);
+  if (p->tokens == 0 && p->kv_tokens == 0) return TF_OK;
+  TFK_REQUIRE(p->offsets && (p->query || p->tokens == 0) && ((p->key && p->value) || p->kv_tokens == 0), TF_ERR_INVALID_ARG, "%s: null pointer", who);
+  TFK_REQUIRE(p->kv_offsets || p->tokens == p->kv_tokens, TF_ERR_INVALID_ARG, "%s: keys of another number than queries need kv_offsets", who);
+  const int64_t* strides[] = {p->query_strides, p->key_strides, p->value_strides};
+  for (const int64_t* s : strides)
+    for (int i = 0; i < 2; ++i)
+      TFK_REQUIRE(s[i] >= 0 && s[i] % 8 == 0 && s[i] < (1 << 24), TF_ERR_INVALID_ARG, "%s: strides must be multiples of 8 elements, below 2^24", who);
+  TFK_REQUIRE(((reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value)) & 15) == 0,
+              TF_ERR_INVALID_ARG, "%s: operands must begin at 16-byte boundaries", who);
+  return TF_OK;
+}
+PackedArgs packed_args(const tf_packed_attention_t& p) {
+  return {p.offsets, p.kv_offsets ? p.kv_offsets : p.offsets, (int)p.sequences, (int)p.tokens, (int)p.kv_tokens, (int)p.heads, (int)p.kv_heads,
+          make_divider((unsigned)(p.heads / p.kv_heads)), (int)p.query_strides[0], (int)p.key_strides[0], (int)p.value_strides[0], (int)p.query_strides[1], (int)p.key_strides[1],
+          (int)p.value_strides[1], nullptr};
+}
+
+// Rows per workgroup, from the sequences' mean length, which is all that the host knows.
+int packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads) {
+  const int64_t mean = sequences > 0 ? tokens / sequences * (heads / kv_heads) : 0, all = tokens * heads;
+  if (mean >= 512 && all / 256 + sequences / 2 * kv_heads >= 256) return 256;
+  if (mean >= 96 && all / 128 + sequences / 2 * kv_heads >= 256) return 128;
+  return 64;
+}
+
+}  // namespace
+}  // namespace tfk
+
+extern "C" int tf_flash_attention_packed(const tf_packed_attention_t* p, void* out, float* lse, void* stream) {
+  using namespace tfk;
+  constexpr const char* who = "tf_flash_attention_packed";
+  if (int rc = check_packed(who, p)) return rc;
+  if (p->tokens == 0) return TF_OK;
+  TFK_REQUIRE(out && (reinterpret_cast<uintptr_t>(out) & 15) == 0, TF_ERR_INVALID_ARG, "%s: out must begin at a 16-byte boundary", who);
+  PackedCall c = {p->query, p->key, p->value, out, packed_args(*p), (float)(p->softmax_scale * 1.4426950408889634), p->dtype == TF_DTYPE_BF16,
+                  p->causal != 0, packed_rows(p->tokens, p->sequences, p->heads, p->kv_heads), static_cast<hipStream_t>(stream)};
+  c.args.lse = lse;
+  return p->D == 128 ? run_attention_packed_d128(c) : run_attention_packed_d64(c);
+}
+
+extern "C" int tf_flash_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads) {
+  if (tokens < 0 || sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
+  return tfk::packed_rows(tokens, sequences, heads, kv_heads);
+}

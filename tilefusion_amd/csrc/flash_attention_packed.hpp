@@ -1,0 +1,23 @@
+// Attention over packed sequences: what the C entry points (flash_attention_packed.hip) and the kernels' source files share.
+#pragma once
+
+#include "packed_sequences.hpp"
+
+namespace tfk {
+
+struct PackedCall {
+  const void *query, *key, *value;
+  void* out;
+  PackedArgs args;
+  float scale_log2;
+  bool bf16, causal;
+  int rows;   // per workgroup: 256, 128 or 64
+  hipStream_t stream;
+};
+int run_attention_packed_d64(const PackedCall& c);
+int run_attention_packed_d128(const PackedCall& c);
+
+// Tiles of `rows` that sequences of `all` rows together can make.
+inline int64_t most_tiles(int64_t all, int64_t sequences, int64_t rows) { return (all + sequences * (rows - 1)) / rows; }
+
+}  // namespace tfk

@@ -1,0 +1,130 @@
+// Sequences packed one behind the other, for attention: which rows of queries, and which keys, a workgroup takes.
+//
+// The query heads of a group read the same keys: they are rows of one problem, row r being head r % group of token r / group, so that a tile of rows
+// spans few tokens (less of a causal tile is masked, short sequences fill theirs) and keys are fetched once for a group.
+//
+// Sequence b is tokens offsets[b] .. offsets[b + 1] - 1 of the queries and kv_offsets[b] .. of the keys.  The host does not know them: a launch has
+// as many workgroups as there can be tiles, and each finds its own.  Offsets are in device memory and may hold anything; what they
+// name beyond the tensors is cut off.
+#pragma once
+
+#include "common.hpp"
+#include "paged_cache.hpp"
+
+namespace tfk {
+
+struct PackedArgs {
+  const int *offsets, *kv_offsets;   // [sequences + 1]
+  int sequences, tokens, kv_tokens, heads, kv_heads;
+  Divider group;   // query heads that share a head of keys
+  int query_row, key_row, value_row, query_head, key_head, value_head;   // strides in elements
+  float* lse;   // [heads][tokens], or null
+};
+
+struct PackedTile {
+  int sequence;   // -1: none
+  int from_end;   // tiles of the sequence behind it
+  int q0, lq, k0, lkv;   // tokens and keys: the first, how many
+};
+
+// rows [begin, begin + length) of a sequence, within `rows`
+struct PackedRange { int begin, length; };
+TFK_DEVICE PackedRange packed_range(int begin, int end, int rows) {
+  const int b = min(max(begin, 0), rows);
+  return {b, max(min(end, rows) - b, 0)};
+}
+
+TFK_DEVICE int wave_sum(int x) {
+#pragma unroll
+  for (int d = 1; d < kWaveSize; d *= 2) x += __shfl_xor(x, d);
+  return __builtin_amdgcn_readfirstlane(x);
+}
+TFK_DEVICE int wave_max(int x) {
+#pragma unroll
+  for (int d = 1; d < kWaveSize; d *= 2) x = max(x, __shfl_xor(x, d));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// The (blockIdx.x / kv_heads)-th of the tiles of `rows` rows that the sequences make, most keys first.  Tile e from a sequence's end ends
+// e * rows rows in front of it and counts as ceil(lkv * group / rows) - e (causal or not: the longest sequences first, and their last
+// tokens).  The largest number that more tiles reach than come before this one is found by halving, each step a
+// sum over the sequences, 64 at a time: with a few dozen sequences some hundred cycles a step, where a sorted list would be a launch of its own.
+TFK_DEVICE PackedTile packed_tile(const PackedArgs& a, int rows) {
+  const int rank = (int)blockIdx.x / a.kv_heads, lane = threadIdx.x % kWaveSize;
+  struct Own { int tiles, level; };   // of a lane's sequence
+  auto own = [&](int b) __attribute__((always_inline)) -> Own {
+    if (b >= a.sequences) return {0, 0};
+    const int lq = packed_range(a.offsets[b], a.offsets[b + 1], a.tokens).length;
+    const int lkv = packed_range(a.kv_offsets[b], a.kv_offsets[b + 1], a.kv_tokens).length;
+    return {(lq * (int)a.group.d + rows - 1) / rows, (lkv * (int)a.group.d + rows - 1) / rows};
+  };
+  const Own first = own(lane);   // (kept: mostly all there are)
+  auto of = [&](int b0) __attribute__((always_inline)) -> Own { return b0 == 0 ? first : own(b0 + lane); };
+  int most = -0x7fffffff, least = 0x7fffffff;
+  for (int b0 = 0; b0 < a.sequences; b0 += kWaveSize) {
+    const Own o = of(b0);
+    if (o.tiles > 0) {
+      most = max(most, o.level);
+      least = min(least, o.level - o.tiles + 1);
+    }
+  }
+  int high = wave_max(most) + 1, low = -wave_max(-least);   // none reaches `high`, all reach `low`
+  auto count = [&](int level) __attribute__((always_inline)) {
+    int n = 0;
+    for (int b0 = 0; b0 < a.sequences; b0 += kWaveSize) {
+      const Own o = of(b0);
+      n += min(max(o.level - level + 1, 0), o.tiles);
+    }
+    return wave_sum(n);
+  };
+  PackedTile tile = {-1, 0, 0, 0, 0, 0};
+  if (low >= high || count(low) <= rank) return tile;
+  int above = 0;   // tiles that reach `high`
+  while (high - low > 1) {
+    const int middle = low + (high - low) / 2, n = count(middle);
+    if (n > rank) {
+      low = middle;
+    } else {
+      high = middle;
+      above = n;
+    }
+  }
+  int left = rank - above;   // of the tiles that count `low`, one a sequence
+  for (int b0 = 0; b0 < a.sequences; b0 += kWaveSize) {
+    const Own o = of(b0);
+    const bool has = o.level >= low && o.level - low < o.tiles;
+    const unsigned long long all = __builtin_amdgcn_ballot_w64(has);
+    const int n = __builtin_popcountll(all);
+    if (left >= n) {
+      left -= n;
+      continue;
+    }
+    const bool mine = has && __builtin_popcountll(all & ((1ull << lane) - 1)) == left;
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(mine));
+    tile.sequence = b0 + at;
+    tile.from_end = __builtin_amdgcn_readlane(o.level, at) - low;
+    break;
+  }
+  if (tile.sequence < 0) return tile;
+  const PackedRange q = packed_range(read_uniform(a.offsets + tile.sequence), read_uniform(a.offsets + tile.sequence + 1), a.tokens);
+  const PackedRange k = packed_range(read_uniform(a.kv_offsets + tile.sequence), read_uniform(a.kv_offsets + tile.sequence + 1), a.kv_tokens);
+  tile.q0 = q.begin;
+  tile.lq = q.length;
+  tile.k0 = k.begin;
+  tile.lkv = k.length;
+  return tile;
+}
+
+// Rows in front of the first sequence and behind the last: `use` for each of them, the workgroups sharing them out.
+template <typename Use>
+TFK_DEVICE void rows_outside(const int* offsets, int sequences, int rows, Use use) {
+  const int from = min(max(read_uniform(offsets), 0), rows), to = min(max(read_uniform(offsets + sequences), from), rows);
+  const int outside = from + rows - to;
+  for (int i = blockIdx.x; i < outside; i += gridDim.x) use(i < from ? i : to + i - from);
+}
+template <typename T>
+TFK_DEVICE void clear_row(T* row, int elements) {
+  using V8 = T __attribute__((ext_vector_type(8)));
+  for (int c = threadIdx.x; c < elements / 8; c += blockDim.x) *reinterpret_cast<V8*>(row + 8 * c) = V8{};
+}
+}  // namespace tfk

@@ -1,6 +1,6 @@
 // PyTorch operator bindings: registers torch.ops.tilefusion.{gemm, fused_two_gemms,
 // flash_attention, flash_attention_fwd, flash_attention_fwd_kt, flash_decode, scatter_nd, quantize_rows, gemm_int8, gated_ffn, gated_ffn_backward,
-// linear_cross_entropy, linear_cross_entropy_backward, append_paged_kv, flash_decode_paged} for the CUDA dispatch key (HIP tensors
+// linear_cross_entropy, linear_cross_entropy_backward, append_paged_kv, flash_decode_paged, flash_attention_packed} for the CUDA dispatch key (HIP tensors
 // are "cuda" tensors on PyTorch-ROCm) and forwards to the C ABI in tilefusion_c.h on the
 // caller's current stream.
 //
@@ -703,6 +703,59 @@ void flash_decode_paged(const at::Tensor& query, const at::Tensor& key_cache, co
   check_status(tf_flash_decode_paged(&cache, query.data_ptr(), strides, out.data_ptr(), h, softmax_scale, ws.get(), bytes, current_stream()), op);
 }
 
+// ---- attention over packed sequences ------------------------------------------------------------
+namespace {
+tf_packed_attention_t packed_attention(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const at::Tensor& offsets,
+                                       const std::optional<at::Tensor>& kv_offsets, double softmax_scale, bool causal, const char* op) {
+  tf_packed_attention_t p = {};
+  TORCH_CHECK(query.is_cuda(), "tilefusion::", op, ": query must be a CUDA tensor.");
+  p.dtype = operand_dtype(query, op);
+  TORCH_CHECK(query.dim() == 3 && key.dim() == 3, "tilefusion::", op, ": query must be [tokens, heads, D], key and value [kv_tokens, kv_heads, D].");
+  p.tokens = query.size(0);
+  p.heads = query.size(1);
+  p.D = query.size(2);
+  p.kv_tokens = key.size(0);
+  p.kv_heads = key.size(1);
+  check_rows(query, "query", p.tokens, p.heads, p.D, query, op, p.query_strides);
+  check_rows(key, "key", p.kv_tokens, p.kv_heads, p.D, query, op, p.key_strides);
+  check_rows(value, "value", p.kv_tokens, p.kv_heads, p.D, query, op, p.value_strides);
+  check_int32(offsets, "offsets", query, op);
+  TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) > 0 && offsets.is_contiguous(), "tilefusion::", op, ": offsets must be [sequences + 1] and contiguous.");
+  p.sequences = offsets.size(0) - 1;
+  p.offsets = offsets.data_ptr<int32_t>();
+  if (kv_offsets.has_value()) {
+    check_int32(*kv_offsets, "kv_offsets", query, op);
+    TORCH_CHECK(kv_offsets->sizes() == offsets.sizes() && kv_offsets->is_contiguous(), "tilefusion::", op, ": kv_offsets must have the shape of offsets and be contiguous.");
+    p.kv_offsets = kv_offsets->data_ptr<int32_t>();
+  } else {
+    TORCH_CHECK(p.tokens == p.kv_tokens, "tilefusion::", op, ": keys of another number (", p.kv_tokens, ") than queries (", p.tokens, ") need kv_offsets.");
+  }
+  p.query = query.data_ptr();
+  p.key = key.data_ptr();
+  p.value = value.data_ptr();
+  p.softmax_scale = softmax_scale;
+  p.causal = causal ? 1 : 0;
+  return p;
+}
+void check_lse(const at::Tensor& lse, const tf_packed_attention_t& p, const at::Tensor& like, const char* op) {
+  check_operand(lse, "lse", like, op);
+  TORCH_CHECK(lse.scalar_type() == at::kFloat, "tilefusion::", op, ": lse must be float32.");
+  check_sizes(lse, "lse", p.heads, p.tokens, op);
+}
+}  // namespace
+
+// flash_attention_packed(query [T,H,D], key, value [S,Hkv,D], offsets, kv_offsets [sequences + 1] int32 -> out [T,H,D], lse [H,T] fp32 where it is given)
+void flash_attention_packed(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const at::Tensor& offsets,
+                            const std::optional<at::Tensor>& kv_offsets, double softmax_scale, bool causal, at::Tensor& out,
+                            const std::optional<at::Tensor>& lse) {
+  constexpr const char* op = "flash_attention_packed";
+  const tf_packed_attention_t p = packed_attention(query, key, value, offsets, kv_offsets, softmax_scale, causal, op);
+  check_result(out, "out", p.tokens, p.heads, p.D, query, op);
+  if (lse.has_value()) check_lse(*lse, p, query, op);
+  const c10::DeviceGuard there(query.device());
+  check_status(tf_flash_attention_packed(&p, out.data_ptr(), lse.has_value() ? lse->data_ptr<float>() : nullptr, current_stream()), op);
+}
+
 }  // namespace kernels
 
 // Self-registering op table: each REGISTER_OP adds (schema, installer) at load time, and the
@@ -790,6 +843,11 @@ REGISTER_OP(flash_decode_paged,
             "flash_decode_paged(Tensor query, Tensor key_cache, Tensor value_cache, Tensor page_table, Tensor lengths, "
             "float softmax_scale, Tensor(a!) out) -> ()",
             &kernels::flash_decode_paged);
+
+REGISTER_OP(flash_attention_packed,
+            "flash_attention_packed(Tensor query, Tensor key, Tensor value, Tensor offsets, Tensor? kv_offsets, "
+            "float softmax_scale, bool causal, Tensor(a!) out, Tensor(b!)? lse) -> ()",
+            &kernels::flash_attention_packed);
 
 TORCH_LIBRARY(tilefusion, m) { KernelRegistry::instance().register_with_torch(m); }
 TORCH_LIBRARY_IMPL(tilefusion, CUDA, m) { KernelRegistry::instance().register_implementations(m); }

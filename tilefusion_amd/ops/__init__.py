@@ -11,6 +11,7 @@
 
 from .append_paged_kv import append_paged_kv, rotation_tables  # noqa: F401
 from .flash_attention import FlashAttention, flash_attention
+from .flash_attention_packed import flash_attention_packed  # noqa: F401
 from .flash_decode import flash_decode
 from .flash_decode_paged import flash_decode_paged  # noqa: F401
 from .fused_two_gemms import fused_two_gemms
