@@ -14,8 +14,8 @@ int check_packed(const char* who, const tf_packed_attention_t* p) {
               TF_ERR_INVALID_ARG, "%s: tokens and kv_tokens must be below 2^24, sequences at most 65536", who);
   TFK_REQUIRE(p->heads > 0 && p->heads <= 1024 && p->kv_heads > 0 && p->heads % p->kv_heads == 0, TF_ERR_INVALID_ARG,
               "%s: heads must be a multiple of kv_heads, at most 1024 (got %lld and %lld)", who, (long long)p->heads, (long long)p->kv_heads);
-  TFK_REQUIRE(std::max(p->tokens, p->kv_tokens) * (p->heads / p->kv_heads) < (1ll << 31) - 256, TF_ERR_INVALID_ARG,
-              "%s: tokens times the heads of a group must be below 2^31 - 256", who);
+  TFK_REQUIRE(std::max(p->tokens, p->kv_tokens) * (p->heads / p->kv_heads) < (1ll << 30), TF_ERR_INVALID_ARG,
+              "%s: tokens times the heads of a group must be below 2^30", who);
   TFK_REQUIRE(p->softmax_scale == p->softmax_scale && p->softmax_scale - p->softmax_scale == 0.0, TF_ERR_INVALID_ARG,
               "%s: softmax_scale must be finite", who);
   if (p->tokens == 0 && p->kv_tokens == 0) return TF_OK;
@@ -56,6 +56,30 @@ extern "C" int tf_flash_attention_packed(const tf_packed_attention_t* p, void* o
                   p->causal != 0, packed_rows(p->tokens, p->sequences, p->heads, p->kv_heads), static_cast<hipStream_t>(stream)};
   c.args.lse = lse;
   return p->D == 128 ? run_attention_packed_d128(c) : run_attention_packed_d64(c);
+}
+
+extern "C" size_t tf_flash_attention_packed_backward_workspace_bytes(int64_t tokens, int64_t heads) {
+  if (tokens < 0 || heads <= 0) return 0;
+  return (size_t)tokens * (size_t)heads * 8;
+}
+
+extern "C" int tf_flash_attention_packed_backward(const tf_packed_attention_t* p, const void* grad_out, const void* out, const float* lse,
+                                                  void* grad_query, void* grad_key, void* grad_value, void* workspace, size_t workspace_bytes,
+                                                  void* stream) {
+  using namespace tfk;
+  constexpr const char* who = "tf_flash_attention_packed_backward";
+  if (int rc = check_packed(who, p)) return rc;
+  TFK_REQUIRE((grad_key == nullptr) == (grad_value == nullptr) || p->kv_tokens == 0, TF_ERR_INVALID_ARG, "%s: grad_key and grad_value are both asked for or neither", who);
+  if (p->tokens == 0 && p->kv_tokens == 0) return TF_OK;
+  TFK_REQUIRE((grad_out && out && lse && workspace) || p->tokens == 0, TF_ERR_INVALID_ARG, "%s: null pointer", who);
+  TFK_REQUIRE(((reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(grad_query) |
+                reinterpret_cast<uintptr_t>(grad_key) | reinterpret_cast<uintptr_t>(grad_value) | reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
+              TF_ERR_INVALID_ARG, "%s: operands must begin at 16-byte boundaries", who);
+  const size_t need = tf_flash_attention_packed_backward_workspace_bytes(p->tokens, p->heads);
+  TFK_REQUIRE(workspace_bytes >= need || p->tokens == 0, TF_ERR_INVALID_ARG, "%s: workspace holds %zu bytes, %zu needed", who, workspace_bytes, need);
+  const PackedGradCall c = {p->query, p->key, p->value, out, grad_out, lse, grad_query, grad_key, grad_value, workspace, packed_args(*p),
+                            (float)p->softmax_scale, p->dtype == TF_DTYPE_BF16, p->causal != 0, static_cast<hipStream_t>(stream)};
+  return p->D == 128 ? run_attention_packed_backward_d128(c) : run_attention_packed_backward_d64(c);
 }
 
 extern "C" int tf_flash_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads) {

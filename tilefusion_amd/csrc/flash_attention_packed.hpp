@@ -17,6 +17,19 @@ struct PackedCall {
 int run_attention_packed_d64(const PackedCall& c);
 int run_attention_packed_d128(const PackedCall& c);
 
+struct PackedGradCall {
+  const void *query, *key, *value, *out, *grad_out;
+  const float* lse;
+  void *grad_query, *grad_key, *grad_value;   // grad_query, or grad_key and grad_value, may be null
+  void* stats;   // room for 8 bytes a row
+  PackedArgs args;
+  float scale;
+  bool bf16, causal;
+  hipStream_t stream;
+};
+int run_attention_packed_backward_d64(const PackedGradCall& c);
+int run_attention_packed_backward_d128(const PackedGradCall& c);
+
 // Tiles of `rows` that sequences of `all` rows together can make.
 inline int64_t most_tiles(int64_t all, int64_t sequences, int64_t rows) { return (all + sequences * (rows - 1)) / rows; }
 

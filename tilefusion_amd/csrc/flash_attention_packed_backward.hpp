@@ -1,0 +1,572 @@
+// Gradients of attention over packed sequences (the forward pass: flash_attention_packed_kernel.hpp), in a source file per head dimension.
+//
+// With P = exp(scale Q K^T - lse) and delta = rowsum(dO o O):   dV = P^T dO,   dS = P o (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q.
+// P is made again from the forward pass's log-sum-exp.  Three kernels, no atomics, so that the same bits come out every time:
+//   * stats: delta, and lse in units of log2, beside each other in the order of rows that the others read them in;
+//   * keys: a workgroup takes 128 keys and walks the rows that see them (all heads of a group are rows, so a group's sum is the same sum);
+//   * queries: a workgroup takes 128 rows and walks their keys.  That makes P and dO V^T twice, 7 products instead of 5; sums of dQ from the
+//     key side would need atomics in fp32, whose order changes results, and a pass of their own over 4 bytes an element.
+// Both walk tiles of 32 in a ring in LDS (global_load_lds), their own 32 keys or rows of a wavefront in registers as the second operand of the
+// first two products, whose accumulators are the second operand of the last ones as they are: a lane holds one key (row), its registers
+// four rows (keys).  The tile is read from LDS as rows and, transposed, as columns; one swizzle serves both.  Two workgroups of four wavefronts share a
+// CU, so that one's exponentials run beside the other's products.
+#pragma once
+
+#include "flash_attention.hpp"
+#include "flash_attention_packed.hpp"
+
+namespace tfk {
+namespace {
+
+constexpr int kGradWaves = 4, kGradTile = 32, kGradOwn = kGradWaves * 32;   // keys (rows) of a workgroup
+constexpr float kLog2E = 1.4426950408889634f;
+
+// 16 rows that read one logical 16-byte chunk hit 16 different bank groups, and 8 rows that read 32 bytes transposed hit 8 different windows.
+template <int CH>
+__host__ __device__ constexpr int swz_both(int row, int c) {
+  const int pair = CH >= 16 ? row & 7 : (row >> 1) & 3;
+  return c ^ (pair << 1 | ((row >> 3) & 1));
+}
+
+// Where a lane finds its part of a fragment in a tile [rows][D]: rows lr, chunk 4 kk + lg (rows), or rows 4 lg .. + 3 and 16 more, columns
+// 16 db .. + 15, transposed (columns).  The swizzle is an exclusive or of chunk numbers, so that kk and db are one more of the offset in a tile at a multiple of 256 bytes.
+struct FragmentOffsets { unsigned row, column; };
+template <int D>
+TFK_DEVICE FragmentOffsets fragment_offsets() {
+  const int lane = threadIdx.x & 63, lr = lane & 15, lg = lane >> 4, row = 4 * lg + (lr >> 2), col = 4 * (lr & 3);
+  return {(unsigned)(lr * D * 2 + swz_both<D / 8>(lr, lg) * 16), (unsigned)(row * D * 2 + swz_both<D / 8>(row, col / 8) * 16 + (col % 8) * 2)};
+}
+template <typename T>
+TFK_DEVICE typename Vec<T>::v8 row_fragment(unsigned tile, const FragmentOffsets& off, int kk, int block_bytes) {
+  return lds_read_b128<typename Vec<T>::v8>((opaque(tile + off.row) ^ (kk << 6)) + block_bytes);
+}
+template <typename T, int D>
+TFK_DEVICE typename Vec<T>::v8 column_fragment(unsigned tile, const FragmentOffsets& off, int db) {
+  using V4 = typename Vec<T>::v4;
+  const unsigned at = opaque(tile + off.column) ^ (db << 5);
+  const V4 lo = lds_read_tr4<V4>(at), hi = lds_read_tr4<V4>(at + 16 * D * 2);
+  typename Vec<T>::v8 f;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    f[t] = lo[t];
+    f[4 + t] = hi[t];
+  }
+  return f;
+}
+
+// One in the sign's place of each 16-bit half that is an infinity or a NaN: an exponent of ones, into which one more carries.
+template <typename T>
+TFK_DEVICE unsigned not_finite_halves(unsigned two) {
+  return ((two & 0x7fff7fffu) + (std::is_same_v<T, bf16_t> ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+// Zeros in the place of what is not finite.
+template <typename T>
+TFK_DEVICE void clean(typename Vec<T>::v8& f) {
+  uint4_t x = __builtin_bit_cast(uint4_t, f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] &= ~((not_finite_halves<T>(x[e]) >> 15) * 0xffffu);
+  f = __builtin_bit_cast(typename Vec<T>::v8, x);
+}
+
+// fp16: P is taken 2^15 times as large (its smallest number is then 2^-39), and dS times a power of two a lane, by which the largest so far is
+// 2^14 to 2^15; both are divided out of the fp32 sums.  bf16 has the range.
+template <typename T>
+constexpr float kUpP = std::is_same_v<T, bf16_t> ? 0.f : 15.f;
+TFK_DEVICE float power_for(float largest) {   // 2^(14 - floor(log2 largest)), within fp32
+  const int e = (int)(__builtin_bit_cast(unsigned, largest) >> 23 & 255u);
+  return __builtin_bit_cast(float, (unsigned)min(max(127 + 14 + 127 - e, 27), 227) << 23);
+}
+
+struct GradArgs {
+  PackedArgs packed;      // of query, key and value
+  const void *query, *key, *value, *out, *grad_out;   // out, grad_out [tokens][heads][D]
+  const float* lse;       // [heads][tokens]
+  float2_t* stats;        // [kv_heads][tokens * group]: lse * log2 e, delta
+  void *grad_query, *grad_key, *grad_value;            // contiguous
+  float scale, scale_log2;
+};
+
+// Every row of a tile is 16 lanes wide at most; a thread takes 8 elements of a row of out and grad_out.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void packed_stats_kernel(GradArgs a) {
+  using V8 = typename Vec<T>::v8;
+  constexpr int kLanes = D / 8;
+  const int64_t row = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes, all = (int64_t)a.packed.tokens * a.packed.heads;
+  const int64_t at = (row < all ? row : all - 1) * D + threadIdx.x % kLanes * 8;
+  const V8 o = *reinterpret_cast<const V8*>(static_cast<const T*>(a.out) + at), g = *reinterpret_cast<const V8*>(static_cast<const T*>(a.grad_out) + at);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum = fmaf((float)o[i], (float)g[i], sum);
+#pragma unroll
+  for (int d = 1; d < kLanes; d *= 2) sum += __shfl_xor(sum, d);
+  if (row >= all || threadIdx.x % kLanes != 0) return;
+  const int token = (int)(row / a.packed.heads), head = (int)(row % a.packed.heads), group = (int)a.packed.group.d;
+  const float2_t x = {a.lse[(size_t)head * a.packed.tokens + token] * kLog2E, sum};
+  a.stats[((size_t)(head / group) * a.packed.tokens + token) * group + head % group] = x;
+}
+
+// Columns 16 db + 4 lg .. of row lr, times `factor` (of the lane's row lr), to row st_row of `to` (the lane's pointer to that row's segment).
+template <typename T, int kDB>
+TFK_DEVICE void store_transposed(const float4_t (&acc)[kDB], float factor, T* to, bool there) {
+  using V2 = typename Vec<T>::v2;
+  const int lane = threadIdx.x & 63, st_row = lane >> 2, st_seg = lane & 3, src_lane = st_row + 16 * (((st_seg & 1) << 1) | (st_seg >> 1));
+#pragma unroll
+  for (int db = 0; db < kDB; db += 2) {
+    unsigned x[2], y[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const V2 hx = {(T)(acc[db][2 * h] * factor), (T)(acc[db][2 * h + 1] * factor)};
+      const V2 hy = {(T)(acc[db + 1][2 * h] * factor), (T)(acc[db + 1][2 * h + 1] * factor)};
+      x[h] = __builtin_bit_cast(unsigned, hx);
+      y[h] = __builtin_bit_cast(unsigned, hy);
+#if defined(__HIP_DEVICE_COMPILE__)
+      auto sw = __builtin_amdgcn_permlane16_swap(x[h], y[h], false, false);
+      x[h] = sw[0];
+      y[h] = sw[1];
+#endif
+    }
+    uint4_t v;
+    v[0] = (unsigned)__builtin_amdgcn_ds_bpermute(4 * src_lane, (int)x[0]);
+    v[1] = (unsigned)__builtin_amdgcn_ds_bpermute(4 * src_lane, (int)x[1]);
+    v[2] = (unsigned)__builtin_amdgcn_ds_bpermute(4 * src_lane, (int)y[0]);
+    v[3] = (unsigned)__builtin_amdgcn_ds_bpermute(4 * src_lane, (int)y[1]);
+    if (there) *reinterpret_cast<uint4_t*>(to + 16 * db + 8 * st_seg) = v;
+  }
+}
+
+// What a lane's dS were multiplied by so far (fp16).
+struct Power {
+  float up = 0.f;   // 0: nothing but zeros seen
+};
+// Four dS of a lane, times its power of two, into half `h` of an operand whose first half may be there; `acc` are the sums that hold it.
+template <typename T, int kDB>
+TFK_DEVICE void to_operand(const float4_t& ds, int h, typename Vec<T>::v8& f, Power& power, float4_t (&acc)[kDB]) {
+  if constexpr (std::is_same_v<T, bf16_t>) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) f[4 * h + t] = (T)ds[t];
+  } else {
+    const float big = fmaxf(fmaxf(__builtin_fabsf(ds[0]), __builtin_fabsf(ds[1])), fmaxf(__builtin_fabsf(ds[2]), __builtin_fabsf(ds[3])));
+    // (infinities and NaN go through as they are)
+    const bool finite = big < INFINITY;
+    if (__builtin_amdgcn_ballot_w64(finite && (big * power.up > 32768.f || (power.up == 0.f && big > 0.f))) != 0) {
+      const float largest = quad_max(finite ? big : 0.f);
+      if (largest * power.up > 32768.f || (power.up == 0.f && largest > 0.f)) {
+        const float up = power_for(largest), factor = power.up == 0.f ? 1.f : up / power.up;
+        power.up = up;
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) acc[db] *= factor;
+        if (h == 1) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) f[t] = (T)((float)f[t] * factor);
+        }
+      }
+    }
+    const float by = power.up == 0.f ? 1.f : power.up;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) f[4 * h + t] = (T)(ds[t] * by);
+  }
+}
+
+template <int D>
+constexpr int grad_stage_bytes() { return 2 * kGradTile * D * 2 + kGradTile * 8; }
+constexpr int kGradStages = 4;
+
+// ---- dK and dV of 128 keys ------------------------------------------------------------------------
+template <typename T, int D, bool kCausal>
+__global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_keys_kernel(GradArgs g) {
+  using V8 = typename Vec<T>::v8;
+  constexpr int kChunks = D / 8, kRowsPerInstr = 64 / kChunks, kTileBytes = kGradTile * D * 2;
+  constexpr int kStage = grad_stage_bytes<D>(), kPerWave = kTileBytes / 1024 / kGradWaves, kRequests = 2 * kPerWave + 1;
+  constexpr int kKK = D / 32, kDB = D / 16, kKB = 2;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const PackedArgs& a = g.packed;
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  T* const grad_key = static_cast<T*>(g.grad_key);
+  T* const grad_value = static_cast<T*>(g.grad_value);
+  rows_outside(a.kv_offsets, a.sequences, a.kv_tokens, [&](int row) {
+    clear_row(grad_key + (size_t)row * a.kv_heads * D, a.kv_heads * D);
+    clear_row(grad_value + (size_t)row * a.kv_heads * D, a.kv_heads * D);
+  });
+  const PackedTile tile = packed_key_tile(a, kGradOwn);
+  if (tile.sequence < 0) return;
+  const int head = (int)blockIdx.x % a.kv_heads, group = (int)a.group.d;
+  const int shift = tile.lkv - tile.lq, rows = tile.lq * group, key0 = tile.from_end * kGradOwn;   // (counted from the front)
+  const T* const Q = static_cast<const T*>(g.query) + (size_t)tile.q0 * a.query_row + (size_t)head * group * a.query_head;
+  const T* const dO = static_cast<const T*>(g.grad_out) + ((size_t)tile.q0 * a.heads + (size_t)head * group) * D;
+  const float2_t* const stats = g.stats + ((size_t)head * a.tokens + tile.q0) * group;
+
+  // ---- this wavefront's keys: blocks wave and wave + 4 of 16 (so that all have as much behind the diagonal) ----
+  V8 kf[kKB][kKK], vf[kKB][kKK];
+  int row_min[kKB];   // the first row that sees key lr of a block
+#pragma unroll
+  for (int kb = 0; kb < kKB; ++kb) {
+    const int key = key0 + 16 * (kGradWaves * kb + wave) + lr;
+    row_min[kb] = kCausal ? max(key - shift, 0) * group : 0;
+    const size_t at = tile.k0 + min(key, tile.lkv - 1);
+    const T* k = static_cast<const T*>(g.key) + at * a.key_row + (size_t)head * a.key_head;
+    const T* v = static_cast<const T*>(g.value) + at * a.value_row + (size_t)head * a.value_head;
+#pragma unroll
+    for (int kk = 0; kk < kKK; ++kk) {
+      kf[kb][kk] = *reinterpret_cast<const V8*>(k + 32 * kk + 8 * lg);
+      vf[kb][kk] = *reinterpret_cast<const V8*>(v + 32 * kk + 8 * lg);
+    }
+  }
+  const int tiles = (rows + kGradTile - 1) / kGradTile;
+  const int first = kCausal ? min(tiles, max(key0 - shift, 0) * group / kGradTile) : 0;
+  // tiles from here on are masked for none of this wavefront's keys, but for the last one's rows behind the last
+  const int last_min = __builtin_amdgcn_readfirstlane(kCausal ? max(key0 + 16 * (kGradWaves * (kKB - 1) + wave) + 15 - shift, 0) * group : 0);
+  const int n_masked = min(tiles, (last_min + kGradTile - 1) / kGradTile), n_full = rows / kGradTile;
+  const int first_min = __builtin_amdgcn_readfirstlane(kCausal ? max(key0 + 16 * wave - shift, 0) * group : 0);
+
+  const unsigned smem_base = lds_address(smem);
+  auto request_tile = [&](int t) __attribute__((always_inline)) {
+    const unsigned stage = smem_base + t % kGradStages * kStage;
+    const int r0 = min(t, tiles - 1) * kGradTile;
+#pragma unroll
+    for (int i = 0; i < kPerWave; ++i) {
+      const int instr = wave + kGradWaves * i, row_l = instr * kRowsPerInstr + lane / kChunks;
+      const int row = min(r0 + row_l, rows - 1), token = divide(a.group, row), hg = row - token * group;
+      const int col = swz_both<kChunks>(row_l, lane % kChunks) * 8;
+      lds_dma_16B(Q + (size_t)token * a.query_row + (size_t)hg * a.query_head + col, stage + instr * 1024);
+      lds_dma_16B(dO + ((size_t)token * a.heads + hg) * D + col, stage + kTileBytes + instr * 1024);
+    }
+    // 8 rows' statistics, a lane each number
+    if (lane < 16) {
+      const float* from = reinterpret_cast<const float*>(stats + min(r0 + 8 * wave + lane / 2, rows - 1)) + lane % 2;
+      asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "{m0}"(stage + 2 * kTileBytes + wave * 64) : "memory");
+    }
+  };
+
+  const FragmentOffsets off = fragment_offsets<D>();
+  float4_t dk[kKB][kDB], dv[kKB][kDB];
+  Power power[kKB];
+#pragma unroll
+  for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) dk[kb][db] = dv[kb][db] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](int t, auto mask_c) __attribute__((always_inline)) {
+    constexpr bool kMask = decltype(mask_c)::value;
+    const unsigned stage = smem_base + t % kGradStages * kStage;
+    V8 pf[kKB], sf[kKB];
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+      float4_t s[kKB], dp[kKB];
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb) s[kb] = dp[kb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < kKK; ++kk) {
+        const V8 q = row_fragment<T>(stage, off, kk, rb * 16 * D * 2), o = row_fragment<T>(stage + kTileBytes, off, kk, rb * 16 * D * 2);
+#pragma unroll
+        for (int kb = 0; kb < kKB; ++kb) s[kb] = mfma_t<T>(q, kf[kb][kk], s[kb]);
+#pragma unroll
+        for (int kb = 0; kb < kKB; ++kb) dp[kb] = mfma_t<T>(o, vf[kb][kk], dp[kb]);
+        if (kk % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // (more of them ahead cost registers that there are not)
+      }
+      // rows 16 rb + 4 lg + r: their lse and delta
+      const float4_t x0 = lds_read_b128<float4_t>(stage + 2 * kTileBytes + (16 * rb + 4 * lg) * 8);
+      const float4_t x1 = lds_read_b128<float4_t>(stage + 2 * kTileBytes + (16 * rb + 4 * lg) * 8 + 16);
+      const float base[4] = {kUpP<T> - x0[0], kUpP<T> - x0[2], kUpP<T> - x1[0], kUpP<T> - x1[2]}, delta[4] = {x0[1], x0[3], x1[1], x1[3]};
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb) {
+        float4_t ds;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[kb][r], g.scale_log2, base[r])), d = p * (dp[kb][r] - delta[r]);
+          if constexpr (kMask) {
+            const int row = t * kGradTile + 16 * rb + 4 * lg + r;
+            const bool sees = row >= row_min[kb] && row < rows;
+            p = sees ? p : 0.f;
+            d = sees ? d : 0.f;
+          }
+          pf[kb][4 * rb + r] = (T)p;
+          ds[r] = d;
+        }
+        to_operand<T, kDB>(ds, rb, sf[kb], power[kb], dk[kb]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // Infinities and NaN in rows that a part of the keys does not see (there a weight of zero would make NaN of them) are taken out of the products.  Of Q
+    // that leaves the right NaN: a row with them has NaN weights.  Those of dO go to the keys that see them one by one.
+    bool found = false;
+    if constexpr (kMask) {
+      unsigned seen = 0;
+#pragma unroll
+      for (int i = 0; i < 2 * kTileBytes / 1024; ++i) {
+        const uint4_t x = lds_read_b128<uint4_t>(stage + lane * 16 + i * 1024);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen |= not_finite_halves<T>(x[e]);
+      }
+      found = __builtin_amdgcn_ballot_w64(seen != 0) != 0;
+      for (int i = 0; found && i < kTileBytes / 1024; ++i) {
+        const uint4_t x = lds_read_b128<uint4_t>(stage + kTileBytes + lane * 16 + i * 1024);
+        unsigned mine = 0;   // a bit for each of the eight
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned bits = not_finite_halves<T>(x[e]);
+          mine |= ((bits >> 15 & 1u) | (bits >> 30 & 2u)) << (2 * e);
+        }
+        for (;;) {
+          const unsigned long long lanes = __builtin_amdgcn_ballot_w64(mine != 0);
+          if (lanes == 0) break;
+          const int from = __builtin_ctzll(lanes), e = __builtin_ctz(__builtin_amdgcn_readlane(mine, from));
+          const unsigned pair = e < 4 ? (e < 2 ? x[0] : x[1]) : (e < 6 ? x[2] : x[3]);
+          const unsigned short bits = (unsigned short)(__builtin_amdgcn_readlane(pair, from) >> (e % 2 * 16));
+          const float value = (float)__builtin_bit_cast(T, bits);
+          const int row_l = i * kRowsPerInstr + from / kChunks, col = swz_both<kChunks>(row_l, from % kChunks) * 8 + e, row = t * kGradTile + row_l;
+#pragma unroll
+          for (int kb = 0; kb < kKB; ++kb) {
+            const float to_key = row >= row_min[kb] && row < rows ? value : 0.f;
+#pragma unroll
+            for (int db = 0; db < kDB; ++db)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) dv[kb][db][r] += 16 * db + 4 * lg + r == col ? to_key : 0.f;
+          }
+          if (lane == from) mine &= mine - 1;
+        }
+      }
+    }
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) {
+      V8 o = column_fragment<T, D>(stage + kTileBytes, off, db), q = column_fragment<T, D>(stage, off, db);
+      if (found) {
+        clean<T>(o);
+        clean<T>(q);
+      }
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb) dv[kb][db] = mfma_t<T>(o, pf[kb], dv[kb][db]);
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb) dk[kb][db] = mfma_t<T>(q, sf[kb], dk[kb][db]);
+      if (db % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (first < tiles) {
+#pragma unroll
+    for (int kb = 0; kb < kKB; ++kb)
+#pragma unroll
+      for (int kk = 0; kk < kKK; ++kk) asm volatile("" : "+v"(kf[kb][kk]), "+v"(vf[kb][kk]));   // (waited for here, not among the tiles)
+#pragma unroll
+    for (int t = 0; t < kGradStages - 1; ++t) request_tile(first + t);
+    for (int t = first; t < tiles; ++t) {
+      barrier_keep_vmem<(kGradStages - 2) * kRequests>();   // tile t has landed, tile t-1 has been read
+      request_tile(t + kGradStages - 1);
+      if ((t + 1) * kGradTile <= first_min) continue;   // (none of the rows sees a key of this wavefront's)
+      if (t < n_masked || t >= n_full) compute(t, std::true_type{});
+      else compute(t, std::false_type{});
+    }
+    wait_vmem_all();   // the requests past the last tile must not outlive the workgroup's LDS
+  }
+
+  const int st_row = lane >> 2;
+#pragma unroll
+  for (int kb = 0; kb < kKB; ++kb) {
+    const int key = key0 + 16 * (kGradWaves * kb + wave) + st_row;
+    const bool there = key < tile.lkv;
+    const size_t at = ((size_t)(tile.k0 + (there ? key : 0)) * a.kv_heads + head) * D;
+    constexpr float kDownP = std::is_same_v<T, bf16_t> ? 1.f : 1.f / 32768.f;
+    float down = g.scale * kDownP;
+    if constexpr (!std::is_same_v<T, bf16_t>) {
+      // (in two steps: the power alone may be beyond what is left of fp32's range)
+      if (power[kb].up != 0.f) {
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) dk[kb][db] *= 1.f / power[kb].up;
+      }
+    }
+    store_transposed<T, kDB>(dk[kb], down, grad_key + at, there);
+    store_transposed<T, kDB>(dv[kb], kDownP, grad_value + at, there);
+  }
+}
+
+// ---- dQ of 128 rows --------------------------------------------------------------------------------
+template <typename T, int D, bool kCausal>
+__global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_queries_kernel(GradArgs g) {
+  using V8 = typename Vec<T>::v8;
+  constexpr int kChunks = D / 8, kRowsPerInstr = 64 / kChunks, kTileBytes = kGradTile * D * 2;
+  constexpr int kStage = 2 * kTileBytes, kPerWave = kTileBytes / 1024 / kGradWaves, kRequests = 2 * kPerWave;
+  constexpr int kKK = D / 32, kDB = D / 16, kQB = 2;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const PackedArgs& a = g.packed;
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  T* const grad_query = static_cast<T*>(g.grad_query);
+  rows_outside(a.offsets, a.sequences, a.tokens, [&](int row) { clear_row(grad_query + (size_t)row * a.heads * D, a.heads * D); });
+  const PackedTile tile = packed_tile(a, kGradOwn);
+  if (tile.sequence < 0) return;
+  const int head = (int)blockIdx.x % a.kv_heads, group = (int)a.group.d;
+  const int Lkv = tile.lkv, shift = tile.lkv - tile.lq, rows = tile.lq * group;
+  const int tile_row0 = ((rows + kGradOwn - 1) / kGradOwn - 1 - tile.from_end) * kGradOwn;
+  const T* const Q = static_cast<const T*>(g.query) + (size_t)tile.q0 * a.query_row + (size_t)head * group * a.query_head;
+  const size_t at_head = ((size_t)tile.q0 * a.heads + (size_t)head * group) * D;
+  const T* const dO = static_cast<const T*>(g.grad_out) + at_head;
+  const T* const K = static_cast<const T*>(g.key) + (size_t)tile.k0 * a.key_row + (size_t)head * a.key_head;
+  const T* const V = static_cast<const T*>(g.value) + (size_t)tile.k0 * a.value_row + (size_t)head * a.value_head;
+  const float2_t* const stats = g.stats + ((size_t)head * a.tokens + tile.q0) * group;
+  auto limit_of = [&](int row) __attribute__((always_inline)) { return kCausal ? min(Lkv - 1, divide(a.group, min(row, rows - 1)) + shift) : Lkv - 1; };
+
+  // ---- this wavefront's rows: blocks wave and wave + 4 of 16 ----------------------------------
+  V8 qf[kQB][kKK], of[kQB][kKK];
+  float base[kQB], delta[kQB];
+  int limit[kQB];
+#pragma unroll
+  for (int qb = 0; qb < kQB; ++qb) {
+    const int row = min(tile_row0 + 16 * (kGradWaves * qb + wave) + lr, rows - 1), token = divide(a.group, row), hg = row - token * group;
+    limit[qb] = limit_of(row);
+    const float2_t x = stats[row];
+    base[qb] = kUpP<T> - x[0];
+    delta[qb] = x[1];
+#pragma unroll
+    for (int kk = 0; kk < kKK; ++kk) {
+      qf[qb][kk] = *reinterpret_cast<const V8*>(Q + (size_t)token * a.query_row + (size_t)hg * a.query_head + 32 * kk + 8 * lg);
+      of[qb][kk] = *reinterpret_cast<const V8*>(dO + ((size_t)token * a.heads + hg) * D + 32 * kk + 8 * lg);
+    }
+  }
+  const int n_end = limit_of(tile_row0 + kGradOwn - 1) + 1, tiles = n_end <= 0 ? 0 : (n_end + kGradTile - 1) / kGradTile;
+  // of this wavefront: tiles that every row sees whole, and those that any row sees
+  const int n_plain = max(0, (__builtin_amdgcn_readfirstlane(limit_of(tile_row0 + 16 * wave)) + 1) / kGradTile);
+  const int last = __builtin_amdgcn_readfirstlane(limit_of(tile_row0 + 16 * (kGradWaves * (kQB - 1) + wave) + 15));
+  const int n_compute = last < 0 ? 0 : last / kGradTile + 1;
+
+  const unsigned smem_base = lds_address(smem);
+  auto request_tile = [&](int t) __attribute__((always_inline)) {
+    const unsigned stage = smem_base + t % kGradStages * kStage;
+    const int n0 = min(t, tiles - 1) * kGradTile;
+#pragma unroll
+    for (int i = 0; i < kPerWave; ++i) {
+      const int instr = wave + kGradWaves * i, row_l = instr * kRowsPerInstr + lane / kChunks;
+      const size_t key = min(n0 + row_l, Lkv - 1);
+      const int col = swz_both<kChunks>(row_l, lane % kChunks) * 8;
+      lds_dma_16B(K + key * a.key_row + col, stage + instr * 1024);
+      lds_dma_16B(V + key * a.value_row + col, stage + kTileBytes + instr * 1024);
+    }
+  };
+  const FragmentOffsets off = fragment_offsets<D>();
+  float4_t dq[kQB][kDB];
+  Power power[kQB];
+#pragma unroll
+  for (int qb = 0; qb < kQB; ++qb)
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) dq[qb][db] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+  auto compute = [&](int t, auto mask_c) __attribute__((always_inline)) {
+    constexpr bool kMask = decltype(mask_c)::value;
+    const unsigned stage = smem_base + t % kGradStages * kStage;
+    V8 sf[kQB];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      float4_t s[kQB], dp[kQB];
+#pragma unroll
+      for (int qb = 0; qb < kQB; ++qb) s[qb] = dp[qb] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < kKK; ++kk) {
+        const V8 k = row_fragment<T>(stage, off, kk, kb * 16 * D * 2), v = row_fragment<T>(stage + kTileBytes, off, kk, kb * 16 * D * 2);
+#pragma unroll
+        for (int qb = 0; qb < kQB; ++qb) s[qb] = mfma_t<T>(k, qf[qb][kk], s[qb]);
+#pragma unroll
+        for (int qb = 0; qb < kQB; ++qb) dp[qb] = mfma_t<T>(v, of[qb][kk], dp[qb]);
+      }
+#pragma unroll
+      for (int qb = 0; qb < kQB; ++qb) {
+        float4_t ds;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float d = __builtin_amdgcn_exp2f(fmaf(s[qb][r], g.scale_log2, base[qb])) * (dp[qb][r] - delta[qb]);
+          if (kMask && t * kGradTile + 16 * kb + 4 * lg + r > limit[qb]) d = 0.f;
+          ds[r] = d;
+        }
+        to_operand<T, kDB>(ds, kb, sf[qb], power[qb], dq[qb]);
+      }
+    }
+    // Infinities and NaN in keys that a part of the rows does not see are taken out of the product: the rows that see them have NaN weights.
+    bool found = false;
+    if constexpr (kMask) {
+      unsigned seen = 0;
+#pragma unroll
+      for (int i = 0; i < kTileBytes / 1024; ++i) {
+        const uint4_t x = lds_read_b128<uint4_t>(stage + lane * 16 + i * 1024);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen |= not_finite_halves<T>(x[e]);
+      }
+      found = __builtin_amdgcn_ballot_w64(seen != 0) != 0;
+    }
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) {
+      V8 k = column_fragment<T, D>(stage, off, db);
+      if (found) clean<T>(k);
+#pragma unroll
+      for (int qb = 0; qb < kQB; ++qb) dq[qb][db] = mfma_t<T>(k, sf[qb], dq[qb][db]);
+    }
+  };
+
+  if (tiles > 0) {
+#pragma unroll
+    for (int qb = 0; qb < kQB; ++qb) {
+#pragma unroll
+      for (int kk = 0; kk < kKK; ++kk) asm volatile("" : "+v"(qf[qb][kk]), "+v"(of[qb][kk]));   // (waited for here, not among the tiles)
+      asm volatile("" : "+v"(base[qb]), "+v"(delta[qb]));
+    }
+#pragma unroll
+    for (int t = 0; t < kGradStages - 1; ++t) request_tile(t);
+    for (int t = 0; t < tiles; ++t) {
+      barrier_keep_vmem<(kGradStages - 2) * kRequests>();   // tile t has landed, tile t-1 has been read
+      request_tile(t + kGradStages - 1);
+      if (t < n_plain) compute(t, std::false_type{});
+      else if (t < n_compute) compute(t, std::true_type{});
+    }
+    wait_vmem_all();
+  }
+
+  const int st_row = lane >> 2;
+#pragma unroll
+  for (int qb = 0; qb < kQB; ++qb) {
+    const int row = tile_row0 + 16 * (kGradWaves * qb + wave) + st_row;
+    const bool there = row < rows;
+    const int token = divide(a.group, there ? row : 0), hg = (there ? row : 0) - token * group;
+    float down = g.scale;
+    if constexpr (!std::is_same_v<T, bf16_t>) {
+      down *= 1.f / 32768.f;
+      if (power[qb].up != 0.f) {
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) dq[qb][db] *= 1.f / power[qb].up;
+      }
+    }
+    store_transposed<T, kDB>(dq[qb], down, grad_query + at_head + ((size_t)token * a.heads + hg) * D, there);
+  }
+}
+
+template <typename T, int D, bool kCausal>
+int launch_grad(const GradArgs& g, hipStream_t st) {
+  const PackedArgs& a = g.packed;
+  const int64_t all = (int64_t)a.tokens * a.heads;
+  constexpr int kRows = 256 / (D / 8);
+  if (all > 0)
+    if (int rc = launch_kernel(packed_stats_kernel<T, D>, dim3((unsigned)((all + kRows - 1) / kRows)), dim3(256), 0, st, g)) return rc;
+  if (g.grad_key && a.kv_tokens > 0) {
+    auto kern = packed_grad_keys_kernel<T, D, kCausal>;
+    constexpr int lds = kGradStages * grad_stage_bytes<D>();
+    TFK_LDS_OPT_IN(kern, lds);
+    const int64_t tiles = most_tiles(a.kv_tokens, a.sequences, kGradOwn) * a.kv_heads;
+    if (int rc = launch_kernel(kern, dim3((unsigned)std::max<int64_t>(tiles, 1)), dim3(kGradWaves * 64), lds, st, g)) return rc;
+  }
+  if (g.grad_query && a.tokens > 0) {
+    auto kern = packed_grad_queries_kernel<T, D, kCausal>;
+    constexpr int lds = kGradStages * 2 * kGradTile * D * 2;
+    TFK_LDS_OPT_IN(kern, lds);
+    const int64_t tiles = most_tiles((int64_t)a.tokens * a.group.d, a.sequences, kGradOwn) * a.kv_heads;
+    if (int rc = launch_kernel(kern, dim3((unsigned)std::max<int64_t>(tiles, 1)), dim3(kGradWaves * 64), lds, st, g)) return rc;
+  }
+  return TF_OK;
+}
+template <int D>
+int run_grad(const PackedGradCall& c) {
+  const GradArgs g = {c.args, c.query, c.key, c.value, c.out, c.grad_out, c.lse, static_cast<float2_t*>(c.stats), c.grad_query, c.grad_key, c.grad_value,
+                      c.scale, c.scale * kLog2E};
+  if (c.bf16) return c.causal ? launch_grad<bf16_t, D, true>(g, c.stream) : launch_grad<bf16_t, D, false>(g, c.stream);
+  return c.causal ? launch_grad<half_t, D, true>(g, c.stream) : launch_grad<half_t, D, false>(g, c.stream);
+}
+
+}  // namespace
+}  // namespace tfk

@@ -49,13 +49,15 @@ TFK_DEVICE int wave_max(int x) {
 // e * rows rows in front of it and counts as ceil(lkv * group / rows) - e (causal or not: the longest sequences first, and their last
 // tokens).  The largest number that more tiles reach than come before this one is found by halving, each step a
 // sum over the sequences, 64 at a time: with a few dozen sequences some hundred cycles a step, where a sorted list would be a launch of its own.
-TFK_DEVICE PackedTile packed_tile(const PackedArgs& a, int rows) {
+template <bool kKeys>
+TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows) {
   const int rank = (int)blockIdx.x / a.kv_heads, lane = threadIdx.x % kWaveSize;
   struct Own { int tiles, level; };   // of a lane's sequence
   auto own = [&](int b) __attribute__((always_inline)) -> Own {
     if (b >= a.sequences) return {0, 0};
-    const int lq = packed_range(a.offsets[b], a.offsets[b + 1], a.tokens).length;
     const int lkv = packed_range(a.kv_offsets[b], a.kv_offsets[b + 1], a.kv_tokens).length;
+    if constexpr (kKeys) return {(lkv + rows - 1) / rows, (lkv + rows - 1) / rows};
+    const int lq = packed_range(a.offsets[b], a.offsets[b + 1], a.tokens).length;
     return {(lq * (int)a.group.d + rows - 1) / rows, (lkv * (int)a.group.d + rows - 1) / rows};
   };
   const Own first = own(lane);   // (kept: mostly all there are)
@@ -114,6 +116,9 @@ TFK_DEVICE PackedTile packed_tile(const PackedArgs& a, int rows) {
   tile.lkv = k.length;
   return tile;
 }
+TFK_DEVICE PackedTile packed_tile(const PackedArgs& a, int rows) { return find_tile<false>(a, rows); }
+// The same of the tiles of `keys` keys, from_end counted from a sequence's first key, which the most rows see.
+TFK_DEVICE PackedTile packed_key_tile(const PackedArgs& a, int keys) { return find_tile<true>(a, keys); }
 
 // Rows in front of the first sequence and behind the last: `use` for each of them, the workgroups sharing them out.
 template <typename Use>

@@ -1,6 +1,6 @@
 // PyTorch operator bindings: registers torch.ops.tilefusion.{gemm, fused_two_gemms,
 // flash_attention, flash_attention_fwd, flash_attention_fwd_kt, flash_decode, scatter_nd, quantize_rows, gemm_int8, gated_ffn, gated_ffn_backward,
-// linear_cross_entropy, linear_cross_entropy_backward, append_paged_kv, flash_decode_paged, flash_attention_packed} for the CUDA dispatch key (HIP tensors
+// linear_cross_entropy, linear_cross_entropy_backward, append_paged_kv, flash_decode_paged, flash_attention_packed, flash_attention_packed_backward} for the CUDA dispatch key (HIP tensors
 // are "cuda" tensors on PyTorch-ROCm) and forwards to the C ABI in tilefusion_c.h on the
 // caller's current stream.
 //
@@ -756,6 +756,33 @@ void flash_attention_packed(const at::Tensor& query, const at::Tensor& key, cons
   check_status(tf_flash_attention_packed(&p, out.data_ptr(), lse.has_value() ? lse->data_ptr<float>() : nullptr, current_stream()), op);
 }
 
+// flash_attention_packed_backward(grad_out, query, key, value, out, lse, .. -> grad_query [T,H,D], grad_key and grad_value [S,Hkv,D]), the gradients that are
+// given
+void flash_attention_packed_backward(const at::Tensor& grad_out, const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const at::Tensor& out,
+                                     const at::Tensor& lse, const at::Tensor& offsets, const std::optional<at::Tensor>& kv_offsets, double softmax_scale,
+                                     bool causal, const std::optional<at::Tensor>& grad_query, const std::optional<at::Tensor>& grad_key,
+                                     const std::optional<at::Tensor>& grad_value) {
+  constexpr const char* op = "flash_attention_packed_backward";
+  const tf_packed_attention_t p = packed_attention(query, key, value, offsets, kv_offsets, softmax_scale, causal, op);
+  check_result(grad_out, "grad_out", p.tokens, p.heads, p.D, query, op);
+  check_result(out, "out", p.tokens, p.heads, p.D, query, op);
+  check_lse(lse, p, query, op);
+  TORCH_CHECK(grad_key.has_value() == grad_value.has_value(), "tilefusion::", op, ": grad_key and grad_value are asked for both or neither.");
+  if (grad_query.has_value()) check_result(*grad_query, "grad_query", p.tokens, p.heads, p.D, query, op);
+  if (grad_key.has_value()) {
+    check_result(*grad_key, "grad_key", p.kv_tokens, p.kv_heads, p.D, query, op);
+    check_result(*grad_value, "grad_value", p.kv_tokens, p.kv_heads, p.D, query, op);
+  }
+  const c10::DeviceGuard there(query.device());
+  const size_t bytes = tf_flash_attention_packed_backward_workspace_bytes(p.tokens, p.heads);
+  c10::DataPtr ws;
+  if (bytes > 0) ws = scratch(bytes, query);
+  const auto at_or_null = [](const std::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; };
+  check_status(tf_flash_attention_packed_backward(&p, grad_out.data_ptr(), out.data_ptr(), lse.data_ptr<float>(), at_or_null(grad_query), at_or_null(grad_key),
+                                                  at_or_null(grad_value), ws.get(), bytes, current_stream()),
+               op);
+}
+
 }  // namespace kernels
 
 // Self-registering op table: each REGISTER_OP adds (schema, installer) at load time, and the
@@ -848,6 +875,11 @@ REGISTER_OP(flash_attention_packed,
             "flash_attention_packed(Tensor query, Tensor key, Tensor value, Tensor offsets, Tensor? kv_offsets, "
             "float softmax_scale, bool causal, Tensor(a!) out, Tensor(b!)? lse) -> ()",
             &kernels::flash_attention_packed);
+
+REGISTER_OP(flash_attention_packed_backward,
+            "flash_attention_packed_backward(Tensor grad_out, Tensor query, Tensor key, Tensor value, Tensor out, Tensor lse, Tensor offsets, "
+            "Tensor? kv_offsets, float softmax_scale, bool causal, Tensor(a!)? grad_query, Tensor(b!)? grad_key, Tensor(c!)? grad_value) -> ()",
+            &kernels::flash_attention_packed_backward);
 
 TORCH_LIBRARY(tilefusion, m) { KernelRegistry::instance().register_with_torch(m); }
 TORCH_LIBRARY_IMPL(tilefusion, CUDA, m) { KernelRegistry::instance().register_implementations(m); }

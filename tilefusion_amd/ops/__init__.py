@@ -5,13 +5,14 @@
     gemm_int8, quantize_rows                                  products of 8-bit integers with scales
     gated_ffn, gated_ffn_backward                             the gated feed-forward block
     linear_cross_entropy, linear_cross_entropy_backward       the cross entropy of a linear head
+    flash_attention_packed, flash_attention_packed_backward   attention over packed sequences
     append_paged_kv, rotation_tables                          rotated keys, and values, into a paged cache
     flash_decode_paged                                        one new token of every sequence over that cache
 """
 
 from .append_paged_kv import append_paged_kv, rotation_tables  # noqa: F401
 from .flash_attention import FlashAttention, flash_attention
-from .flash_attention_packed import flash_attention_packed  # noqa: F401
+from .flash_attention_packed import flash_attention_packed, flash_attention_packed_backward  # noqa: F401
 from .flash_decode import flash_decode
 from .flash_decode_paged import flash_decode_paged  # noqa: F401
 from .fused_two_gemms import fused_two_gemms
