@@ -18,7 +18,7 @@
 namespace tfk {
 namespace {
 
-constexpr int kGradWaves = 4, kGradTile = 32, kGradOwn = kGradWaves * 32;   // keys (rows) of a workgroup
+constexpr int kGradWaves = 4, kGradTile = 32;
 constexpr float kLog2E = 1.4426950408889634f;
 
 // 16 rows that read one logical 16-byte chunk hit 16 different bank groups, and 8 rows that read 32 bytes transposed hit 8 different windows.
@@ -77,6 +77,11 @@ TFK_DEVICE float power_for(float largest) {   // 2^(14 - floor(log2 largest)), w
   return __builtin_bit_cast(float, (unsigned)min(max(127 + 14 + 127 - e, 27), 227) << 23);
 }
 
+// 16 bytes a lane from base + offset to LDS; base is wavefront-uniform.
+TFK_DEVICE void lds_dma_from(const void* base, unsigned offset, unsigned lds_addr) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "{m0}"(lds_addr) : "memory");
+}
+
 struct GradArgs {
   PackedArgs packed;      // of query, key and value
   const void *query, *key, *value, *out, *grad_out;   // out, grad_out [tokens][heads][D]
@@ -84,6 +89,7 @@ struct GradArgs {
   float2_t* stats;        // [kv_heads][tokens * group]: lse * log2 e, delta
   void *grad_query, *grad_key, *grad_value;            // contiguous
   float scale, scale_log2;
+  unsigned group_factor;   // ceil(2^32 / group): the high half of n * it is n / group for n < 2^22, where group is not 1
 };
 
 // Every row of a tile is 16 lanes wide at most; a thread takes 8 elements of a row of out and grad_out.
@@ -172,12 +178,12 @@ constexpr int grad_stage_bytes() { return 2 * kGradTile * D * 2 + kGradTile * 8;
 constexpr int kGradStages = 4;
 
 // ---- dK and dV of 128 keys ------------------------------------------------------------------------
-template <typename T, int D, bool kCausal>
-__global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_keys_kernel(GradArgs g) {
+template <typename T, int D, bool kCausal, int kKB>
+__global__ __launch_bounds__(kGradWaves * 64, D * kKB > 256 ? 1 : 2) void packed_grad_keys_kernel(GradArgs g) {
   using V8 = typename Vec<T>::v8;
   constexpr int kChunks = D / 8, kRowsPerInstr = 64 / kChunks, kTileBytes = kGradTile * D * 2;
   constexpr int kStage = grad_stage_bytes<D>(), kPerWave = kTileBytes / 1024 / kGradWaves, kRequests = 2 * kPerWave + 1;
-  constexpr int kKK = D / 32, kDB = D / 16, kKB = 2;
+  constexpr int kKK = D / 32, kDB = D / 16, kGradOwn = kGradWaves * 16 * kKB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const PackedArgs& a = g.packed;
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
@@ -223,19 +229,22 @@ __global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_keys_kernel(Gr
   const unsigned smem_base = lds_address(smem);
   auto request_tile = [&](int t) __attribute__((always_inline)) {
     const unsigned stage = smem_base + t % kGradStages * kStage;
-    const int r0 = min(t, tiles - 1) * kGradTile;
+    // (from the token of the tile's first row, behind which 32 bits reach any row of it)
+    const int r0 = min(t, tiles - 1) * kGradTile, token0 = divide(a.group, r0), skipped = token0 * group, last = rows - 1 - skipped;
+    const T* const q = Q + (size_t)token0 * a.query_row;
+    const T* const o = dO + (size_t)token0 * a.heads * D;
 #pragma unroll
     for (int i = 0; i < kPerWave; ++i) {
       const int instr = wave + kGradWaves * i, row_l = instr * kRowsPerInstr + lane / kChunks;
-      const int row = min(r0 + row_l, rows - 1), token = divide(a.group, row), hg = row - token * group;
+      const int row = min(r0 - skipped + row_l, last), token = group == 1 ? row : (int)__umulhi((unsigned)row, g.group_factor), hg = row - token * group;
       const int col = swz_both<kChunks>(row_l, lane % kChunks) * 8;
-      lds_dma_16B(Q + (size_t)token * a.query_row + (size_t)hg * a.query_head + col, stage + instr * 1024);
-      lds_dma_16B(dO + ((size_t)token * a.heads + hg) * D + col, stage + kTileBytes + instr * 1024);
+      lds_dma_from(q, (unsigned)(token * a.query_row + hg * a.query_head + col) * 2u, stage + instr * 1024);
+      lds_dma_from(o, (unsigned)((token * a.heads + hg) * D + col) * 2u, stage + kTileBytes + instr * 1024);
     }
     // 8 rows' statistics, a lane each number
     if (lane < 16) {
-      const float* from = reinterpret_cast<const float*>(stats + min(r0 + 8 * wave + lane / 2, rows - 1)) + lane % 2;
-      asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(from), "{m0}"(stage + 2 * kTileBytes + wave * 64) : "memory");
+      const unsigned at = (unsigned)min(8 * wave + lane / 2, rows - 1 - r0) * 8u + lane % 2 * 4u;
+      asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(at), "s"(stats + r0), "{m0}"(stage + 2 * kTileBytes + wave * 64) : "memory");
     }
   };
 
@@ -293,7 +302,7 @@ __global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_keys_kernel(Gr
     bool found = false;
     if constexpr (kMask) {
       unsigned seen = 0;
-#pragma unroll
+#pragma unroll 2
       for (int i = 0; i < 2 * kTileBytes / 1024; ++i) {
         const uint4_t x = lds_read_b128<uint4_t>(stage + lane * 16 + i * 1024);
 #pragma unroll
@@ -350,12 +359,19 @@ __global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_keys_kernel(Gr
       for (int kk = 0; kk < kKK; ++kk) asm volatile("" : "+v"(kf[kb][kk]), "+v"(vf[kb][kk]));   // (waited for here, not among the tiles)
 #pragma unroll
     for (int t = 0; t < kGradStages - 1; ++t) request_tile(first + t);
-    for (int t = first; t < tiles; ++t) {
+    auto next_tile = [&](int t) __attribute__((always_inline)) {
       barrier_keep_vmem<(kGradStages - 2) * kRequests>();   // tile t has landed, tile t-1 has been read
       request_tile(t + kGradStages - 1);
-      if ((t + 1) * kGradTile <= first_min) continue;   // (none of the rows sees a key of this wavefront's)
-      if (t < n_masked || t >= n_full) compute(t, std::true_type{});
-      else compute(t, std::false_type{});
+    };
+    for (int t = first; t < tiles; ++t) {
+      for (; t >= n_masked && t < n_full; ++t) {
+        next_tile(t);
+        compute(t, std::false_type{});
+      }
+      if (t >= tiles) break;
+      next_tile(t);
+      // (otherwise none of the rows sees a key of this wavefront's)
+      if ((t + 1) * kGradTile > first_min) compute(t, std::true_type{});
     }
     wait_vmem_all();   // the requests past the last tile must not outlive the workgroup's LDS
   }
@@ -381,12 +397,12 @@ __global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_keys_kernel(Gr
 }
 
 // ---- dQ of 128 rows --------------------------------------------------------------------------------
-template <typename T, int D, bool kCausal>
-__global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_queries_kernel(GradArgs g) {
+template <typename T, int D, bool kCausal, int kQB>
+__global__ __launch_bounds__(kGradWaves * 64, D * kQB > 256 ? 1 : 2) void packed_grad_queries_kernel(GradArgs g) {
   using V8 = typename Vec<T>::v8;
   constexpr int kChunks = D / 8, kRowsPerInstr = 64 / kChunks, kTileBytes = kGradTile * D * 2;
   constexpr int kStage = 2 * kTileBytes, kPerWave = kTileBytes / 1024 / kGradWaves, kRequests = 2 * kPerWave;
-  constexpr int kKK = D / 32, kDB = D / 16, kQB = 2;
+  constexpr int kKK = D / 32, kDB = D / 16, kGradOwn = kGradWaves * 16 * kQB;
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   const PackedArgs& a = g.packed;
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
@@ -434,13 +450,14 @@ __global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_queries_kernel
   auto request_tile = [&](int t) __attribute__((always_inline)) {
     const unsigned stage = smem_base + t % kGradStages * kStage;
     const int n0 = min(t, tiles - 1) * kGradTile;
+    const T* const k = K + (size_t)n0 * a.key_row;
+    const T* const v = V + (size_t)n0 * a.value_row;
 #pragma unroll
     for (int i = 0; i < kPerWave; ++i) {
-      const int instr = wave + kGradWaves * i, row_l = instr * kRowsPerInstr + lane / kChunks;
-      const size_t key = min(n0 + row_l, Lkv - 1);
+      const int instr = wave + kGradWaves * i, row_l = instr * kRowsPerInstr + lane / kChunks, key = min(row_l, Lkv - 1 - n0);
       const int col = swz_both<kChunks>(row_l, lane % kChunks) * 8;
-      lds_dma_16B(K + key * a.key_row + col, stage + instr * 1024);
-      lds_dma_16B(V + key * a.value_row + col, stage + kTileBytes + instr * 1024);
+      lds_dma_from(k, (unsigned)(key * a.key_row + col) * 2u, stage + instr * 1024);
+      lds_dma_from(v, (unsigned)(key * a.value_row + col) * 2u, stage + kTileBytes + instr * 1024);
     }
   };
   const FragmentOffsets off = fragment_offsets<D>();
@@ -484,7 +501,7 @@ __global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_queries_kernel
     bool found = false;
     if constexpr (kMask) {
       unsigned seen = 0;
-#pragma unroll
+#pragma unroll 2
       for (int i = 0; i < kTileBytes / 1024; ++i) {
         const uint4_t x = lds_read_b128<uint4_t>(stage + lane * 16 + i * 1024);
 #pragma unroll
@@ -537,6 +554,24 @@ __global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_queries_kernel
   }
 }
 
+template <typename T, int D, bool kCausal, int kKB>
+int launch_grad_keys(const GradArgs& g, hipStream_t st) {
+  const PackedArgs& a = g.packed;
+  auto kern = packed_grad_keys_kernel<T, D, kCausal, kKB>;
+  constexpr int lds = kGradStages * grad_stage_bytes<D>();
+  TFK_LDS_OPT_IN(kern, lds);
+  const int64_t tiles = most_tiles(a.kv_tokens, a.sequences, kGradWaves * 16 * kKB) * a.kv_heads;
+  return launch_kernel(kern, dim3((unsigned)std::max<int64_t>(tiles, 1)), dim3(kGradWaves * 64), lds, st, g);
+}
+template <typename T, int D, bool kCausal, int kQB>
+int launch_grad_queries(const GradArgs& g, hipStream_t st) {
+  const PackedArgs& a = g.packed;
+  auto kern = packed_grad_queries_kernel<T, D, kCausal, kQB>;
+  constexpr int lds = kGradStages * 2 * kGradTile * D * 2;
+  TFK_LDS_OPT_IN(kern, lds);
+  const int64_t tiles = most_tiles((int64_t)a.tokens * a.group.d, a.sequences, kGradWaves * 16 * kQB) * a.kv_heads;
+  return launch_kernel(kern, dim3((unsigned)std::max<int64_t>(tiles, 1)), dim3(kGradWaves * 64), lds, st, g);
+}
 template <typename T, int D, bool kCausal>
 int launch_grad(const GradArgs& g, hipStream_t st) {
   const PackedArgs& a = g.packed;
@@ -545,25 +580,17 @@ int launch_grad(const GradArgs& g, hipStream_t st) {
   if (all > 0)
     if (int rc = launch_kernel(packed_stats_kernel<T, D>, dim3((unsigned)((all + kRows - 1) / kRows)), dim3(256), 0, st, g)) return rc;
   if (g.grad_key && a.kv_tokens > 0) {
-    auto kern = packed_grad_keys_kernel<T, D, kCausal>;
-    constexpr int lds = kGradStages * grad_stage_bytes<D>();
-    TFK_LDS_OPT_IN(kern, lds);
-    const int64_t tiles = most_tiles(a.kv_tokens, a.sequences, kGradOwn) * a.kv_heads;
-    if (int rc = launch_kernel(kern, dim3((unsigned)std::max<int64_t>(tiles, 1)), dim3(kGradWaves * 64), lds, st, g)) return rc;
+    if (int rc = launch_grad_keys<T, D, kCausal, 2>(g, st)) return rc;
   }
   if (g.grad_query && a.tokens > 0) {
-    auto kern = packed_grad_queries_kernel<T, D, kCausal>;
-    constexpr int lds = kGradStages * 2 * kGradTile * D * 2;
-    TFK_LDS_OPT_IN(kern, lds);
-    const int64_t tiles = most_tiles((int64_t)a.tokens * a.group.d, a.sequences, kGradOwn) * a.kv_heads;
-    if (int rc = launch_kernel(kern, dim3((unsigned)std::max<int64_t>(tiles, 1)), dim3(kGradWaves * 64), lds, st, g)) return rc;
+    if (int rc = launch_grad_queries<T, D, kCausal, 2>(g, st)) return rc;
   }
   return TF_OK;
 }
 template <int D>
 int run_grad(const PackedGradCall& c) {
   const GradArgs g = {c.args, c.query, c.key, c.value, c.out, c.grad_out, c.lse, static_cast<float2_t*>(c.stats), c.grad_query, c.grad_key, c.grad_value,
-                      c.scale, c.scale * kLog2E};
+                      c.scale, c.scale * kLog2E, (unsigned)(((1ull << 32) + c.args.group.d - 1) / c.args.group.d)};
   if (c.bf16) return c.causal ? launch_grad<bf16_t, D, true>(g, c.stream) : launch_grad<bf16_t, D, false>(g, c.stream);
   return c.causal ? launch_grad<half_t, D, true>(g, c.stream) : launch_grad<half_t, D, false>(g, c.stream);
 }
