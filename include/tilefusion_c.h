@@ -343,7 +343,7 @@ TF_API int tf_flash_attention_packed(const tf_packed_attention_t* p, void* out, 
  * group's heads are summed in fp32.  A null grad_query, or null grad_key and grad_value, are not computed.  Rows of no sequence, rows that see no key and keys that
  * no row sees have zeros.  P = exp(S - lse) and dS are rounded to dtype as operands of the products that follow (in fp16 times powers of two, so that
  * the type's range is not theirs).  No atomics: the same bits every time.  The workspace begins at a 16-byte boundary and may hold anything. */
-TF_API size_t tf_flash_attention_packed_backward_workspace_bytes(int64_t tokens, int64_t heads);
+TF_API size_t tf_flash_attention_packed_backward_workspace_bytes(const tf_packed_attention_t* p);
 TF_API int tf_flash_attention_packed_backward(const tf_packed_attention_t* p, const void* grad_out, const void* out, const float* lse,
                                               void* grad_query, void* grad_key, void* grad_value, void* workspace, size_t workspace_bytes,
                                               void* stream);

@@ -73,7 +73,7 @@ SIGNATURES = {
     "tf_flash_decode_paged_workspace_bytes": (_sz, [_i64] * 4),
     "tf_flash_decode_paged": (_i, [ctypes.POINTER(PagedCache), _vp, ctypes.POINTER(_i64), _vp, _i64, _d, _vp, _sz, _vp]),
     "tf_flash_attention_packed": (_i, [ctypes.POINTER(PackedAttention), _vp, _vp, _vp]),
-    "tf_flash_attention_packed_backward_workspace_bytes": (_sz, [_i64] * 2),
+    "tf_flash_attention_packed_backward_workspace_bytes": (_sz, [ctypes.POINTER(PackedAttention)]),
     "tf_flash_attention_packed_backward": (_i, [ctypes.POINTER(PackedAttention)] + [_vp] * 7 + [_sz, _vp]),
     "tf_product_kernel_index": (_i, [_i64, _i64, _i64, _i]),
     "tf_product_cols_plan": (_i, [_i64, _i64, _i64, ctypes.POINTER(_i)]),

@@ -43,6 +43,14 @@ int packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_hea
   return 64;
 }
 
+// Parts that the rows behind a tile of keys are cut into: where there are fewer tiles than the chip runs workgroups at a time, and rows enough.
+int grad_parts(const tf_packed_attention_t& p) {
+  const int64_t tiles = std::max<int64_t>(1, (p.kv_tokens / kGradKeys + p.sequences / 2) * p.kv_heads);
+  const int64_t rows = p.sequences > 0 ? p.tokens / p.sequences * (p.heads / p.kv_heads) : 0;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, rows / 512, 8}));
+}
+size_t stats_bytes(const tf_packed_attention_t& p) { return ((size_t)p.tokens * (size_t)p.heads * 8 + 255) / 256 * 256; }
+
 }  // namespace
 }  // namespace tfk
 
@@ -58,9 +66,11 @@ extern "C" int tf_flash_attention_packed(const tf_packed_attention_t* p, void* o
   return p->D == 128 ? run_attention_packed_d128(c) : run_attention_packed_d64(c);
 }
 
-extern "C" size_t tf_flash_attention_packed_backward_workspace_bytes(int64_t tokens, int64_t heads) {
-  if (tokens < 0 || heads <= 0) return 0;
-  return (size_t)tokens * (size_t)heads * 8;
+extern "C" size_t tf_flash_attention_packed_backward_workspace_bytes(const tf_packed_attention_t* p) {
+  using namespace tfk;
+  if (!p || p->tokens < 0 || p->kv_tokens < 0 || p->sequences < 0 || p->kv_heads <= 0 || p->heads < p->kv_heads || p->D <= 0) return 0;
+  const int parts = grad_parts(*p);
+  return stats_bytes(*p) + (parts > 1 ? (size_t)parts * 2 * (size_t)p->kv_tokens * (size_t)p->kv_heads * (size_t)p->D * sizeof(float) : 0);
 }
 
 extern "C" int tf_flash_attention_packed_backward(const tf_packed_attention_t* p, const void* grad_out, const void* out, const float* lse,
@@ -71,13 +81,14 @@ extern "C" int tf_flash_attention_packed_backward(const tf_packed_attention_t* p
   if (int rc = check_packed(who, p)) return rc;
   TFK_REQUIRE((grad_key == nullptr) == (grad_value == nullptr) || p->kv_tokens == 0, TF_ERR_INVALID_ARG, "%s: grad_key and grad_value are both asked for or neither", who);
   if (p->tokens == 0 && p->kv_tokens == 0) return TF_OK;
-  TFK_REQUIRE((grad_out && out && lse && workspace) || p->tokens == 0, TF_ERR_INVALID_ARG, "%s: null pointer", who);
+  TFK_REQUIRE((grad_out && out && lse) || p->tokens == 0, TF_ERR_INVALID_ARG, "%s: null pointer", who);
   TFK_REQUIRE(((reinterpret_cast<uintptr_t>(grad_out) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(grad_query) |
                 reinterpret_cast<uintptr_t>(grad_key) | reinterpret_cast<uintptr_t>(grad_value) | reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
               TF_ERR_INVALID_ARG, "%s: operands must begin at 16-byte boundaries", who);
-  const size_t need = tf_flash_attention_packed_backward_workspace_bytes(p->tokens, p->heads);
-  TFK_REQUIRE(workspace_bytes >= need || p->tokens == 0, TF_ERR_INVALID_ARG, "%s: workspace holds %zu bytes, %zu needed", who, workspace_bytes, need);
-  const PackedGradCall c = {p->query, p->key, p->value, out, grad_out, lse, grad_query, grad_key, grad_value, workspace, packed_args(*p),
+  const size_t need = tf_flash_attention_packed_backward_workspace_bytes(p);
+  TFK_REQUIRE((workspace && workspace_bytes >= need) || need == 0, TF_ERR_INVALID_ARG, "%s: workspace holds %zu bytes, %zu needed", who, workspace_bytes, need);
+  const PackedGradCall c = {p->query, p->key, p->value, out, grad_out, lse, grad_query, grad_key, grad_value, workspace,
+                            static_cast<char*>(workspace) + stats_bytes(*p), grad_parts(*p), packed_args(*p),
                             (float)p->softmax_scale, p->dtype == TF_DTYPE_BF16, p->causal != 0, static_cast<hipStream_t>(stream)};
   return p->D == 128 ? run_attention_packed_backward_d128(c) : run_attention_packed_backward_d64(c);
 }

@@ -1,10 +1,11 @@
 // Gradients of attention over packed sequences (the forward pass: flash_attention_packed_kernel.hpp), in a source file per head dimension.
 //
 // With P = exp(scale Q K^T - lse) and delta = rowsum(dO o O):   dV = P^T dO,   dS = P o (dO V^T - delta),   dQ = scale dS K,   dK = scale dS^T Q.
-// P is made again from the forward pass's log-sum-exp.  Three kernels, no atomics, so that the same bits come out every time:
-//   * stats: delta, and lse in units of log2, beside each other in the order of rows that the others read them in;
-//   * keys: a workgroup takes 128 keys and walks the rows that see them (all heads of a group are rows, so a group's sum is the same sum);
-//   * queries: a workgroup takes 128 rows and walks their keys.  That makes P and dO V^T twice, 7 products instead of 5; sums of dQ from the
+// P is made again from the forward pass's log-sum-exp.  No atomics, so that the same bits come out every time:
+//   * a first kernel leaves delta, and lse in units of log2, beside each other in the order of rows that the second reads them in;
+//   * of the second's workgroups some take 128 keys and walk the rows that see them (all heads of a group are rows, so a group's sum is the same sum), or,
+//     where there would be few of those, a part of the rows, and a third kernel adds the parts up;
+//   * the others take 128 rows and walk their keys.  That makes P and dO V^T twice, 7 products instead of 5; sums of dQ from the
 //     key side would need atomics in fp32, whose order changes results, and a pass of their own over 4 bytes an element.
 // Both walk tiles of 32 in a ring in LDS (global_load_lds), their own 32 keys or rows of a wavefront in registers as the second operand of the
 // first two products, whose accumulators are the second operand of the last ones as they are: a lane holds one key (row), its registers
@@ -19,6 +20,7 @@ namespace tfk {
 namespace {
 
 constexpr int kGradWaves = 4, kGradTile = 32;
+static_assert(kGradKeys == kGradWaves * 16 * 2, "");
 constexpr float kLog2E = 1.4426950408889634f;
 
 // 16 rows that read one logical 16-byte chunk hit 16 different bank groups, and 8 rows that read 32 bytes transposed hit 8 different windows.
@@ -89,6 +91,8 @@ struct GradArgs {
   float2_t* stats;        // [kv_heads][tokens * group]: lse * log2 e, delta
   void *grad_query, *grad_key, *grad_value;            // contiguous
   float scale, scale_log2;
+  int key_groups, parts;   // workgroups for dK and dV; parts that the rows of each of their tiles are cut into
+  float* partial;          // parts > 1: [parts][dK, dV][kv_tokens][kv_heads][D] in fp32
   unsigned group_factor;   // ceil(2^32 / group): the high half of n * it is n / group for n < 2^22, where group is not 1
 };
 
@@ -178,26 +182,28 @@ constexpr int grad_stage_bytes() { return 2 * kGradTile * D * 2 + kGradTile * 8;
 constexpr int kGradStages = 4;
 
 // ---- dK and dV of 128 keys ------------------------------------------------------------------------
+// `group_no` of `groups` workgroups.
 template <typename T, int D, bool kCausal, int kKB>
-__global__ __launch_bounds__(kGradWaves * 64, D * kKB > 256 ? 1 : 2) void packed_grad_keys_kernel(GradArgs g) {
+TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int groups) {
   using V8 = typename Vec<T>::v8;
   constexpr int kChunks = D / 8, kRowsPerInstr = 64 / kChunks, kTileBytes = kGradTile * D * 2;
   constexpr int kStage = grad_stage_bytes<D>(), kPerWave = kTileBytes / 1024 / kGradWaves, kRequests = 2 * kPerWave + 1;
   constexpr int kKK = D / 32, kDB = D / 16, kGradOwn = kGradWaves * 16 * kKB;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
   const PackedArgs& a = g.packed;
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   T* const grad_key = static_cast<T*>(g.grad_key);
   T* const grad_value = static_cast<T*>(g.grad_value);
-  rows_outside(a.kv_offsets, a.sequences, a.kv_tokens, [&](int row) {
-    clear_row(grad_key + (size_t)row * a.kv_heads * D, a.kv_heads * D);
-    clear_row(grad_value + (size_t)row * a.kv_heads * D, a.kv_heads * D);
-  });
-  const PackedTile tile = packed_key_tile(a, kGradOwn);
+  if (g.parts == 1) {
+    rows_outside(a.kv_offsets, a.sequences, a.kv_tokens, group_no, groups, [&](int row) {
+      clear_row(grad_key + (size_t)row * a.kv_heads * D, a.kv_heads * D);
+      clear_row(grad_value + (size_t)row * a.kv_heads * D, a.kv_heads * D);
+    });
+  }
+  const int part = group_no / a.kv_heads % g.parts, head = group_no % a.kv_heads, group = (int)a.group.d;
+  const PackedTile tile = packed_key_tile(a, kGradOwn, group_no / a.kv_heads / g.parts);
   if (tile.sequence < 0) return;
-  const int head = (int)blockIdx.x % a.kv_heads, group = (int)a.group.d;
   const int shift = tile.lkv - tile.lq, rows = tile.lq * group, key0 = tile.from_end * kGradOwn;   // (counted from the front)
   const T* const Q = static_cast<const T*>(g.query) + (size_t)tile.q0 * a.query_row + (size_t)head * group * a.query_head;
   const T* const dO = static_cast<const T*>(g.grad_out) + ((size_t)tile.q0 * a.heads + (size_t)head * group) * D;
@@ -220,7 +226,9 @@ __global__ __launch_bounds__(kGradWaves * 64, D * kKB > 256 ? 1 : 2) void packed
     }
   }
   const int tiles = (rows + kGradTile - 1) / kGradTile;
-  const int first = kCausal ? min(tiles, max(key0 - shift, 0) * group / kGradTile) : 0;
+  const int all_first = kCausal ? min(tiles, max(key0 - shift, 0) * group / kGradTile) : 0;
+  // of the tiles that see these keys, this part's
+  const int first = all_first + (int)((int64_t)(tiles - all_first) * part / g.parts), end = all_first + (int)((int64_t)(tiles - all_first) * (part + 1) / g.parts);
   // tiles from here on are masked for none of this wavefront's keys, but for the last one's rows behind the last
   const int last_min = __builtin_amdgcn_readfirstlane(kCausal ? max(key0 + 16 * (kGradWaves * (kKB - 1) + wave) + 15 - shift, 0) * group : 0);
   const int n_masked = min(tiles, (last_min + kGradTile - 1) / kGradTile), n_full = rows / kGradTile;
@@ -352,7 +360,7 @@ __global__ __launch_bounds__(kGradWaves * 64, D * kKB > 256 ? 1 : 2) void packed
     }
   };
 
-  if (first < tiles) {
+  if (first < end) {
 #pragma unroll
     for (int kb = 0; kb < kKB; ++kb)
 #pragma unroll
@@ -363,12 +371,12 @@ __global__ __launch_bounds__(kGradWaves * 64, D * kKB > 256 ? 1 : 2) void packed
       barrier_keep_vmem<(kGradStages - 2) * kRequests>();   // tile t has landed, tile t-1 has been read
       request_tile(t + kGradStages - 1);
     };
-    for (int t = first; t < tiles; ++t) {
-      for (; t >= n_masked && t < n_full; ++t) {
+    for (int t = first; t < end; ++t) {
+      for (; t >= n_masked && t < min(n_full, end); ++t) {
         next_tile(t);
         compute(t, std::false_type{});
       }
-      if (t >= tiles) break;
+      if (t >= end) break;
       next_tile(t);
       // (otherwise none of the rows sees a key of this wavefront's)
       if ((t + 1) * kGradTile > first_min) compute(t, std::true_type{});
@@ -379,6 +387,19 @@ __global__ __launch_bounds__(kGradWaves * 64, D * kKB > 256 ? 1 : 2) void packed
   const int st_row = lane >> 2;
 #pragma unroll
   for (int kb = 0; kb < kKB; ++kb) {
+    if (g.parts > 1) {
+      const int key = key0 + 16 * (kGradWaves * kb + wave) + lr;
+      if (key >= tile.lkv) continue;
+      const float down_k = std::is_same_v<T, bf16_t> || power[kb].up == 0.f ? 1.f : 1.f / power[kb].up;
+      const size_t all = (size_t)a.kv_tokens * a.kv_heads * D, at = ((size_t)(tile.k0 + key) * a.kv_heads + head) * D + 4 * lg;
+      float* to = g.partial + 2 * part * all + at;
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        *reinterpret_cast<float4_t*>(to + 16 * db) = dk[kb][db] * down_k;
+        *reinterpret_cast<float4_t*>(to + all + 16 * db) = dv[kb][db];
+      }
+      continue;
+    }
     const int key = key0 + 16 * (kGradWaves * kb + wave) + st_row;
     const bool there = key < tile.lkv;
     const size_t at = ((size_t)(tile.k0 + (there ? key : 0)) * a.kv_heads + head) * D;
@@ -398,21 +419,20 @@ __global__ __launch_bounds__(kGradWaves * 64, D * kKB > 256 ? 1 : 2) void packed
 
 // ---- dQ of 128 rows --------------------------------------------------------------------------------
 template <typename T, int D, bool kCausal, int kQB>
-__global__ __launch_bounds__(kGradWaves * 64, D * kQB > 256 ? 1 : 2) void packed_grad_queries_kernel(GradArgs g) {
+TFK_DEVICE void grad_queries(const GradArgs& g, char* smem, int group_no, int groups) {
   using V8 = typename Vec<T>::v8;
   constexpr int kChunks = D / 8, kRowsPerInstr = 64 / kChunks, kTileBytes = kGradTile * D * 2;
   constexpr int kStage = 2 * kTileBytes, kPerWave = kTileBytes / 1024 / kGradWaves, kRequests = 2 * kPerWave;
   constexpr int kKK = D / 32, kDB = D / 16, kGradOwn = kGradWaves * 16 * kQB;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
   const PackedArgs& a = g.packed;
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   T* const grad_query = static_cast<T*>(g.grad_query);
-  rows_outside(a.offsets, a.sequences, a.tokens, [&](int row) { clear_row(grad_query + (size_t)row * a.heads * D, a.heads * D); });
-  const PackedTile tile = packed_tile(a, kGradOwn);
+  rows_outside(a.offsets, a.sequences, a.tokens, group_no, groups, [&](int row) { clear_row(grad_query + (size_t)row * a.heads * D, a.heads * D); });
+  const PackedTile tile = packed_tile(a, kGradOwn, group_no / a.kv_heads);
   if (tile.sequence < 0) return;
-  const int head = (int)blockIdx.x % a.kv_heads, group = (int)a.group.d;
+  const int head = group_no % a.kv_heads, group = (int)a.group.d;
   const int Lkv = tile.lkv, shift = tile.lkv - tile.lq, rows = tile.lq * group;
   const int tile_row0 = ((rows + kGradOwn - 1) / kGradOwn - 1 - tile.from_end) * kGradOwn;
   const T* const Q = static_cast<const T*>(g.query) + (size_t)tile.q0 * a.query_row + (size_t)head * group * a.query_head;
@@ -554,43 +574,67 @@ __global__ __launch_bounds__(kGradWaves * 64, D * kQB > 256 ? 1 : 2) void packed
   }
 }
 
-template <typename T, int D, bool kCausal, int kKB>
-int launch_grad_keys(const GradArgs& g, hipStream_t st) {
-  const PackedArgs& a = g.packed;
-  auto kern = packed_grad_keys_kernel<T, D, kCausal, kKB>;
-  constexpr int lds = kGradStages * grad_stage_bytes<D>();
-  TFK_LDS_OPT_IN(kern, lds);
-  const int64_t tiles = most_tiles(a.kv_tokens, a.sequences, kGradWaves * 16 * kKB) * a.kv_heads;
-  return launch_kernel(kern, dim3((unsigned)std::max<int64_t>(tiles, 1)), dim3(kGradWaves * 64), lds, st, g);
+// Both in one launch: the keys' workgroups first, which take longer, and the queries' where CUs have room.
+template <typename T, int D, bool kCausal, int kKB, int kQB>
+__global__ __launch_bounds__(kGradWaves * 64, 2) void packed_grad_kernel(GradArgs g) {
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  const int no = (int)blockIdx.x;
+  if (no < g.key_groups) grad_keys<T, D, kCausal, kKB>(g, smem, no, g.key_groups);
+  else grad_queries<T, D, kCausal, kQB>(g, smem, no - g.key_groups, (int)gridDim.x - g.key_groups);
 }
-template <typename T, int D, bool kCausal, int kQB>
-int launch_grad_queries(const GradArgs& g, hipStream_t st) {
+
+// dK and dV: the sums of the parts' sums.  A thread takes 4 elements.
+template <typename T>
+__global__ __launch_bounds__(256) void packed_grad_parts_kernel(GradArgs g, int d) {
+  using V4 = typename Vec<T>::v4;
   const PackedArgs& a = g.packed;
-  auto kern = packed_grad_queries_kernel<T, D, kCausal, kQB>;
-  constexpr int lds = kGradStages * 2 * kGradTile * D * 2;
-  TFK_LDS_OPT_IN(kern, lds);
-  const int64_t tiles = most_tiles((int64_t)a.tokens * a.group.d, a.sequences, kGradWaves * 16 * kQB) * a.kv_heads;
-  return launch_kernel(kern, dim3((unsigned)std::max<int64_t>(tiles, 1)), dim3(kGradWaves * 64), lds, st, g);
+  const size_t all = (size_t)a.kv_tokens * a.kv_heads * d, at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= all) return;
+  const int row = (int)(at / ((size_t)a.kv_heads * d)), from = read_uniform(a.kv_offsets), to = read_uniform(a.kv_offsets + a.sequences);
+  const bool there = row >= from && row < to;   // (rows of no sequence have no parts)
+  float4_t dk = {0.f, 0.f, 0.f, 0.f}, dv = dk;
+  for (int p = 0; p < (there ? g.parts : 0); ++p) {
+    dk += *reinterpret_cast<const float4_t*>(g.partial + 2 * p * all + at);
+    dv += *reinterpret_cast<const float4_t*>(g.partial + (2 * p + 1) * all + at);
+  }
+  constexpr float kDownP = std::is_same_v<T, bf16_t> ? 1.f : 1.f / 32768.f;
+  V4 k, v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    k[e] = (T)(dk[e] * (g.scale * kDownP));
+    v[e] = (T)(dv[e] * kDownP);
+  }
+  *reinterpret_cast<V4*>(static_cast<T*>(g.grad_key) + at) = k;
+  *reinterpret_cast<V4*>(static_cast<T*>(g.grad_value) + at) = v;
 }
+
 template <typename T, int D, bool kCausal>
-int launch_grad(const GradArgs& g, hipStream_t st) {
+int launch_grad(GradArgs g, hipStream_t st) {
   const PackedArgs& a = g.packed;
   const int64_t all = (int64_t)a.tokens * a.heads;
   constexpr int kRows = 256 / (D / 8);
   if (all > 0)
     if (int rc = launch_kernel(packed_stats_kernel<T, D>, dim3((unsigned)((all + kRows - 1) / kRows)), dim3(256), 0, st, g)) return rc;
-  if (g.grad_key && a.kv_tokens > 0) {
-    if (int rc = launch_grad_keys<T, D, kCausal, 2>(g, st)) return rc;
-  }
-  if (g.grad_query && a.tokens > 0) {
-    if (int rc = launch_grad_queries<T, D, kCausal, 2>(g, st)) return rc;
+  const bool of_keys = g.grad_key && a.kv_tokens > 0, of_queries = g.grad_query && a.tokens > 0;
+  constexpr int kKB = 2, kQB = 2;
+  auto kern = packed_grad_kernel<T, D, kCausal, kKB, kQB>;
+  constexpr int lds = kGradStages * grad_stage_bytes<D>();
+  TFK_LDS_OPT_IN(kern, lds);
+  // (rows of no sequence are cleared by whatever workgroups there are)
+  g.key_groups = of_keys ? (int)std::max<int64_t>(most_tiles(a.kv_tokens, a.sequences, kGradKeys) * a.kv_heads * g.parts, 1) : 0;
+  const int64_t query_groups = of_queries ? std::max<int64_t>(most_tiles((int64_t)a.tokens * a.group.d, a.sequences, kGradWaves * 16 * kQB) * a.kv_heads, 1) : 0;
+  if (g.key_groups + query_groups > 0)
+    if (int rc = launch_kernel(kern, dim3((unsigned)(g.key_groups + query_groups)), dim3(kGradWaves * 64), lds, st, g)) return rc;
+  if (of_keys && g.parts > 1) {
+    const int64_t threads = (int64_t)a.kv_tokens * a.kv_heads * D / 4;
+    return launch_kernel(packed_grad_parts_kernel<T>, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, g, D);
   }
   return TF_OK;
 }
 template <int D>
 int run_grad(const PackedGradCall& c) {
   const GradArgs g = {c.args, c.query, c.key, c.value, c.out, c.grad_out, c.lse, static_cast<float2_t*>(c.stats), c.grad_query, c.grad_key, c.grad_value,
-                      c.scale, c.scale * kLog2E, (unsigned)(((1ull << 32) + c.args.group.d - 1) / c.args.group.d)};
+                      c.scale, c.scale * kLog2E, 0, c.parts, static_cast<float*>(c.partial), (unsigned)(((1ull << 32) + c.args.group.d - 1) / c.args.group.d)};
   if (c.bf16) return c.causal ? launch_grad<bf16_t, D, true>(g, c.stream) : launch_grad<bf16_t, D, false>(g, c.stream);
   return c.causal ? launch_grad<half_t, D, true>(g, c.stream) : launch_grad<half_t, D, false>(g, c.stream);
 }

@@ -42,12 +42,12 @@ __global__ __launch_bounds__(kWavesT * 64, 1) void flash_attention_packed_kernel
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  rows_outside(a.offsets, a.sequences, a.tokens, [&](int row) {
+  rows_outside(a.offsets, a.sequences, a.tokens, (int)blockIdx.x, (int)gridDim.x, [&](int row) {
     clear_row(O + (size_t)row * a.heads * D, a.heads * D);
     if (!a.lse) return;
     for (int h = tid; h < a.heads; h += kWavesT * 64) a.lse[(size_t)h * a.tokens + row] = -INFINITY;
   });
-  const PackedTile tile = packed_tile(a, kBM);
+  const PackedTile tile = packed_tile(a, kBM, (int)blockIdx.x / a.kv_heads);
   if (tile.sequence < 0) return;
   // Neighbours in the grid, which run on different XCDs, are of different heads of keys: with 8 of them the tiles of a
   // sequence that read the same keys read them from one L2.

@@ -45,13 +45,13 @@ TFK_DEVICE int wave_max(int x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 
-// The (blockIdx.x / kv_heads)-th of the tiles of `rows` rows that the sequences make, most keys first.  Tile e from a sequence's end ends
+// The `rank`-th of the tiles of `rows` rows that the sequences make, most keys first.  Tile e from a sequence's end ends
 // e * rows rows in front of it and counts as ceil(lkv * group / rows) - e (causal or not: the longest sequences first, and their last
 // tokens).  The largest number that more tiles reach than come before this one is found by halving, each step a
 // sum over the sequences, 64 at a time: with a few dozen sequences some hundred cycles a step, where a sorted list would be a launch of its own.
 template <bool kKeys>
-TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows) {
-  const int rank = (int)blockIdx.x / a.kv_heads, lane = threadIdx.x % kWaveSize;
+TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows, int rank) {
+  const int lane = threadIdx.x % kWaveSize;
   struct Own { int tiles, level; };   // of a lane's sequence
   auto own = [&](int b) __attribute__((always_inline)) -> Own {
     if (b >= a.sequences) return {0, 0};
@@ -116,16 +116,16 @@ TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows) {
   tile.lkv = k.length;
   return tile;
 }
-TFK_DEVICE PackedTile packed_tile(const PackedArgs& a, int rows) { return find_tile<false>(a, rows); }
+TFK_DEVICE PackedTile packed_tile(const PackedArgs& a, int rows, int rank) { return find_tile<false>(a, rows, rank); }
 // The same of the tiles of `keys` keys, from_end counted from a sequence's first key, which the most rows see.
-TFK_DEVICE PackedTile packed_key_tile(const PackedArgs& a, int keys) { return find_tile<true>(a, keys); }
+TFK_DEVICE PackedTile packed_key_tile(const PackedArgs& a, int keys, int rank) { return find_tile<true>(a, keys, rank); }
 
-// Rows in front of the first sequence and behind the last: `use` for each of them, the workgroups sharing them out.
+// Rows in front of the first sequence and behind the last: `use` for each of them, `groups` workgroups sharing them out.
 template <typename Use>
-TFK_DEVICE void rows_outside(const int* offsets, int sequences, int rows, Use use) {
+TFK_DEVICE void rows_outside(const int* offsets, int sequences, int rows, int group_no, int groups, Use use) {
   const int from = min(max(read_uniform(offsets), 0), rows), to = min(max(read_uniform(offsets + sequences), from), rows);
   const int outside = from + rows - to;
-  for (int i = blockIdx.x; i < outside; i += gridDim.x) use(i < from ? i : to + i - from);
+  for (int i = group_no; i < outside; i += groups) use(i < from ? i : to + i - from);
 }
 template <typename T>
 TFK_DEVICE void clear_row(T* row, int elements) {

@@ -774,7 +774,7 @@ void flash_attention_packed_backward(const at::Tensor& grad_out, const at::Tenso
     check_result(*grad_value, "grad_value", p.kv_tokens, p.kv_heads, p.D, query, op);
   }
   const c10::DeviceGuard there(query.device());
-  const size_t bytes = tf_flash_attention_packed_backward_workspace_bytes(p.tokens, p.heads);
+  const size_t bytes = tf_flash_attention_packed_backward_workspace_bytes(&p);
   c10::DataPtr ws;
   if (bytes > 0) ws = scratch(bytes, query);
   const auto at_or_null = [](const std::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; };
