@@ -49,7 +49,7 @@ int grad_parts(const tf_packed_attention_t& p) {
   const int64_t rows = p.sequences > 0 ? p.tokens / p.sequences * (p.heads / p.kv_heads) : 0;
   return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, rows / 512, 8}));
 }
-size_t stats_bytes(const tf_packed_attention_t& p) { return ((size_t)p.tokens * (size_t)p.heads * 8 + 255) / 256 * 256; }
+size_t stats_bytes(const tf_packed_attention_t& p) { return ((size_t)p.tokens * (size_t)p.heads * 16 + 255) / 256 * 256; }
 
 }  // namespace
 }  // namespace tfk

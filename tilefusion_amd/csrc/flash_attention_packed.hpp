@@ -21,7 +21,7 @@ struct PackedGradCall {
   const void *query, *key, *value, *out, *grad_out;
   const float* lse;
   void *grad_query, *grad_key, *grad_value;   // grad_query, or grad_key and grad_value, may be null
-  void* stats;     // room for 8 bytes a row
+  void* stats;     // room for 16 bytes a row
   void* partial;   // parts > 1: room for parts times dK and dV in fp32
   int parts;       // that the rows behind a tile of keys are cut into
   PackedArgs args;
