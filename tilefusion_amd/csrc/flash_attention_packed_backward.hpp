@@ -209,11 +209,9 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
 
   // ---- this wavefront's keys: blocks wave and wave + 4 of 16 (so that all have as much behind the diagonal) ----
   V8 kf[kKB][kKK], vf[kKB][kKK];
-  int row_min[kKB];   // the first row that sees key lr of a block
 #pragma unroll
   for (int kb = 0; kb < kKB; ++kb) {
     const int key = key0 + 16 * (kGradWaves * kb + wave) + lr;
-    row_min[kb] = kCausal ? max(key - shift, 0) * group : 0;
     const size_t at = tile.k0 + min(key, tile.lkv - 1);
     const T* k = static_cast<const T*>(g.key) + at * a.key_row + (size_t)head * a.key_head;
     const T* v = static_cast<const T*>(g.value) + at * a.value_row + (size_t)head * a.value_head;
@@ -235,6 +233,7 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
   const unsigned smem_base = lds_address(smem);
   auto request_tile = [&](int t) __attribute__((always_inline)) {
     const unsigned stage = smem_base + t % kGradStages * kStage;
+    const int lane = (int)opaque((unsigned)tid & 63u);   // (what follows from it is made again for each tile: registers are short)
     // (from the token of the tile's first row, behind which 32 bits reach any row of it)
     const int r0 = min(t, tiles - 1) * kGradTile, token0 = divide(a.group, r0), skipped = token0 * group, last = rows - 1 - skipped;
     const T* const q = Q + (size_t)token0 * a.query_row;
@@ -263,6 +262,13 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
     constexpr bool kMask = decltype(mask_c)::value;
     const unsigned stage = smem_base + t % kGradStages * kStage;
     V8 pf[kKB], sf[kKB];
+    [[maybe_unused]] int row_min[kKB];   // the first row of the tile that sees key lr of a block
+    if constexpr (kMask) {
+      const int own = (int)opaque((unsigned)lr);
+#pragma unroll
+      for (int kb = 0; kb < kKB; ++kb)
+        row_min[kb] = (kCausal ? max(key0 + 16 * (kGradWaves * kb + wave) + own - shift, 0) * group : 0) - t * kGradTile;
+    }
     [[maybe_unused]] float odd = 0.f;   // NaN where a score or dP is not finite, as all are of a row of Q or dO with an infinity or a NaN
     const unsigned row_at = opaque(stage + off.row), column_at = opaque(stage + off.column);
 #pragma unroll
@@ -296,8 +302,8 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
           float p = __builtin_amdgcn_exp2f(fmaf(s[kb][r], g.scale_log2, base[r])), d = p * (dp[kb][r] - delta[r]);
           if constexpr (kMask) {
             odd = fmaf(s[kb][r], 0.f, fmaf(dp[kb][r], 0.f, odd));
-            const int row = t * kGradTile + 16 * rb + 4 * lg + r;
-            const bool sees = row >= row_min[kb] && row < rows;
+            const int row = 16 * rb + 4 * lg + r;
+            const bool sees = row >= row_min[kb] && row < rows - t * kGradTile;
             p = sees ? p : 0.f;
             d = sees ? d : 0.f;
           }
@@ -328,10 +334,10 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
           const unsigned pair = e < 4 ? (e < 2 ? x[0] : x[1]) : (e < 6 ? x[2] : x[3]);
           const unsigned short bits = (unsigned short)(__builtin_amdgcn_readlane(pair, from) >> (e % 2 * 16));
           const float value = (float)__builtin_bit_cast(T, bits);
-          const int row_l = i * kRowsPerInstr + from / kChunks, col = swz_both<kChunks>(row_l, from % kChunks) * 8 + e, row = t * kGradTile + row_l;
+          const int row_l = i * kRowsPerInstr + from / kChunks, col = swz_both<kChunks>(row_l, from % kChunks) * 8 + e;
 #pragma unroll
           for (int kb = 0; kb < kKB; ++kb) {
-            const float to_key = row >= row_min[kb] && row < rows ? value : 0.f;
+            const float to_key = row_l >= row_min[kb] && row_l < rows - t * kGradTile ? value : 0.f;
 #pragma unroll
             for (int db = 0; db < kDB; ++db)
 #pragma unroll
