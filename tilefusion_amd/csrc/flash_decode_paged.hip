@@ -4,14 +4,17 @@
 // No counterpart in the reference.  HBM-bound: every key and value is read once, for all query heads of its group together (4 G flops a
 // byte for a group of G), so the products run on the matrix pipe whatever G is: S^T = K Q^T and O^T = V^T P^T with a block of 16 queries, of
 // which a group fills G columns (a larger group is several blocks, which read the keys again).
-//   * Work is cut without the host knowing the lengths: all (sequence, key head) items are laid end to end in blocks of kBlockKeys keys and
-//     every workgroup takes an equal range of them, whatever items that range cuts through.  An item in one workgroup's range is
+//   * Work is cut without the host knowing the lengths: all (sequence, key head) items are laid end to end, in blocks of kBlockKeys keys and what
+//     an item costs besides, and every workgroup takes an equal range of that, whatever items that range cuts through.  An item in one workgroup's range is
 //     written by it, of any other every workgroup leaves its part (fp32 rows, maximum, sum) and the last to arrive puts the
 //     parts together.  A workgroup has at most two parts, so the workspace depends on the sequences' number alone.
 //   * A wavefront takes every kWaves-th tile of 16 keys of the range and shares nothing with the others up to the end of an item: tiles of K and V
-//     go from their pages to LDS directly, three tiles ahead, and are waited for by count, with no barrier.
+//     go from their pages to registers, 24 KiB ahead, which with 8 wavefronts on a CU is what its share of HBM needs on the way; keys are fragments
+//     as they are loaded, values pass through 4 KiB of LDS for their transposition, with no barrier.
 //   * Pages are whole tiles: a tile's page is looked up with a scalar load, one tile before it is needed, and the lanes' offsets
 //     within a tile are constants of the launch.
+// 16 texts of 32768 keys, 8 heads x 128: 346 us, 6.2 TB/s; 60 texts of 17 to 8001 keys, 8 x 64: 43 us, 3.7 TB/s, of which 12 go to the launch, the
+// ranges, the first pages and the last parts, as one text of 1999 keys shows, which takes no less.
 #include <algorithm>
 
 #include "flash_attention.hpp"
@@ -20,12 +23,13 @@
 namespace tfk {
 namespace {
 
-constexpr int kWaves = 4, kThreads = kWaves * kWaveSize, kTileKeys = 16, kStages = 4;
-constexpr int kTilesPerBlock = 8, kBlockKeys = kTilesPerBlock * kTileKeys;
+constexpr int kWaves = 8, kThreads = kWaves * kWaveSize, kTileKeys = 16;
+constexpr int kBlockKeys = kWaves * kTileKeys;   // a tile each
+constexpr int tiles_ahead(int d) { return d == 128 ? 3 : 4; }   // of a wavefront, in registers: 24 or 16 KiB
 constexpr int kQueries = 16;   // of an item: one block of MFMA columns
-// Workgroups of a launch: those that LDS lets run at once.
-__host__ __device__ constexpr int tile_bytes(int d) { return 2 * kTileKeys * d * 2; }
-__host__ __device__ constexpr int resident(int d) { return kCUs * (kMaxLdsBytes / (kStages * kWaves * tile_bytes(d))); }
+// Workgroups of a launch, one on a CU.  (Two of half the size: the older one is served first and is done at two thirds of the time, the other
+// goes on alone and takes in less than the CU's share.  16 of 8 heads x 32768 x 128: 321 us, as two 354.)
+constexpr int kGroups = kCUs;
 
 struct DecodeArgs {
   const void* query;
@@ -46,6 +50,24 @@ TFK_DEVICE int keys_of(const DecodeArgs& a, int length) {
   return length > (int64_t)a.table.width * a.table.page.d ? -1 : max(length, 0);
 }
 TFK_DEVICE int blocks_of(int keys) { return (max(keys, 0) + kBlockKeys - 1) / kBlockKeys; }
+// An item costs the time of its blocks and of kOverhead more: to begin with new queries and pages, and to come together.  Ranges are of equal
+// cost (60 texts of 17 to 8001 keys, 8 heads x 64: the workgroups with many short ones were done at 60 us, the others at 30).
+__host__ __device__ constexpr int overhead(int d) { return d == 128 ? 1 : 2; }
+template <int D>
+TFK_DEVICE int cost_of(int keys) { return keys > 0 ? blocks_of(keys) + overhead(D) : 0; }
+
+// 16 bytes at base + offset, zeros where that is not within `bytes`; `base` and `bytes` are wavefront-uniform.  kOnce: whole lines, which no
+// cache need keep (a key's line is loaded in two halves: 16 of 8 heads x 32768 x 128 341 us with the hint, 335 without).
+template <typename V, bool kOnce>
+TFK_DEVICE V load_below(const void* base, unsigned bytes, unsigned offset) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kRaw32Bit = 0x00020000, kStreaming = kOnce ? 2 : 0;
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, kRaw32Bit);
+  return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(rsrc, offset, 0, kStreaming));
+#else
+  return V{};
+#endif
+}
 
 TFK_DEVICE int wave_prefix(int x) {   // inclusive sum over the lanes
   const int lane = threadIdx.x % kWaveSize;
@@ -105,27 +127,27 @@ TFK_DEVICE void store_weighed(const Weighed& w, T* to) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 1) void flash_decode_paged_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void flash_decode_paged_kernel(DecodeArgs a) {
   using V4 = typename Vec<T>::v4;
   using V8 = typename Vec<T>::v8;
   constexpr int kChunks = D / 8, kRowsPerLoad = kWaveSize / kChunks;   // 16-byte pieces of a row; rows of one load
   constexpr int kLoads = kTileKeys / kRowsPerLoad;                      // ... of a tile's keys, as of its values
-  constexpr int kKK = D / 32, kDB = D / 16, kColumns = D / 4;
-  constexpr int kKeyBytes = kTileKeys * D * 2, kStage = tile_bytes(D);
+  constexpr int kKK = D / 32, kDB = D / 16, kColumns = D / 4, kAhead = tiles_ahead(D);
+  constexpr int kRoom = kQueries * D * 4;   // bytes of LDS of a wavefront: its rows at the end, before that a tile of values
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   __shared__ float s_stats[kWaves][kQueries][2];
-  __shared__ bool s_last;
+  __shared__ bool s_last[2];
 
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int items_of = a.kv_heads * a.blocks_of_group;   // of a sequence
 
-  // ---- this workgroup's range of blocks ---------------------------------------------------------
-  auto own_blocks = [&](int b) __attribute__((always_inline)) { return b < a.sequences ? blocks_of(keys_of(a, a.lengths[b])) : 0; };
-  const int first_own = wave_prefix(own_blocks(lane));   // (kept: mostly all there are)
+  // ---- this workgroup's range of the items' costs ---------------------------------------------------------
+  auto own_cost = [&](int b) __attribute__((always_inline)) { return b < a.sequences ? cost_of<D>(keys_of(a, a.lengths[b])) : 0; };
+  const int first_own = wave_prefix(own_cost(lane));   // (kept: mostly all there are)
   int total = __builtin_amdgcn_readlane(first_own, 63);
-  for (int b0 = kWaveSize; b0 < a.sequences; b0 += kWaveSize) total += __builtin_amdgcn_readlane(wave_prefix(own_blocks(b0 + lane)), 63);
-  const unsigned blocks = (unsigned)total * (unsigned)items_of;   // (below 2^31: the host has seen the tables' width)
+  for (int b0 = kWaveSize; b0 < a.sequences; b0 += kWaveSize) total += __builtin_amdgcn_readlane(wave_prefix(own_cost(b0 + lane)), 63);
+  const unsigned cost = (unsigned)total * (unsigned)items_of;   // (below 2^31: the host has seen the tables' width)
   // sequences without a key, and those that the table cannot hold
   for (int b = blockIdx.x; b < a.sequences; b += gridDim.x) {
     const int n = keys_of(a, read_uniform(a.lengths + b));
@@ -133,20 +155,20 @@ __global__ __launch_bounds__(kThreads, 1) void flash_decode_paged_kernel(DecodeA
     const float v = n < 0 ? __builtin_nanf("") : 0.f;
     for (int i = tid; i < a.heads * D; i += kThreads) static_cast<T*>(a.out)[(int64_t)b * a.heads * D + i] = (T)v;
   }
-  // (no more workgroups than blocks; the first `longer` have one block more)
-  const unsigned groups = min(gridDim.x, blocks);
+  // (the first `longer` workgroups have a range that is longer by one)
+  const unsigned groups = min(gridDim.x, cost);
   if (blockIdx.x >= groups) return;
-  const unsigned quota = blocks / groups, longer = blocks - quota * groups;
+  const unsigned quota = cost / groups, longer = cost - quota * groups;
   const unsigned begin = blockIdx.x * quota + min(blockIdx.x, longer), end = begin + quota + (blockIdx.x < longer ? 1 : 0);
-  auto group_of = [&](unsigned block) __attribute__((always_inline)) {
+  auto group_of = [&](unsigned at) __attribute__((always_inline)) {
     const unsigned split = longer * (quota + 1);
-    return block < split ? block / (quota + 1) : longer + (block - split) / quota;
+    return at < split ? at / (quota + 1) : longer + (at - split) / quota;
   };
   // the sequence in which the range begins
   int b = 0;
-  unsigned before = 0;   // blocks of the sequences in front of it
+  unsigned before = 0;   // the cost of the sequences in front of it
   for (int b0 = 0; b0 < a.sequences; b0 += kWaveSize) {
-    const int up_to = b0 == 0 ? first_own : wave_prefix(own_blocks(b0 + lane));
+    const int up_to = b0 == 0 ? first_own : wave_prefix(own_cost(b0 + lane));
     const bool passed = before + (unsigned)up_to * (unsigned)items_of <= begin;
     const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(passed));
     b = b0 + n;
@@ -154,241 +176,289 @@ __global__ __launch_bounds__(kThreads, 1) void flash_decode_paged_kernel(DecodeA
     if (n < kWaveSize) break;
   }
 
-  // ---- LDS: where loads leave their rows and fragments find them ------------------------------
-  const unsigned wave_base = lds_address(smem) + wave * kStages * kStage;
-  unsigned key_off[kLoads], value_off[kLoads];   // bytes from a tile's first row in memory
+  // ---- what a lane loads of a tile, bytes from its first row in memory, and where the values go in LDS ----
+  const int key_step = (int)a.key_strides[1] * 2, value_step = (int)a.value_strides[1] * 2;
+  const unsigned key_off = (unsigned)(lr * key_step + 16 * lg);   // chunk 4 kk + lg of key lr: a fragment as it is
+  unsigned value_off[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) value_off[i] = (unsigned)((i * kRowsPerLoad + lane / kChunks) * value_step + lane % kChunks * 16);
+  const unsigned room = lds_address(smem) + wave * kRoom;
+  // (the swizzle is an exclusive or of chunk numbers: rows of one load to the next, and columns 16 db, differ by constants)
+  unsigned v_to[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
     const int row = i * kRowsPerLoad + lane / kChunks;
-    key_off[i] = (unsigned)(row * (int)a.key_strides[1] + swz_k<kChunks>(row, lane % kChunks) * 8) * 2u;
-    value_off[i] = (unsigned)(row * (int)a.value_strides[1] + swz_v<kChunks>(row, lane % kChunks) * 8) * 2u;
+    v_to[i] = room + row * D * 2 + swz_v<kChunks>(row, lane % kChunks) * 16;
   }
-  // (the swizzles are exclusive ors of chunk numbers: fragment kk of the keys is 64 kk further in that sense, db of the values 32 db)
-  const unsigned k_at = lr * D * 2 + swz_k<kChunks>(lr, lg) * 16;
   const int v_row = 4 * lg + (lr >> 2), v_col = 4 * (lr & 3);
-  const unsigned v_at = kKeyBytes + v_row * D * 2 + swz_v<kChunks>(v_row, v_col / 8) * 16 + (v_col % 8) * 2;
+  const unsigned v_at = room + v_row * D * 2 + swz_v<kChunks>(v_row, v_col / 8) * 16 + (v_col % 8) * 2;
 
-  for (unsigned at = begin; at < end; ++b) {
-    const int keys = keys_of(a, read_uniform(a.lengths + b));
-    const unsigned of_item = blocks_of(keys), of_sequence = of_item * (unsigned)items_of;
-    while (at < end && at < before + of_sequence) {
-      // ---- one item, or what of it is in the range: blocks [first, last) --------------------
-      const int item = (int)((at - before) / of_item);
-      const unsigned item_begin = before + (unsigned)item * of_item;
-      const int first = (int)(at - item_begin), last = (int)min(of_item, end - item_begin);
-      at = item_begin + last;
-      const int head = item / a.blocks_of_group, query0 = item % a.blocks_of_group * kQueries;
-      const int queries = min(kQueries, a.group - query0);
-      const int h0 = head * a.group + query0;
-      arrivals_t* const word = a.arrivals + ((int64_t)b * items_of + item) * kArrivalsPitch;
-      // the workgroups that have a part of it
-      const bool whole = first == 0 && last == (int)of_item;
-      const unsigned part_first = whole ? blockIdx.x : group_of(item_begin);
-      const int parts = whole ? 1 : (int)(group_of(item_begin + of_item - 1) - part_first) + 1;
-      if (parts > 1 && tid == 0 && blockIdx.x == part_first) open_arrivals(word, a.tag);
+  // Items of which this workgroup has a part, the range's first and last at most: they are put together when all else is done, so
+  // that nothing waits for stores and counts in between.
+  struct Part {
+    int parts = 0, first = 0, h0 = 0, queries = 0, b = 0;   // workgroups, the first of them; heads; sequence
+    arrivals_t* word = nullptr;
+  } mine[2];   // [1]: of an item that begins in this range
 
-      V8 qf[kKK];
-      const T* q = static_cast<const T*>(a.query) + b * a.query_token + (h0 + min(lr, queries - 1)) * a.query_head;
-#pragma unroll
-      for (int kk = 0; kk < kKK; ++kk) qf[kk] = *reinterpret_cast<const V8*>(q + 32 * kk + 8 * lg);
-
-      const int tile_end = min(last * kTilesPerBlock, (keys + kTileKeys - 1) / kTileKeys);
-      bool lost = false;   // a page that the cache does not have
-      const T* const keys_at = static_cast<const T*>(a.key) + head * a.key_strides[2];
-      const T* const values_at = static_cast<const T*>(a.value) + head * a.value_strides[2];
-      auto page_for = [&](int tile) __attribute__((always_inline)) { return page_of(a.table, b, min(tile, tile_end - 1) * kTileKeys); };
-      auto request = [&](int tile, int page, int stage) __attribute__((always_inline)) {
-        const unsigned dst = wave_base + stage * kStage;
-        lost |= page < 0;
-        page = max(page, 0);
-        const int key0 = tile * kTileKeys, row = key0 - divide(a.table.page, key0) * (int)a.table.page.d;
-        const T* k = keys_at + page * a.key_strides[0] + row * a.key_strides[1];
-        const T* v = values_at + page * a.value_strides[0] + row * a.value_strides[1];
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(key_off[i]), "s"(k), "{m0}"(dst + i * 1024) : "memory");
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(value_off[i]), "s"(v), "{m0}"(dst + kKeyBytes + i * 1024) : "memory");
-      };
-
-      float4_t o[kDB];
-#pragma unroll
-      for (int db = 0; db < kDB; ++db) o[db] = float4_t{0.f, 0.f, 0.f, 0.f};
-      // Weights are taken 2^kUp times as large in fp16 and enter the product as a number and its remainder: a weight's smallest remainder is
-      // then 2^-31 of the largest weight.
-      constexpr float kUp = std::is_same_v<T, bf16_t> ? 0.f : 7.f, kLazy = kUp + 8.f;
-      float top = -INFINITY, sum = 0.f;   // reference of query lr; this lane's part of its weights' sum
-
-      int tile = first * kTilesPerBlock + wave, ahead = tile;   // the next to compute, to request
-      int pages[kStages - 1];
-#pragma unroll
-      for (int n = 0; n < kStages - 1; ++n) pages[n] = page_for(tile + n * kWaves);
-      int next_page = page_for(tile + (kStages - 1) * kWaves);
-#pragma unroll
-      for (int kk = 0; kk < kKK; ++kk) asm volatile("" : "+v"(qf[kk]));   // (waited for here, not among the tiles)
-#pragma unroll
-      for (int n = 0; n < kStages - 1; ++n, ahead += kWaves)
-        if (ahead < tile_end) request(ahead, pages[n], n);
-      for (int n = 0; tile < tile_end; ++n, tile += kWaves) {
-        const unsigned stage = wave_base + n % kStages * kStage;
-        if (ahead < tile_end) {
-          request(ahead, next_page, (n + kStages - 1) % kStages);
-          ahead += kWaves;
-          next_page = page_for(ahead);
-          wait_vmem<(kStages - 1) * 2 * kLoads>();
-        } else {   // (the last tiles have all been asked for)
-          const int behind = (tile_end - 1 - tile) / kWaves;
-          if (behind >= 2) wait_vmem<2 * 2 * kLoads>();
-          else if (behind == 1) wait_vmem<2 * kLoads>();
-          else wait_vmem_all();
-        }
-        const int left = keys - tile * kTileKeys;   // keys of the tile, one at least
-        if (left < kTileKeys) {
-          // rows behind the last key hold anything: their weight is zero, and zero times an infinity is none
-          const V8 zeros = {};
-#pragma unroll
-          for (int i = 0; i < kLoads; ++i)
-            if (i * kRowsPerLoad + lane / kChunks >= left)
-              *(__attribute__((address_space(3))) V8*)(size_t)(stage + kKeyBytes + i * 1024 + lane * 16) = zeros;
-        }
-        const unsigned ka = opaque(stage + k_at), va = opaque(stage + v_at);
-        float4_t s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < kKK; ++kk) s = mfma_t<T>(lds_read_b128<V8>(ka ^ (kk << 6)), qf[kk], s);
-        V4 vf[kDB];
-#pragma unroll
-        for (int db = 0; db < kDB; ++db) vf[db] = lds_read_tr4<V4>(va ^ (db << 5));
-        float big = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[r] = 4 * lg + r < left ? s[r] * a.scale_log2 : -INFINITY;
-          big = fmaxf(big, s[r]);
-        }
-        if (__builtin_amdgcn_ballot_w64(big > top + kLazy) != 0) {   // (the first finite score, too)
-          const float higher = fmaxf(top, quad_max(big) - kUp);
-          const float factor = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - higher);
-          top = higher;
-          sum *= factor;
-#pragma unroll
-          for (int db = 0; db < kDB; ++db) o[db] *= factor;
-        }
-        const float reference = top == -INFINITY ? 0.f : top;
-        V4 p, rest;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float w = __builtin_amdgcn_exp2f(s[r] - reference);
-          sum += w;
-          const SplitWeight<T> two = split_weight<T>(w);
-          p[r] = two.whole;
-          rest[r] = two.rest;
-        }
-#pragma unroll
-        for (int db = 0; db < kDB; ++db) {
-          o[db] = mfma_16x16x16<T>(vf[db], p, o[db]);
-          o[db] = mfma_16x16x16<T>(vf[db], rest, o[db]);
-        }
-        // the tile's reads are done before its room is asked for again
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  // One item, or what of it is in the range: blocks [first, first + blocks).
+  struct Segment {
+    int b, h0, queries, head, keys, first, blocks;
+    unsigned begin, cost;   // where the item begins, and what it costs
+  };
+  // The next segment of the range from `at` on, which is moved behind it; no blocks: there is none.  An item's overhead stands in front of its
+  // blocks, and a range may end in it.  b and `before` are those of the segment in front, or of the range's beginning.
+  unsigned at = begin;
+  auto next_segment = [&]() __attribute__((always_inline)) -> Segment {
+    Segment g = {};
+    while (at < end && g.blocks == 0) {
+      int keys = keys_of(a, read_uniform(a.lengths + b));
+      unsigned of_item = cost_of<D>(keys);
+      while (at >= before + of_item * (unsigned)items_of) {   // (ends: the range is within the sum)
+        before += of_item * (unsigned)items_of;
+        keys = keys_of(a, read_uniform(a.lengths + ++b));
+        of_item = cost_of<D>(keys);
       }
-
-      // ---- the wavefronts together, in their tiles' room ------------------------------------------
-      sum += __shfl_xor(sum, 16);
-      sum += __shfl_xor(sum, 32);
-      if (lost) sum = __builtin_nanf("");
-      if (lg == 0) {
-        s_stats[wave][lr][0] = top;
-        s_stats[wave][lr][1] = sum;
-      }
-      float* const s_rows = reinterpret_cast<float*>(smem + wave * kStages * kStage);   // [kQueries][D]
-#pragma unroll
-      for (int db = 0; db < kDB; ++db) *reinterpret_cast<float4_t*>(s_rows + lr * D + ((db ^ (lr & (kDB - 1))) * 16 + 4 * lg)) = o[db];
-      __syncthreads();
-      T* const out = static_cast<T*>(a.out) + ((int64_t)b * a.heads + h0) * D;
-      float* const part = a.part + ((int64_t)blockIdx.x * 2 + (blockIdx.x == part_first ? 1 : 0)) * part_floats<D>();
-      for (int i = tid; i < queries * kColumns; i += kThreads) {
-        const int qi = i / kColumns, c = i % kColumns;
-        Weighed w;
-#pragma unroll
-        for (int v = 0; v < kWaves; ++v)
-          add_weighed(w, s_stats[v][qi][0], s_stats[v][qi][1],
-                      *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(smem + v * kStages * kStage) + qi * D +
-                                                         (((c / 4) ^ (qi & (kDB - 1))) * 16 + 4 * (c % 4))));
-        if (parts == 1) {
-          store_weighed(w, out + qi * D + 4 * c);
-          continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) store_shared(part + qi * D + 4 * c + e, w.o[e]);
-        if (c == 0) {
-          store_shared(part + kQueries * D + 2 * qi, w.m);
-          store_shared(part + kQueries * D + 2 * qi + 1, w.l);
-        }
-      }
-      if (parts > 1) {
-        wait_vmem_all();
-        __syncthreads();
-        if (tid == 0) s_last = arrive(word, a.tag, (unsigned)parts);
-        __syncthreads();
-        if (s_last) {
-          // The parts lie in the second room of the first workgroup and in the first rooms of the others.  kBatch of them are on their way at a
-          // time, and where an item has few queries several threads share the parts of a column.
-          constexpr int kBatch = 8;
-          constexpr unsigned kPitch = 2 * part_floats<D>() * 4, kSecond = part_floats<D>() * 4;
-          const float* const from = a.part + (int64_t)part_first * 2 * part_floats<D>();
-          const int units = queries * kColumns;
-          const int sharing = units * 8 <= kThreads ? 8 : units * 4 <= kThreads ? 4 : units * 2 <= kThreads ? 2 : 1;
-          Weighed* const s_shared = reinterpret_cast<Weighed*>(smem);   // [sharing][units]
-          for (int i = tid; i < units * sharing; i += kThreads) {
-            const int unit = i % units, share = i / units, qi = unit / kColumns, c = unit % kColumns;
-            Weighed w;
-            for (int s0 = share; s0 < parts; s0 += kBatch * sharing) {
-              float2_t ml[kBatch];
-              float4_t x[kBatch];
-#pragma unroll
-              for (int u = 0; u < kBatch; ++u) {
-                const int s = min(s0 + u * sharing, parts - 1);
-                const unsigned slot = (unsigned)s * kPitch + (s == 0 ? kSecond : 0u);
-                ml[u] = load_shared_8B(from, slot + (kQueries * D + 2 * qi) * 4);
-                x[u] = load_shared_16B<float4_t>(from, slot + (qi * D + 4 * c) * 4);
-              }
-#pragma unroll
-              for (int u = 0; u < kBatch; ++u)
-                if (s0 + u * sharing < parts) add_weighed(w, ml[u][0], ml[u][1], x[u]);
-            }
-            if (sharing == 1) store_weighed(w, out + qi * D + 4 * c);
-            else s_shared[share * units + unit] = w;
-          }
-          if (sharing > 1) {
-            __syncthreads();
-            if (tid < units) {
-              Weighed w = s_shared[tid];
-              for (int k = 1; k < sharing; ++k) {
-                const Weighed& x = s_shared[k * units + tid];
-                add_weighed(w, x.m, x.l, x.o);
-              }
-              store_weighed(w, out + tid / kColumns * D + 4 * (tid % kColumns));
-            }
-          }
-        }
-      }
-      __syncthreads();   // the room is the next item's
+      const unsigned item = (at - before) / of_item, item_begin = before + item * of_item, stop = min(item_begin + of_item, end);
+      const int head = (int)item / a.blocks_of_group, query0 = (int)item % a.blocks_of_group * kQueries;
+      const int first = max((int)(at - item_begin) - overhead(D), 0), last = max((int)(stop - item_begin) - overhead(D), 0);
+      g = {b, head * a.group + query0, min(kQueries, a.group - query0), head, keys, first, last - first, item_begin, of_item};
+      at = stop;
     }
-    before += of_sequence;
+    return g;
+  };
+
+  V8 qf[kKK], k[kAhead][kKK], v[kAhead][kLoads];
+  bool lost = false, next_lost = false;   // a page that the cache does not have
+  int next_page = 0;
+  // This wavefront's tile of a block of a segment.
+  auto page_for = [&](const Segment& g, int block) __attribute__((always_inline)) {
+    // (within the table: keys_of; what the entry holds is looked at when it is needed, so that nothing waits for it here)
+    return read_uniform(a.table.pages + g.b * a.table.stride + divide(a.table.page, min((g.first + block) * kWaves + wave, (g.keys - 1) / kTileKeys) * kTileKeys));
+  };
+  // Tiles past the end are asked for as well, and rows behind the last key: the bounds check of a buffer load returns zeros there and fetches nothing.
+  // (With a branch around loads the compiler waits for all of them where its two ways meet.  Zeros, because what the cache holds behind
+  // the last key may be infinite, and its weight of zero would make NaN of it.)
+  auto load = [&](const Segment& g, int n, int block, int page, bool& none) __attribute__((always_inline)) {
+    const int tile = (g.first + block) * kWaves + wave, key0 = min(tile, (g.keys - 1) / kTileKeys) * kTileKeys;
+    const int rows = block < g.blocks ? min(kTileKeys, g.keys - tile * kTileKeys) : 0;
+    const bool there = page >= 0 && page < a.table.cache_pages;
+    none |= rows > 0 && !there;
+    page = there ? page : 0;
+    const int row = key0 - divide(a.table.page, key0) * (int)a.table.page.d;
+    const T* kp = static_cast<const T*>(a.key) + page * a.key_strides[0] + row * a.key_strides[1] + g.head * a.key_strides[2];
+    const T* vp = static_cast<const T*>(a.value) + page * a.value_strides[0] + row * a.value_strides[1] + g.head * a.value_strides[2];
+    const unsigned key_bytes = rows > 0 ? (unsigned)((rows - 1) * key_step + D * 2) : 0u;
+    const unsigned value_bytes = rows > 0 ? (unsigned)((rows - 1) * value_step + D * 2) : 0u;
+#pragma unroll
+    for (int kk = 0; kk < kKK; ++kk) k[n][kk] = load_below<V8, false>(kp, key_bytes, key_off + 64 * kk);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) v[n][i] = load_below<V8, true>(vp, value_bytes, value_off[i]);
+    __builtin_amdgcn_sched_barrier(0);   // the requests leave before the next tile is consumed
+  };
+  // What a segment's first blocks need, asked for.
+  auto start = [&](const Segment& g) __attribute__((always_inline)) {
+    const T* q = static_cast<const T*>(a.query) + g.b * a.query_token + (g.h0 + min(lr, g.queries - 1)) * a.query_head;
+    int pages[kAhead];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) pages[n] = page_for(g, n);
+    next_page = page_for(g, kAhead);   // (asked for a tile before it is needed)
+#pragma unroll
+    for (int kk = 0; kk < kKK; ++kk) qf[kk] = *reinterpret_cast<const V8*>(q + 32 * kk + 8 * lg);
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) load(g, n, n, pages[n], next_lost);
+  };
+
+  Segment now = next_segment();
+  if (now.blocks > 0) start(now);
+  while (now.blocks > 0) {
+    lost = next_lost;
+    next_lost = false;
+    float4_t o[kDB];
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) o[db] = float4_t{0.f, 0.f, 0.f, 0.f};
+    // Weights are taken 2^kUp times as large in fp16 and enter the product as a number and its remainder: a weight's smallest remainder is
+    // then 2^-31 of the largest weight.
+    constexpr float kUp = std::is_same_v<T, bf16_t> ? 0.f : 7.f, kLazy = kUp + 8.f;
+    float top = -INFINITY, sum = 0.f;   // reference of query lr; this lane's part of its weights' sum
+
+    auto consume = [&](int n, int left) __attribute__((always_inline)) {   // left: keys of the tile; it may have none
+      float4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < kKK; ++kk) s = mfma_t<T>(k[n][kk], qf[kk], s);
+      // (LDS serves a wavefront in order: what the last tile has read is read)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) *(__attribute__((address_space(3))) V8*)(size_t)v_to[i] = v[n][i];
+      V4 vf[kDB];
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) vf[db] = lds_read_tr4<V4>(v_at ^ (db << 5));
+      float big = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[r] = 4 * lg + r < left ? s[r] * a.scale_log2 : -INFINITY;
+        big = fmaxf(big, s[r]);
+      }
+      if (__builtin_amdgcn_ballot_w64(big > top + kLazy) != 0) {   // (the first finite score, too)
+        const float higher = fmaxf(top, quad_max(big) - kUp);
+        const float factor = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - higher);
+        top = higher;
+        sum *= factor;
+#pragma unroll
+        for (int db = 0; db < kDB; ++db) o[db] *= factor;
+      }
+      const float reference = top == -INFINITY ? 0.f : top;
+      V4 p, rest;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float w = __builtin_amdgcn_exp2f(s[r] - reference);
+        sum += w;
+        const SplitWeight<T> two = split_weight<T>(w);
+        p[r] = two.whole;
+        rest[r] = two.rest;
+      }
+#pragma unroll
+      for (int db = 0; db < kDB; ++db) {
+        o[db] = mfma_16x16x16<T>(vf[db], p, o[db]);
+        o[db] = mfma_16x16x16<T>(vf[db], rest, o[db]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // (the queries came first: waited for here, they are not waited for among the tiles, and all that is ahead with them)
+#pragma unroll
+    for (int kk = 0; kk < kKK; ++kk) asm volatile("" : "+v"(qf[kk]));
+    auto consume_block = [&](int n, int block) __attribute__((always_inline)) {
+      consume(n, now.keys - ((now.first + block) * kWaves + wave) * kTileKeys);
+    };
+    // (whole rounds, and then what is left: the loads on their way at a loop's beginning are always the same, and the compiler waits for no more
+    // than it needs)
+    int block = 0;
+    for (; block + kAhead <= now.blocks; block += kAhead) {
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) {
+        consume_block(n, block + n);
+        load(now, n, block + n + kAhead, next_page, lost);
+        next_page = page_for(now, block + n + 1 + kAhead);
+      }
+      barrier_only();   // (the wavefronts in step: the older ones are served first, and would leave the others behind)
+    }
+#pragma unroll
+    for (int n = 0; n < kAhead - 1; ++n)
+      if (block + n < now.blocks) consume_block(n, block + n);
+
+    // ---- the next segment is on its way while this one's wavefronts come together ---------------
+    const Segment done = now;
+    now = next_segment();
+    if (now.blocks > 0) start(now);
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (lost) sum = __builtin_nanf("");
+    if (lg == 0) {
+      s_stats[wave][lr][0] = top;
+      s_stats[wave][lr][1] = sum;
+    }
+    float* const s_rows = reinterpret_cast<float*>(smem + wave * kRoom);   // [kQueries][D]
+#pragma unroll
+    for (int db = 0; db < kDB; ++db) *reinterpret_cast<float4_t*>(s_rows + lr * D + ((db ^ (lr & (kDB - 1))) * 16 + 4 * lg)) = o[db];
+    barrier_lds_only();
+    // the workgroups that have a part of the item
+    const bool whole = done.first == 0 && done.blocks + overhead(D) == (int)done.cost;
+    const unsigned part_first = whole ? blockIdx.x : group_of(done.begin + overhead(D));
+    const int parts = whole ? 1 : (int)(group_of(done.begin + done.cost - 1) - part_first) + 1;
+    const bool begins = blockIdx.x == part_first;
+    T* const out = static_cast<T*>(a.out) + ((int64_t)done.b * a.heads + done.h0) * D;
+    float* const part = a.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * part_floats<D>();
+    if (parts > 1) {
+      arrivals_t* const word = a.arrivals + ((int64_t)done.b * items_of + done.h0 / a.group * a.blocks_of_group + done.h0 % a.group / kQueries) * kArrivalsPitch;
+      if (begins && tid == 0) open_arrivals(word, a.tag);
+      const Part p = {parts, (int)part_first, done.h0, done.queries, done.b, word};
+      if (begins) mine[1] = p;
+      else mine[0] = p;
+    }
+    for (int i = tid; i < done.queries * kColumns; i += kThreads) {
+      const int qi = i / kColumns, c = i % kColumns;
+      Weighed w;
+#pragma unroll
+      for (int x = 0; x < kWaves; ++x)
+        add_weighed(w, s_stats[x][qi][0], s_stats[x][qi][1],
+                    *reinterpret_cast<const float4_t*>(reinterpret_cast<const float*>(smem + x * kRoom) + qi * D +
+                                                       (((c / 4) ^ (qi & (kDB - 1))) * 16 + 4 * (c % 4))));
+      if (parts == 1) {
+        store_weighed(w, out + qi * D + 4 * c);
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) store_shared(part + qi * D + 4 * c + e, w.o[e]);
+      if (c == 0) {
+        store_shared(part + kQueries * D + 2 * qi, w.m);
+        store_shared(part + kQueries * D + 2 * qi + 1, w.l);
+      }
+    }
+    barrier_lds_only();   // the room is the next item's
+  }
+
+  if (mine[0].parts + mine[1].parts == 0) return;
+  wait_vmem_all();
+  __syncthreads();
+  if (lane == 0 && wave < 2) s_last[wave] = mine[wave].parts > 0 && arrive(mine[wave].word, a.tag, (unsigned)mine[wave].parts);
+  __syncthreads();
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    if (!s_last[which]) continue;
+    // The parts lie in the second room of the first workgroup and in the first rooms of the others.  kBatch of them are on their way at a
+    // time, and where an item has few queries several threads share the parts of a column.
+    constexpr int kBatch = 8;
+    constexpr unsigned kPitch = 2 * part_floats<D>() * 4, kSecond = part_floats<D>() * 4;
+    const Part& p = mine[which];
+    const float* const from = a.part + (int64_t)p.first * 2 * part_floats<D>();
+    T* const out = static_cast<T*>(a.out) + ((int64_t)p.b * a.heads + p.h0) * D;
+    const int units = p.queries * kColumns, parts = p.parts;
+    const int sharing = units * 8 <= kThreads ? 8 : units * 4 <= kThreads ? 4 : units * 2 <= kThreads ? 2 : 1;
+    Weighed* const s_shared = reinterpret_cast<Weighed*>(smem);   // [sharing][units]
+    for (int i = tid; i < units * sharing; i += kThreads) {
+      const int unit = i % units, share = i / units, qi = unit / kColumns, c = unit % kColumns;
+      Weighed w;
+      for (int s0 = share; s0 < parts; s0 += kBatch * sharing) {
+        float2_t ml[kBatch];
+        float4_t x[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int s = min(s0 + u * sharing, parts - 1);
+          const unsigned slot = (unsigned)s * kPitch + (s == 0 ? kSecond : 0u);
+          ml[u] = load_shared_8B(from, slot + (kQueries * D + 2 * qi) * 4);
+          x[u] = load_shared_16B<float4_t>(from, slot + (qi * D + 4 * c) * 4);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+          if (s0 + u * sharing < parts) add_weighed(w, ml[u][0], ml[u][1], x[u]);
+      }
+      if (sharing == 1) store_weighed(w, out + qi * D + 4 * c);
+      else s_shared[share * units + unit] = w;
+    }
+    if (sharing > 1) {
+      __syncthreads();
+      if (tid < units) {
+        Weighed w = s_shared[tid];
+        for (int k = 1; k < sharing; ++k) {
+          const Weighed& x = s_shared[k * units + tid];
+          add_weighed(w, x.m, x.l, x.o);
+        }
+        store_weighed(w, out + tid / kColumns * D + 4 * (tid % kColumns));
+      }
+      __syncthreads();
+    }
   }
 }
 
 int blocks_of_group(int64_t heads, int64_t kv_heads) { return (int)((heads / kv_heads + kQueries - 1) / kQueries); }
-size_t part_bytes(int64_t D) { return (size_t)resident((int)D) * 2 * kQueries * (size_t)(D + 2) * sizeof(float); }
+size_t part_bytes(int64_t D) { return (size_t)kGroups * 2 * kQueries * (size_t)(D + 2) * sizeof(float); }
 
 template <typename T, int D>
 int launch_decode_paged(const DecodeArgs& a, hipStream_t st) {
   auto kern = flash_decode_paged_kernel<T, D>;
-  constexpr int lds = kStages * kWaves * tile_bytes(D);
+  constexpr int lds = kWaves * kQueries * D * 4;
   TFK_LDS_OPT_IN(kern, lds);
-  // (blocks that there can be: a launch of a few sequences with short tables asks for no more workgroups than those)
-  const int64_t most = (int64_t)a.sequences * a.kv_heads * a.blocks_of_group * (((int64_t)a.table.width * a.table.page.d + kBlockKeys - 1) / kBlockKeys);
-  return launch_kernel(kern, dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, resident(D)))), dim3(kThreads), lds, st, a);
+  // (what there can be: a launch of a few sequences with short tables asks for no more workgroups than that)
+  const int64_t most = (int64_t)a.sequences * a.kv_heads * a.blocks_of_group * (((int64_t)a.table.width * a.table.page.d + kBlockKeys - 1) / kBlockKeys + overhead(D));
+  return launch_kernel(kern, dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(most, kGroups))), dim3(kThreads), lds, st, a);
 }
 
 }  // namespace
@@ -412,7 +482,7 @@ extern "C" int tf_flash_decode_paged(const tf_paged_cache_t* cache, const void* 
   TFK_REQUIRE(softmax_scale == softmax_scale && softmax_scale - softmax_scale == 0.0, TF_ERR_INVALID_ARG, "%s: softmax_scale must be finite", who);
   if (cache->sequences == 0) return TF_OK;
   TFK_REQUIRE(cache->table_width < (1ll << 31) / cache->page_size &&
-                  cache->sequences * (cache->table_width * cache->page_size / kBlockKeys + 1) <
+                  cache->sequences * (cache->table_width * cache->page_size / kBlockKeys + 3) <
                       (1ll << 31) / (cache->kv_heads * blocks_of_group(heads, cache->kv_heads)),
               TF_ERR_INVALID_ARG, "%s: the table has room for 2^31 tokens a sequence, or 2^31 blocks of 128 keys in all", who);
   TFK_REQUIRE(cache->sequences * heads < (1 << 24), TF_ERR_INVALID_ARG, "%s: sequences * heads must be below 2^24", who);
