@@ -283,7 +283,7 @@ TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* 
 
 /* A cache of keys and values in pages: token p of sequence b is row p % page_size of page page_table[b][p / page_size].  key and value
  * [pages, page_size, kv_heads, D] of dtype (fp16 or bf16), D 64 or 128, in any order of the first three dimensions: strides in elements from page to
- * page, token to token and head to head, multiples of 8; both begin at 16-byte boundaries.  page_table [sequences, table_width] int32, rows table_stride
+ * page, token to token and head to head, multiples of 8, no less than D (or zero where there is one); both begin at 16-byte boundaries.  page_table [sequences, table_width] int32, rows table_stride
  * apart, and lengths [sequences] int32 are in device memory and may hold anything: a page that the cache does not have is
  * never read or written.  Table entries beyond a sequence's length are not looked at.  (No counterpart in the reference.) */
 typedef struct {

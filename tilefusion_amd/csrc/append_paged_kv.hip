@@ -189,8 +189,9 @@ int check_paged_cache(const char* who, const tf_paged_cache_t* c) {
   TFK_REQUIRE(c->sequences >= 0 && c->sequences <= (1 << 20) && c->table_width >= 0 && c->table_width < (1ll << 31) && c->table_stride >= 0,
               TF_ERR_INVALID_ARG, "%s: at most 2^20 sequences, table_width below 2^31", who);
   for (int i = 0; i < 3; ++i)
-    TFK_REQUIRE(c->key_strides[i] >= 0 && c->value_strides[i] >= 0 && c->key_strides[i] % 8 == 0 && c->value_strides[i] % 8 == 0, TF_ERR_INVALID_ARG,
-                "%s: the cache's strides must be multiples of 8 elements", who);
+    for (const int64_t stride : {c->key_strides[i], c->value_strides[i]})
+      TFK_REQUIRE((stride == 0 || stride >= c->D) && stride % 8 == 0, TF_ERR_INVALID_ARG,
+                  "%s: the cache's strides must be multiples of 8 elements and no less than a row, or zero where there is one", who);
   TFK_REQUIRE(((reinterpret_cast<uintptr_t>(c->key) | reinterpret_cast<uintptr_t>(c->value)) & 15) == 0, TF_ERR_INVALID_ARG,
               "%s: the cache must begin at a 16-byte boundary", who);
   return TF_OK;

@@ -624,7 +624,7 @@ tf_paged_cache_t paged_cache(const at::Tensor& key_cache, const at::Tensor& valu
     bool whole = x.t.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.t.data_ptr()) % 16 == 0;
     for (int i = 0; i < 3; ++i) {
       x.strides[i] = x.t.size(i) > 1 ? x.t.stride(i) : 0;
-      whole = whole && x.strides[i] % 8 == 0 && (x.t.size(i) == 1 || x.strides[i] > 0);
+      whole = whole && x.strides[i] % 8 == 0 && (x.t.size(i) == 1 || x.strides[i] >= x.t.size(3));
     }
     TORCH_CHECK(whole, "tilefusion::", op, ": rows of ", x.name, " must lie in one piece each, in places of their own at 16-byte boundaries.");
   }
