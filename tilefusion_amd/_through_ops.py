@@ -46,3 +46,19 @@ def gated_ffn_backward(*args: Any) -> None:
 
 def linear_cross_entropy_backward(*args: Any) -> None:
     return None
+
+
+def flash_decode_paged(*args: Any) -> None:
+    return None
+
+
+def append_paged_kv(*args: Any) -> None:
+    return None
+
+
+def flash_attention_packed(*args: Any) -> None:
+    return None
+
+
+def flash_attention_packed_backward(*args: Any) -> None:
+    return None

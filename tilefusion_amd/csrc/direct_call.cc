@@ -365,6 +365,112 @@ PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssi
   END_HANDLE_TH_ERRORS
 }
 
+// ---- attention over packed sequences and paged caches: [n, heads, D], rows in one piece at 16-byte boundaries as they come ----
+bool rows_in_place(const at::Tensor* t, int n) {
+  for (int i = 0; i < n; ++i)
+    if (t[i].dim() != 3 || t[i].stride(2) != 1 || t[i].stride(0) % 8 != 0 || t[i].stride(1) % 8 != 0 || reinterpret_cast<uintptr_t>(t[i].data_ptr()) % 16 != 0 ||
+        !is_half_type(t[i]))
+      return false;
+  return true;
+}
+bool scale_of(PyObject* arg, const at::Tensor& query, double* out) {
+  if (arg != Py_None && !PyFloat_CheckExact(arg)) return false;
+  *out = arg == Py_None ? 1.0 / std::sqrt((double)query.size(2)) : PyFloat_AS_DOUBLE(arg);
+  return query.size(2) > 0;
+}
+// A tensor or None; false: something else, or a tensor that is not plain (as `plain` has it).
+bool plain_or_none(const c10::OperatorHandle& op, PyObject* arg, std::optional<at::Tensor>* out) {
+  if (arg == Py_None) return true;
+  at::Tensor t[1];
+  if (!plain(op, &arg, 1, t)) return false;
+  *out = t[0];
+  return true;
+}
+
+// (query, key_cache, value_cache, page_table, lengths, softmax_scale or None) -> output, or None
+PyObject* flash_decode_paged(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[5], out;
+  double scale;
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, double, at::Tensor&);
+  static const auto op = find_op<Op>("tilefusion::flash_decode_paged");
+  if (nargs != 6 || !plain(op, args, 5, t) || !rows_in_place(t, 1) || !scale_of(args[5], t[0], &scale)) Py_RETURN_NONE;
+  {
+    NoGil unlocked;
+    out = empty_output(t[0].sizes(), t[0]);
+    op.redispatch(kCuda, t[0], t[1], t[2], t[3], t[4], scale, out);
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (query, key, value, cos, sin, key_cache, value_cache, page_table, lengths, offsets or None, interleaved, keep) -> (query,) or (query, key), or None
+PyObject* append_paged_kv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[9], query;
+  std::optional<at::Tensor> offsets, key;
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, at::Tensor&, at::Tensor&, const at::Tensor&,
+                  const at::Tensor&, const std::optional<at::Tensor>&, bool, at::Tensor&, const std::optional<at::Tensor>&);
+  static const auto op = find_op<Op>("tilefusion::append_paged_kv");
+  if (nargs != 12 || !plain(op, args, 9, t) || !rows_in_place(t, 3) || !t[3].is_contiguous() || !t[4].is_contiguous() ||
+      !plain_or_none(op, args[9], &offsets) || !PyBool_Check(args[10]) || !PyBool_Check(args[11]))
+    Py_RETURN_NONE;
+  const bool keep = args[11] == Py_True;
+  {
+    NoGil unlocked;
+    query = empty_output(t[0].sizes(), t[0]);
+    if (keep) key = empty_output(t[1].sizes(), t[1]);
+    op.redispatch(kCuda, t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], offsets, args[10] == Py_True, query, key);
+  }
+  return keep ? tuple_of({query, *key}) : tuple_of({query});
+  END_HANDLE_TH_ERRORS
+}
+
+// (query, key, value, offsets, kv_offsets or None, softmax_scale or None, causal, keep) -> (out,) or (out, lse), or None
+PyObject* flash_attention_packed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[4], out;
+  std::optional<at::Tensor> kv_offsets, lse;
+  double scale;
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&, double, bool, at::Tensor&,
+                  const std::optional<at::Tensor>&);
+  static const auto op = find_op<Op>("tilefusion::flash_attention_packed");
+  if (nargs != 8 || !plain(op, args, 4, t) || !rows_in_place(t, 3) || !plain_or_none(op, args[4], &kv_offsets) || !scale_of(args[5], t[0], &scale) ||
+      !PyBool_Check(args[6]) || !PyBool_Check(args[7]))
+    Py_RETURN_NONE;
+  const bool keep = args[7] == Py_True;
+  {
+    NoGil unlocked;
+    out = empty_output(t[0].sizes(), t[0]);
+    if (keep) lse = empty_output({t[0].size(1), t[0].size(0)}, t[0], at::kFloat);
+    op.redispatch(kCuda, t[0], t[1], t[2], t[3], kv_offsets, scale, args[6] == Py_True, out, lse);
+  }
+  return keep ? tuple_of({out, *lse}) : tuple_of({out});
+  END_HANDLE_TH_ERRORS
+}
+
+// (grad_out, query, key, value, out, lse, offsets, kv_offsets or None, softmax_scale or None, causal) -> (grad_query, grad_key, grad_value), or None
+PyObject* flash_attention_packed_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  at::Tensor t[7];
+  std::optional<at::Tensor> kv_offsets, grads[3];
+  double scale;
+  using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                  const std::optional<at::Tensor>&, double, bool, const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
+                  const std::optional<at::Tensor>&);
+  static const auto op = find_op<Op>("tilefusion::flash_attention_packed_backward");
+  if (nargs != 10 || !plain(op, args, 7, t) || !rows_in_place(t, 5) || !t[0].is_contiguous() || !t[4].is_contiguous() || !t[5].is_contiguous() ||
+      !plain_or_none(op, args[7], &kv_offsets) || !scale_of(args[8], t[1], &scale) || !PyBool_Check(args[9]))
+    Py_RETURN_NONE;
+  {
+    NoGil unlocked;
+    for (int i = 0; i < 3; ++i) grads[i] = empty_output(t[1 + i].sizes(), t[1 + i]);
+    op.redispatch(kCuda, t[0], t[1], t[2], t[3], t[4], t[5], t[6], kv_offsets, scale, args[9] == Py_True, grads[0], grads[1], grads[2]);
+  }
+  return tuple_of({*grads[0], *grads[1], *grads[2]});
+  END_HANDLE_TH_ERRORS
+}
+
 template <PyObject* (*kFunction)(PyObject*, PyObject* const*, Py_ssize_t)>
 constexpr PyMethodDef method(const char* name) {
   return {name, (PyCFunction)(void (*)(void))kFunction, METH_FASTCALL, nullptr};
@@ -374,6 +480,9 @@ PyMethodDef methods[] = {method<gemm>("gemm"), method<fused_two_gemms>("fused_tw
                          method<quantize_rows>("quantize_rows"), method<gemm_int8>("gemm_int8"), method<gated_ffn>("gated_ffn"),
                          method<gated_ffn_backward>("gated_ffn_backward"), method<linear_cross_entropy>("linear_cross_entropy"),
                          method<linear_cross_entropy_backward>("linear_cross_entropy_backward"),
+                         method<flash_decode_paged>("flash_decode_paged"), method<append_paged_kv>("append_paged_kv"),
+                         method<flash_attention_packed>("flash_attention_packed"),
+                         method<flash_attention_packed_backward>("flash_attention_packed_backward"),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -4,6 +4,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
+from .. import _direct
 from ._autograd import refuse_gradients, rows_in_place
 
 __all__ = ["append_paged_kv", "rotation_tables"]
@@ -52,6 +53,12 @@ def append_paged_kv(
     page in the cache, or no row in the tables, leaves the cache as it is and its rotated rows are NaN; tokens of no sequence (behind
     offsets[-1], or of one that is shorter than its new tokens, as an idle slot of length 0) leave it as it is too, and their rows are zero.  Pages that
     new tokens go to belong to one sequence.  There is no gradient."""
+    if not torch.compiler.is_compiling():
+        direct = _direct.append_paged_kv(
+            query, key, value, cos, sin, key_cache, value_cache, page_table, lengths, offsets, interleaved, keep
+        )
+        if direct is not None:
+            return direct if keep else direct[0]
     op = "append_paged_kv"
     refuse_gradients(op, query, key, value, cos, sin, key_cache, value_cache)
     if query.dim() != 3 or key.dim() != 3:

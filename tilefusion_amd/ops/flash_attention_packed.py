@@ -5,6 +5,7 @@ from typing import Any, Optional, Tuple, Union
 
 import torch
 
+from .. import _direct
 from ._autograd import not_captured, records, refuse_transforms, rows_in_place
 
 __all__ = ["flash_attention_packed", "flash_attention_packed_backward"]
@@ -103,6 +104,10 @@ def flash_attention_packed(
     tensors.  Rows that see no key (more queries than keys) and rows of no sequence (behind offsets[-1]) are zero, their lse -inf.  Scores, maxima
     and sums are fp32; the weights are rounded to the type for the product with V.  Under autograd out carries the backward pass (once: no gradient of a
     gradient, no forward mode), and lse none; neither the call nor that pass is captured into a graph."""
+    if not torch.compiler.is_compiling():
+        direct = _direct.flash_attention_packed(query, key, value, offsets, kv_offsets, softmax_scale, causal, keep)   # (no gradient is asked for)
+        if direct is not None:
+            return direct if keep else direct[0]
     op = "flash_attention_packed"
     scale = _scale(query, softmax_scale, op)
     if records(op, query, key, value):
@@ -129,6 +134,12 @@ def flash_attention_packed_backward(
     exp(scores - lse) and the gradients of the scores are rounded to the type on the way, as operands of the products that follow (in fp16 times powers of
     two, so that the type's range is not theirs); sums, those over the heads of a group among them, are fp32.  The same bits every time.  Rows of no
     sequence, rows that see no key and keys that no row sees have zeros."""
+    if not torch.compiler.is_compiling():
+        direct = _direct.flash_attention_packed_backward(
+            grad_out, query, key, value, out, lse, offsets, kv_offsets, softmax_scale, causal
+        )
+        if direct is not None:
+            return direct
     op = "flash_attention_packed_backward"
     scale = _scale(query, softmax_scale, op)
     refuse_transforms(op, grad_out, query, key, value, out, lse)

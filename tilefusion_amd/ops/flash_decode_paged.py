@@ -5,6 +5,7 @@ from typing import Optional
 
 import torch
 
+from .. import _direct
 from ._autograd import refuse_gradients, rows_in_place
 
 __all__ = ["flash_decode_paged"]
@@ -30,6 +31,10 @@ def flash_decode_paged(
     Returns [sequences, heads, D].  The cache is cut evenly over the chip whatever the lengths are, which only the device knows: a call can be
     captured and replayed with other lengths and tables in the same tensors.  A sequence of length 0 has rows of zeros, one that is
     longer than its row of the table, or names a page that the cache does not have within its length, NaN.  There is no gradient."""
+    if not torch.compiler.is_compiling():
+        direct = _direct.flash_decode_paged(query, key_cache, value_cache, page_table, lengths, softmax_scale)
+        if direct is not None:
+            return direct
     op = "flash_decode_paged"
     refuse_gradients(op, query, key_cache, value_cache)
     if query.dim() != 3:
