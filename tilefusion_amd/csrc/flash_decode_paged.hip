@@ -69,16 +69,6 @@ TFK_DEVICE V load_below(const void* base, unsigned bytes, unsigned offset) {
 #endif
 }
 
-TFK_DEVICE int wave_prefix(int x) {   // inclusive sum over the lanes
-  const int lane = threadIdx.x % kWaveSize;
-#pragma unroll
-  for (int d = 1; d < kWaveSize; d *= 2) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
-  return x;
-}
-
 // Position of (query, element) in a workgroup's part.
 template <int D>
 constexpr int part_floats() { return kQueries * (D + 2); }

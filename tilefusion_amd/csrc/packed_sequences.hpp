@@ -34,21 +34,10 @@ TFK_DEVICE PackedRange packed_range(int begin, int end, int rows) {
   return {b, max(min(end, rows) - b, 0)};
 }
 
-TFK_DEVICE int wave_sum(int x) {
-#pragma unroll
-  for (int d = 1; d < kWaveSize; d *= 2) x += __shfl_xor(x, d);
-  return __builtin_amdgcn_readfirstlane(x);
-}
-TFK_DEVICE int wave_max(int x) {
-#pragma unroll
-  for (int d = 1; d < kWaveSize; d *= 2) x = max(x, __shfl_xor(x, d));
-  return __builtin_amdgcn_readfirstlane(x);
-}
-
 // The `rank`-th of the tiles of `rows` rows that the sequences make, most keys first.  Tile e from a sequence's end ends
 // e * rows rows in front of it and counts as ceil(lkv * group / rows) - e (causal or not: the longest sequences first, and their last
 // tokens).  The largest number that more tiles reach than come before this one is found by halving, each step a
-// sum over the sequences, 64 at a time: with a few dozen sequences some hundred cycles a step, where a sorted list would be a launch of its own.
+// sum over the sequences, 64 at a time: a hundred cycles a step with up to 64 sequences, where a sorted list would be a launch of its own.
 template <bool kKeys>
 TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows, int rank) {
   const int lane = threadIdx.x % kWaveSize;

@@ -48,6 +48,28 @@ __host__ __device__ inline int page_of(const PageTable& t, int64_t b, int64_t po
   return page >= 0 && page < t.cache_pages ? page : -1;
 }
 
+// `use` of what all lanes up to one's own have, in steps that stay within registers (rows of 16 lanes by shifts of 1, 2, 4 and 8, then a row's
+// last lane to the next row, and the 32nd to the upper half): a tenth of the time of six exchanges through LDS.  All lanes call.
+template <typename Use>
+TFK_DEVICE int wave_scan(int x, int identity, Use use) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  x = use(x, __builtin_amdgcn_update_dpp(identity, x, 0x111, 0xf, 0xf, false));
+  x = use(x, __builtin_amdgcn_update_dpp(identity, x, 0x112, 0xf, 0xf, false));
+  x = use(x, __builtin_amdgcn_update_dpp(identity, x, 0x114, 0xf, 0xf, false));
+  x = use(x, __builtin_amdgcn_update_dpp(identity, x, 0x118, 0xf, 0xf, false));
+  x = use(x, __builtin_amdgcn_update_dpp(identity, x, 0x142, 0xa, 0xf, false));
+  x = use(x, __builtin_amdgcn_update_dpp(identity, x, 0x143, 0xc, 0xf, false));
+#endif
+  return x;
+}
+TFK_DEVICE int wave_prefix(int x) {   // sum up to a lane, its own included
+  return wave_scan(x, 0, [](int a, int b) { return a + b; });
+}
+TFK_DEVICE int wave_sum(int x) { return __builtin_amdgcn_readlane(wave_prefix(x), kWaveSize - 1); }
+TFK_DEVICE int wave_max(int x) {
+  return __builtin_amdgcn_readlane(wave_scan(x, -0x7fffffff, [](int a, int b) { return max(a, b); }), kWaveSize - 1);
+}
+
 // The sequence that holds token t of packed ones, those before it ending at or in front of t: -1 in front of the first, n behind the last.
 // A wavefront looks at 64 ends at a time (all lanes call).  Offsets that do not ascend give some number within -1 .. n.
 TFK_DEVICE int find_sequence(const int* __restrict__ offsets, int n, int t) {
