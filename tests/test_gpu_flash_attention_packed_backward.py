@@ -126,6 +126,17 @@ def test_gradients_of_different_sizes_in_one_call():
         _check([400], dtype=torch.float16, rows=(q, k, v, do * (weight if order == 1 else weight.flip(0))[:, None, None].half()))
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_an_infinite_gradient_beside_large_ones_in_fp16(causal):
+    # small ones, by which the powers of two are chosen, then one that is infinite among ones that are 2^18 times as large
+    for d in (64, 128):
+        q, k, v, do = _rows(64, 64, 2, 1, d, torch.float16, seed=d)
+        do[:32] *= 2.0 ** -8
+        do[32:] *= 2.0 ** 10
+        do[33, 1, 5] = math.inf
+        _check([64], h=2, hkv=1, d=d, causal=causal, rows=(q, k, v, do))
+
+
 def test_long_rows_of_small_weights_in_fp16():
     # weights of 2^-13, of which fp16 alone keeps ten bits less than of larger ones
     _check([4], [9000], dtype=torch.float16, causal=False, scale=0.01)

@@ -154,10 +154,12 @@ TFK_DEVICE void to_operand(const float4_t& ds, int h, typename Vec<T>::v8& f, Po
     for (int t = 0; t < 4; ++t) f[4 * h + t] = (T)ds[t];
   } else {
     const float big = fmaxf(fmaxf(__builtin_fabsf(ds[0]), __builtin_fabsf(ds[1])), fmaxf(__builtin_fabsf(ds[2]), __builtin_fabsf(ds[3])));
-    // (infinities and NaN go through as they are)
-    const bool finite = big < INFINITY;
-    if (__builtin_amdgcn_ballot_w64(finite && (big * power.up > 32768.f || (power.up == 0.f && big > 0.f))) != 0) {
-      const float largest = quad_max(finite ? big : 0.f);
+    // (infinities and NaN go through as they are, and do not count for those beside them)
+    if (__builtin_amdgcn_ballot_w64(big * power.up > 32768.f || (power.up == 0.f && big > 0.f)) != 0) {
+      float finite = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) finite = fmaxf(finite, __builtin_fabsf(ds[t]) < INFINITY ? __builtin_fabsf(ds[t]) : 0.f);
+      const float largest = quad_max(finite);
       if (largest * power.up > 32768.f || (power.up == 0.f && largest > 0.f)) {
         const float up = power_for(largest), factor = power.up == 0.f ? 1.f : up / power.up;
         power.up = up;
