@@ -5,6 +5,8 @@
 //
 // Every byte is read and written once, with nothing to share but a token's row of cos and sin: bound by HBM for prompts and by a chain of
 // dependent loads (sequence, length, page and angles, store) for a step of a few tokens.
+// 9 prompts of 77 to 2999, 32/8 heads x 128, fp16: 39 us, 5.2 TB/s (one row a thread 45, two 42, three 39, four 39); a token each of 64: 3.8 us of
+// the GPU's time.
 #include <algorithm>
 #include <limits>
 
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
 
 template <typename T, int D, bool kNeighbours, bool kVector>
 int launch_append(const AppendArgs& a, int64_t tokens, hipStream_t st) {
-  constexpr int kUnroll = 2, kRows = kThreads / (D / 8) * kUnroll;
+  constexpr int kUnroll = 3, kRows = kThreads / (D / 8) * kUnroll;
   const int rows = a.heads + 2 * a.kv_heads;
   return launch_kernel(append_kernel<T, D, kNeighbours, kVector, kUnroll>, dim3((unsigned)tokens, (unsigned)((rows + kRows - 1) / kRows)),
                        dim3(kThreads), 0, st, a);
