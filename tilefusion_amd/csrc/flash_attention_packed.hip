@@ -25,6 +25,9 @@ int check_packed(const char* who, const tf_packed_attention_t* p) {
   for (const int64_t* s : strides)
     for (int i = 0; i < 2; ++i)
       TFK_REQUIRE(s[i] >= 0 && s[i] % 8 == 0 && s[i] < (1 << 24), TF_ERR_INVALID_ARG, "%s: strides must be multiples of 8 elements, below 2^24", who);
+  // (the backward pass addresses a tile of 32 rows, whose tokens are 33 at most, in 32 bits from the first one's)
+  TFK_REQUIRE(33 * p->query_strides[0] + p->heads / p->kv_heads * p->query_strides[1] < (1ll << 31) - p->D, TF_ERR_INVALID_ARG,
+              "%s: the heads of a group must lie within 2^31 elements", who);
   TFK_REQUIRE(((reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value)) & 15) == 0,
               TF_ERR_INVALID_ARG, "%s: operands must begin at 16-byte boundaries", who);
   return TF_OK;
