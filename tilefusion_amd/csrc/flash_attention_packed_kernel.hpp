@@ -125,14 +125,10 @@ __global__ __launch_bounds__(kWavesT * 64, 1) void flash_attention_packed_kernel
   };
 
   // ---- LDS -> registers (see flash_attention.hpp for which lane holds what) ------------------
-  unsigned k_off[kKK], v_off[kDB];
-#pragma unroll
-  for (int kk = 0; kk < kKK; ++kk) k_off[kk] = lr * D * 2 + swz_k<kChunks>(lr, 4 * kk + lg) * 16;
-#pragma unroll
-  for (int db = 0; db < kDB; ++db) {
-    const int row = 4 * lg + (lr >> 2), col = db * 16 + 4 * (lr & 3);
-    v_off[db] = row * D * 2 + swz_v<kChunks>(row, col / 8) * 16 + (col % 8) * 2;
-  }
+  // (a swizzle is an exclusive or of chunk numbers: kk and db are one more of the address of the first)
+  const int v_row = 4 * lg + (lr >> 2), v_col = 4 * (lr & 3);
+  const unsigned k_off = lr * D * 2 + swz_k<kChunks>(lr, lg) * 16;
+  const unsigned v_off = v_row * D * 2 + swz_v<kChunks>(v_row, v_col / 8) * 16 + (v_col % 8) * 2 + kTileBytes;
   float4_t o_acc[kDB][kQB];
   float neg_m[kQB], l_sum[kQB];   // minus a row's reference; this lane's part of its weights' sum
   bool unset[kQB];                // no score above -inf seen yet
@@ -149,7 +145,7 @@ __global__ __launch_bounds__(kWavesT * 64, 1) void flash_attention_packed_kernel
   V8 pb[kJ][kQB];  // weights, B operand of the second product
   auto stage_of = [&](int it) __attribute__((always_inline)) { return smem_base + (it % kStages) * kStageBytes; };
   auto k_reads = [&](int buf, int it, int kk) __attribute__((always_inline)) {
-    const unsigned ka = opaque(stage_of(it) + k_off[kk]);
+    const unsigned ka = opaque((stage_of(it) + k_off) ^ (kk << 6));
 #pragma unroll
     for (int kb = 0; kb < kKB; ++kb) kf[buf][kb] = lds_read_b128<V8>(ka + kb * 16 * D * 2);
   };
@@ -165,7 +161,7 @@ __global__ __launch_bounds__(kWavesT * 64, 1) void flash_attention_packed_kernel
   };
   auto v_reads = [&](int it, int j) __attribute__((always_inline)) {
 #pragma unroll
-    for (int db = 0; db < kDB; ++db) vf[j][db] = v_frag(opaque(stage_of(it) + v_off[db]) + kTileBytes, j);
+    for (int db = 0; db < kDB; ++db) vf[j][db] = v_frag(opaque((stage_of(it) + v_off) ^ (db << 5)), j);
   };
   // S^T = K Q^T; the fragments of step 0 are on their way.  req_tile >= 0: its requests go out between the products.
   auto qk_tile = [&](int it, int req_tile, auto lean_c) __attribute__((always_inline)) {
@@ -175,7 +171,7 @@ __global__ __launch_bounds__(kWavesT * 64, 1) void flash_attention_packed_kernel
       for (int qb = 0; qb < kQB; ++qb) s[kb][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < kKK; ++kk) {
-      const unsigned ka = kk + 1 < kKK ? opaque(stage_of(it) + k_off[kk + 1 < kKK ? kk + 1 : 0]) : 0u;
+      const unsigned ka = kk + 1 < kKK ? opaque((stage_of(it) + k_off) ^ ((kk + 1) << 6)) : 0u;
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kb = 0; kb < kKB; ++kb) {
