@@ -62,16 +62,14 @@ def test_lengths(dtype, d, causal, lengths):
     _check(lengths, d=d, dtype=dtype, causal=causal, tail=5)
 
 
-def _rows_of(tokens, sequences, h, hkv):
-    return _capi.load().tf_flash_attention_packed_rows(tokens, sequences, h, hkv)
-
-
-@pytest.mark.parametrize("rows,lengths,h,hkv", [(64, [100, 31], 4, 2), (128, [700, 300, 41, 200], 32, 8), (256, [1500, 4, 1200], 32, 8),
-                                                (256, [4100], 16, 16), (128, [130] * 40, 8, 8), (256, [2049, 2047], 40, 8)])
+# rows of a workgroup for D = 64 and 128
+@pytest.mark.parametrize("rows,lengths,h,hkv", [((64, 64), [100, 31], 4, 2), ((64, 128), [500, 300, 41], 32, 8), ((256, 256), [700, 300, 41, 200], 32, 8),
+                                                ((256, 256), [1500, 4, 1200], 32, 8), ((256, 256), [4100], 16, 16), ((128, 128), [130] * 40, 8, 8),
+                                                ((256, 256), [2049, 2047], 40, 8)])
 @pytest.mark.parametrize("causal", [False, True])
 def test_every_kernel(rows, lengths, h, hkv, causal):
-    assert _rows_of(sum(lengths), len(lengths), h, hkv) == rows
-    for d in (64, 128):
+    for d, n in zip((64, 128), rows):
+        assert _capi.load().tf_flash_attention_packed_rows(sum(lengths), len(lengths), h, hkv, d) == n
         for dtype in (torch.float16, torch.bfloat16):
             _check(lengths, h=h, hkv=hkv, d=d, dtype=dtype, causal=causal)
 

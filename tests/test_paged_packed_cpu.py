@@ -128,8 +128,13 @@ def test_parts_of_the_gradients_rows():
 
 def test_rows_of_a_workgroup():
     rows = _capi.load().tf_flash_attention_packed_rows
-    assert rows(100, 4, 4, 2) == 64 and rows(2000, 14, 32, 8) == 256 and rows(16384, 1, 32, 8) == 256 and rows(5000, 40, 8, 8) == 128
-    assert rows(-1, 1, 4, 2) == 0 == rows(10, 1, 3, 2) == rows(10, 1, 4, 0) and rows(0, 0, 4, 2) == 64
+    for d in (64, 128):
+        assert rows(100, 4, 4, 2, d) == 64 and rows(2000, 14, 32, 8, d) == 256 == rows(16384, 1, 32, 8, d) and rows(5200, 40, 8, 8, d) == 128
+        # short texts leave most of a large tile empty
+        assert rows(3000, 1000, 8, 8, d) == 64 and rows(30000, 300, 8, 8, d) == 128
+    # one round of workgroups: 64 rows for two on a CU (D = 64) or one
+    assert rows(800, 1, 32, 8, 64) == 64 and rows(800, 1, 32, 8, 128) == 128 and rows(512, 1, 32, 8, 128) == 64
+    assert rows(-1, 1, 4, 2, 64) == 0 == rows(10, 1, 3, 2, 64) == rows(10, 1, 4, 0, 64) == rows(10, 1, 4, 2, 96) and rows(0, 0, 4, 2, 64) == 64
 
 
 def test_pages_and_divisions():

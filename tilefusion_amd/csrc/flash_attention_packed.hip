@@ -1,6 +1,7 @@
 // Attention over packed sequences: the C entry points, and which instance of the kernels a call runs.
 #include <algorithm>
 
+#include "flash_attention.hpp"
 #include "flash_attention_packed.hpp"
 
 namespace tfk {
@@ -38,11 +39,15 @@ PackedArgs packed_args(const tf_packed_attention_t& p) {
           (int)p.value_strides[1], nullptr};
 }
 
-// Rows per workgroup, from the sequences' mean length, which is all that the host knows.
-int packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads) {
-  const int64_t mean = sequences > 0 ? tokens / sequences * (heads / kv_heads) : 0, all = tokens * heads;
-  if (mean >= 512 && all / 256 + sequences / 2 * kv_heads >= 256) return 256;
-  if (mean >= 96 && all / 128 + sequences / 2 * kv_heads >= 256) return 128;
+// Rows per workgroup, from the sequences' mean length, which is all that the host knows of them.  A tile of 64 keys takes 1.45 us with 256 rows, 1.0 with
+// 128 and 0.77 with 64 (D = 128), and a CU has room for one workgroup (two with 64 rows and D = 64): the largest for which the next smaller
+// one would go round more than once, or whose rows sequences fill.  us with 256 / 128 / 64 rows, 32 heads x 128: 858 tokens behind 6000 keys 144 / 102 / 147, 512
+// of them 148 / 102 / 79; 60 texts of 20 to 400 in groups of 4 heads 70 / 86 / 121; 37 of 1 to 300, 16/4 heads x 64: 12.1 / 9.8 / 10.9.
+int packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t D) {
+  const int64_t mean = sequences > 0 ? tokens / sequences * (heads / kv_heads) : 0;
+  const auto tiles = [&](int64_t rows) { return tokens * heads / rows + sequences / 2 * kv_heads; };
+  if (tiles(128) > kCUs && mean >= 256) return 256;
+  if (tiles(64) > (D == 64 ? 2 : 1) * kCUs && mean >= 64) return 128;
   return 64;
 }
 
@@ -65,7 +70,7 @@ extern "C" int tf_flash_attention_packed(const tf_packed_attention_t* p, void* o
   if (p->tokens == 0) return TF_OK;
   TFK_REQUIRE(out && (reinterpret_cast<uintptr_t>(out) & 15) == 0, TF_ERR_INVALID_ARG, "%s: out must begin at a 16-byte boundary", who);
   PackedCall c = {p->query, p->key, p->value, out, packed_args(*p), (float)(p->softmax_scale * 1.4426950408889634), p->dtype == TF_DTYPE_BF16,
-                  p->causal != 0, packed_rows(p->tokens, p->sequences, p->heads, p->kv_heads), static_cast<hipStream_t>(stream)};
+                  p->causal != 0, packed_rows(p->tokens, p->sequences, p->heads, p->kv_heads, p->D), static_cast<hipStream_t>(stream)};
   c.args.lse = lse;
   return p->D == 128 ? run_attention_packed_d128(c) : run_attention_packed_d64(c);
 }
@@ -97,7 +102,7 @@ extern "C" int tf_flash_attention_packed_backward(const tf_packed_attention_t* p
   return p->D == 128 ? run_attention_packed_backward_d128(c) : run_attention_packed_backward_d64(c);
 }
 
-extern "C" int tf_flash_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads) {
-  if (tokens < 0 || sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0) return 0;
-  return tfk::packed_rows(tokens, sequences, heads, kv_heads);
+extern "C" int tf_flash_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t D) {
+  if (tokens < 0 || sequences < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || (D != 64 && D != 128)) return 0;
+  return tfk::packed_rows(tokens, sequences, heads, kv_heads, D);
 }
