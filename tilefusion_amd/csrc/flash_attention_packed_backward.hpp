@@ -142,39 +142,46 @@ TFK_DEVICE void store_transposed(const float4_t (&acc)[kDB], float factor, T* to
   }
 }
 
-// What a lane's dS were multiplied by so far (fp16).
+// What a lane's dS are multiplied by (fp16): at first as much as numbers can be, so that nothing has to be known of whether there were any.
 struct Power {
-  float up = 0.f;   // 0: nothing but zeros seen
+  float up = 0x1p100f;
 };
-// Four dS of a lane, times its power of two, into half `h` of an operand whose first half may be there; `acc` are the sums that hold it.
-template <typename T, int kDB>
-TFK_DEVICE void to_operand(const float4_t& ds, int h, typename Vec<T>::v8& f, Power& power, float4_t (&acc)[kDB]) {
-  if constexpr (std::is_same_v<T, bf16_t>) {
+// Four dS of a lane for each of kN operands, times its power of two, into halves `h`, of which the first may be there; `acc` are the sums that hold them.
+// (One question for all of them: in fp16 every branch here parts the products in front of it from those behind.)
+template <typename T, int kN, int kDB>
+TFK_DEVICE void to_operands(const float4_t (&ds)[kN], int h, typename Vec<T>::v8 (&f)[kN], Power (&power)[kN], float4_t (&acc)[kN][kDB]) {
+  if constexpr (!std::is_same_v<T, bf16_t>) {
+    bool beyond = false;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) f[4 * h + t] = (T)ds[t];
-  } else {
-    const float big = fmaxf(fmaxf(__builtin_fabsf(ds[0]), __builtin_fabsf(ds[1])), fmaxf(__builtin_fabsf(ds[2]), __builtin_fabsf(ds[3])));
-    // (infinities and NaN go through as they are, and do not count for those beside them)
-    if (__builtin_amdgcn_ballot_w64(big * power.up > 32768.f || (power.up == 0.f && big > 0.f)) != 0) {
-      float finite = 0.f;
+    for (int n = 0; n < kN; ++n) {
+      const float4_t& d = ds[n];
+      beyond |= fmaxf(fmaxf(__builtin_fabsf(d[0]), __builtin_fabsf(d[1])), fmaxf(__builtin_fabsf(d[2]), __builtin_fabsf(d[3]))) * power[n].up > 32768.f;
+    }
+    if (__builtin_amdgcn_ballot_w64(beyond) != 0) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) finite = fmaxf(finite, __builtin_fabsf(ds[t]) < INFINITY ? __builtin_fabsf(ds[t]) : 0.f);
-      const float largest = quad_max(finite);
-      if (largest * power.up > 32768.f || (power.up == 0.f && largest > 0.f)) {
-        const float up = power_for(largest), factor = power.up == 0.f ? 1.f : up / power.up;
-        power.up = up;
+      for (int n = 0; n < kN; ++n) {
+        // (infinities and NaN go through as they are, and do not count for those beside them)
+        float finite = 0.f;
 #pragma unroll
-        for (int db = 0; db < kDB; ++db) acc[db] *= factor;
-        if (h == 1) {
+        for (int t = 0; t < 4; ++t) finite = fmaxf(finite, __builtin_fabsf(ds[n][t]) < INFINITY ? __builtin_fabsf(ds[n][t]) : 0.f);
+        const float largest = quad_max(finite);
+        if (largest * power[n].up > 32768.f) {
+          const float up = power_for(largest), factor = up / power[n].up;
+          power[n].up = up;
 #pragma unroll
-          for (int t = 0; t < 4; ++t) f[t] = (T)((float)f[t] * factor);
+          for (int db = 0; db < kDB; ++db) acc[n][db] *= factor;
+          if (h == 1) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) f[n][t] = (T)((float)f[n][t] * factor);
+          }
         }
       }
     }
-    const float by = power.up == 0.f ? 1.f : power.up;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) f[4 * h + t] = (T)(ds[t] * by);
   }
+#pragma unroll
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) f[n][4 * h + t] = (T)(std::is_same_v<T, bf16_t> ? ds[n][t] : ds[n][t] * power[n].up);
 }
 
 template <int D>
@@ -288,6 +295,7 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
         for (int kb = 0; kb < kKB; ++kb) dp[kb] = mfma_t<T>(o, vf[kb][kk], dp[kb]);
         if (kk % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // (more of them ahead cost registers that there are not)
       }
+      float4_t ds[kKB];
       // rows 16 rb + 4 lg + r: their lse and delta
       float base[4], delta[4];
 #pragma unroll
@@ -298,7 +306,6 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
       }
 #pragma unroll
       for (int kb = 0; kb < kKB; ++kb) {
-        float4_t ds;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float p = __builtin_amdgcn_exp2f(fmaf(s[kb][r], g.scale_log2, base[r])), d = p * (dp[kb][r] - delta[r]);
@@ -310,10 +317,10 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
             d = sees ? d : 0.f;
           }
           pf[kb][4 * rb + r] = (T)p;
-          ds[r] = d;
+          ds[kb][r] = d;
         }
-        to_operand<T, kDB>(ds, rb, sf[kb], power[kb], dk[kb]);
       }
+      to_operands<T, kKB, kDB>(ds, rb, sf, power, dk);
       __builtin_amdgcn_sched_barrier(0);
     }
     // Infinities and NaN in rows that a part of the keys does not see (there a weight of zero would make NaN of them) are taken out of the products.  Of Q
@@ -395,7 +402,7 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
     if (g.parts > 1) {
       const int key = key0 + 16 * (kGradWaves * kb + wave) + lr;
       if (key >= tile.lkv) continue;
-      const float down_k = std::is_same_v<T, bf16_t> || power[kb].up == 0.f ? 1.f : 1.f / power[kb].up;
+      const float down_k = std::is_same_v<T, bf16_t> ? 1.f : 1.f / power[kb].up;
       const size_t all = (size_t)a.kv_tokens * a.kv_heads * D, at = ((size_t)(tile.k0 + key) * a.kv_heads + head) * D + 4 * lg;
       float* to = g.partial + 2 * part * all + at;
 #pragma unroll
@@ -412,10 +419,8 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
     float down = g.scale * kDownP;
     if constexpr (!std::is_same_v<T, bf16_t>) {
       // (in two steps: the power alone may be beyond what is left of fp32's range)
-      if (power[kb].up != 0.f) {
 #pragma unroll
-        for (int db = 0; db < kDB; ++db) dk[kb][db] *= 1.f / power[kb].up;
-      }
+      for (int db = 0; db < kDB; ++db) dk[kb][db] *= 1.f / power[kb].up;
     }
     store_transposed<T, kDB>(dk[kb], down, grad_key + at, there);
     store_transposed<T, kDB>(dv[kb], kDownP, grad_value + at, there);
@@ -513,9 +518,9 @@ TFK_DEVICE void grad_queries(const GradArgs& g, char* smem, int group_no, int gr
 #pragma unroll
         for (int qb = 0; qb < kQB; ++qb) dp[qb] = mfma_t<T>(v, of[qb][kk], dp[qb]);
       }
+      float4_t ds[kQB];
 #pragma unroll
       for (int qb = 0; qb < kQB; ++qb) {
-        float4_t ds;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float d = __builtin_amdgcn_exp2f(fmaf(s[qb][r], g.scale_log2, base[qb])) * (dp[qb][r] - delta[qb]);
@@ -523,10 +528,10 @@ TFK_DEVICE void grad_queries(const GradArgs& g, char* smem, int group_no, int gr
             odd = fmaf(s[qb][r], 0.f, odd);
             if (t * kGradTile + 16 * kb + 4 * lg + r > limit[qb]) d = 0.f;
           }
-          ds[r] = d;
+          ds[qb][r] = d;
         }
-        to_operand<T, kDB>(ds, kb, sf[qb], power[qb], dq[qb]);
       }
+      to_operands<T, kQB, kDB>(ds, kb, sf, power, dq);
     }
     // Infinities and NaN in keys that a part of the rows does not see are taken out of the product: the rows that see them have NaN weights.
     bool found = false;
@@ -567,10 +572,8 @@ TFK_DEVICE void grad_queries(const GradArgs& g, char* smem, int group_no, int gr
     float down = g.scale;
     if constexpr (!std::is_same_v<T, bf16_t>) {
       down *= 1.f / 32768.f;
-      if (power[qb].up != 0.f) {
 #pragma unroll
-        for (int db = 0; db < kDB; ++db) dq[qb][db] *= 1.f / power[qb].up;
-      }
+      for (int db = 0; db < kDB; ++db) dq[qb][db] *= 1.f / power[qb].up;
     }
     store_transposed<T, kDB>(dq[qb], down, grad_query + at_head + ((size_t)token * a.heads + hg) * D, there);
   }
