@@ -187,6 +187,13 @@ TFK_DEVICE void to_operands(const float4_t (&ds)[kN], int h, typename Vec<T>::v8
 template <int D>
 constexpr int grad_stage_bytes() { return 2 * kGradTile * D * 2 + kGradTile * 16; }
 constexpr int kGradStages = 4;
+// Fragments of a wavefront's own values that stay in LDS behind the ring and are read again for each 16 rows: in fp16 with D = 128 the powers of two leave too few
+// registers for all of them, and what the compiler put into scratch instead was fetched in front of a wait for every request of the ring
+// (4 x 2048 x 32 heads: 787 us, 672 so).  Two workgroups share a CU's LDS, which has room for three.
+template <typename T, int D>
+constexpr int kGradHeld = std::is_same_v<T, bf16_t> || D < 128 ? 0 : 3;
+template <typename T, int D>
+constexpr int grad_lds_bytes() { return kGradStages * grad_stage_bytes<D>() + kGradWaves * kGradHeld<T, D> * 1024; }
 
 // ---- dK and dV of 128 keys ------------------------------------------------------------------------
 // `group_no` of `groups` workgroups.
@@ -230,6 +237,11 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
       vf[kb][kk] = *reinterpret_cast<const V8*>(v + 32 * kk + 8 * lg);
     }
   }
+  constexpr int kHeld = kGradHeld<T, D>;   // the last ones of the last block
+  const unsigned smem_base = lds_address(smem), held = smem_base + kGradStages * kStage + wave * kHeld * 1024;
+  auto held_at = [&]() __attribute__((always_inline)) { return held + opaque((unsigned)tid & 63u) * 16; };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) *(__attribute__((address_space(3))) V8*)(size_t)(held_at() + i * 1024) = vf[kKB - 1][kKK - kHeld + i];
   const int tiles = (rows + kGradTile - 1) / kGradTile;
   const int all_first = kCausal ? min(tiles, max(key0 - shift, 0) * group / kGradTile) : 0;
   // of the tiles that see these keys, this part's
@@ -239,7 +251,6 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
   const int n_masked = min(tiles, (last_min + kGradTile - 1) / kGradTile), n_full = rows / kGradTile;
   const int first_min = __builtin_amdgcn_readfirstlane(kCausal ? max(key0 + 16 * wave - shift, 0) * group : 0);
 
-  const unsigned smem_base = lds_address(smem);
   auto request_tile = [&](int t) __attribute__((always_inline)) {
     const unsigned stage = smem_base + t % kGradStages * kStage;
     const int lane = (int)opaque((unsigned)tid & 63u);   // (what follows from it is made again for each tile: registers are short)
@@ -280,6 +291,7 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
     }
     [[maybe_unused]] float odd = 0.f;   // NaN where a score or dP is not finite, as all are of a row of Q or dO with an infinity or a NaN
     const unsigned row_at = opaque(stage + off.row), column_at = opaque(stage + off.column);
+    [[maybe_unused]] const unsigned held_from = kHeld > 0 ? held_at() : 0u;
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
       float4_t s[kKB], dp[kKB];
@@ -292,7 +304,8 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
 #pragma unroll
         for (int kb = 0; kb < kKB; ++kb) s[kb] = mfma_t<T>(q, kf[kb][kk], s[kb]);
 #pragma unroll
-        for (int kb = 0; kb < kKB; ++kb) dp[kb] = mfma_t<T>(o, vf[kb][kk], dp[kb]);
+        for (int kb = 0; kb < kKB; ++kb)
+          dp[kb] = mfma_t<T>(o, kb == kKB - 1 && kk >= kKK - kHeld ? lds_read_b128<V8>(held_from + (kk - kKK + kHeld) * 1024) : vf[kb][kk], dp[kb]);
         if (kk % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // (more of them ahead cost registers that there are not)
       }
       float4_t ds[kKB];
@@ -376,7 +389,10 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
 #pragma unroll
     for (int kb = 0; kb < kKB; ++kb)
 #pragma unroll
-      for (int kk = 0; kk < kKK; ++kk) asm volatile("" : "+v"(kf[kb][kk]), "+v"(vf[kb][kk]));   // (waited for here, not among the tiles)
+      for (int kk = 0; kk < kKK; ++kk) {   // (waited for here, not among the tiles)
+        asm volatile("" : "+v"(kf[kb][kk]));
+        if (kb < kKB - 1 || kk < kKK - kHeld) asm volatile("" : "+v"(vf[kb][kk]));
+      }
 #pragma unroll
     for (int t = 0; t < kGradStages - 1; ++t) request_tile(first + t);
     auto next_tile = [&](int t) __attribute__((always_inline)) {
@@ -554,11 +570,18 @@ TFK_DEVICE void grad_queries(const GradArgs& g, char* smem, int group_no, int gr
     }
 #pragma unroll
     for (int t = 0; t < kGradStages - 1; ++t) request_tile(t);
-    for (int t = 0; t < tiles; ++t) {
+    auto next_tile = [&](int t) __attribute__((always_inline)) {
       barrier_keep_vmem<(kGradStages - 2) * kRequests>();   // tile t has landed, tile t-1 has been read
       request_tile(t + kGradStages - 1);
-      if (t < n_plain) compute(t, std::false_type{});
-      else if (t < n_compute) compute(t, std::true_type{});
+    };
+    int t = 0;
+    for (; t < min(n_plain, tiles); ++t) {
+      next_tile(t);
+      compute(t, std::false_type{});
+    }
+    for (; t < tiles; ++t) {
+      next_tile(t);
+      if (t < n_compute) compute(t, std::true_type{});
     }
     wait_vmem_all();
   }
@@ -623,7 +646,8 @@ int launch_grad(GradArgs g, hipStream_t st) {
   const bool of_keys = g.grad_key && a.kv_tokens > 0, of_queries = g.grad_query && a.tokens > 0;
   constexpr int kKB = 2, kQB = 2;
   auto kern = packed_grad_kernel<T, D, kCausal, kKB, kQB>;
-  constexpr int lds = kGradStages * grad_stage_bytes<D>();
+  constexpr int lds = grad_lds_bytes<T, D>();
+  static_assert(2 * lds <= kMaxLdsBytes, "two workgroups do not fit in a CU's LDS");
   TFK_LDS_OPT_IN(kern, lds);
   // (rows of no sequence are cleared by whatever workgroups there are)
   g.key_groups = of_keys ? (int)std::max<int64_t>(most_tiles(a.kv_tokens, a.sequences, kGradKeys) * a.kv_heads * g.parts, 1) : 0;
