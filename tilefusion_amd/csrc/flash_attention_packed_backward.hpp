@@ -187,13 +187,14 @@ TFK_DEVICE void to_operands(const float4_t (&ds)[kN], int h, typename Vec<T>::v8
 template <int D>
 constexpr int grad_stage_bytes() { return 2 * kGradTile * D * 2 + kGradTile * 16; }
 constexpr int kGradStages = 4;
-// Fragments of a wavefront's own values that stay in LDS behind the ring and are read again for each 16 rows: in fp16 with D = 128 the powers of two leave too few
-// registers for all of them, and what the compiler put into scratch instead was fetched in front of a wait for every request of the ring
-// (4 x 2048 x 32 heads: 787 us, 672 so).  Two workgroups share a CU's LDS, which has room for three.
-template <typename T, int D>
-constexpr int kGradHeld = std::is_same_v<T, bf16_t> || D < 128 ? 0 : 3;
-template <typename T, int D>
-constexpr int grad_lds_bytes() { return kGradStages * grad_stage_bytes<D>() + kGradWaves * kGradHeld<T, D> * 1024; }
+// Fragments of a wavefront's own values that stay in LDS behind the ring and are read again for each 16 rows, with D = 128: the powers of two (fp16) and masks
+// (causal) leave too few registers for all of them, and what the compiler put into scratch instead was fetched behind a wait for every request of
+// the ring (4 x 2048 x 32 heads, causal: fp16 787 us, 672 so, bf16 523 and 504; not causal, bf16: 825 and 830).  Two workgroups share a CU's LDS, which has
+// room for three.
+template <typename T, int D, bool kCausal>
+constexpr int kGradHeld = D == 128 && (kCausal || !std::is_same_v<T, bf16_t>) ? 3 : 0;
+template <typename T, int D, bool kCausal>
+constexpr int grad_lds_bytes() { return kGradStages * grad_stage_bytes<D>() + kGradWaves * kGradHeld<T, D, kCausal> * 1024; }
 
 // ---- dK and dV of 128 keys ------------------------------------------------------------------------
 // `group_no` of `groups` workgroups.
@@ -237,7 +238,7 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
       vf[kb][kk] = *reinterpret_cast<const V8*>(v + 32 * kk + 8 * lg);
     }
   }
-  constexpr int kHeld = kGradHeld<T, D>;   // the last ones of the last block
+  constexpr int kHeld = kGradHeld<T, D, kCausal>;   // the last ones of the last block
   const unsigned smem_base = lds_address(smem), held = smem_base + kGradStages * kStage + wave * kHeld * 1024;
   auto held_at = [&]() __attribute__((always_inline)) { return held + opaque((unsigned)tid & 63u) * 16; };
 #pragma unroll
@@ -646,7 +647,7 @@ int launch_grad(GradArgs g, hipStream_t st) {
   const bool of_keys = g.grad_key && a.kv_tokens > 0, of_queries = g.grad_query && a.tokens > 0;
   constexpr int kKB = 2, kQB = 2;
   auto kern = packed_grad_kernel<T, D, kCausal, kKB, kQB>;
-  constexpr int lds = grad_lds_bytes<T, D>();
+  constexpr int lds = grad_lds_bytes<T, D, kCausal>();
   static_assert(2 * lds <= kMaxLdsBytes, "two workgroups do not fit in a CU's LDS");
   TFK_LDS_OPT_IN(kern, lds);
   // (rows of no sequence are cleared by whatever workgroups there are)
