@@ -11,6 +11,8 @@
 // first two products, whose accumulators are the second operand of the last ones as they are: a lane holds one key (row), its registers
 // four rows (keys).  The tile is read from LDS as rows and, transposed, as columns; one swizzle serves both.  Two workgroups of four wavefronts share a
 // CU, so that one's exponentials run beside the other's products.
+// 4 texts of 2048, 32/8 heads x 128, causal, bf16: 504 us, of which 28 are the first kernel's (HBM) and 475 the second's (7 products at 1.0 PFLOP/s); fp16 645.  11 texts of
+// 30 to 1001, 16/4 heads x 64, fp16: 68 us, 5 + 57 + 5.
 #pragma once
 
 #include "flash_attention.hpp"

@@ -28,7 +28,7 @@ constexpr int kBlockKeys = kWaves * kTileKeys;   // a tile each
 constexpr int tiles_ahead(int d) { return d == 128 ? 3 : 4; }   // of a wavefront, in registers: 24 or 16 KiB
 constexpr int kQueries = 16;   // of an item: one block of MFMA columns
 // Workgroups of a launch, one on a CU.  (Two of half the size: the older one is served first and is done at two thirds of the time, the other
-// goes on alone and takes in less than the CU's share.  16 of 8 heads x 32768 x 128: 321 us, as two 354.)
+// goes on alone and takes in less than the CU's share: they were done at 235 and 343 us with 16 of 8 heads x 32768 x 128.)
 constexpr int kGroups = kCUs;
 
 struct DecodeArgs {
