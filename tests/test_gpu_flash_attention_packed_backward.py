@@ -306,3 +306,24 @@ def test_refusals():
     assert nothing[0].shape == (0, 4, 64) and (nothing[1] == 0).all() and (nothing[2] == 0).all()
     nothing = ops.flash_attention_packed_backward(do, q, k[:0], v[:0], out, lse, of, torch.zeros(3, dtype=torch.int32, device=DEV))
     assert (nothing[0] == 0).all() and nothing[1].shape == (0, 2, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_no_queries_or_no_keys_at_all(dtype):
+    q, k, v, do = _rows(0, 50, 4, 2, 64, dtype)
+    of, kv = _offsets([0, 0]), _offsets([20, 30])
+    out, lse = ops.flash_attention_packed(q, k, v, of, kv, keep=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (4, 0)
+    grads = ops.flash_attention_packed_backward(do, q, k, v, out, lse, of, kv)
+    assert grads[0].shape == q.shape and (grads[1] == 0).all() and (grads[2] == 0).all()
+    q, k, v, do = _rows(50, 0, 4, 2, 64, dtype)
+    for causal in (False, True):
+        out, lse = ops.flash_attention_packed(q, k, v, kv, of, None, causal, True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+        grads = ops.flash_attention_packed_backward(do, q, k, v, out, lse, kv, of, None, causal)
+        assert (grads[0] == 0).all() and grads[1].shape == k.shape == grads[2].shape
+    # no sequence: rows of none
+    out, lse = ops.flash_attention_packed(q, q[:, :2], q[:, :2], _offsets([]), keep=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    for g in ops.flash_attention_packed_backward(do, q, q[:, :2], q[:, :2], out, lse, _offsets([])):
+        assert (g == 0).all()

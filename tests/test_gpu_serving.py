@@ -133,3 +133,24 @@ def test_a_layer_under_autograd_is_its_calls_one_by_one(dtype):
     assert torch.equal(x.grad, torch.cat(grads, dim=1))
     for a, b in zip(w, grad_w):
         assert torch.equal(a.grad, b)
+
+
+def test_compiled_calls_are_the_eager_ones():
+    server = _Server(torch.bfloat16, False)
+    server.prompts([40, 3, 0, 18])
+    _, (q, k, v) = server.projection(SLOTS)
+    lengths = server.lengths + torch.tensor([1, 1, 0, 1], dtype=torch.int32, device=DEV)
+
+    def step(q, k, v, key, value):
+        turned = ops.append_paged_kv(q, k, v, server.cos, server.sin, key, value, server.table, lengths)
+        return turned, ops.flash_decode_paged(turned, key, value, server.table, lengths)
+
+    def texts(q, k, v):
+        return ops.flash_attention_packed(q, k, v, torch.tensor([0, 1, 4], dtype=torch.int32, device=DEV))
+
+    caches = [[x.clone(memory_format=torch.preserve_format) for x in (server.key, server.value)] for _ in range(2)]
+    with torch.no_grad():
+        want, got = step(q, k, v, *caches[0]), torch.compile(step, backend="eager")(q, k, v, *caches[1])
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(*caches))
+        assert torch.equal(texts(q, k, v), torch.compile(texts, backend="eager")(q, k, v))

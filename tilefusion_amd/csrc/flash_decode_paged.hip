@@ -203,11 +203,13 @@ __global__ __launch_bounds__(kThreads, 2) void flash_decode_paged_kernel(DecodeA
     while (at < end && g.blocks == 0) {
       int keys = keys_of(a, read_uniform(a.lengths + b));
       unsigned of_item = cost_of<D>(keys);
-      while (at >= before + of_item * (unsigned)items_of) {   // (ends: the range is within the sum)
+      // (the range is within the sum; bounded all the same, for lengths that a program changes while they are read)
+      while (at >= before + of_item * (unsigned)items_of && b + 1 < a.sequences) {
         before += of_item * (unsigned)items_of;
         keys = keys_of(a, read_uniform(a.lengths + ++b));
         of_item = cost_of<D>(keys);
       }
+      if (at - before >= of_item * (unsigned)items_of) break;
       const unsigned item = (at - before) / of_item, item_begin = before + item * of_item, stop = min(item_begin + of_item, end);
       const int head = (int)item / a.blocks_of_group, query0 = (int)item % a.blocks_of_group * kQueries;
       const int first = max((int)(at - item_begin) - overhead(D), 0), last = max((int)(stop - item_begin) - overhead(D), 0);

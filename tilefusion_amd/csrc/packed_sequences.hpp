@@ -103,6 +103,7 @@ TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows, int rank) {
   tile.lq = q.length;
   tile.k0 = k.begin;
   tile.lkv = k.length;
+  if ((kKeys ? k.length : q.length) == 0) tile.sequence = -1;   // (offsets that a program changes while they are read)
   return tile;
 }
 TFK_DEVICE PackedTile packed_tile(const PackedArgs& a, int rows, int rank) { return find_tile<false>(a, rows, rank); }
