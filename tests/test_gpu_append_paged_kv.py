@@ -212,3 +212,73 @@ def test_refusals():
             ops.rotation_tables(positions, rotated, device=DEV)
     empty = ops.append_paged_kv(q[:0], k[:0], v[:0], cos, sin, cache.key, cache.value, cache.table, cache.lengths, torch.zeros(3, dtype=torch.int32, device=DEV))
     assert empty.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("through_the_dispatcher", [False, True])
+def test_autograd_sees_that_the_cache_has_changed(through_the_dispatcher):
+    # what was saved of the cache for a backward pass is not what it was: that raises, as for any change in place
+    g = torch.Generator().manual_seed(4)
+    lengths = [40, 33]
+    cache = ref.Cache(lengths, 16, 2, 64, torch.float16)
+    q, k, v = _rows(2, 4, 2, 64, torch.float16)
+    cos, sin = ops.rotation_tables(41, 64, device=DEV)
+    if through_the_dispatcher:   # (tables in pieces are made whole, which the direct call leaves to the wrapper)
+        cos, sin = (torch.cat([x, x], dim=1)[:, :32] for x in (cos, sin))
+
+    def append():
+        return ops.append_paged_kv(q, k, v, cos, sin, cache.key, cache.value, cache.table, cache.lengths, None, False, True)
+
+    for saved in (cache.key, cache.value):
+        x = torch.randn(saved[0].shape, generator=g).half().to(DEV).requires_grad_()
+        loss = (x * saved[0]).sum()
+        loss.backward(retain_graph=True)
+        append()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    # a sequence's pages, attended to where they lie
+    rows = cache.table[0, :1].long()
+    one = slice(int(rows), int(rows) + 1)
+    q1 = torch.randn(16, 4, 64, generator=g).half().to(DEV).requires_grad_()
+    offsets = _offsets([16])
+    out = ops.flash_attention_packed(q1, cache.key[one].squeeze(0), cache.value[one].squeeze(0), offsets)
+    append()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    # the inputs have not changed, and a call without tokens changes nothing
+    versions = [x._version for x in (q, k, v, cache.table, cache.lengths, cache.key, cache.value)]
+    ops.append_paged_kv(q[:0], k[:0], v[:0], cos, sin, cache.key, cache.value, cache.table, cache.lengths, torch.zeros(3, dtype=torch.int32, device=DEV))
+    assert versions == [x._version for x in (q, k, v, cache.table, cache.lengths, cache.key, cache.value)]
+    append()
+    assert versions[:5] == [x._version for x in (q, k, v, cache.table, cache.lengths)]
+
+
+def test_a_cache_of_inference_tensors():
+    # (they count no changes, inside inference mode and outside)
+    with torch.inference_mode():
+        cache = ref.Cache([40, 33], 16, 2, 64, torch.float16)
+        q, k, v = _rows(2, 4, 2, 64, torch.float16)
+        cos, sin = ops.rotation_tables(41, 64, device=DEV)
+        want = ops.append_paged_kv(q, k, v, cos, sin, cache.key, cache.value, cache.table, cache.lengths)
+        stored = cache.key.clone()
+    got = ops.append_paged_kv(q, k, v, cos, sin, cache.key, cache.value, cache.table, cache.lengths)
+    assert torch.equal(got, want) and torch.equal(cache.key.nan_to_num(), stored.nan_to_num())
+
+
+def test_results_that_a_program_hands_in_count_as_changed():
+    # torch.ops.tilefusion: the results are arguments, which may be anyone's
+    lengths = [5, 3]
+    cache = ref.Cache(lengths, 16, 2, 64, torch.float16)
+    q, k, v = _rows(2, 4, 2, 64, torch.float16)
+    cos, sin = ops.rotation_tables(41, 64, device=DEV)
+    offsets, direct = _offsets([1, 1]), torch.ops.tilefusion
+    outs = {name: torch.zeros(shape, dtype=dtype, device=DEV) for name, shape, dtype in
+            [("q", q.shape, q.dtype), ("k", k.shape, k.dtype), ("decoded", q.shape, q.dtype), ("out", q.shape, q.dtype), ("lse", (4, 2), torch.float32),
+             ("dq", q.shape, q.dtype), ("dk", k.shape, k.dtype), ("dv", k.shape, k.dtype)]}
+    before = {name: x._version for name, x in outs.items()}
+    direct.append_paged_kv(q, k, v, cos, sin, cache.key, cache.value, cache.table, cache.lengths, offsets, False, outs["q"], outs["k"])
+    direct.flash_decode_paged(q, cache.key, cache.value, cache.table, cache.lengths, 0.125, outs["decoded"])
+    direct.flash_attention_packed(q, k, v, offsets, None, 0.125, True, outs["out"], outs["lse"])
+    after_forward = {name: outs[name]._version for name in ("out", "lse")}
+    direct.flash_attention_packed_backward(q, q, k, v, outs["out"], outs["lse"], offsets, None, 0.125, True, outs["dq"], outs["dk"], outs["dv"])
+    assert all(outs[name]._version > n for name, n in before.items())
+    assert after_forward == {name: outs[name]._version for name in ("out", "lse")}

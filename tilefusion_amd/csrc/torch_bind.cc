@@ -59,6 +59,15 @@ c10::DataPtr scratch(size_t bytes, const at::Tensor& like) {
   return from->allocate(bytes);
 }
 
+// What is written is the caller's: autograd, which counts a tensor's changes and not the kernels that make them, raises where it has saved the
+// tensor, instead of going on with what is there now.  (Inference tensors count none.)
+void mark_written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void mark_written(const std::optional<at::Tensor>& t) {
+  if (t.has_value()) mark_written(*t);
+}
+
 void check_status(int status, const char* op) {
   TORCH_CHECK(status == TF_OK, "tilefusion::", op, " failed (status ", status, "): ", tf_last_error());
 }
@@ -683,6 +692,8 @@ void append_paged_kv(const at::Tensor& query, const at::Tensor& key, const at::T
                                   cos.size(0), 2 * cos.size(1), interleaved ? 1 : 0, offsets.has_value() ? offsets->data_ptr<int32_t>() : nullptr, t, h,
                                   query_out.data_ptr(), key_out.has_value() ? key_out->data_ptr() : nullptr, current_stream()),
                op);
+  for (const at::Tensor* t : {&key_cache, &value_cache, &query_out}) mark_written(*t);
+  mark_written(key_out);
 }
 
 // flash_decode_paged(query [sequences,H,D], the cache, its table and lengths -> out [sequences,H,D])
@@ -701,6 +712,7 @@ void flash_decode_paged(const at::Tensor& query, const at::Tensor& key_cache, co
   const size_t bytes = tf_flash_decode_paged_workspace_bytes(cache.sequences, h, cache.kv_heads, cache.D);
   const c10::DataPtr ws = scratch(bytes, query);
   check_status(tf_flash_decode_paged(&cache, query.data_ptr(), strides, out.data_ptr(), h, softmax_scale, ws.get(), bytes, current_stream()), op);
+  mark_written(out);
 }
 
 // ---- attention over packed sequences ------------------------------------------------------------
@@ -754,6 +766,8 @@ void flash_attention_packed(const at::Tensor& query, const at::Tensor& key, cons
   if (lse.has_value()) check_lse(*lse, p, query, op);
   const c10::DeviceGuard there(query.device());
   check_status(tf_flash_attention_packed(&p, out.data_ptr(), lse.has_value() ? lse->data_ptr<float>() : nullptr, current_stream()), op);
+  mark_written(out);
+  mark_written(lse);
 }
 
 // flash_attention_packed_backward(grad_out, query, key, value, out, lse, .. -> grad_query [T,H,D], grad_key and grad_value [S,Hkv,D]), the gradients that are
@@ -781,6 +795,7 @@ void flash_attention_packed_backward(const at::Tensor& grad_out, const at::Tenso
   check_status(tf_flash_attention_packed_backward(&p, grad_out.data_ptr(), out.data_ptr(), lse.data_ptr<float>(), at_or_null(grad_query), at_or_null(grad_key),
                                                   at_or_null(grad_value), ws.get(), bytes, current_stream()),
                op);
+  for (const auto* t : {&grad_query, &grad_key, &grad_value}) mark_written(*t);
 }
 
 }  // namespace kernels

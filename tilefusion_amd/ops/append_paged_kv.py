@@ -52,7 +52,8 @@ def append_paged_kv(
     Returns the rotated queries [tokens, heads, D], or (queries, keys).  The rotation is in fp32 and rounded once.  A token whose position has no
     page in the cache, or no row in the tables, leaves the cache as it is and its rotated rows are NaN; tokens of no sequence (behind
     offsets[-1], or of one that is shorter than its new tokens, as an idle slot of length 0) leave it as it is too, and their rows are zero.  Pages that
-    new tokens go to belong to one sequence.  There is no gradient."""
+    new tokens go to belong to one sequence.  There is no gradient; the caches count as changed in place, so that a backward pass that has saved
+    some of them raises."""
     if not torch.compiler.is_compiling():
         direct = _direct.append_paged_kv(
             query, key, value, cos, sin, key_cache, value_cache, page_table, lengths, offsets, interleaved, keep
