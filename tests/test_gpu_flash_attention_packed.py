@@ -219,3 +219,43 @@ def test_refusals():
     assert ops.flash_attention_packed(q[:0], k[:0], v[:0], torch.zeros(3, dtype=torch.int32, device=DEV)).shape == (0, 4, 64)
     out = ops.flash_attention_packed(q, k[:0], v[:0], offsets, torch.zeros(3, dtype=torch.int32, device=DEV))
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("ahead,n", [(20.6, 60001), (25.5, 200001)])
+@pytest.mark.parametrize("m,h,hkv,d", [(1, 1, 1, 64), (5, 6, 1, 128), (2500, 8, 8, 128), (4200, 8, 8, 64), (4200, 8, 8, 128)])
+def test_weights_far_below_the_largest_count_in_fp16(ahead, n, m, h, hkv, d):
+    # one key ahead of equal ones by 20.6 or 25.5 (in units of log2), whose weights are together 4% or 0.4% of the sum: among those of a row whose
+    # largest is 1 fp16 has 2^-20.6 only to 4%, and nothing for 2^-25.5
+    rows = _capi.load().tf_flash_attention_packed_rows(m, 1, h, hkv, d)
+    assert rows == {1: 64, 5: 64, 2500: 128, 4200: 256}[m]
+    key, value = torch.zeros(n, hkv, d), torch.ones(n, hkv, d)
+    key[n // 3, :, 0], value[n // 3] = ahead, -1.0
+    q = torch.zeros(m, h, d)
+    q[..., 0] = 1.0
+    q, key, value = (x.half().to(DEV) for x in (q, key, value))
+    out, lse = ops.flash_attention_packed(q, key, value, _offsets([m]), _offsets([n]), math.log(2.0), False, True)
+    # all rows, heads and columns are one number
+    score = key[:, 0, 0].double() * math.log(2.0)
+    p = torch.softmax(score, 0)
+    v = value[:, 0, 0].double()
+    want, want_lse = (p * v).sum(), torch.logsumexp(score, 0)
+    # Relative errors of weights move the result by their part of sum p |v - out|: a rounding of 2^-11, exp2 and its argument 2^-20, the score's (one product that is not
+    # zero, scaled) 2^-22 of it.  Below fp16's normal numbers a rounding is of 2^-25, with the largest at 2^7 or more 2^-32 of that.  Sums in fp32: a tile of 64
+    # after the other, whose parts are added as a tree or by the product in two steps, so n / 32 + 64 roundings of 2^-24 at most.
+    distance = (v - want).abs()
+    sums = (n / 32 + 64) * 2.0 ** -24
+    bound = 2.0 ** -11 * want.abs() + 2.01 * ((2.0 ** -11 + 2.0 ** -20 + ahead * 2.0 ** -22) * (p * distance).sum() + 2.0 ** -32 * p.max() * distance.sum() + sums)
+    ref.assert_within(out, want.expand_as(out), bound.expand_as(out), "out")
+    ref.assert_within(lse, want_lse.expand_as(lse), torch.full_like(lse, sums + (1.0 + ahead) * 2.0 ** -21), "lse")
+
+
+def test_weights_far_above_the_first_in_fp16():
+    # the first keys' scores set a reference that those behind them exceed by up to 8, which does not raise it, and by more: weights stay within the type
+    for rise in (1.0, 7.9, 8.0, 8.1, 15.0, 40.0):
+        q, k, v = _rows(300, 300, 2, 1, 64, torch.float16)
+        k.mul_(0.01)
+        k[200:, 0, 0] = rise
+        q[:, :, 0] = 1.0
+        v[250:, 0, 1] = 60000.0
+        for causal in (False, True):
+            _check([300], h=2, hkv=1, dtype=torch.float16, causal=causal, scale=math.log(2.0), rows=(q, k, v))

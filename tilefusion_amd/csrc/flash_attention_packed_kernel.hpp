@@ -203,8 +203,9 @@ __global__ __launch_bounds__(kWavesT * 64, 1) void flash_attention_packed_kernel
           if constexpr (decltype(mask_c)::value)
             if (it * kBN + kb * 16 + 4 * lg + r > limit[qb]) s[kb][qb][r] = -INFINITY;
         }
-    // The reference is raised when some score is more than kLazy (log2 units) above it; weights reach 2^kLazy until then.
-    constexpr float kLazy = 8.f;
+    // The reference is set 2^kUp below the largest score and raised when some score is more than kLazy (log2 units) above it; weights reach 2^kLazy until
+    // then.  In fp16, whose smallest number is 2^-24, a weight's smallest step is so 2^-31 of the largest weight or less; bf16 has the range.
+    constexpr float kUp = std::is_same_v<T, bf16_t> ? 0.f : 7.f, kLazy = kUp + 8.f;
     float mx[kQB];
     bool grow = false;
 #pragma unroll
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(kWavesT * 64, 1) void flash_attention_packed_kernel
 #pragma unroll
       for (int qb = 0; qb < kQB; ++qb) {
         const float qmax = quad_max(mx[qb]);
-        float shift_m = unset[qb] ? qmax : fmaxf(0.f, qmax);
+        float shift_m = unset[qb] ? qmax - kUp : fmaxf(0.f, qmax - kUp);
         const float alpha = unset[qb] ? 1.f : __builtin_amdgcn_exp2f(-shift_m);
         if (unset[qb] && qmax == -INFINITY) shift_m = 0.f;
         else unset[qb] = false;
