@@ -322,8 +322,8 @@ TF_API int tf_flash_decode_paged(const tf_paged_cache_t* cache, const void* quer
                                  double softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Attention over sequences packed one behind the other.  query [tokens, heads, D], key and value [kv_tokens, kv_heads, D] of dtype (fp16 or bf16), D 64
- * or 128; head h attends head h / (heads / kv_heads) of the keys; strides in elements from token to token and head to head, multiples of 8 below
- * 2^24, the heads of a group within 2^31 elements, 16-byte boundaries.  offsets and kv_offsets [sequences + 1] int32 in device memory, ascending: sequence b is queries offsets[b] .. offsets[b+1] - 1
+ * or 128; head h attends head h / (heads / kv_heads) of the keys; strides in elements from token to token, below 2^24, and from head to head, below 2^40, all
+ * multiples of 8; the heads of query that share a head of keys within 2^31 elements; 16-byte boundaries.  offsets and kv_offsets [sequences + 1] int32 in device memory, ascending: sequence b is queries offsets[b] .. offsets[b+1] - 1
  * and keys kv_offsets[b] .. kv_offsets[b+1] - 1 (null: the same as the queries).  What they name beyond the tensors is cut off.  causal: query i of a
  * sequence of m queries and n keys sees keys up to i + n - m, the last one all.  tokens and kv_tokens < 2^24.  (No counterpart in the reference, whose attention has one
  * length and one head count, include/kernels/ops.hpp:47-52.) */

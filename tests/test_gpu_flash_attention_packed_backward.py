@@ -327,3 +327,36 @@ def test_no_queries_or_no_keys_at_all(dtype):
     assert (out == 0).all() and (lse == -math.inf).all()
     for g in ops.flash_attention_packed_backward(do, q, q[:, :2], q[:, :2], out, lse, _offsets([])):
         assert (g == 0).all()
+
+
+def _spread(x, token, head):
+    """x with rows `token` and heads `head` elements apart, in memory that is not touched otherwise."""
+    n, h, d = x.shape
+    y = torch.empty((n - 1) * token + (h - 1) * head + d, dtype=x.dtype, device=DEV).as_strided(x.shape, (token, head, 1))
+    return y.copy_(x)
+
+
+# heads of keys as far apart as those of 2^17 tokens x 128, beyond 32 bits, and heads of queries that are copied (2^31 elements in a group)
+@pytest.mark.parametrize("h,hkv,of_query,of_keys", [(4, 2, 1 << 24, 1 << 24), (4, 4, 1 << 30, 1 << 30), (4, 2, 1 << 30, 1 << 31), (2, 2, 64, 1 << 32)])
+def test_heads_far_from_each_other(h, hkv, of_query, of_keys):
+    for d, dtype in ((64, torch.float16), (128, torch.bfloat16)):
+        q, k, v, do = _rows(170, 170, h, hkv, d, dtype)
+        of = _offsets([100, 70])
+        far = _spread(q, d, max(of_query, 170 * d)), _spread(k, d, of_keys), _spread(v, d, of_keys)
+        out, lse = ops.flash_attention_packed(q, k, v, of, keep=True)
+        for own in (far, (far[0], k, v), (q, *far[1:])):
+            assert all(torch.equal(a, b) for a, b in zip(ops.flash_attention_packed(*own, of, keep=True), (out, lse)))
+            got = ops.flash_attention_packed_backward(do, *own, out, lse, of)
+            assert all(torch.equal(a, b) for a, b in zip(got, ops.flash_attention_packed_backward(do, q, k, v, out, lse, of)))
+        leaves = [x.detach().requires_grad_() for x in far]
+        ops.flash_attention_packed(*leaves, of).backward(do)
+        assert all(torch.equal(x.grad, g) for x, g in zip(leaves, got))
+        del far, own, leaves
+
+
+def test_tokens_far_from_each_other():
+    # further apart than 32-bit offsets reach within a tile: copied
+    q, k, v, do = _rows(40, 40, 2, 1, 64, torch.bfloat16)
+    of = _offsets([25, 15])
+    want = ops.flash_attention_packed(q, k, v, of)
+    assert torch.equal(ops.flash_attention_packed(_spread(q, 1 << 24, 64), _spread(k, 1 << 25, 64), _spread(v, 1 << 24, 64), of), want)

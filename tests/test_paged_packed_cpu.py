@@ -246,3 +246,46 @@ def test_the_comparison_passes_its_own_rounding_and_sees_mistakes(dtype):
     # a turn keeps a pair's length, and the product of two turned by one angle
     pairs = lambda y: y[..., :16] ** 2 + y[..., 16:32] ** 2
     torch.testing.assert_close(pairs(turned), pairs(x.double()), rtol=1e-6, atol=1e-6)
+
+
+def test_heads_of_packed_operands_lie_anywhere():
+    # a [heads, tokens, D] of 2^17 tokens x 128, turned: heads 2^24 elements apart.  (What is refused in these calls is another argument, so that none runs.)
+    lib = _capi.load()
+    size = lib.tf_flash_attention_packed_backward_workspace_bytes
+
+    def refused(message, **changed):
+        p = _packed(**changed)
+        for status in (lib.tf_flash_attention_packed(p, P + 8, P, None),
+                       lib.tf_flash_attention_packed_backward(p, P, P, P, P + 8, P, P, P, size(p), None)):
+            assert status == BAD and message in lib.tf_last_error(), (changed, lib.tf_last_error())
+
+    far = 1 << 24
+    for name in ("query_strides", "key_strides", "value_strides"):
+        refused(b"boundar", **{name: _i64(128, far)})
+        refused(b"boundar", **{name: _i64(128, far)}, D=128)
+        refused(b"strides", **{name: _i64(far, 128)})
+        refused(b"strides", **{name: _i64(128, far + 4)})
+        refused(b"strides", **{name: _i64(128, -far)})
+        refused(b"strides", **{name: _i64(128, 1 << 40)})
+    for name in ("key_strides", "value_strides"):
+        refused(b"boundar", **{name: _i64(128, 1 << 34)})
+    # the heads of a group are reached from one another in 32 bits, one head alone is not
+    refused(b"within 2^31", query_strides=_i64(128, 1 << 30))
+    refused(b"boundar", query_strides=_i64(128, 1 << 30), heads=2)
+    refused(b"boundar", query_strides=_i64(128, 1 << 34), heads=2)
+
+
+def test_the_wrapper_copies_what_the_kernels_do_not_reach():
+    from tilefusion_amd.ops.flash_attention_packed import _within_reach
+
+    def rows(n, heads, token, head):
+        return torch.empty((n - 1) * token + (heads - 1) * head + 64, dtype=torch.float16).as_strided((n, heads, 64), (token, head, 1))
+
+    near = rows(2, 2, 128, 64)
+    for q, k, copied in ((near, near, (False, False)), (rows(2, 2, 64, 1 << 24), near, (False, False)), (rows(2, 2, 64, 1 << 24), rows(2, 2, 64, 1 << 24), (False, False)),
+                         (rows(2, 2, 1 << 24, 64), near, (True, False)), (near, rows(2, 2, 1 << 24, 64), (False, True)), (rows(1, 2, 1 << 24, 64), near, (False, False)),
+                         (rows(2, 2, 64, 1 << 30), rows(2, 1, 64, 64), (True, False)), (rows(2, 2, 64, 1 << 30), rows(2, 2, 64, 64), (False, False))):
+        got_q, got_k, got_v = _within_reach(q, k, k)
+        assert [got_q is not q, got_k is not k, got_v is not k] == [copied[0], copied[1], copied[1]]
+        assert not copied[0] or (got_q.is_contiguous() and got_q.shape == q.shape)
+        assert not copied[1] or (got_k.is_contiguous() and got_k.shape == k.shape)

@@ -373,6 +373,13 @@ bool rows_in_place(const at::Tensor* t, int n) {
       return false;
   return true;
 }
+// ... and near enough to one another for attention over packed sequences (as the C entry points have it); what is not, the wrapper copies
+bool within_reach(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value) {
+  constexpr int64_t kToken = 1 << 24;
+  const int64_t group = key.size(1) > 0 ? query.size(1) / key.size(1) : 1;
+  return query.stride(0) < kToken && key.stride(0) < kToken && value.stride(0) < kToken &&
+         (group <= 1 || (query.stride(1) < (1ll << 31) && 33 * query.stride(0) + group * query.stride(1) < (1ll << 31) - query.size(2)));
+}
 bool scale_of(PyObject* arg, const at::Tensor& query, double* out) {
   if (arg != Py_None && !PyFloat_CheckExact(arg)) return false;
   *out = arg == Py_None ? 1.0 / std::sqrt((double)query.size(2)) : PyFloat_AS_DOUBLE(arg);
@@ -435,8 +442,8 @@ PyObject* flash_attention_packed(PyObject*, PyObject* const* args, Py_ssize_t na
   using Op = void(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&, double, bool, at::Tensor&,
                   const std::optional<at::Tensor>&);
   static const auto op = find_op<Op>("tilefusion::flash_attention_packed");
-  if (nargs != 8 || !plain(op, args, 4, t) || !rows_in_place(t, 3) || !plain_or_none(op, args[4], &kv_offsets) || !scale_of(args[5], t[0], &scale) ||
-      !PyBool_Check(args[6]) || !PyBool_Check(args[7]))
+  if (nargs != 8 || !plain(op, args, 4, t) || !rows_in_place(t, 3) || !within_reach(t[0], t[1], t[2]) || !plain_or_none(op, args[4], &kv_offsets) ||
+      !scale_of(args[5], t[0], &scale) || !PyBool_Check(args[6]) || !PyBool_Check(args[7]))
     Py_RETURN_NONE;
   const bool keep = args[7] == Py_True;
   {
@@ -459,7 +466,7 @@ PyObject* flash_attention_packed_backward(PyObject*, PyObject* const* args, Py_s
                   const std::optional<at::Tensor>&, double, bool, const std::optional<at::Tensor>&, const std::optional<at::Tensor>&,
                   const std::optional<at::Tensor>&);
   static const auto op = find_op<Op>("tilefusion::flash_attention_packed_backward");
-  if (nargs != 10 || !plain(op, args, 7, t) || !rows_in_place(t, 5) || !t[0].is_contiguous() || !t[4].is_contiguous() || !t[5].is_contiguous() ||
+  if (nargs != 10 || !plain(op, args, 7, t) || !rows_in_place(t, 5) || !within_reach(t[1], t[2], t[3]) || !t[0].is_contiguous() || !t[4].is_contiguous() || !t[5].is_contiguous() ||
       !plain_or_none(op, args[7], &kv_offsets) || !scale_of(args[8], t[1], &scale) || !PyBool_Check(args[9]))
     Py_RETURN_NONE;
   {

@@ -22,21 +22,24 @@ int check_packed(const char* who, const tf_packed_attention_t* p) {
   if (p->tokens == 0 && p->kv_tokens == 0) return TF_OK;
   TFK_REQUIRE(p->offsets && (p->query || p->tokens == 0) && ((p->key && p->value) || p->kv_tokens == 0), TF_ERR_INVALID_ARG, "%s: null pointer", who);
   TFK_REQUIRE(p->kv_offsets || p->tokens == p->kv_tokens, TF_ERR_INVALID_ARG, "%s: keys of another number than queries need kv_offsets", who);
+  // A tile of up to 64 tokens is addressed in 32 bits from its first one, and its head in 64.
   const int64_t* strides[] = {p->query_strides, p->key_strides, p->value_strides};
   for (const int64_t* s : strides)
-    for (int i = 0; i < 2; ++i)
-      TFK_REQUIRE(s[i] >= 0 && s[i] % 8 == 0 && s[i] < (1 << 24), TF_ERR_INVALID_ARG, "%s: strides must be multiples of 8 elements, below 2^24", who);
-  // (the backward pass addresses a tile of 32 rows, whose tokens are 33 at most, in 32 bits from the first one's)
-  TFK_REQUIRE(33 * p->query_strides[0] + p->heads / p->kv_heads * p->query_strides[1] < (1ll << 31) - p->D, TF_ERR_INVALID_ARG,
+    TFK_REQUIRE(s[0] >= 0 && s[0] % 8 == 0 && s[0] < (1 << 24) && s[1] >= 0 && s[1] % 8 == 0 && s[1] < (1ll << 40), TF_ERR_INVALID_ARG,
+                "%s: strides must be multiples of 8 elements, from token to token below 2^24 and from head to head below 2^40", who);
+  // (the backward pass addresses a tile of 32 rows, whose tokens are 33 at most, in 32 bits from the first one's; one head alone is no step further)
+  const int64_t group = p->heads / p->kv_heads;
+  TFK_REQUIRE(33 * p->query_strides[0] + (group > 1 ? group * p->query_strides[1] : 0) < (1ll << 31) - p->D, TF_ERR_INVALID_ARG,
               "%s: the heads of a group must lie within 2^31 elements", who);
   TFK_REQUIRE(((reinterpret_cast<uintptr_t>(p->query) | reinterpret_cast<uintptr_t>(p->key) | reinterpret_cast<uintptr_t>(p->value)) & 15) == 0,
               TF_ERR_INVALID_ARG, "%s: operands must begin at 16-byte boundaries", who);
   return TF_OK;
 }
 PackedArgs packed_args(const tf_packed_attention_t& p) {
+  const int64_t group = p.heads / p.kv_heads;
   return {p.offsets, p.kv_offsets ? p.kv_offsets : p.offsets, (int)p.sequences, (int)p.tokens, (int)p.kv_tokens, (int)p.heads, (int)p.kv_heads,
-          make_divider((unsigned)(p.heads / p.kv_heads)), (int)p.query_strides[0], (int)p.key_strides[0], (int)p.value_strides[0], (int)p.query_strides[1], (int)p.key_strides[1],
-          (int)p.value_strides[1], nullptr};
+          make_divider((unsigned)group), (int)p.query_strides[0], (int)p.key_strides[0], (int)p.value_strides[0],
+          group > 1 ? (int)p.query_strides[1] : 0, group * p.query_strides[1], p.key_strides[1], p.value_strides[1], nullptr};
 }
 
 // Rows per workgroup, from the sequences' mean length, which is all that the host knows of them.  A tile of 64 keys takes 1.45 us with 256 rows, 1.0 with

@@ -222,7 +222,7 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
   const PackedTile tile = packed_key_tile(a, kGradOwn, group_no / a.kv_heads / g.parts);
   if (tile.sequence < 0) return;
   const int shift = tile.lkv - tile.lq, rows = tile.lq * group, key0 = tile.from_end * kGradOwn;   // (counted from the front)
-  const T* const Q = static_cast<const T*>(g.query) + (size_t)tile.q0 * a.query_row + (size_t)head * group * a.query_head;
+  const T* const Q = static_cast<const T*>(g.query) + (size_t)tile.q0 * a.query_row + head * a.query_group;
   const T* const dO = static_cast<const T*>(g.grad_out) + ((size_t)tile.q0 * a.heads + (size_t)head * group) * D;
   const float4_t* const stats = g.stats + ((size_t)head * a.tokens + tile.q0) * group;
 
@@ -232,8 +232,8 @@ TFK_DEVICE void grad_keys(const GradArgs& g, char* smem, int group_no, int group
   for (int kb = 0; kb < kKB; ++kb) {
     const int key = key0 + 16 * (kGradWaves * kb + wave) + lr;
     const size_t at = tile.k0 + min(key, tile.lkv - 1);
-    const T* k = static_cast<const T*>(g.key) + at * a.key_row + (size_t)head * a.key_head;
-    const T* v = static_cast<const T*>(g.value) + at * a.value_row + (size_t)head * a.value_head;
+    const T* k = static_cast<const T*>(g.key) + at * a.key_row + head * a.key_head;
+    const T* v = static_cast<const T*>(g.value) + at * a.value_row + head * a.value_head;
 #pragma unroll
     for (int kk = 0; kk < kKK; ++kk) {
       kf[kb][kk] = *reinterpret_cast<const V8*>(k + 32 * kk + 8 * lg);
@@ -464,11 +464,11 @@ TFK_DEVICE void grad_queries(const GradArgs& g, char* smem, int group_no, int gr
   const int head = group_no % a.kv_heads, group = (int)a.group.d;
   const int Lkv = tile.lkv, shift = tile.lkv - tile.lq, rows = tile.lq * group;
   const int tile_row0 = ((rows + kGradOwn - 1) / kGradOwn - 1 - tile.from_end) * kGradOwn;
-  const T* const Q = static_cast<const T*>(g.query) + (size_t)tile.q0 * a.query_row + (size_t)head * group * a.query_head;
+  const T* const Q = static_cast<const T*>(g.query) + (size_t)tile.q0 * a.query_row + head * a.query_group;
   const size_t at_head = ((size_t)tile.q0 * a.heads + (size_t)head * group) * D;
   const T* const dO = static_cast<const T*>(g.grad_out) + at_head;
-  const T* const K = static_cast<const T*>(g.key) + (size_t)tile.k0 * a.key_row + (size_t)head * a.key_head;
-  const T* const V = static_cast<const T*>(g.value) + (size_t)tile.k0 * a.value_row + (size_t)head * a.value_head;
+  const T* const K = static_cast<const T*>(g.key) + (size_t)tile.k0 * a.key_row + head * a.key_head;
+  const T* const V = static_cast<const T*>(g.value) + (size_t)tile.k0 * a.value_row + head * a.value_head;
   const float4_t* const stats = g.stats + ((size_t)head * a.tokens + tile.q0) * group;
   auto limit_of = [&](int row) __attribute__((always_inline)) { return kCausal ? min(Lkv - 1, divide(a.group, min(row, rows - 1)) + shift) : Lkv - 1; };
 

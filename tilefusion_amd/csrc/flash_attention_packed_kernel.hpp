@@ -58,9 +58,9 @@ __global__ __launch_bounds__(kWavesT * 64, 1) void flash_attention_packed_kernel
   // Causal tiles end at the last row, in 64s: the tile that is not full is the one with the fewest keys.  Rows in front of the first are none.
   const int tile_row0 = kCausal ? (rows + 63) / 64 * 64 - (tile.from_end + 1) * kBM : ((rows + kBM - 1) / kBM - 1 - tile.from_end) * kBM;
   const int q_row0 = tile_row0 + wave * kRowsPerWave;
-  Q += (size_t)tile.q0 * a.query_row + (size_t)head * group * a.query_head;
-  K += (size_t)tile.k0 * a.key_row + (size_t)head * a.key_head;
-  V += (size_t)tile.k0 * a.value_row + (size_t)head * a.value_head;
+  Q += (size_t)tile.q0 * a.query_row + head * a.query_group;
+  K += (size_t)tile.k0 * a.key_row + head * a.key_head;
+  V += (size_t)tile.k0 * a.value_row + head * a.value_head;
   const size_t o_row = (size_t)a.heads * D;
   O += tile.q0 * o_row + (size_t)head * group * D;
   float* const lse = a.lse ? a.lse + (size_t)head * group * a.tokens + tile.q0 : nullptr;

@@ -17,7 +17,8 @@ struct PackedArgs {
   const int *offsets, *kv_offsets;   // [sequences + 1]
   int sequences, tokens, kv_tokens, heads, kv_heads;
   Divider group;   // query heads that share a head of keys
-  int query_row, key_row, value_row, query_head, key_head, value_head;   // strides in elements
+  int query_row, key_row, value_row, query_head;   // strides in elements; query_head: from one to the next of the heads of a group
+  int64_t query_group, key_head, value_head;       // ... from one head of keys to the next (that of a long text's head-major tensor is its tokens * D)
   float* lse;   // [heads][tokens], or null
 };
 

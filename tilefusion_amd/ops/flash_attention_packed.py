@@ -17,6 +17,18 @@ def _scale(query: torch.Tensor, softmax_scale: Optional[float], op: str) -> floa
     return 1.0 / math.sqrt(query.size(-1)) if softmax_scale is None else softmax_scale
 
 
+def _within_reach(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor) -> Tuple[torch.Tensor, ...]:
+    """query, key and value as they are where the kernels read them so, otherwise copies: rows in one piece, tokens less than 2^24 elements apart, and the
+    heads of a group, which 32-bit offsets reach from one another, within 2^31 (those of a long text's [heads, tokens, D] may not be)."""
+    query, key, value = (rows_in_place(t) for t in (query, key, value))
+    query, key, value = (t.contiguous() if t.dim() == 3 and t.size(0) > 1 and t.stride(0) >= 2**24 else t for t in (query, key, value))
+    if query.dim() == 3 and key.dim() == 3 and query.size(1) > key.size(1) > 0:
+        group = query.size(1) // key.size(1)
+        if 33 * query.stride(0) + group * query.stride(1) >= 2**31 - query.size(2):
+            query = query.contiguous()
+    return query, key, value
+
+
 def _forward(
     query: torch.Tensor,
     key: torch.Tensor,
@@ -27,7 +39,7 @@ def _forward(
     causal: bool,
     keep: bool,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    query, key, value = (rows_in_place(t) for t in (query, key, value))
+    query, key, value = _within_reach(query, key, value)
     out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     lse = torch.empty(query.size(1), query.size(0), dtype=torch.float32, device=query.device) if keep else None
     torch.ops.tilefusion.flash_attention_packed(query, key, value, offsets, kv_offsets, softmax_scale, causal, out, lse)
@@ -49,7 +61,7 @@ def _backward(
     of_keys: bool,
 ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
     """The gradients that are asked for, None in the place of the others."""
-    query, key, value = (rows_in_place(t) for t in (query, key, value))
+    query, key, value = _within_reach(query, key, value)
     grad_out, out = (rows_in_place(t.contiguous()) for t in (grad_out, out))
     grad_query = torch.empty(query.shape, dtype=query.dtype, device=query.device) if of_query else None
     grad_key, grad_value = (torch.empty(t.shape, dtype=t.dtype, device=t.device) if of_keys else None for t in (key, value))
@@ -93,7 +105,8 @@ def flash_attention_packed(
 
     Args:
         query: [tokens, heads, D] fp16 or bf16, D 64 or 128; key, value: [kv_tokens, kv_heads, D], head h reads head h // (heads // kv_heads) of them.
-            Slices of one projection are read where they are.
+            Slices of one projection and head-major tensors are read where they are; tokens 2^24 elements apart or more, and queries whose heads that
+            share one of the keys reach 2^31 elements, are copied.
         offsets: [sequences + 1] int32, ascending: sequence b is tokens offsets[b] .. offsets[b + 1] - 1.
         kv_offsets: the same of the keys, where a sequence has keys from before (a prompt in pieces); None: as the queries.
         softmax_scale: 1 / sqrt(D) where it is None.
