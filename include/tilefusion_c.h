@@ -307,7 +307,7 @@ typedef struct {
  * The rotated queries go to query_out [tokens, heads, D], the keys to key_out [tokens, kv_heads, D] as well unless it is null.
  * A token whose position has no page in the cache or no row in the tables changes nothing in the cache; its rows of query_out and key_out are NaN.  Tokens that
  * belong to no sequence, and those of a sequence that is not as long as its new tokens, change nothing either, and their rows are zero.
- * Pages that new tokens go to belong to one sequence.  tokens < 2^24. */
+ * Pages that new tokens go to belong to one sequence.  No rows of the cache may lie on each other.  tokens < 2^24. */
 TF_API int tf_append_paged_kv(const tf_paged_cache_t* cache, const void* query, const void* key, const void* value, const int64_t* strides,
                               const float* cos, const float* sin, int64_t positions, int64_t rotated, int interleaved, const int32_t* offsets,
                               int64_t tokens, int64_t heads, void* query_out, void* key_out, void* stream);

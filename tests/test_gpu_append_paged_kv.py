@@ -282,3 +282,27 @@ def test_results_that_a_program_hands_in_count_as_changed():
     direct.flash_attention_packed_backward(q, q, k, v, outs["out"], outs["lse"], offsets, None, 0.125, True, outs["dq"], outs["dk"], outs["dv"])
     assert all(outs[name]._version > n for name, n in before.items())
     assert after_forward == {name: outs[name]._version for name in ("out", "lse")}
+
+
+def test_caches_whose_rows_lie_on_each_other_are_refused():
+    cache = ref.Cache([40, 3], 16, 2, 64, torch.float16)
+    q, k, v = _rows(2, 4, 2, 64, torch.float16)
+    cos, sin = ops.rotation_tables(64, 64, device=DEV)
+    pages = cache.key.shape[0]
+    # each page half of the one in front of it
+    half = torch.zeros((pages + 1) * 1024, dtype=torch.float16, device=DEV).as_strided((pages, 16, 2, 64), (1024, 128, 64, 1))
+    for caches in ((half, cache.value), (cache.key, half)):
+        with pytest.raises(RuntimeError, match="on each other"):
+            ops.append_paged_kv(q, k, v, cos, sin, *caches, cache.table, cache.lengths)
+    assert (half == 0).all()
+    # (read it may be)
+    ops.flash_decode_paged(q, half, half, cache.table, cache.lengths)
+    # keys and values side by side, of two layers in one tensor, in an order of dimensions that is neither of the usual ones
+    both = torch.zeros(2, 16, pages, 2, 2, 64, dtype=torch.float16, device=DEV)
+    key, value = (both[1, :, :, i].transpose(0, 1) for i in range(2))
+    got = ops.append_paged_kv(q, k, v, cos, sin, key, value, cache.table, cache.lengths)
+    want = ops.append_paged_kv(q, k, v, cos, sin, cache.key, cache.value, cache.table, cache.lengths)
+    assert torch.equal(got, want) and (both[0] == 0).all()
+    for b, n in enumerate([40, 3]):
+        place = cache.places(b, n - 1, n)
+        assert torch.equal(key[place], cache.key[place]) and torch.equal(value[place], cache.value[place])

@@ -289,3 +289,23 @@ def test_the_wrapper_copies_what_the_kernels_do_not_reach():
         assert [got_q is not q, got_k is not k, got_v is not k] == [copied[0], copied[1], copied[1]]
         assert not copied[0] or (got_q.is_contiguous() and got_q.shape == q.shape)
         assert not copied[1] or (got_k.is_contiguous() and got_k.shape == k.shape)
+
+
+def test_new_tokens_have_places_of_their_own():
+    # rows of the cache that would lie on each other in part: two tokens' rows would be written to one place, in no order
+    lib = _capi.load()
+
+    def call(**changed):   # (refused in any case: half of an odd number is turned)
+        status = lib.tf_append_paged_kv(_cache(**changed), P, P, P, _i64(256, 64, 128, 64, 128, 64), P, P, 100, 33, 0, None, 3, 4, P, P, None)
+        assert status == BAD
+        return b"on each other" in lib.tf_last_error()
+
+    # 8 pages of 16 tokens, 2 heads x 64, strides of page, token and head
+    for strides in ((2048, 64, 1024), (2048, 128, 64), (64, 1024, 512), (64, 512, 1 << 20), (1 << 33, 64, 1024), (4096, 128, 2048), (1 << 62, 64, 1024)):
+        assert not call(key_strides=_i64(*strides)) and not call(value_strides=_i64(*strides)), strides
+    for strides in ((1024, 64, 1024), (2048, 64, 64), (2040, 128, 64), (64, 64, 64), (64, 504, 1 << 20), (2048, 0, 1024), (0, 64, 1024), (2048, 64, 0),
+                    (2048, 64, 960), (128, 64, 1 << 20)):
+        assert call(key_strides=_i64(*strides)) and call(value_strides=_i64(*strides)), strides
+    # the stride of one alone says nothing
+    assert not call(kv_heads=1, key_strides=_i64(1024, 64, 0)) and not call(pages=1, key_strides=_i64(64, 64, 1024))
+    assert not call(page_size=1, key_strides=_i64(128, 0, 64), value_strides=_i64(128, 64, 64))

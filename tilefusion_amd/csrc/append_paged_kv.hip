@@ -8,7 +8,9 @@
 // 9 prompts of 77 to 2999, 32/8 heads x 128, fp16: 39 us, 5.2 TB/s (one row a thread 45, two 42, three 39, four 39); a token each of 64: 3.8 us of
 // the GPU's time.
 #include <algorithm>
+#include <iterator>
 #include <limits>
+#include <utility>
 
 #include "paged_cache.hpp"
 
@@ -179,6 +181,20 @@ int launch_append(const AppendArgs& a, int64_t tokens, bool neighbours, hipStrea
   return vector ? launch_append<T, D, false, true>(a, tokens, st) : launch_append<T, D, false, false>(a, tokens, st);
 }
 
+// No row of a cache lies on another: every dimension's steps lead past all that those with smaller steps reach, as in whatever order and slice of a
+// tensor (not every cache without overlaps is of this kind, but all that are made by turning and cutting are).
+bool rows_apart(const tf_paged_cache_t& c, const int64_t (&strides)[3]) {
+  std::pair<int64_t, int64_t> steps[] = {{strides[0], c.pages}, {strides[1], c.page_size}, {strides[2], c.kv_heads}};
+  std::sort(std::begin(steps), std::end(steps));
+  __int128 reach = c.D;
+  for (const auto& [stride, count] : steps) {
+    if (count == 1) continue;
+    if (stride < reach) return false;
+    reach += (__int128)stride * (count - 1);
+  }
+  return true;
+}
+
 }  // namespace
 
 int check_paged_cache(const char* who, const tf_paged_cache_t* c) {
@@ -210,6 +226,8 @@ extern "C" int tf_append_paged_kv(const tf_paged_cache_t* cache, const void* que
   using namespace tfk;
   constexpr const char* who = "tf_append_paged_kv";
   if (int rc = check_paged_cache(who, cache)) return rc;
+  TFK_REQUIRE(rows_apart(*cache, cache->key_strides) && rows_apart(*cache, cache->value_strides), TF_ERR_INVALID_ARG,
+              "%s: rows of the cache lie on each other", who);
   TFK_REQUIRE(tokens >= 0 && tokens < (1 << 24) && heads > 0 && heads <= 65536, TF_ERR_INVALID_ARG, "%s: tokens below 2^24, heads 1 .. 65536", who);
   TFK_REQUIRE(rotated > 0 && rotated % 2 == 0 && rotated <= cache->D && positions >= 0, TF_ERR_INVALID_ARG,
               "%s: rotated must be even and at most the head dim (got %lld)", who, (long long)rotated);
