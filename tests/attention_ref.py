@@ -109,3 +109,64 @@ def rotate(x, position, cos, sin, interleaved):
     size = torch.zeros_like(y)
     size[..., a], size[..., b] = (xa * c).abs() + (xb * s).abs(), (xa * s).abs() + (xb * c).abs()
     return y, half_step(x.dtype) * y.abs() + 2.0 ** -22 * size + torch.finfo(x.dtype).tiny * half_step(x.dtype)
+
+
+# ---- gradients without a formula of them: of a loss in 64 bits, by autograd and by differences -------------------------------
+def loss(q, k, v, do, lengths, scale, causal):
+    """sum(do * attention) over packed sequences, all in 64 bits."""
+    total, group, a = 0.0, q.shape[1] // k.shape[1], 0
+    for n in lengths:
+        masked = torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1) if causal else torch.zeros(n, n, dtype=torch.bool, device=q.device)
+        for head in range(q.shape[1]):
+            rows, keys = (slice(a, a + n), head), (slice(a, a + n), head // group)
+            score = (q[rows] @ k[keys].t().contiguous() * scale).masked_fill(masked, -math.inf)
+            total = total + ((torch.softmax(score, 1) @ v[keys]) * do[rows].double()).sum()
+        a += n
+    return total
+
+
+def gradients(q, k, v, do, out, lse, lengths, scale, causal):
+    """The gradients of `loss` in q, k and v by autograd in 64 bits, and how far off those of a kernel may be that starts from `out` and `lse` as they are
+    (rounded, and with the forward pass's errors).
+
+    Of P = exp(s - lse) the relative error is that of its score, of lse, of exp2 and its argument, and one rounding.  Of dS = P (dP - delta) it is that and a
+    rounding, and P times the errors of dP and delta: sums of D products in fp32, and what do makes of the error of out.  All that is weighed with
+    what it multiplies; sums in fp32 over keys or over a group's rows; one rounding of the result."""
+    leaves = [x.double().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(loss(*leaves, do, lengths, scale, causal), leaves)
+    bounds = [torch.zeros_like(x) for x in grads]
+    dtype, d, group, step, a = q.dtype, q.shape[-1], q.shape[1] // k.shape[1], half_step(q.dtype), 0
+    for n in lengths:
+        masked = torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1) if causal else torch.zeros(n, n, dtype=torch.bool, device=q.device)
+        for head in range(q.shape[1]):
+            rows, keys = (slice(a, a + n), head), (slice(a, a + n), head // group)
+            o, l = attend(q[rows], k[keys], v[keys], scale, masked)[:2]
+            qd, kd, vd, gd = (x.double() for x in (q[rows], k[keys], v[keys], do[rows]))
+            s = qd @ kd.t().contiguous() * scale
+            p = torch.exp(s - l[:, None]).masked_fill(masked, 0.0)
+            off_p = qd.abs() @ kd.abs().t().contiguous() * abs(scale) * (d + 8) * 2.0 ** -24 + 2.0 ** -20 + (l[:, None].abs() + s.abs()) * 2.0 ** -22
+            off_p = off_p + (lse[head, a:a + n].double() - l).abs()[:, None]
+            dp, delta = gd @ vd.t().contiguous(), (gd * o).sum(1, keepdim=True)
+            off_d = (d + 4) * 2.0 ** -24 * (gd.abs() @ vd.abs().t().contiguous() + (gd * o).abs().sum(1, keepdim=True))
+            off_d = off_d + (gd * (out[rows].double() - o)).sum(1, keepdim=True).abs()
+            ds = (p * (dp - delta)).abs()
+            err = p * off_d + (off_p + step) * ds
+            bounds[0][rows] += abs(scale) * ((err + n * 2.0 ** -24 * ds) @ kd.abs())
+            bounds[1][keys] += abs(scale) * ((err + n * group * 2.0 ** -24 * ds).t().contiguous() @ qd.abs())
+            bounds[2][keys] += ((off_p + step + n * group * 2.0 ** -24) * p).t().contiguous() @ gd.abs()
+        a += n
+    return grads, [1.02 * e + step * x.abs() + 2 * step * torch.finfo(dtype).tiny for e, x in zip(bounds, grads)]
+
+
+def assert_slopes(got, q, k, v, do, lengths, scale, causal, bounds, seed=1):
+    """Each gradient against differences of `loss` along a way that goes up wherever the gradient does: nothing cancels in their product, so that what is
+    allowed is a few hundredths of it, and the differences' own error (of the third order in steps of 10^-4) nothing beside it."""
+    g, h = torch.Generator().manual_seed(seed), 1e-4
+    inputs = [x.double() for x in (q, k, v)]
+    for n, (name, grad, bound) in enumerate(zip(("grad_query", "grad_key", "grad_value"), got, bounds)):
+        way = torch.randn(grad.shape, generator=g, dtype=torch.float64).abs().to(grad.device) * grad.double().sign()
+        ahead, behind = ([x + (h * way if i == n else 0.0) * sign for i, x in enumerate(inputs)] for sign in (1.0, -1.0))
+        slope = ((loss(*ahead, do, lengths, scale, causal) - loss(*behind, do, lengths, scale, causal)) / (2 * h)).item()
+        rise, allowed = (grad.double() * way).sum().item(), (bound * way.abs()).sum().item() + 1e-5 * abs(slope)
+        assert allowed < 0.1 * rise, f"{name}: {allowed} of {rise} would pass anything"
+        assert abs(rise - slope) <= allowed, f"{name}: {rise}, by differences {slope}, allowed {allowed}"

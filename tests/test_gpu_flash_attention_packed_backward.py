@@ -360,3 +360,18 @@ def test_tokens_far_from_each_other():
     of = _offsets([25, 15])
     want = ops.flash_attention_packed(q, k, v, of)
     assert torch.equal(ops.flash_attention_packed(_spread(q, 1 << 24, 64), _spread(k, 1 << 25, 64), _spread(v, 1 << 24, 64), of), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths,h,hkv,d", [([25, 15], 2, 1, 64), ([25, 15], 4, 2, 128), ([130, 47, 1], 4, 2, 64), ([200], 6, 2, 128)])
+def test_gradients_of_the_loss_by_autograd_and_by_differences(dtype, causal, lengths, h, hkv, d):
+    # (from the definition of the forward pass alone, in 64 bits)
+    q, k, v, do = _rows(sum(lengths), sum(lengths), h, hkv, d, dtype)
+    of = _offsets(lengths)
+    out, lse = ops.flash_attention_packed(q, k, v, of, None, None, causal, True)
+    got = ops.flash_attention_packed_backward(do, q, k, v, out, lse, of, None, None, causal)
+    want, bounds = ref.gradients(q, k, v, do, out, lse, lengths, d ** -0.5, causal)
+    for name, a, b, c in zip(("grad_query", "grad_key", "grad_value"), got, want, bounds):
+        ref.assert_within(a, b, c, name)
+    ref.assert_slopes(got, q, k, v, do, lengths, d ** -0.5, causal, bounds)

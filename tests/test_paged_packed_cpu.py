@@ -309,3 +309,38 @@ def test_new_tokens_have_places_of_their_own():
     # the stride of one alone says nothing
     assert not call(kv_heads=1, key_strides=_i64(1024, 64, 0)) and not call(pages=1, key_strides=_i64(64, 64, 1024))
     assert not call(page_size=1, key_strides=_i64(128, 0, 64), value_strides=_i64(128, 64, 64))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_the_comparisons_of_gradients_see_factors(dtype, causal):
+    g = torch.Generator().manual_seed(5)
+    lengths = [25, 15]
+    q, do = (torch.randn(40, 4, 64, generator=g).to(dtype) for _ in range(2))
+    k, v = (torch.randn(40, 2, 64, generator=g).to(dtype) for _ in range(2))
+    problem = (q, k, v, do, lengths, 0.125, causal)
+    out, lse = torch.empty_like(q), torch.empty(4, 40)
+    for a, b in ((0, 25), (25, 40)):
+        masked = torch.ones(b - a, b - a).triu(1).bool() if causal else None
+        for head in range(4):
+            o, l, _, _ = ref.attend(q[a:b, head], k[a:b, head // 2], v[a:b, head // 2], 0.125, masked)
+            out[a:b, head], lse[head, a:b] = o.to(dtype), l.float()
+    want, bounds = ref.gradients(q, k, v, do, out, lse, lengths, 0.125, causal)
+    right = [x.to(dtype) for x in want]
+    for a, b, c in zip(right, want, bounds):
+        ref.assert_within(a, b, c)
+    ref.assert_slopes(right, *problem, bounds)
+    # (the mistakes are planted in the oracle: a factor in one gradient, and a head that is left out of a group's sum)
+    for n in range(3):
+        for factor in (0.7, 0.9, 1.1, 1.3, 2.0, 0.125, -1.0):
+            wrong = [x * factor if i == n else x for i, x in enumerate(want)]
+            with pytest.raises(AssertionError):
+                ref.assert_within(wrong[n].to(dtype), want[n], bounds[n])
+            with pytest.raises(AssertionError):
+                ref.assert_slopes([x.to(dtype) for x in wrong], *problem, bounds)
+    less = do.clone()
+    less[:, 1] = 0.0
+    wrong = ref.gradients(q, k, v, less, out, lse, lengths, 0.125, causal)[0]
+    for n in (1, 2):
+        with pytest.raises(AssertionError):
+            ref.assert_within(wrong[n].to(dtype), want[n], bounds[n])
