@@ -306,3 +306,20 @@ def test_caches_whose_rows_lie_on_each_other_are_refused():
     for b, n in enumerate([40, 3]):
         place = cache.places(b, n - 1, n)
         assert torch.equal(key[place], cache.key[place]) and torch.equal(value[place], cache.value[place])
+
+
+def test_offsets_beyond_32_bits():
+    # 8 GiB of keys, of which three pages are written, the last one among them
+    d, page = 128, 16
+    pages = 2 ** 33 // (page * d * 2)
+    key, value = (torch.empty(pages, page, 1, d, dtype=torch.float16, device=DEV) for _ in range(2))
+    cache = ref.Cache([40], page, 1, d, torch.float16)
+    where = [pages - 1, 0, pages // 2 + 3]
+    q, k, v = _rows(40, 4, 1, d, torch.float16)
+    cos, sin = ops.rotation_tables(41, d, device=DEV)
+    got = ops.append_paged_kv(q, k, v, cos, sin, key, value, torch.tensor([where], dtype=torch.int32, device=DEV), cache.lengths, _offsets([40]))
+    want = ops.append_paged_kv(q, k, v, cos, sin, cache.key, cache.value, cache.table, cache.lengths, _offsets([40]))
+    assert torch.equal(got, want)
+    for i, p in enumerate(where):
+        rows, own = min(page, 40 - i * page), cache.table[0, i].long()
+        assert torch.equal(key[p, :rows], cache.key[own, :rows]) and torch.equal(value[p, :rows], cache.value[own, :rows])

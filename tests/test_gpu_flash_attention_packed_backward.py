@@ -375,3 +375,37 @@ def test_gradients_of_the_loss_by_autograd_and_by_differences(dtype, causal, len
     for name, a, b, c in zip(("grad_query", "grad_key", "grad_value"), got, want, bounds):
         ref.assert_within(a, b, c, name)
     ref.assert_slopes(got, q, k, v, do, lengths, d ** -0.5, causal, bounds)
+
+
+def test_offsets_beyond_32_bits():
+    # tokens that lie 2^20 elements apart: the last of them 10 GiB behind the first
+    lengths, h, hkv, d = [100, 4000, 900], 4, 2, 64
+    t = sum(lengths)
+    q, k, v, do = _rows(t, t, h, hkv, d, torch.float16)
+    of = _offsets(lengths)
+    out, lse = ops.flash_attention_packed(q, k, v, of, keep=True)
+    want = ops.flash_attention_packed_backward(do, q, k, v, out, lse, of)
+    far = [_spread(x, 1 << 20, d) for x in (q, k, v)]
+    assert all(torch.equal(a, b) for a, b in zip(ops.flash_attention_packed(*far, of, keep=True), (out, lse)))
+    assert all(torch.equal(a, b) for a, b in zip(ops.flash_attention_packed_backward(do, *far, out, lse, of), want))
+
+
+def test_results_beyond_32_bits():
+    # 2^32 elements of queries, results and gradients: sequences at both ends and around the middle, a head from each end and one between
+    tokens, h, d, n = 1 << 18, 128, 128, 128
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, do = (torch.randn(tokens, h, d, dtype=torch.bfloat16, device=DEV, generator=g) for _ in range(2))
+    k, v = (torch.randn(tokens, 1, d, dtype=torch.bfloat16, device=DEV, generator=g) for _ in range(2))
+    of = _offsets([n] * (tokens // n))
+    out, lse = ops.flash_attention_packed(q, k, v, of, keep=True)
+    grads = ops.flash_attention_packed_backward(do, q, k, v, out, lse, of)
+    for a in (0, tokens // 2 - n, tokens // 2, tokens - n):
+        s = slice(a, a + n)
+        want, bound = _want(q[s], k[s], v[s], do[s], out[s], lse[:, s], [n], [n], d ** -0.5, True)
+        for name, x, b, c in zip(("grad_query", "grad_key", "grad_value"), grads, want, bound):
+            ref.assert_within(x[s], b, c, f"{name} from {a}")
+        masked = torch.ones(n, n, dtype=torch.bool, device=DEV).triu(1)
+        for head in (0, 63, 127):
+            o, l, off, off_l = ref.attend(q[s, head], k[s, 0], v[s, 0], d ** -0.5, masked, ref.half_step(torch.bfloat16) + 2.0 ** -20)
+            ref.assert_within(out[s, head], o, off, f"out from {a}")
+            ref.assert_within(lse[head, s], l, off_l, f"lse from {a}")
