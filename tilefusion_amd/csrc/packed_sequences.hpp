@@ -30,9 +30,9 @@ struct PackedTile {
 
 // rows [begin, begin + length) of a sequence, within `rows`
 struct PackedRange { int begin, length; };
-TFK_DEVICE PackedRange packed_range(int begin, int end, int rows) {
-  const int b = min(max(begin, 0), rows);
-  return {b, max(min(end, rows) - b, 0)};
+__host__ __device__ inline PackedRange packed_range(int begin, int end, int rows) {
+  const int b = begin < 0 ? 0 : begin < rows ? begin : rows, e = end < rows ? end : rows;
+  return {b, e > b ? e - b : 0};   // (compared first: an end near -2^31 less b is a large number)
 }
 
 // The `rank`-th of the tiles of `rows` rows that the sequences make, most keys first.  Tile e from a sequence's end ends
