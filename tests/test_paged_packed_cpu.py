@@ -346,7 +346,7 @@ def test_the_comparisons_of_gradients_see_factors(dtype, causal):
             ref.assert_within(wrong[n].to(dtype), want[n], bounds[n])
 
 
-def test_ranges_of_packed_sequences():
+def test_ranges_and_tiles_of_packed_sequences():
     subprocess.check_call(["make", "-C", CPP, "test_packed_sequences_host"], stdout=subprocess.DEVNULL)
     out = subprocess.run([os.path.join(CPP, "test_packed_sequences_host")], capture_output=True, text=True, timeout=60)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr

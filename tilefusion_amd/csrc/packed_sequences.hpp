@@ -35,6 +35,17 @@ __host__ __device__ inline PackedRange packed_range(int begin, int end, int rows
   return {b, e > b ? e - b : 0};   // (compared first: an end near -2^31 less b is a large number)
 }
 
+// A sequence's queries and keys, the tiles of `rows` rows (or keys) that it makes, and how far its last (first) one counts: see find_tile.
+struct SequenceTiles {
+  PackedRange q, k;
+  int tiles, level;
+};
+template <bool kKeys>
+__host__ __device__ inline SequenceTiles sequence_tiles(PackedRange q, PackedRange k, int group, int rows) {
+  const auto tiles_of = [&](int n) { return (n + rows - 1) / rows; };
+  return {q, k, kKeys ? tiles_of(k.length) : tiles_of(q.length * group), kKeys ? tiles_of(k.length) : tiles_of(k.length * group)};
+}
+
 // The `rank`-th of the tiles of `rows` rows that the sequences make, most keys first.  Tile e from a sequence's end ends
 // e * rows rows in front of it and counts as ceil(lkv * group / rows) - e (causal or not: the longest sequences first, and their last
 // tokens).  The largest number that more tiles reach than come before this one is found by halving, each step a
@@ -42,19 +53,16 @@ __host__ __device__ inline PackedRange packed_range(int begin, int end, int rows
 template <bool kKeys>
 TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows, int rank) {
   const int lane = threadIdx.x % kWaveSize;
-  struct Own { int tiles, level; };   // of a lane's sequence
-  auto own = [&](int b) __attribute__((always_inline)) -> Own {
-    if (b >= a.sequences) return {0, 0};
-    const int lkv = packed_range(a.kv_offsets[b], a.kv_offsets[b + 1], a.kv_tokens).length;
-    if constexpr (kKeys) return {(lkv + rows - 1) / rows, (lkv + rows - 1) / rows};
-    const int lq = packed_range(a.offsets[b], a.offsets[b + 1], a.tokens).length;
-    return {(lq * (int)a.group.d + rows - 1) / rows, (lkv * (int)a.group.d + rows - 1) / rows};
+  auto own = [&](int b) __attribute__((always_inline)) -> SequenceTiles {   // a lane's
+    if (b >= a.sequences) return {};
+    return sequence_tiles<kKeys>(packed_range(a.offsets[b], a.offsets[b + 1], a.tokens), packed_range(a.kv_offsets[b], a.kv_offsets[b + 1], a.kv_tokens),
+                                 (int)a.group.d, rows);
   };
-  const Own first = own(lane);   // (kept: mostly all there are)
-  auto of = [&](int b0) __attribute__((always_inline)) -> Own { return b0 == 0 ? first : own(b0 + lane); };
+  const SequenceTiles first = own(lane);   // (kept: mostly all there are)
+  auto of = [&](int b0) __attribute__((always_inline)) -> SequenceTiles { return b0 == 0 ? first : own(b0 + lane); };
   int most = -0x7fffffff, least = 0x7fffffff;
   for (int b0 = 0; b0 < a.sequences; b0 += kWaveSize) {
-    const Own o = of(b0);
+    const SequenceTiles o = of(b0);
     if (o.tiles > 0) {
       most = max(most, o.level);
       least = min(least, o.level - o.tiles + 1);
@@ -64,13 +72,13 @@ TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows, int rank) {
   auto count = [&](int level) __attribute__((always_inline)) {
     int n = 0;
     for (int b0 = 0; b0 < a.sequences; b0 += kWaveSize) {
-      const Own o = of(b0);
+      const SequenceTiles o = of(b0);
       n += min(max(o.level - level + 1, 0), o.tiles);
     }
     return wave_sum(n);
   };
-  PackedTile tile = {-1, 0, 0, 0, 0, 0};
-  if (low >= high || count(low) <= rank) return tile;
+  constexpr PackedTile none = {-1, 0, 0, 0, 0, 0};
+  if (low >= high || count(low) <= rank) return none;
   int above = 0;   // tiles that reach `high`
   while (high - low > 1) {
     const int middle = low + (high - low) / 2, n = count(middle);
@@ -83,7 +91,7 @@ TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows, int rank) {
   }
   int left = rank - above;   // of the tiles that count `low`, one a sequence
   for (int b0 = 0; b0 < a.sequences; b0 += kWaveSize) {
-    const Own o = of(b0);
+    const SequenceTiles o = of(b0);
     const bool has = o.level >= low && o.level - low < o.tiles;
     const unsigned long long all = __builtin_amdgcn_ballot_w64(has);
     const int n = __builtin_popcountll(all);
@@ -93,19 +101,11 @@ TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows, int rank) {
     }
     const bool mine = has && __builtin_popcountll(all & ((1ull << lane) - 1)) == left;
     const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(mine));
-    tile.sequence = b0 + at;
-    tile.from_end = __builtin_amdgcn_readlane(o.level, at) - low;
-    break;
+    // (the ranges that the tile has been counted by: of ones that are read again, and that a program has changed meanwhile, it may be no tile)
+    const auto of_lane = [&](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, at); };
+    return {b0 + at, of_lane(o.level) - low, of_lane(o.q.begin), of_lane(o.q.length), of_lane(o.k.begin), of_lane(o.k.length)};
   }
-  if (tile.sequence < 0) return tile;
-  const PackedRange q = packed_range(read_uniform(a.offsets + tile.sequence), read_uniform(a.offsets + tile.sequence + 1), a.tokens);
-  const PackedRange k = packed_range(read_uniform(a.kv_offsets + tile.sequence), read_uniform(a.kv_offsets + tile.sequence + 1), a.kv_tokens);
-  tile.q0 = q.begin;
-  tile.lq = q.length;
-  tile.k0 = k.begin;
-  tile.lkv = k.length;
-  if ((kKeys ? k.length : q.length) == 0) tile.sequence = -1;   // (offsets that a program changes while they are read)
-  return tile;
+  return none;
 }
 TFK_DEVICE PackedTile packed_tile(const PackedArgs& a, int rows, int rank) { return find_tile<false>(a, rows, rank); }
 // The same of the tiles of `keys` keys, from_end counted from a sequence's first key, which the most rows see.
