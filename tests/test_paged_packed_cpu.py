@@ -350,3 +350,9 @@ def test_ranges_and_tiles_of_packed_sequences():
     subprocess.check_call(["make", "-C", CPP, "test_packed_sequences_host"], stdout=subprocess.DEVNULL)
     out = subprocess.run([os.path.join(CPP, "test_packed_sequences_host")], capture_output=True, text=True, timeout=60)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
+
+
+def test_ranges_of_equal_cost():
+    subprocess.check_call(["make", "-C", CPP, "test_equal_ranges_host"], stdout=subprocess.DEVNULL)
+    out = subprocess.run([os.path.join(CPP, "test_equal_ranges_host")], capture_output=True, text=True, timeout=60)
+    assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr

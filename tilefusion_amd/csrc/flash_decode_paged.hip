@@ -145,15 +145,10 @@ __global__ __launch_bounds__(kThreads, 2) void flash_decode_paged_kernel(DecodeA
     const float v = n < 0 ? __builtin_nanf("") : 0.f;
     for (int i = tid; i < a.heads * D; i += kThreads) static_cast<T*>(a.out)[(int64_t)b * a.heads * D + i] = (T)v;
   }
-  // (the first `longer` workgroups have a range that is longer by one)
   const unsigned groups = min(gridDim.x, cost);
   if (blockIdx.x >= groups) return;
-  const unsigned quota = cost / groups, longer = cost - quota * groups;
-  const unsigned begin = blockIdx.x * quota + min(blockIdx.x, longer), end = begin + quota + (blockIdx.x < longer ? 1 : 0);
-  auto group_of = [&](unsigned at) __attribute__((always_inline)) {
-    const unsigned split = longer * (quota + 1);
-    return at < split ? at / (quota + 1) : longer + (at - split) / quota;
-  };
+  const EqualRanges ranges = equal_ranges(cost, groups);
+  const unsigned begin = range_begin(ranges, blockIdx.x), end = range_begin(ranges, blockIdx.x + 1);
   // the sequence in which the range begins
   int b = 0;
   unsigned before = 0;   // the cost of the sequences in front of it
@@ -353,8 +348,9 @@ __global__ __launch_bounds__(kThreads, 2) void flash_decode_paged_kernel(DecodeA
     barrier_lds_only();
     // the workgroups that have a part of the item
     const bool whole = done.first == 0 && done.blocks + overhead(D) == (int)done.cost;
-    const unsigned part_first = whole ? blockIdx.x : group_of(done.begin + overhead(D));
-    const int parts = whole ? 1 : (int)(group_of(done.begin + done.cost - 1) - part_first) + 1;
+    // (workgroups that there are, also for lengths that a program changes while they are read)
+    const unsigned part_first = whole ? blockIdx.x : range_of(ranges, done.begin + overhead(D));
+    const int parts = whole ? 1 : (int)(range_of(ranges, done.begin + done.cost - 1) - part_first) + 1;
     const bool begins = blockIdx.x == part_first;
     T* const out = static_cast<T*>(a.out) + ((int64_t)done.b * a.heads + done.h0) * D;
     float* const part = a.part + ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * part_floats<D>();

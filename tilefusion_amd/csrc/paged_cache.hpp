@@ -34,6 +34,18 @@ __host__ __device__ inline int read_uniform(const int* p) {
 #endif
 }
 
+// `cost` units in `groups` ranges of equal length, the first `longer` of them longer by one; 0 < groups <= cost.
+struct EqualRanges {
+  unsigned groups, quota, longer;
+};
+__host__ __device__ inline EqualRanges equal_ranges(unsigned cost, unsigned groups) { return {groups, cost / groups, cost % groups}; }
+__host__ __device__ inline unsigned range_begin(const EqualRanges& r, unsigned no) { return no * r.quota + (no < r.longer ? no : r.longer); }
+// The range that holds a unit, the last one for units that there are not.
+__host__ __device__ inline unsigned range_of(const EqualRanges& r, unsigned at) {
+  const unsigned split = r.longer * (r.quota + 1), no = at < split ? at / (r.quota + 1) : r.longer + (at - split) / r.quota;
+  return no < r.groups ? no : r.groups - 1;
+}
+
 struct PageTable {
   const int* pages;   // [sequences][stride], `width` of each row
   int64_t stride;
