@@ -356,3 +356,19 @@ def test_ranges_of_equal_cost():
     subprocess.check_call(["make", "-C", CPP, "test_equal_ranges_host"], stdout=subprocess.DEVNULL)
     out = subprocess.run([os.path.join(CPP, "test_equal_ranges_host")], capture_output=True, text=True, timeout=60)
     assert out.returncode == 0 and out.stdout.strip() == "ok", out.stdout + out.stderr
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 1e300, 2.4e38, -2.4e38])
+def test_scales_beyond_fp32_are_refused(scale):
+    # (the kernels scale by softmax_scale log2(e) in fp32, of which these make an infinity; the alignment of out is refused where the scale is not)
+    lib = _capi.load()
+
+    def statuses(scale):
+        p = _packed(softmax_scale=scale)
+        calls = [lambda: lib.tf_flash_attention_packed(p, P + 8, P, None),
+                 lambda: lib.tf_flash_attention_packed_backward(p, P, P, P, P + 8, P, P, P, 1 << 20, None),
+                 lambda: lib.tf_flash_decode_paged(_cache(), P, _i64(256, 64), P + 8, 4, scale, P, 1 << 30, None)]
+        return [(call(), lib.tf_last_error()) for call in calls]
+
+    assert all(status == BAD and b"softmax_scale" in error for status, error in statuses(scale))
+    assert all(status == BAD and b"boundar" in error for status, error in statuses(math.copysign(2.3e38, scale)))

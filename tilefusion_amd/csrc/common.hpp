@@ -165,6 +165,11 @@ TFK_DEVICE bool arrive(arrivals_t* word, arrivals_t tag, unsigned parts) {
 arrivals_t next_arrivals_tag();
 void set_error(const char* fmt, ...);
 int hip_fail(hipError_t e, const char* what);
+// The scale of softmax as the kernels have it, in fp32 times log2(e), is a finite number.
+inline bool is_softmax_scale(double scale) {
+  const double in_log2 = scale * 1.4426950408889634;
+  return in_log2 >= -3.4028234663852886e38 && in_log2 <= 3.4028234663852886e38;
+}
 // Ordinary (coarse-grained) memory of the current device, for which hardware atomics are defined: on host, managed or fine-grained
 // memory an update may be lost.
 bool is_ordinary_device_memory(const void* p);

@@ -17,8 +17,7 @@ int check_packed(const char* who, const tf_packed_attention_t* p) {
               "%s: heads must be a multiple of kv_heads, at most 1024 (got %lld and %lld)", who, (long long)p->heads, (long long)p->kv_heads);
   TFK_REQUIRE(std::max(p->tokens, p->kv_tokens) * (p->heads / p->kv_heads) < (1ll << 30), TF_ERR_INVALID_ARG,
               "%s: tokens times the heads of a group must be below 2^30", who);
-  TFK_REQUIRE(p->softmax_scale == p->softmax_scale && p->softmax_scale - p->softmax_scale == 0.0, TF_ERR_INVALID_ARG,
-              "%s: softmax_scale must be finite", who);
+  TFK_REQUIRE(is_softmax_scale(p->softmax_scale), TF_ERR_INVALID_ARG, "%s: softmax_scale must be finite, times log2(e) in fp32 too", who);
   if (p->tokens == 0 && p->kv_tokens == 0) return TF_OK;
   TFK_REQUIRE(p->offsets && (p->query || p->tokens == 0) && ((p->key && p->value) || p->kv_tokens == 0), TF_ERR_INVALID_ARG, "%s: null pointer", who);
   TFK_REQUIRE(p->kv_offsets || p->tokens == p->kv_tokens, TF_ERR_INVALID_ARG, "%s: keys of another number than queries need kv_offsets", who);

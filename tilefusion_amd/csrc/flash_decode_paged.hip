@@ -467,7 +467,7 @@ extern "C" int tf_flash_decode_paged(const tf_paged_cache_t* cache, const void* 
   TFK_REQUIRE(cache->page_size % 16 == 0, TF_ERR_UNSUPPORTED, "%s: page_size must be a multiple of 16 (got %lld)", who, (long long)cache->page_size);
   TFK_REQUIRE(cache->key_strides[1] < (1 << 26) && cache->value_strides[1] < (1 << 26), TF_ERR_UNSUPPORTED,
               "%s: the cache's strides from token to token must be below 2^26 elements", who);
-  TFK_REQUIRE(softmax_scale == softmax_scale && softmax_scale - softmax_scale == 0.0, TF_ERR_INVALID_ARG, "%s: softmax_scale must be finite", who);
+  TFK_REQUIRE(is_softmax_scale(softmax_scale), TF_ERR_INVALID_ARG, "%s: softmax_scale must be finite, times log2(e) in fp32 too", who);
   if (cache->sequences == 0) return TF_OK;
   TFK_REQUIRE(cache->table_width < (1ll << 31) / cache->page_size &&
                   cache->sequences * (cache->table_width * cache->page_size / kBlockKeys + 3) <
