@@ -372,3 +372,10 @@ def test_scales_beyond_fp32_are_refused(scale):
 
     assert all(status == BAD and b"softmax_scale" in error for status, error in statuses(scale))
     assert all(status == BAD and b"boundar" in error for status, error in statuses(math.copysign(2.3e38, scale)))
+
+
+@pytest.mark.parametrize("name", ["flash_decode_paged", "flash_attention_packed", "flash_attention_packed_backward"])
+def test_a_head_dimension_of_zero_is_refused_by_name(name):
+    q, calls = _calls()
+    with pytest.raises(RuntimeError, match=f"{name}: query must be"):
+        calls[name](q[..., :0])

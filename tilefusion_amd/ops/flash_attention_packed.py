@@ -12,7 +12,7 @@ __all__ = ["flash_attention_packed", "flash_attention_packed_backward"]
 
 
 def _scale(query: torch.Tensor, softmax_scale: Optional[float], op: str) -> float:
-    if query.dim() != 3:
+    if query.dim() != 3 or query.size(-1) == 0:
         raise RuntimeError(f"{op}: query must be [tokens, heads, D], got {list(query.shape)}")
     return 1.0 / math.sqrt(query.size(-1)) if softmax_scale is None else softmax_scale
 

@@ -37,7 +37,7 @@ def flash_decode_paged(
             return direct
     op = "flash_decode_paged"
     refuse_gradients(op, query, key_cache, value_cache)
-    if query.dim() != 3:
+    if query.dim() != 3 or query.size(-1) == 0:
         raise RuntimeError(f"{op}: query must be [sequences, heads, D], got {list(query.shape)}")
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(query.size(-1))
