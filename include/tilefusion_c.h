@@ -283,7 +283,7 @@ TF_API int tf_linear_cross_entropy_backward(const float* grad_loss, const void* 
 
 /* A cache of keys and values in pages: token p of sequence b is row p % page_size of page page_table[b][p / page_size].  key and value
  * [pages, page_size, kv_heads, D] of dtype (fp16 or bf16), D 64 or 128, in any order of the first three dimensions: strides in elements from page to
- * page, token to token and head to head, multiples of 8, no less than D (or zero where there is one); both begin at 16-byte boundaries.  page_table [sequences, table_width] int32, rows table_stride
+ * page, token to token (for decoding below 2^26) and head to head, multiples of 8, no less than D (or zero where there is one); both begin at 16-byte boundaries.  page_table [sequences, table_width] int32, rows table_stride
  * apart, and lengths [sequences] int32 are in device memory and may hold anything: a page that the cache does not have is
  * never read or written.  Table entries beyond a sequence's length are not looked at.  (No counterpart in the reference.) */
 typedef struct {
@@ -336,7 +336,8 @@ typedef struct {
   int causal, dtype;
 } tf_packed_attention_t;
 /* out [tokens, heads, D] = softmax(softmax_scale * Q K^T) V per sequence and head, and where lse is not null lse [heads, tokens] fp32 = log sum exp of the
- * scaled scores.  Scores, maxima and sums in fp32; the weights are rounded to dtype for the product with V.  Rows that see no key, and rows of no
+ * scaled scores.  Scores, maxima and sums in fp32; the weights are rounded to dtype for the product with V (in fp16 2^7 to 2^15 times as large, so that those
+ * far below the largest count).  softmax_scale times log2(e) has to be finite in fp32, here as for the gradients and for decoding.  Rows that see no key, and rows of no
  * sequence, are zero and their lse -inf. */
 TF_API int tf_flash_attention_packed(const tf_packed_attention_t* p, void* out, float* lse, void* stream);
 /* Gradients of query, key and value (contiguous, of dtype) from that of out (grad_out [tokens, heads, D]) and the out and lse that the forward call gave.  A

@@ -8,11 +8,12 @@
 //   * the others take 128 rows and walk their keys.  That makes P and dO V^T twice, 7 products instead of 5; sums of dQ from the
 //     key side would need atomics in fp32, whose order changes results, and a pass of their own over 4 bytes an element.
 // Both walk tiles of 32 in a ring in LDS (global_load_lds), their own 32 keys or rows of a wavefront in registers as the second operand of the
-// first two products, whose accumulators are the second operand of the last ones as they are: a lane holds one key (row), its registers
+// first two products, whose accumulators are the second operand of the last ones as they are, P and dS rounded to the type for that (gradients 2.3e-3 to 2.4e-3 from 64 bits in bf16
+// and 2.9e-4 in fp16, relative, over the tensor, where the results' own rounding is 1.7e-3 and 2.1e-4): a lane holds one key (row), its registers
 // four rows (keys).  The tile is read from LDS as rows and, transposed, as columns; one swizzle serves both.  Two workgroups of four wavefronts share a
 // CU, so that one's exponentials run beside the other's products.
-// 4 texts of 2048, 32/8 heads x 128, causal, bf16: 504 us, of which 28 are the first kernel's (HBM) and 475 the second's (7 products at 1.0 PFLOP/s); fp16 645.  11 texts of
-// 30 to 1001, 16/4 heads x 64, fp16: 68 us, 5 + 57 + 5.
+// 4 texts of 2048, 32/8 heads x 128, causal, bf16: 487 to 515 us (as the board's clock is), of which 28 are the first kernel's (HBM) and the rest the second's (7 products at 1.0
+// PFLOP/s); fp16 628 to 647, bound by the questions for powers of two between its products.  11 texts of 30 to 1001, 16/4 heads x 64, fp16: 66 us, 5 + 54 + 6.
 #pragma once
 
 #include "flash_attention.hpp"

@@ -6,10 +6,14 @@
 //   * rows that are the heads of a group of one token after the other (packed_sequences.hpp), and tiles that the device deals out;
 //   * scores that are scaled in fp32, and weights that are summed in fp32 before they are rounded for the product: the log-sum-exp leaves in
 //     fp32 for the backward pass, and a rounding of scaled queries, or a sum of rounded weights, would put 2^-9 (bf16) into it;
+//   * weights that enter the product as one number of the type, which half a step each puts into the result: 2.0e-3 from 64 bits in bf16 (relative, over the
+//     tensor), 1.6e-3 of them the result's own rounding, and 2.2e-4 against 1.9e-4 in fp16.  A number and its remainder, as decoding over pages has
+//     it, whose products are free beside its loads, would be half as many matrix instructions again where those are what bounds;
 //   * rows without a key (more queries than keys), which are zero;
 //   * infinities and NaN among the values of a tile that is masked in part reach the rows that see them and no others.
 // A fragment's address is the first one's, exclusive or a constant, which leaves the registers that masked tiles need.  Bound by the products with the exponentials beside them
-// on long sequences (one of 8192, 32/8 heads x 128, bf16: 451 us, 1.2 PFLOP/s), by what a workgroup takes to begin and end, 8 us, on ragged ones (14 of 64 to 4001: 275 us).
+// on long sequences (one of 8192, 32/8 heads x 128, bf16: 448 to 469 us, 1.2 PFLOP/s, as the board's clock is), by what a workgroup takes to begin and end, 8 us, on ragged ones
+// (14 of 64 to 4001: 257 to 269 us).
 #pragma once
 
 #include "flash_attention.hpp"

@@ -13,8 +13,9 @@
 //     as they are loaded, values pass through 4 KiB of LDS for their transposition, with no barrier.
 //   * Pages are whole tiles: a tile's page is looked up with a scalar load, one tile before it is needed, and the lanes' offsets
 //     within a tile are constants of the launch.
-// 16 texts of 32768 keys, 8 heads x 128: 346 us, 6.2 TB/s; 60 texts of 17 to 8001 keys, 8 x 64: 43 us, 3.7 TB/s, of which 12 go to the launch, the
-// ranges, the first pages and the last parts, as one text of 1999 keys shows, which takes no less.
+// 16 texts of 32768 keys, 8 heads x 128: 343 us, 6.3 TB/s, where the same bytes from one dense cache come at 6.7 (flash_decode.hip); 60 texts of 17 to 8001
+// keys, 8 x 64: 43 us, 3.7 TB/s, of which 12 go to the launch, the ranges, the first pages and the last parts, as one text of 1999 keys shows, which takes
+// no less.  That much is this kernel's arrangement for many texts, and no bound of one: the dense kernel reads as many bytes in 6.3.
 #include <algorithm>
 
 #include "flash_attention.hpp"

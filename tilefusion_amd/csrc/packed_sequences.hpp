@@ -49,7 +49,8 @@ __host__ __device__ inline SequenceTiles sequence_tiles(PackedRange q, PackedRan
 // The `rank`-th of the tiles of `rows` rows that the sequences make, most keys first.  Tile e from a sequence's end ends
 // e * rows rows in front of it and counts as ceil(lkv * group / rows) - e (causal or not: the longest sequences first, and their last
 // tokens).  The largest number that more tiles reach than come before this one is found by halving, each step a
-// sum over the sequences, 64 at a time: a hundred cycles a step with up to 64 sequences, where a sorted list would be a launch of its own.
+// sum over the sequences, 64 at a time: a hundred cycles a step with up to 64 sequences, where a sorted list would be a launch of its own.  (Of more
+// sequences all offsets are read again in each step, by every workgroup: 256 texts of 10 to 200 tokens, 16/4 heads x 64, take 61 us, 1000 of them 571, of whose bytes 66 are.)
 template <bool kKeys>
 TFK_DEVICE PackedTile find_tile(const PackedArgs& a, int rows, int rank) {
   const int lane = threadIdx.x % kWaveSize;

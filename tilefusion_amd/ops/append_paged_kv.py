@@ -41,7 +41,7 @@ def append_paged_kv(
         query: [tokens, heads, D] fp16 or bf16, D 64 or 128; key, value: [tokens, kv_heads, D].  Slices of one projection are read where they are.
         cos, sin: [positions, rotated / 2] fp32 (`rotation_tables`); the first `rotated` elements of a head are turned.
         key_cache, value_cache: [pages, page_size, kv_heads, D], written in place; any order of the first three dimensions in memory
-            (a permuted [pages, kv_heads, page_size, D] is read fastest by `flash_decode_paged`).
+            (a permuted [pages, kv_heads, page_size, D] is read fastest by `flash_decode_paged`), no rows on each other.
         page_table: [sequences, n] int32, the pages of each sequence in their order.
         lengths: [sequences] int32, the lengths with the new tokens.
         offsets: [sequences + 1] int32, ascending: sequence b's new tokens are offsets[b] .. offsets[b + 1] - 1, the last of them at position

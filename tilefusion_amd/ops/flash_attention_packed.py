@@ -115,7 +115,7 @@ def flash_attention_packed(
 
     Returns out [tokens, heads, D], or (out, lse).  The device alone knows the lengths: a call can be captured and replayed with other offsets in the same
     tensors.  Rows that see no key (more queries than keys) and rows of no sequence (behind offsets[-1]) are zero, their lse -inf.  Scores, maxima
-    and sums are fp32; the weights are rounded to the type for the product with V.  Under autograd out carries the backward pass (once: no gradient of a
+    and sums are fp32; the weights are rounded to the type for the product with V, in fp16 2^7 to 2^15 times as large.  Under autograd out carries the backward pass (once: no gradient of a
     gradient, no forward mode), and lse none; neither the call nor that pass is captured into a graph."""
     if not torch.compiler.is_compiling():
         direct = _direct.flash_attention_packed(query, key, value, offsets, kv_offsets, softmax_scale, causal, keep)   # (no gradient is asked for)

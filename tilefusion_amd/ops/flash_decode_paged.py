@@ -23,7 +23,8 @@ def flash_decode_paged(
 
     Args:
         query: [sequences, heads, D] fp16 or bf16, D 64 or 128; head h reads head h // (heads // kv_heads) of the cache.
-        key_cache, value_cache: [pages, page_size, kv_heads, D], page_size a multiple of 16; any order of the first three dimensions in memory.
+        key_cache, value_cache: [pages, page_size, kv_heads, D], page_size a multiple of 16; any order of the first three dimensions in memory,
+            tokens less than 2^26 elements apart.
         page_table: [sequences, n] int32, the pages of each sequence in their order; entries beyond its length may hold anything.
         lengths: [sequences] int32, the new token included (`append_paged_kv` has put it there).
         softmax_scale: 1 / sqrt(D) where it is None.
